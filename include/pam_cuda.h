@@ -85,7 +85,13 @@ enum {
     PAM_OP_PREFILL_TILED = 4,
     PAM_OP_DECODE = 5,
     PAM_OP_APPEND = 6,
-    PAM_OP_BACKWARD = 7
+    PAM_OP_BACKWARD = 7,
+    /* additions: the calls of a speculative step (pamc_plan_step and the following) */
+    PAM_OP_PLAN_STEP = 8,
+    PAM_OP_NORM_ROTATE = 9,
+    PAM_OP_NORM_ROTATE_BACKWARD = 10,
+    PAM_OP_TREE_ATTENTION = 11,
+    PAM_OP_ACCEPT_TREE = 12
 };
 
 /* ------------------------------------------------------------------------
@@ -451,6 +457,162 @@ int32_t pamc_decode_layers(void *ctx, const PamDecodeRequest *requests, int32_t 
 int32_t pamc_prefill_layers(void *ctx, const PamPrefillRequest *requests, int32_t num_layers);
 int32_t pamc_append_layers(void *ctx, const PamAppendRequest *requests, int32_t num_layers,
                            void *const *caches);
+
+/* ------------------------------------------------------------------------
+ * A speculative step: several tokens per request, drafted as a tree, verified
+ * by one pass over the cache.  No counterpart in the reference.
+ *
+ *   pamc_plan_step       lengths (and trees) -> row starts, positions, slots,
+ *                        block tables, ancestor masks
+ *   pamc_norm_rotate     norm of queries and keys for each head, rotation by
+ *                        position, append of keys and values to the pages
+ *   pamc_tree_attention  attention of the step's rows over cache and tree
+ *   pamc_accept_tree     the target model's tokens -> accepted path, slots
+ *   (pamc_reshape_and_cache with those slots appends the accepted rows)
+ *
+ * "Rows" are the new tokens of all requests back to back; request b owns rows
+ * [row_starts[b], row_starts[b + 1]).  Buffers may be device memory of the
+ * context's GPU or host memory (staged inside the call; the pools are device
+ * memory always); memory of another GPU is refused.  While the context's stream
+ * is being captured the calls only record their launches: every buffer must then
+ * be device memory, and the calls that take a workspace must be given one (make one
+ * eager call of each kind first: it loads the kernels).  Two graphs (or streams) that
+ * share a workspace must not run at the same time.
+ * ---------------------------------------------------------------------- */
+
+/* Plan of a step.  new_tokens[b] is taken into [0, max_new_tokens], lengths[b] below zero as
+ * zero; rows beyond num_rows are cut off (the last requests then have fewer or no rows).
+ *   row_starts[b]    sum of the new tokens of the requests before b; row_starts[batch] their sum
+ *   total_lengths[b] lengths[b] + its new tokens
+ *   tables[b][j]     entry j of the request's block list for j < ceil(total / block_size), else 0;
+ *                    the list is row list_index[b] of block_lists (row b without list_index); a
+ *                    row outside [0, num_lists) is an empty list
+ *   positions[r]     lengths[b] + i for the i-th row of request b, with parents lengths[b] + depth
+ *   slots[r]         list[position / block_size] * block_size + position % block_size, -1 where the
+ *                    list has no (or a negative) entry; not with parents, since the nodes of a
+ *                    level share a position (see pamc_accept_tree)
+ *   masks[r]         mask_words words of 32 bits: bit j is set when row r sees the j-th row of its
+ *                    request: itself and its ancestors (without parents: itself and all before)
+ * parents[r] is the index, within its request, of the node a row hangs on; a value that is negative
+ * or not smaller than the row's own index is a root (depth 0).  Trees have at most 1024 nodes.
+ * Rows behind the last request get position -1, slot -1 and an empty mask, which the other calls
+ * of the step skip: a step recorded for num_rows rows can be replayed with fewer. */
+typedef struct PamStepPlanRequest {
+    PamBuffer block_lists; /* int32 [num_lists][list_stride] */
+    PamBuffer list_index;  /* int32 [batch], optional */
+    PamBuffer lengths;     /* int32 [batch] */
+    PamBuffer new_tokens;  /* int32 [batch] */
+    PamBuffer parents;     /* int32 [num_rows], optional */
+    PamBuffer tables;      /* outputs, each optional: int32 [batch][max_num_blocks] */
+    PamBuffer total_lengths; /* uint32 [batch] */
+    PamBuffer row_starts;  /* int32 [batch + 1] */
+    PamBuffer positions;   /* int32 [num_rows] */
+    PamBuffer slots;       /* int64 [num_rows] */
+    PamBuffer masks;       /* uint32 [num_rows][mask_words] */
+    int32_t batch_size, num_lists, list_stride, max_num_blocks, block_size, num_rows, max_new_tokens, mask_words;
+} PamStepPlanRequest;
+int32_t pamc_plan_step(void *ctx, const PamStepPlanRequest *request);
+
+/* n = x * rsqrt(mean(x^2) + epsilon) * weight for each head of q and k, then the first rotary_dim
+ * elements turned by position * inv_freq[i] in the pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1)
+ * when interleaved.  Computed in float32 (the angle in float64), rounded once.
+ * q, k, v are rows of [heads][head_dim] / [kv_heads][head_dim] that start q_stride, k_stride,
+ * v_stride elements apart (0: back to back), so that the parts of one projection's rows need no
+ * copy.  q_out receives the queries; the keys go to k_out, or with their values to the pages
+ * (k_pool and v_pool, [block][kv_head][block_size][head_dim], at slots[r]; a slot outside the
+ * pool is not written), or to both.  q_out may lie over q and k_out over k with equal strides.
+ * Rows with a negative position are skipped: their outputs stay as they were.
+ * cache: the handle that owns the pools; its pools are used then, and it is required for FP8
+ * layers, whose append needs its scales (and cannot be captured).  May be NULL otherwise. */
+typedef struct PamNormRotateRequest {
+    PamBuffer q, k, v;            /* v: with pages only */
+    PamBuffer q_weight, k_weight; /* [head_dim], io type of the layer */
+    PamBuffer inv_freq;           /* float32 [rotary_dim / 2] */
+    PamBuffer positions;          /* int32 [num_rows] */
+    PamBuffer q_out, k_out;       /* k_out optional with pages */
+    PamBuffer k_pool, v_pool, slots; /* slots: int64 [num_rows] */
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride; /* elements, 0: back to back */
+    int32_t num_rows, rotary_dim, interleaved;
+    float epsilon;
+    PamLayerSpec layer;
+} PamNormRotateRequest;
+int32_t pamc_norm_rotate(void *ctx, const PamNormRotateRequest *request, void *cache);
+
+/* Gradient of pamc_norm_rotate.  d_q_out [num_rows][heads][head_dim] and the gradient of the keys
+ * (d_k_out [num_rows][kv_heads][head_dim], or row r's slot of d_k_pool) are given with respect to
+ * the rotated rows; d_q, d_k (rows d_q_stride, d_k_stride elements apart) and the weights'
+ * gradients (float32 [head_dim], optional) are written.  With pages d_v, when wanted, receives
+ * row r's slot of d_v_pool.  A slot outside the pool counts as a gradient of zero; rows with a
+ * negative position are skipped.  FP8 layers are refused (no gradient pools).  The sums over the rows
+ * are taken in a fixed order: equal inputs give equal bits on the same GPU model. */
+typedef struct PamNormRotateBackwardRequest {
+    PamBuffer q, k, q_weight, k_weight, inv_freq, positions;
+    PamBuffer d_q_out, d_k_out, d_k_pool, d_v_pool, slots;
+    PamBuffer d_q, d_k, d_v, d_q_weight, d_k_weight;
+    PamBuffer workspace;          /* optional, see pamc_norm_rotate_backward_workspace */
+    int64_t q_stride, k_stride, d_q_stride, d_k_stride, d_v_stride; /* elements, 0: back to back */
+    int32_t num_rows, rotary_dim, interleaved;
+    float epsilon;
+    PamLayerSpec layer;
+} PamNormRotateBackwardRequest;
+int32_t pamc_norm_rotate_backward(void *ctx, const PamNormRotateBackwardRequest *request);
+/* Bytes of workspace the request needs (only sizes and which buffers are given are read), or -1. */
+int64_t pamc_norm_rotate_backward_workspace(void *ctx, const PamNormRotateBackwardRequest *request);
+
+/* Attention of the rows of a step: row i of request b sees the cache_lengths[b] tokens that
+ * its pages hold and the rows of its own request that masks names (without masks: itself and
+ * all before).  q, k, v are the step's rows (k and v are not in the pages yet), q_stride,
+ * k_stride, v_stride elements apart (0: back to back); softmax scale 1 / sqrt(head_dim).
+ * With a window W (layer.window_size, else the engine's default) a row at position p sees
+ * only keys at positions > p - W, in the cache and in the tree; with masks that needs positions (a
+ * position below the cache length counts as the cache length; without masks and positions row i
+ * stands at cache_lengths[b] + i).  A row that sees nothing is written as zero; values a row
+ * does not see do not reach it, whatever they hold; rows outside every request stay as they
+ * were.  Requests beyond max_new_tokens rows are cut off there. */
+typedef struct PamTreeAttentionRequest {
+    PamBuffer q, k, v, k_pool, v_pool;
+    PamBuffer block_tables;       /* int32 [batch][max_num_blocks] */
+    PamBuffer cache_lengths;      /* uint32 [batch] */
+    PamBuffer row_starts;         /* int32 [batch + 1] */
+    PamBuffer masks;              /* uint32 [num_rows][mask_words], optional */
+    PamBuffer positions;          /* int32 [num_rows], optional */
+    PamBuffer output;             /* [num_rows][heads][head_dim] */
+    PamBuffer k_scale, v_scale;   /* FP8 only */
+    PamBuffer workspace;          /* optional, see pamc_tree_attention_workspace */
+    int64_t q_stride, k_stride, v_stride; /* elements, 0: back to back */
+    int32_t batch_size, max_num_blocks, num_rows, max_new_tokens, mask_words;
+    PamLayerSpec layer;
+} PamTreeAttentionRequest;
+int32_t pamc_tree_attention(void *ctx, const PamTreeAttentionRequest *request);
+/* Bytes of workspace the request needs (only its sizes, types and alignments are read), or -1. */
+int64_t pamc_tree_attention_workspace(void *ctx, const PamTreeAttentionRequest *request);
+
+/* Acceptance of drafted trees (greedy): a node is accepted when it is a root, or its parent is
+ * accepted and draft_tokens[node] == target_tokens[parent], the token the target model puts after
+ * the parent.  The deepest accepted node, the lowest index among equals, ends the accepted path.
+ *   accepted_counts[b]  nodes on the path (0 for a request without rows)
+ *   accepted_rows[b]    their rows, root first, -1 behind them; the first max_path of them
+ *   next_tokens[b]      target_tokens of the path's end, -1 for a request without rows
+ *   new_lengths[b]      lengths[b] + accepted_counts[b]
+ *   slots[r]            slot of position lengths[b] + depth for rows on the path, -1 for all others
+ *                       (pamc_reshape_and_cache skips those); needs block_tables; -1 too where the
+ *                       table ends or its entry is negative
+ * parents as in pamc_plan_step; at most max_tree (<= 1024) nodes of a request are looked at. */
+typedef struct PamAcceptRequest {
+    PamBuffer row_starts;         /* int32 [batch + 1] */
+    PamBuffer parents;            /* int32 [num_rows] */
+    PamBuffer draft_tokens;       /* int32 [num_rows] */
+    PamBuffer target_tokens;      /* int32 [num_rows] */
+    PamBuffer lengths;            /* int32 [batch] */
+    PamBuffer block_tables;       /* int32 [batch][max_num_blocks]; needed for slots */
+    PamBuffer slots;              /* outputs, each optional: int64 [num_rows] */
+    PamBuffer accepted_counts;    /* int32 [batch] */
+    PamBuffer accepted_rows;      /* int32 [batch][max_path] */
+    PamBuffer next_tokens;        /* int32 [batch] */
+    PamBuffer new_lengths;        /* uint32 [batch] */
+    int32_t batch_size, num_rows, max_tree, max_path, max_num_blocks, block_size;
+} PamAcceptRequest;
+int32_t pamc_accept_tree(void *ctx, const PamAcceptRequest *request);
 
 /* ------------------------------------------------------------------------
  * Outputs of a cache sharded by KV head over several GPUs

@@ -16,6 +16,8 @@ _API = {
                   "SchedulerSequence", "SequenceStatus"],
     "engine": ["BatchKVCacheManager", "ContinuousBatchingScheduler", "DeviceBuffer", "KVCacheManager",
                "PagedAttentionEngine", "PagedAttentionInference"],
+    "step_requests": ["PagedAcceptRequest", "PagedNormRotateBackwardRequest", "PagedNormRotateRequest",
+                      "PagedStepPlanRequest", "PagedTreeAttentionRequest"],
 }
 _WHERE = {name: mod for mod, names in _API.items() for name in names}
 __all__ = sorted(_WHERE)

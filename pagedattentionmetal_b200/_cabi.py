@@ -86,6 +86,45 @@ class PamBackwardRequest(C.Structure):
                 ("d_k_pool", PamBuffer), ("d_v_pool", PamBuffer), ("seq_len", c_int32), ("layer", PamLayerSpec)]
 
 
+class PamStepPlanRequest(C.Structure):
+    _fields_ = [(x, PamBuffer) for x in ("block_lists", "list_index", "lengths", "new_tokens", "parents", "tables",
+                                         "total_lengths", "row_starts", "positions", "slots", "masks")] + \
+               [(x, c_int32) for x in ("batch_size", "num_lists", "list_stride", "max_num_blocks", "block_size",
+                                       "num_rows", "max_new_tokens", "mask_words")]
+
+
+class PamNormRotateRequest(C.Structure):
+    _fields_ = [(x, PamBuffer) for x in ("q", "k", "v", "q_weight", "k_weight", "inv_freq", "positions", "q_out", "k_out",
+                                         "k_pool", "v_pool", "slots")] + \
+               [(x, c_int64) for x in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride")] + \
+               [("num_rows", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32), ("epsilon", C.c_float),
+                ("layer", PamLayerSpec)]
+
+
+class PamNormRotateBackwardRequest(C.Structure):
+    _fields_ = [(x, PamBuffer) for x in ("q", "k", "q_weight", "k_weight", "inv_freq", "positions", "d_q_out", "d_k_out",
+                                         "d_k_pool", "d_v_pool", "slots", "d_q", "d_k", "d_v", "d_q_weight", "d_k_weight",
+                                         "workspace")] + \
+               [(x, c_int64) for x in ("q_stride", "k_stride", "d_q_stride", "d_k_stride", "d_v_stride")] + \
+               [("num_rows", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32), ("epsilon", C.c_float),
+                ("layer", PamLayerSpec)]
+
+
+class PamTreeAttentionRequest(C.Structure):
+    _fields_ = [(x, PamBuffer) for x in ("q", "k", "v", "k_pool", "v_pool", "block_tables", "cache_lengths", "row_starts",
+                                         "masks", "positions", "output", "k_scale", "v_scale", "workspace")] + \
+               [(x, c_int64) for x in ("q_stride", "k_stride", "v_stride")] + \
+               [(x, c_int32) for x in ("batch_size", "max_num_blocks", "num_rows", "max_new_tokens", "mask_words")] + \
+               [("layer", PamLayerSpec)]
+
+
+class PamAcceptRequest(C.Structure):
+    _fields_ = [(x, PamBuffer) for x in ("row_starts", "parents", "draft_tokens", "target_tokens", "lengths",
+                                         "block_tables", "slots", "accepted_counts", "accepted_rows", "next_tokens",
+                                         "new_lengths")] + \
+               [(x, c_int32) for x in ("batch_size", "num_rows", "max_tree", "max_path", "max_num_blocks", "block_size")]
+
+
 class PamSchedSequence(C.Structure):
     _fields_ = [("id", c_int64), ("status", c_int32), ("num_generated_tokens", c_int32),
                 ("max_new_tokens", c_int32), ("prompt_length", c_int32), ("arrival_order", c_int32)]
@@ -159,6 +198,13 @@ SIGNATURES = {
     "pamc_prefill_layers": (c_int32, [c_void_p, C.POINTER(PamPrefillRequest), c_int32]),
     "pamc_append_layers": (c_int32, [c_void_p, C.POINTER(PamAppendRequest), c_int32, C.POINTER(c_void_p)]),
     "pamc_fused_prefill": (c_int32, [c_void_p, C.POINTER(PamFusedPrefillRequest), c_void_p]),
+    "pamc_plan_step": (c_int32, [c_void_p, C.POINTER(PamStepPlanRequest)]),
+    "pamc_norm_rotate": (c_int32, [c_void_p, C.POINTER(PamNormRotateRequest), c_void_p]),
+    "pamc_norm_rotate_backward": (c_int32, [c_void_p, C.POINTER(PamNormRotateBackwardRequest)]),
+    "pamc_norm_rotate_backward_workspace": (c_int64, [c_void_p, C.POINTER(PamNormRotateBackwardRequest)]),
+    "pamc_tree_attention": (c_int32, [c_void_p, C.POINTER(PamTreeAttentionRequest)]),
+    "pamc_tree_attention_workspace": (c_int64, [c_void_p, C.POINTER(PamTreeAttentionRequest)]),
+    "pamc_accept_tree": (c_int32, [c_void_p, C.POINTER(PamAcceptRequest)]),
     "pamc_backward": (c_int32, [c_void_p, C.POINTER(PamBackwardRequest)]),
     # scheduler
     "pamc_sched_create": (c_void_p, [c_int32, c_int32]),

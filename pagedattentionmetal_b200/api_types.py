@@ -71,7 +71,7 @@ class SequenceStatus(enum.IntEnum):
 
 
 class Operation(enum.IntEnum):
-    """PagedAttentionStats.Operation (PagedAttentionTypes.swift:171-180)"""
+    """PagedAttentionStats.Operation (PagedAttentionTypes.swift:171-180); from planStep on, additions"""
     none = 0
     prefillSinglePass = 1
     prefillMMA = 2
@@ -80,6 +80,11 @@ class Operation(enum.IntEnum):
     decode = 5
     append = 6
     backward = 7
+    planStep = 8
+    normRotate = 9
+    normRotateBackward = 10
+    treeAttention = 11
+    acceptTree = 12
 
 
 @dataclass

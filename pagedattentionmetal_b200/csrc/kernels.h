@@ -178,6 +178,97 @@ bool prefillFp8StagingApplies(const PrefillParams& p);
 cudaError_t launchFp8StagePages(const PrefillParams& p, const int32_t* seqLens, const int32_t* windowStarts, int maxCount,
                                 void* kOut, void* vOut, int32_t* stagedTables, cudaStream_t stream, int* launches);
 
+// ---- plan and acceptance of a speculative step (step_kernels.cu) ----
+constexpr int kMaxTreeNodes = 1024;   // nodes of one request's draft tree (mask of 32 words)
+struct StepPlanParams {
+    const int32_t* lists;         // [numLists][listStride]: the blocks of every request the caller keeps
+    const int32_t* listIndex;     // [batch] row of `lists`, or null: row b
+    const int32_t* lengths;       // [batch] tokens in the cache
+    const int32_t* newTokens;     // [batch]
+    const int32_t* parents;       // [numRows] or null
+    int32_t* tables;              // outputs, each may be null: [batch][maxNumBlocks]
+    uint32_t* totalLengths;       // [batch]
+    int32_t* rowStarts;           // [batch + 1]
+    int32_t* positions;           // [numRows]
+    int64_t* slots;               // [numRows]
+    uint32_t* masks;              // [numRows][maskWords]
+    int batch, numLists, listStride, maxNumBlocks, numRows, maxNew, maskWords, blockSize;
+};
+cudaError_t launchPlanStep(const StepPlanParams& p, cudaStream_t stream, int* launches);
+
+struct AcceptParams {
+    const int32_t* rowStarts;     // [batch + 1]
+    const int32_t* parents;       // [numRows]
+    const int32_t* draft;         // [numRows]
+    const int32_t* target;        // [numRows]
+    const int32_t* lengths;       // [batch]
+    const int32_t* tables;        // [batch][maxNumBlocks] or null (then no slots)
+    int64_t* slots;               // outputs, each may be null: [numRows]
+    int32_t* counts;              // [batch]
+    int32_t* path;                // [batch][maxPath]
+    int32_t* next;                // [batch]
+    uint32_t* newLengths;         // [batch]
+    int batch, numRows, maxTree, maxPath, maxNumBlocks, blockSize;
+};
+cudaError_t launchAcceptTree(const AcceptParams& p, cudaStream_t stream, int* launches);
+
+// ---- norm and rotation of queries and keys (norm_rotate_kernels.cu) ----
+struct NormRotateParams {
+    const void *q, *k, *v;        // rows of [heads][dim], rows qStride / kStride / vStride elements apart
+    const void *qWeight, *kWeight;   // [dim], io type
+    const float* invFreq;         // [rotaryDim / 2]
+    const int32_t* positions;     // [numRows]; negative: the row is skipped
+    void *qOut, *kOut, *vOut;     // rows; kOut and vOut may be null
+    void *kPool, *vPool;          // pages, or null; with them slots
+    const int64_t* slots;         // [numRows]; a slot outside [0, numSlots) is not written
+    int64_t* slotsOut;            // or null: the slots again, -1 for rows that are skipped
+    int64_t numSlots;
+    int64_t qStride, kStride, vStride, qOutStride, kOutStride, vOutStride;   // elements
+    int numRows, heads, kvHeads, headDim, blockSize, rotaryDim, interleaved, ioType;
+    float eps;
+};
+cudaError_t launchNormRotate(const NormRotateParams& p, cudaStream_t stream, int* launches);
+
+struct NormRotateBackwardParams {
+    const void *q, *k, *qWeight, *kWeight;
+    const float* invFreq;
+    const int32_t* positions;
+    const void *dQOut, *dKOut;    // gradients of the rotated rows, contiguous; dKOut null: from the pages
+    const void *dKPool, *dVPool;
+    const int64_t* slots;
+    int64_t numSlots;
+    void *dQ, *dK, *dV;           // written; dV may be null
+    float *dQWeight, *dKWeight;   // [dim], may be null
+    float* partials;              // normRotateBackwardWorkspaceBytes()
+    int64_t qStride, kStride, dQStride, dKStride, dVStride;
+    int numRows, heads, kvHeads, headDim, blockSize, rotaryDim, interleaved, ioType;
+    float eps;
+};
+size_t normRotateBackwardWorkspaceBytes(const NormRotateBackwardParams& p, int smCount);
+cudaError_t launchNormRotateBackward(const NormRotateBackwardParams& p, int smCount, cudaStream_t stream, int* launches);
+
+// ---- attention of draft trees over the cache (tree_kernels.cu) ----
+constexpr int kTreeMaxBatch = 4096;
+struct TreeParams {
+    const void *q, *kNew, *vNew;  // rows of [heads][dim] / [kvHeads][dim], io type
+    const void *kPool, *vPool;
+    const int32_t* tables;        // [batch][maxNumBlocks]
+    const uint32_t* lens;         // [batch]: tokens in the cache
+    const int32_t* rowStarts;     // [batch + 1]
+    const uint32_t* masks;        // [numRows][maskWords], or null: row i sees the rows up to itself
+    const int32_t* positions;     // [numRows], or null: len + i; read with a window only
+    void* out;                    // [numRows][heads][dim]
+    const void *kScale, *vScale;  // FP8: [block][kvHeads] float16
+    int64_t qStride, kStride, vStride;   // elements between rows
+    int batch, heads, kvHeads, headDim, blockSize, maxNumBlocks, numRows, maxNew, maskWords, window, dtype;
+    int poolBlocks;               // table entries are clamped into [0, poolBlocks)
+    float* workspace;             // treeWorkspaceBytes()
+};
+size_t treeWorkspaceBytes(const TreeParams& p, int smCount);
+// Tiles of the longest list the request's bounds allow; the kernels count them in 32 bits.
+int64_t treeTileBound(const TreeParams& p);
+cudaError_t launchTreeAttention(const TreeParams& p, int smCount, cudaStream_t stream, int* launches);
+
 // ---- all-gather of head-sharded outputs (comm.cu) ----
 // local: [rows][slice] on this GPU (slice = heads/N * dim * element bytes, a multiple of 16);
 // staging: N * rows * slice bytes of scratch; full: [rows][N][slice] on every GPU.

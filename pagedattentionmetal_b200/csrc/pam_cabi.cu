@@ -444,6 +444,20 @@ int32_t runCopies(Context* c, Cache* k, const std::vector<std::pair<int32_t, int
     return 0;
 }
 
+// The absmax scratch of FP8 appends to a cache, made by the first one; every append has its own epoch.
+cudaError_t nextAbsmaxEpoch(Cache* k, cudaStream_t stream) {
+    if (!k->amax) {
+        const size_t bytes = static_cast<size_t>(k->maxBlocks) * k->kvHeads * 2 * sizeof(unsigned long long);
+        cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&k->amax), bytes);
+        if (e != cudaSuccess) return e;
+        e = cudaMemsetAsync(k->amax, 0, bytes, stream);
+        if (e != cudaSuccess) return e;
+        k->epoch = 0;
+    }
+    k->epoch += 1;
+    return cudaSuccess;
+}
+
 int32_t appendImpl(Context* c, const PamAppendRequest& rq, Cache* cacheForScratch, const int64_t* hostSlots,
                    const int64_t* deviceSlots = nullptr) {
     // PagedAttentionEngine.swift:585-628; validateAppend :1935-1950
@@ -490,15 +504,8 @@ int32_t appendImpl(Context* c, const PamAppendRequest& rq, Cache* cacheForScratc
         cudaError_t e;
         if (fp8) {
             Cache* k = cacheForScratch;
-            if (!k->amax) {
-                const size_t bytes = static_cast<size_t>(k->maxBlocks) * k->kvHeads * 2 * sizeof(unsigned long long);
-                e = cudaMalloc(reinterpret_cast<void**>(&k->amax), bytes);
-                if (e != cudaSuccess) return e;
-                e = cudaMemsetAsync(k->amax, 0, bytes, c->stream);
-                if (e != cudaSuccess) return e;
-                k->epoch = 0;
-            }
-            k->epoch += 1;
+            e = nextAbsmaxEpoch(k, c->stream);
+            if (e != cudaSuccess) return e;
             e = pam::launchReshapeAndCacheFp8(keys, values, rq.k_pool.ptr, rq.v_pool.ptr, rq.k_scale.ptr, rq.v_scale.ptr,
                                               src, T, l.num_kv_heads, l.block_size, l.head_dim, k->amax, k->epoch,
                                               c->stream, &launches);
@@ -2408,3 +2415,7 @@ void pamc_infer_set_incremental_preemption(void* infer, int32_t on) {
 }
 
 }  // extern "C"
+
+// ------------------------------------------------------------------ speculative step
+
+#include "step_calls.inl"

@@ -1,0 +1,383 @@
+// Attention of draft trees over the paged cache: the choice of kernel, the general kernel and
+// the kernel that joins the records of shared pairs.  The layout of the work is explained in
+// tree_common.cuh.
+//
+//   out_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(q_i . k_j / sqrt(dim)),
+//
+// over the cache tokens of node i's window and the nodes of its mask; a row that sees nothing is
+// zero.  Scores are kept times log2(e), so that the weights are powers of two.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "tree_common.cuh"
+
+namespace pam {
+namespace {
+
+using namespace tree;
+
+// ---- general kernel -----------------------------------------------------------
+
+// Any type, any head_dim up to 256, any strides: float32 products on the CUDA cores out of
+// shared memory.  16 rows (node, head) against 32 keys at a time, 128 threads; warp w owns rows
+// 4 w .. 4 w + 3 from the scores to the result, so that the only block-wide waits are around
+// the tile loads.  Lane (c, z) = (lane / 4, lane % 4) sums the 4 x 4 scores of its warp's rows and
+// keys 4 c .. 4 c + 3 over every fourth 4-element piece of the dimension (8 loads of 16 bytes for
+// 64 products) and, after a sum over z, keeps row z's four.
+constexpr int kGenRows = 16, kGenKeys = 32, kGenThreads = 128;
+
+struct GeneralSmem {
+    static __host__ __device__ int pad(int dim) { return (dim + 15) / 16 * 16; }
+    static __host__ __device__ size_t bytes(int dim, int batch) {
+        const size_t dp = pad(dim);
+        return (kGenRows * dp + kGenKeys * (dp + 4) + kGenKeys * dp + kGenKeys * kGenRows) * sizeof(float) +
+               2 * kGenKeys * sizeof(long long) * 2 + (kGenThreads / 32 + 4) * sizeof(int) + (static_cast<size_t>(batch) + 1) * sizeof(int);
+    }
+};
+
+template <typename QT, typename KT_>
+__global__ void __launch_bounds__(kGenThreads)
+treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    const int D = p.headDim, dp = GeneralSmem::pad(D), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float* sq = reinterpret_cast<float*>(raw);             // [16][dp]
+    float* sk = sq + kGenRows * dp;                        // [32][dp + 4]
+    float* sv = sk + kGenKeys * (dp + 4);                  // [32][dp]
+    float* sp = sv + kGenKeys * dp;                        // [32][16]
+    long long* kAt = reinterpret_cast<long long*>(sp + kGenKeys * kGenRows);   // [32] element offsets, -1: no key
+    long long* vAt = kAt + kGenKeys;
+    long long* blkAt = vAt + kGenKeys;                     // FP8: the block, for its scales
+    int* scratch = reinterpret_cast<int*>(blkAt + 2 * kGenKeys);
+    int* prefix = scratch + kGenThreads / 32 + 4;
+    buildPrefix<kGenRows, kGenKeys, kGenThreads>(p, prefix, scratch);
+    const int blocks = gridDim.x, me = blockIdx.x, total = prefix[p.batch];
+    const int quota = (total + blocks - 1) / blocks;
+    const int begin = static_cast<int>(min(static_cast<long long>(me) * quota, static_cast<long long>(total))), end = min(total, begin + quota);
+    const int group = p.heads / p.kvHeads, c = lane >> 2, z = lane & 3;
+    if (tid == 0) {
+        Header h{};
+        h.lastBlock = -1;
+        *headerOf(p, me) = h;
+    }
+    for (int t = begin; t < end;) {
+        const Segment g = segmentAt<kGenRows, kGenKeys>(p, prefix, t, end);
+        const SeqInfo& s = g.s;
+        const int cacheTiles = s.cacheTiles<kGenKeys>(), rows = s.n * group;
+        const uint32_t hi = lastFirst(p, s, g.rt, kGenRows);
+        __syncthreads();
+        for (int i = tid; i < kGenRows * dp; i += kGenThreads) {
+            const int r = i / dp, d = i - r * dp, rr = g.rt * kGenRows + r;
+            float v = 0.f;
+            if (rr < rows && d < D)
+                v = valueOf(static_cast<const QT*>(p.q) + static_cast<int64_t>(s.start + rr / group) * p.qStride +
+                            static_cast<int64_t>(g.kvh * group + rr % group) * D + d) * scaleLog2;
+            sq[i] = v;
+        }
+        // the row whose softmax this lane keeps
+        const int row = g.rt * kGenRows + 4 * warp + z, node = min(row / group, s.n - 1);
+        const uint32_t first = firstOf(p, s, node);
+        float m = -INFINITY, l = 0.f;
+        float acc[2][4][4];                                // [dims lane * 4 (+ 128)][row][dim]
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[h][r][e] = 0.f;
+        bool odd = false;
+        for (int j = g.first; j < g.last; ++j) {
+            const bool inTree = j >= cacheTiles;
+            const uint32_t k0 = inTree ? static_cast<uint32_t>(j - cacheTiles) * kGenKeys : (s.lo / kGenKeys + j) * kGenKeys;
+            __syncthreads();
+            if (tid < kGenKeys) {
+                const uint32_t key = k0 + tid;
+                kAt[tid] = vAt[tid] = -1;
+                blkAt[tid] = 0;
+                if (inTree) {
+                    if (key < static_cast<uint32_t>(s.n)) {
+                        kAt[tid] = static_cast<int64_t>(s.start + key) * p.kStride + static_cast<int64_t>(g.kvh) * D;
+                        vAt[tid] = static_cast<int64_t>(s.start + key) * p.vStride + static_cast<int64_t>(g.kvh) * D;
+                    }
+                } else if (key >= s.lo && key < s.held) {
+                    int64_t blk;
+                    kAt[tid] = vAt[tid] = poolRow(p, g.b, key, g.kvh, &blk);
+                    blkAt[tid] = blk;
+                }
+            }
+            __syncthreads();
+            for (int i = tid; i < kGenKeys * dp; i += kGenThreads) {
+                const int r = i / dp, d = i - r * dp;
+                float kv = 0.f, vv = 0.f;
+                if (kAt[r] >= 0 && d < D) {
+                    if (inTree) {
+                        kv = valueOf(static_cast<const QT*>(p.kNew) + kAt[r] + d);
+                        vv = valueOf(static_cast<const QT*>(p.vNew) + vAt[r] + d);
+                    } else {
+                        kv = poolValue<KT_>(p, p.kPool, p.kScale, kAt[r] + d, blkAt[r], g.kvh);
+                        vv = poolValue<KT_>(p, p.vPool, p.vScale, vAt[r] + d, blkAt[r], g.kvh);
+                    }
+                    if ((inTree || k0 + r < hi) && isOdd(vv)) { vv = 0.f; odd = true; }   // (some row may not see the key)
+                }
+                sk[r * (dp + 4) + d] = kv;
+                sv[i] = vv;
+            }
+            __syncthreads();
+            float dot[4][4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) dot[r][k] = 0.f;
+            for (int d = 4 * z; d < dp; d += 16) {
+                float4 a[4], b[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4*>(sq + (4 * warp + r) * dp + d);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) b[k] = *reinterpret_cast<const float4*>(sk + (4 * c + k) * (dp + 4) + d);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        dot[r][k] += a[r].x * b[k].x + a[r].y * b[k].y + a[r].z * b[k].z + a[r].w * b[k].w;
+            }
+            float x[4] = {0.f, 0.f, 0.f, 0.f};             // row z's scores of keys 4 c .. 4 c + 3
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float v = dot[r][k];
+                    v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+                    v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+                    if (r == z) x[k] = v;
+                }
+            uint32_t bits = 0u;
+            if (row < rows) {
+                if (inTree) bits = treeBits(p, s, node, static_cast<int>(k0 / 32));
+                else
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t key = k0 + 4 * c + k;
+                        if (key >= first && key < s.held) bits |= 1u << (4 * c + k);
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (!(bits >> (4 * c + k) & 1u)) x[k] = -INFINITY;
+                top = fmaxf(top, x[k]);
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            const float mNew = fmaxf(m, top), base = mNew == -INFINITY ? 0.f : mNew;
+            const float corr = exp2f(m - base);
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                x[k] = exp2f(x[k] - base);
+                sum += x[k];
+                sp[(4 * c + k) * kGenRows + 4 * warp + z] = x[k];
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            l = l * corr + sum;
+            m = mNew;
+            __syncwarp();
+            float f[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) f[r] = __shfl_sync(0xFFFFFFFFu, corr, r);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int d = 4 * lane + 128 * h;
+                if (d >= dp) break;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[h][r][e] *= f[r];
+#pragma unroll 8
+                for (int k = 0; k < kGenKeys; ++k) {
+                    const float4 w = *reinterpret_cast<const float4*>(sp + k * kGenRows + 4 * warp);
+                    const float4 v = *reinterpret_cast<const float4*>(sv + k * dp + d);
+                    const float ww[4] = {w.x, w.y, w.z, w.w}, vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[h][r][e] += ww[r] * vv[e];
+                }
+            }
+            __syncwarp();
+        }
+        odd = __syncthreads_or(odd);
+        const bool whole = g.whole();
+        float* rec = nullptr;
+        if (!whole) {
+            const int which = g.first == 0 ? 1 : 0;
+            rec = recordOf(p, blocks, me, which, kGenRows, dp);
+            if (tid == 0) {
+                Header* h = headerOf(p, me);
+                h->odd[which] = odd ? 1 : 0;
+                if (which == 1) {
+                    h->b = g.b; h->kvh = g.kvh; h->rt = g.rt;
+                    h->lastBlock = (t + g.nT - 1) / quota;
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float lr = __shfl_sync(0xFFFFFFFFu, l, r), mr = __shfl_sync(0xFFFFFFFFu, m, r);
+            const int rl = 4 * warp + r, rr = g.rt * kGenRows + rl;
+            if (rr >= rows) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int d = 4 * lane + 128 * h;
+                if (d >= dp) break;
+                if (whole) {
+                    const float inv = lr == 0.f ? 0.f : 1.f / lr;
+                    QT* out = static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + g.kvh * group + rr % group) * D;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < D) {
+                            float v = acc[h][r][e] * inv;
+                            if (odd) v += leftOut<QT, KT_>(p, s, g.b, g.kvh, rr / group, hi, d + e);
+                            out[d + e] = narrow<QT>(v);
+                        }
+                } else {
+                    *reinterpret_cast<float4*>(rec + rl * dp + d) = make_float4(acc[h][r][0], acc[h][r][1], acc[h][r][2], acc[h][r][3]);
+                }
+            }
+            if (!whole && lane == 0) {
+                rec[kGenRows * dp + rl] = mr;
+                rec[kGenRows * dp + kGenRows + rl] = lr;
+            }
+        }
+        t += g.last - g.first;
+    }
+}
+
+// ---- the records of shared pairs --------------------------------------------------
+
+// Block (i, y): the pair that block i of the attention kernel starts and does not finish, rows
+// 8 y .. 8 y + 7 of its row tile, one warp each.  Its records lie in block i (the second) and in
+// blocks i + 1 .. lastBlock (the first); their sum in that order is the same in every launch.
+template <typename QT, typename KT_>
+__global__ void __launch_bounds__(256)
+treeJoinKernel(const __grid_constant__ TreeParams p, int blocks, int mr, int dimPad) {
+    cudaGridDependencySynchronize();                   // launched early; the records are there from here on
+    const Header h = *headerOf(p, blockIdx.x);
+    if (h.lastBlock < 0) return;
+    const int lane = threadIdx.x & 31, rl = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const SeqInfo s(p, h.b);
+    const int group = p.heads / p.kvHeads, rr = h.rt * mr + rl;
+    if (rl >= mr || rr >= s.n * group) return;
+    const int first = blockIdx.x, count = h.lastBlock - first + 1;
+    auto record = [&](int i) -> const float* { return recordOf(p, blocks, first + i, i == 0 ? 1 : 0, mr, dimPad); };
+    float top = -INFINITY;
+    bool odd = false;
+    for (int i = lane; i < count; i += 32) {
+        top = fmaxf(top, record(i)[mr * dimPad + rl]);
+        odd = odd || headerOf(p, first + i)->odd[i == 0 ? 1 : 0] != 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    odd = __any_sync(0xFFFFFFFFu, odd);
+    const float base = top == -INFINITY ? 0.f : top;
+    const uint32_t hi = odd ? lastFirst(p, s, h.rt, mr) : 0u;
+    QT* out = static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + h.kvh * group + rr % group) * p.headDim;
+    for (int d = 4 * lane; d < p.headDim; d += 128) {
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) {
+            const float* r = record(i);
+            const float f = exp2f(r[mr * dimPad + rl] - base);
+            const float4 o = *reinterpret_cast<const float4*>(r + rl * dimPad + d);
+            l += f * r[mr * dimPad + mr + rl];
+            sum.x += f * o.x; sum.y += f * o.y; sum.z += f * o.z; sum.w += f * o.w;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l, v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < p.headDim) {
+                float x = v[e] * inv;
+                if (odd) x += leftOut<QT, KT_>(p, s, h.b, h.kvh, rr / group, hi, d + e);
+                out[d + e] = narrow<QT>(x);
+            }
+    }
+}
+
+template <typename QT, typename KT_>
+cudaError_t launchJoin(const TreeParams& p, const TreePlan& plan, cudaStream_t stream, int* launches) {
+    if (plan.blocks < 2) return cudaSuccess;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(plan.blocks - 1, (plan.rows + 7) / 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    *launches += 1;
+    return cudaLaunchKernelEx(&cfg, treeJoinKernel<QT, KT_>, p, plan.blocks, plan.rows, plan.dimPad);
+}
+
+// Dynamic shared memory above 48 KB has to be allowed once per device and kernel.
+template <typename K>
+cudaError_t allowSmem(K kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+TreePlan treePlan(const TreeParams& p, int smCount) {
+    TreePlan t{};
+    t.rows = kGenRows;
+    t.keys = kGenKeys;
+    t.dimPad = GeneralSmem::pad(p.headDim);
+    // as many blocks as an SM's shared memory holds, four at most
+    const size_t smem = GeneralSmem::bytes(p.headDim, p.batch);
+    const int perSm = static_cast<int>(std::min<size_t>(4, std::max<size_t>(1, (227u * 1024) / (smem + 1024))));
+    t.blocks = smCount * perSm;
+    return t;
+}
+
+template <typename QT, typename KT_>
+cudaError_t generalOf(const TreeParams& p, const TreePlan& plan, cudaStream_t stream, int* launches) {
+    static std::atomic<unsigned long long> done{0};
+    const size_t smem = GeneralSmem::bytes(p.headDim, p.batch);
+    cudaError_t e = allowSmem(treeGeneralKernel<QT, KT_>, 227 * 1024, done);
+    if (e != cudaSuccess) return e;
+    const float scaleLog2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.headDim));
+    treeGeneralKernel<QT, KT_><<<plan.blocks, kGenThreads, smem, stream>>>(p, scaleLog2);
+    *launches += 1;
+    e = cudaGetLastError();
+    return e == cudaSuccess ? launchJoin<QT, KT_>(p, plan, stream, launches) : e;
+}
+
+}  // namespace
+
+int64_t treeTileBound(const TreeParams& p) {
+    const int64_t rowTiles = (static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) + kGenRows - 1) / kGenRows;
+    const int64_t keyTiles = static_cast<int64_t>(p.maxNumBlocks) * p.blockSize / kGenKeys + 2 + p.maxNew / kGenKeys + 1;
+    return static_cast<int64_t>(p.batch) * p.kvHeads * rowTiles * keyTiles;
+}
+
+size_t treeWorkspaceBytes(const TreeParams& p, int smCount) {
+    const TreePlan t = treePlan(p, smCount);
+    return tree::headerBytes(t.blocks) + static_cast<size_t>(t.blocks) * 2 * tree::recordFloats(t.rows, t.dimPad) * sizeof(float);
+}
+
+cudaError_t launchTreeAttention(const TreeParams& p, int smCount, cudaStream_t stream, int* launches) {
+    const TreePlan plan = treePlan(p, smCount);
+    switch (p.dtype) {
+        case kF32: return generalOf<float, float>(p, plan, stream, launches);
+        case kF16: return generalOf<__half, __half>(p, plan, stream, launches);
+        case kBF16: return generalOf<__nv_bfloat16, __nv_bfloat16>(p, plan, stream, launches);
+        default: return generalOf<__half, uint8_t>(p, plan, stream, launches);
+    }
+}
+
+}  // namespace pam

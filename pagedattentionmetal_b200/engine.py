@@ -22,6 +22,8 @@ from .api_types import (BlockEvictionPolicy, KVCacheError, KVCacheMemoryStats, L
                         PagedAttentionError, PagedAttentionFusedPrefillRequest, PagedAttentionPrefillRequest,
                         PagedAttentionStats,
                         PagedKVAppendRequest, PagedLayerSpec, SchedulerSequence, SequenceStatus)
+from .step_requests import (PagedAcceptRequest, PagedNormRotateBackwardRequest, PagedNormRotateRequest,
+                            PagedStepPlanRequest, PagedTreeAttentionRequest)
 
 
 def _raise(ctx) -> None:
@@ -317,6 +319,51 @@ class PagedAttentionEngine:
                                    request.numNewTokens, _layer(request.layer), _buf(request.kScaleBuffer),
                                    _buf(request.vScaleBuffer))
         _check(self._ctx, lib.pamc_append_to_cache(self._ctx, C.byref(r)))
+
+    # -- a speculative step (no reference counterpart; see include/pam_cuda.h) --
+    def planStep(self, request: "PagedStepPlanRequest") -> None:
+        """Row starts, positions, slots, block tables and ancestor masks of a step, on the
+        GPU, from the lengths of its requests (pamc_plan_step)."""
+        if lib.pamc_plan_step(self._ctx, request._ref) != 0:
+            _raise(self._ctx)
+
+    def normRotate(self, request: "PagedNormRotateRequest", cache: Optional["KVCacheManager"] = None) -> None:
+        """Norm of queries and keys for each head, rotation by position, and the append of
+        keys and values to the pages, in one pass (pamc_norm_rotate).  cache: the manager
+        that owns the pools; required for FP8."""
+        if lib.pamc_norm_rotate(self._ctx, request._ref, cache._h if cache is not None else None) != 0:
+            _raise(self._ctx)
+
+    def normRotateBackward(self, request: "PagedNormRotateBackwardRequest") -> None:
+        """Gradient of normRotate (pamc_norm_rotate_backward)."""
+        if lib.pamc_norm_rotate_backward(self._ctx, request._ref) != 0:
+            _raise(self._ctx)
+
+    def normRotateBackwardWorkspace(self, request: "PagedNormRotateBackwardRequest") -> int:
+        """Bytes of workspace the request needs (required while a stream is being captured)."""
+        n = lib.pamc_norm_rotate_backward_workspace(self._ctx, request._ref)
+        if n < 0:
+            _raise(self._ctx)
+        return int(n)
+
+    def treeAttention(self, request: "PagedTreeAttentionRequest") -> None:
+        """Attention of a step's rows, drafted as trees, over the cache and their own trees
+        (pamc_tree_attention)."""
+        if lib.pamc_tree_attention(self._ctx, request._ref) != 0:
+            _raise(self._ctx)
+
+    def treeAttentionWorkspace(self, request: "PagedTreeAttentionRequest") -> int:
+        """Bytes of workspace the request needs (required while a stream is being captured)."""
+        n = lib.pamc_tree_attention_workspace(self._ctx, request._ref)
+        if n < 0:
+            _raise(self._ctx)
+        return int(n)
+
+    def acceptTree(self, request: "PagedAcceptRequest") -> None:
+        """The accepted path of every drafted tree, the slots of its rows (for
+        reshapeAndCache) and the next token (pamc_accept_tree)."""
+        if lib.pamc_accept_tree(self._ctx, request._ref) != 0:
+            _raise(self._ctx)
 
     # -- batched-layer calls (PagedAttentionEngine.swift:1433-1895) --
     @staticmethod

@@ -1,0 +1,137 @@
+"""Requests of the calls of a speculative step (include/pam_cuda.h: pamc_plan_step,
+pamc_norm_rotate, pamc_norm_rotate_backward, pamc_tree_attention, pamc_accept_tree).
+
+A request is a live C struct: assigning a field writes it, so that a serving loop builds
+a request once over its static buffers and passes it every step without any conversion.
+The buffers assigned to a request are kept alive by it.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _cabi
+from .api_types import PagedLayerSpec
+
+
+def _span(x) -> _cabi.PamBuffer:
+    """A buffer argument with its length; a strided torch view reaches from its first to its last element."""
+    if x is None:
+        return _cabi.PamBuffer(None, 0)
+    if hasattr(x, "is_contiguous") and x.numel() and not x.is_contiguous():
+        last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+        return _cabi.PamBuffer(x.data_ptr(), (last + 1) * x.element_size())
+    return _cabi.buffer(x)
+
+
+class _Request:
+    """Fields by their Python names; `_fields` maps them to the struct's, with the default of a plain number."""
+    _struct: type
+    _fields: dict
+    _required: tuple
+
+    def __init__(self, **values):
+        object.__setattr__(self, "_c", self._struct())
+        object.__setattr__(self, "_values", {})
+        object.__setattr__(self, "_ref", C.byref(self._c))
+        missing = [x for x in self._required if x not in values]
+        if missing:
+            raise TypeError(f"{type(self).__name__} needs {', '.join(missing)}")
+        for name, (field, default) in self._fields.items():
+            setattr(self, name, values.pop(name, default))
+        if values:
+            raise TypeError(f"{type(self).__name__} has no field {', '.join(values)}")
+
+    def __setattr__(self, name, value):
+        if name not in self._fields:
+            raise AttributeError(f"{type(self).__name__} has no field {name}")
+        field, default = self._fields[name]
+        if isinstance(value, PagedLayerSpec):
+            c = _cabi.PamLayerSpec(value.headDim, value.numHeads, value.numKVHeads, value.blockSize,
+                                   int(value.dataType), value.windowSize)
+        elif isinstance(default, float):
+            c = float(value)
+        elif default is None:
+            c = _span(value)
+        else:
+            c = int(value)
+        setattr(self._c, field, c)
+        self._values[name] = value
+
+    def __getattr__(self, name):                     # (a name that is no field must not look for _values)
+        if name in type(self)._fields and "_values" in self.__dict__:
+            return self._values[name]
+        raise AttributeError(f"{type(self).__name__} has no field {name}")
+
+
+def _buffers(**names):
+    return {name: (field, None) for name, field in names.items()}
+
+
+def _numbers(**names):
+    return {name: (field, 0) for name, field in names.items()}
+
+
+class PagedStepPlanRequest(_Request):
+    """PamStepPlanRequest: row starts, positions, slots, block tables and masks from the lengths of a batch."""
+    _struct = _cabi.PamStepPlanRequest
+    _fields = {**_buffers(blockLists="block_lists", listIndex="list_index", lengths="lengths", newTokens="new_tokens",
+                          parents="parents", tables="tables", totalLengths="total_lengths", rowStarts="row_starts",
+                          positions="positions", slots="slots", masks="masks"),
+               **_numbers(batchSize="batch_size", numLists="num_lists", listStride="list_stride",
+                          maxNumBlocks="max_num_blocks", blockSize="block_size", numRows="num_rows",
+                          maxNewTokens="max_new_tokens", maskWords="mask_words")}
+    _required = ("blockLists", "lengths", "newTokens", "batchSize", "numLists", "listStride", "blockSize", "numRows",
+                 "maxNewTokens")
+
+
+class PagedNormRotateRequest(_Request):
+    """PamNormRotateRequest: norm and rotation of queries and keys, append to the pages."""
+    _struct = _cabi.PamNormRotateRequest
+    _fields = {**_buffers(q="q", k="k", v="v", qWeight="q_weight", kWeight="k_weight", invFreq="inv_freq",
+                          positions="positions", qOut="q_out", kOut="k_out", kPool="k_pool", vPool="v_pool",
+                          slots="slots"),
+               **_numbers(qStride="q_stride", kStride="k_stride", vStride="v_stride", qOutStride="q_out_stride",
+                          kOutStride="k_out_stride", numRows="num_rows", rotaryDim="rotary_dim",
+                          interleaved="interleaved"),
+               "epsilon": ("epsilon", 1e-6), "layer": ("layer", PagedLayerSpec(0, 0, 0))}
+    _required = ("q", "k", "qWeight", "kWeight", "positions", "qOut", "numRows", "rotaryDim", "layer")
+
+
+class PagedNormRotateBackwardRequest(_Request):
+    """PamNormRotateBackwardRequest: the gradient of PagedNormRotateRequest."""
+    _struct = _cabi.PamNormRotateBackwardRequest
+    _fields = {**_buffers(q="q", k="k", qWeight="q_weight", kWeight="k_weight", invFreq="inv_freq",
+                          positions="positions", dQOut="d_q_out", dKOut="d_k_out", dKPool="d_k_pool", dVPool="d_v_pool",
+                          slots="slots", dQ="d_q", dK="d_k", dV="d_v", dQWeight="d_q_weight", dKWeight="d_k_weight",
+                          workspace="workspace"),
+               **_numbers(qStride="q_stride", kStride="k_stride", dQStride="d_q_stride", dKStride="d_k_stride",
+                          dVStride="d_v_stride", numRows="num_rows", rotaryDim="rotary_dim",
+                          interleaved="interleaved"),
+               "epsilon": ("epsilon", 1e-6), "layer": ("layer", PagedLayerSpec(0, 0, 0))}
+    _required = ("q", "k", "qWeight", "kWeight", "positions", "dQOut", "dQ", "dK", "numRows", "rotaryDim", "layer")
+
+
+class PagedTreeAttentionRequest(_Request):
+    """PamTreeAttentionRequest: attention of the rows of a step over the cache and their own trees."""
+    _struct = _cabi.PamTreeAttentionRequest
+    _fields = {**_buffers(q="q", k="k", v="v", kPool="k_pool", vPool="v_pool", blockTables="block_tables",
+                          cacheLengths="cache_lengths", rowStarts="row_starts", masks="masks", positions="positions",
+                          output="output", kScaleBuffer="k_scale", vScaleBuffer="v_scale", workspace="workspace"),
+               **_numbers(qStride="q_stride", kStride="k_stride", vStride="v_stride", batchSize="batch_size",
+                          maxNumBlocks="max_num_blocks", numRows="num_rows", maxNewTokens="max_new_tokens",
+                          maskWords="mask_words"),
+               "layer": ("layer", PagedLayerSpec(0, 0, 0))}
+    _required = ("q", "k", "v", "kPool", "vPool", "blockTables", "cacheLengths", "rowStarts", "output", "batchSize",
+                 "maxNumBlocks", "numRows", "maxNewTokens", "layer")
+
+
+class PagedAcceptRequest(_Request):
+    """PamAcceptRequest: the accepted path of every drafted tree, its slots and next token."""
+    _struct = _cabi.PamAcceptRequest
+    _fields = {**_buffers(rowStarts="row_starts", parents="parents", draftTokens="draft_tokens",
+                          targetTokens="target_tokens", lengths="lengths", blockTables="block_tables", slots="slots",
+                          acceptedCounts="accepted_counts", acceptedRows="accepted_rows", nextTokens="next_tokens",
+                          newLengths="new_lengths"),
+               **_numbers(batchSize="batch_size", numRows="num_rows", maxTree="max_tree", maxPath="max_path",
+                          maxNumBlocks="max_num_blocks", blockSize="block_size")}
+    _required = ("rowStarts", "parents", "draftTokens", "targetTokens", "lengths", "batchSize", "numRows", "maxTree")
