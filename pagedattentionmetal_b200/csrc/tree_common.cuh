@@ -173,14 +173,12 @@ __device__ __forceinline__ int64_t poolRow(const TreeParams& p, int b, uint32_t 
     return ((blk * p.kvHeads + kvh) * p.blockSize + (token - page * p.blockSize)) * static_cast<int64_t>(p.headDim);
 }
 
-// FP8: code times scale, rounded to float16 once.
-__device__ __forceinline__ __half dequant(uint8_t code, __half scale) {
-    return __hmul(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3)), scale);
-}
+// A pool's element; FP8: code times scale, in float32.
 template <typename KT_>
 __device__ __forceinline__ float poolValue(const TreeParams& p, const void* pool, const void* scale, int64_t at, int64_t blk, int kvh) {
     if constexpr (sizeof(KT_) == 1)
-        return __half2float(dequant(static_cast<const uint8_t*>(pool)[at], static_cast<const __half*>(scale)[blk * p.kvHeads + kvh]));
+        return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(pool)[at], __NV_E4M3))) *
+               __half2float(static_cast<const __half*>(scale)[blk * p.kvHeads + kvh]);
     else
         return valueOf(static_cast<const KT_*>(pool) + at);
 }
@@ -220,13 +218,14 @@ template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float
 
 }  // namespace tree
 
-// The attention kernels; launchTreeAttention picks one.  Each launches its main kernel over
-// `blocks` blocks and the kernel that joins the records.
+// How a request is launched: the kernel, its tiles, the columns of a record, the blocks.
 struct TreePlan {
-    int variant;       // see treePlan
-    int rows;          // MR
-    int keys;          // KT
-    int dimPad;        // columns of a record
-    int blocks;
+    int variant;       // 0: treeGeneralKernel, 1: treeMmaKernel
+    int rows, keys, dimPad, blocks;
 };
+// tree_mma_kernel.cu: 16-bit and FP8 pools, head_dim up to 128, everything on 16 bytes.
+bool treeMmaApplies(const TreeParams& p);
+TreePlan treeMmaPlan(const TreeParams& p, int smCount);
+cudaError_t launchTreeMma(const TreeParams& p, const TreePlan& plan, cudaStream_t stream);
+
 }  // namespace pam

@@ -333,6 +333,7 @@ cudaError_t allowSmem(K kernel, size_t bytes, std::atomic<unsigned long long>& d
 }
 
 TreePlan treePlan(const TreeParams& p, int smCount) {
+    if (treeMmaApplies(p)) return treeMmaPlan(p, smCount);
     TreePlan t{};
     t.rows = kGenRows;
     t.keys = kGenKeys;
@@ -345,15 +346,19 @@ TreePlan treePlan(const TreeParams& p, int smCount) {
 }
 
 template <typename QT, typename KT_>
-cudaError_t generalOf(const TreeParams& p, const TreePlan& plan, cudaStream_t stream, int* launches) {
+cudaError_t launchGeneral(const TreeParams& p, const TreePlan& plan, cudaStream_t stream) {
     static std::atomic<unsigned long long> done{0};
-    const size_t smem = GeneralSmem::bytes(p.headDim, p.batch);
     cudaError_t e = allowSmem(treeGeneralKernel<QT, KT_>, 227 * 1024, done);
     if (e != cudaSuccess) return e;
     const float scaleLog2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.headDim));
-    treeGeneralKernel<QT, KT_><<<plan.blocks, kGenThreads, smem, stream>>>(p, scaleLog2);
+    treeGeneralKernel<QT, KT_><<<plan.blocks, kGenThreads, GeneralSmem::bytes(p.headDim, p.batch), stream>>>(p, scaleLog2);
+    return cudaGetLastError();
+}
+
+template <typename QT, typename KT_>
+cudaError_t launchOf(const TreeParams& p, const TreePlan& plan, cudaStream_t stream, int* launches) {
+    const cudaError_t e = plan.variant == 1 ? launchTreeMma(p, plan, stream) : launchGeneral<QT, KT_>(p, plan, stream);
     *launches += 1;
-    e = cudaGetLastError();
     return e == cudaSuccess ? launchJoin<QT, KT_>(p, plan, stream, launches) : e;
 }
 
@@ -373,10 +378,10 @@ size_t treeWorkspaceBytes(const TreeParams& p, int smCount) {
 cudaError_t launchTreeAttention(const TreeParams& p, int smCount, cudaStream_t stream, int* launches) {
     const TreePlan plan = treePlan(p, smCount);
     switch (p.dtype) {
-        case kF32: return generalOf<float, float>(p, plan, stream, launches);
-        case kF16: return generalOf<__half, __half>(p, plan, stream, launches);
-        case kBF16: return generalOf<__nv_bfloat16, __nv_bfloat16>(p, plan, stream, launches);
-        default: return generalOf<__half, uint8_t>(p, plan, stream, launches);
+        case kF32: return launchOf<float, float>(p, plan, stream, launches);
+        case kF16: return launchOf<__half, __half>(p, plan, stream, launches);
+        case kBF16: return launchOf<__nv_bfloat16, __nv_bfloat16>(p, plan, stream, launches);
+        default: return launchOf<__half, uint8_t>(p, plan, stream, launches);
     }
 }
 

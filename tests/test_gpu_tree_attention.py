@@ -21,10 +21,10 @@ WEIGHT = {DT.float32: 2.0 ** -24, DT.float16: 2.0 ** -11, DT.bfloat16: 2.0 ** -8
 
 
 def dequantised(codes, scale):
-    """Codes times scale in float16, one rounding."""
+    """Codes times scale."""
     import torch
     value = torch.from_numpy(codes).view(torch.float8_e4m3fn).to(torch.float16).numpy()
-    return (value * scale[:, :, None, None]).astype(np.float16).astype(np.float64)
+    return value.astype(np.float64) * scale.astype(np.float64)[:, :, None, None]
 
 
 class TreeCase:
