@@ -20,8 +20,8 @@ LIB = os.path.join(HERE, "libpam_cuda.so")
 INCLUDE = os.path.join(HERE, "..", "include")
 
 SOURCES = ["cache_kernels.cu", "decode_kernels.cu", "decode_stream_kernel.cu", "prefill_kernels.cu", "prefill_tc_kernel.cu", "backward_kernels.cu", "backward_mma_kernels.cu", "pam_cabi.cu",
-           "comm.cu", "step_kernels.cu", "norm_rotate_kernels.cu", "tree_kernels.cu", "tree_mma_kernel.cu", "block_manager.cpp"]
-HEADERS = ["kernels.h", "step_calls.inl", "tree_common.cuh", "block_manager.h", os.path.join(INCLUDE, "pam_cuda.h")]
+           "comm.cu", "step_kernels.cu", "norm_rotate_kernels.cu", "tree_kernels.cu", "tree_mma_kernel.cu", "tree_tc_kernel.cu", "block_manager.cpp"]
+HEADERS = ["kernels.h", "step_calls.inl", "tree_common.cuh", "tc_common.cuh", "block_manager.h", os.path.join(INCLUDE, "pam_cuda.h")]
 
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",

@@ -263,11 +263,15 @@ struct TreeParams {
     int batch, heads, kvHeads, headDim, blockSize, maxNumBlocks, numRows, maxNew, maskWords, window, dtype;
     int poolBlocks;               // table entries are clamped into [0, poolBlocks)
     float* workspace;             // treeWorkspaceBytes()
+    int* errFlag;                 // device word the tensor-core kernel sets when a bounded wait runs out
+    long long waitCycles;         // that bound; 0: the default
 };
+// Enough for every kernel that a request of these sizes and types may run on.
 size_t treeWorkspaceBytes(const TreeParams& p, int smCount);
 // Tiles of the longest list the request's bounds allow; the kernels count them in 32 bits.
 int64_t treeTileBound(const TreeParams& p);
-cudaError_t launchTreeAttention(const TreeParams& p, int smCount, cudaStream_t stream, int* launches);
+// `bounded`: set when the kernel's waits are bounded and may have raised errFlag.
+cudaError_t launchTreeAttention(const TreeParams& p, int smCount, cudaStream_t stream, int* launches, bool* bounded);
 
 // ---- all-gather of head-sharded outputs (comm.cu) ----
 // local: [rows][slice] on this GPU (slice = heads/N * dim * element bytes, a multiple of 16);

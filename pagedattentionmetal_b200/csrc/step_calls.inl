@@ -550,7 +550,9 @@ int32_t pamc_tree_attention(void* ctx, const PamTreeAttentionRequest* request) {
             if (s->bytes != kUnknownBytes) p.poolBlocks = static_cast<int>(std::min<size_t>(static_cast<size_t>(p.poolBlocks), s->bytes / scaleNeed));
     const double t0 = nowMs();
     if (!capturing) c->arena.reset(c->stream);
-    size_t need = 0;
+    p.errFlag = c->devErr;
+    p.waitCycles = c->waitLimitCycles;
+    const size_t need = pam::treeWorkspaceBytes(p, c->smCount);
     int32_t rc = stepRun(c, "treeAttention", args, n, capturing, [&](int* launches) -> cudaError_t {
         p.q = args[0].device; p.kNew = args[1].device; p.vNew = args[2].device; p.kPool = args[3].device; p.vPool = args[4].device;
         p.tables = static_cast<const int32_t*>(args[5].device);
@@ -560,13 +562,16 @@ int32_t pamc_tree_attention(void* ctx, const PamTreeAttentionRequest* request) {
         p.positions = static_cast<const int32_t*>(args[9].device);
         p.out = args[10].device;
         p.kScale = args[11].device; p.vScale = args[12].device;
-        // (staged copies are better aligned than their sources and may take another kernel)
-        const size_t here = pam::treeWorkspaceBytes(p, c->smCount);
-        need = std::max(need, here);
-        const bool own = rq.workspace.ptr && (rq.workspace.bytes == kUnknownBytes || rq.workspace.bytes >= here);
-        p.workspace = static_cast<float*>(own ? rq.workspace.ptr : c->arena.take(here));
+        p.workspace = static_cast<float*>(rq.workspace.ptr ? rq.workspace.ptr : c->arena.take(need));
         if (!p.workspace) return cudaErrorMemoryAllocation;
-        return pam::launchTreeAttention(p, c->smCount, c->stream, launches);
+        bool bounded = false;
+        cudaError_t e = pam::launchTreeAttention(p, c->smCount, c->stream, launches, &bounded);
+        if (e == cudaSuccess && bounded) {
+            // as in prefillImpl: fetched now when the call waits for the GPU, else by pamc_synchronize
+            if (!c->async && !capturing) e = cudaMemcpyAsync(c->hostErr, c->devErr, sizeof(int), cudaMemcpyDeviceToHost, c->stream);
+            c->errPending = true;
+        }
+        return e;
     });
     if (rc != 0) {
         if (!c->graceful || capturing) return rc;

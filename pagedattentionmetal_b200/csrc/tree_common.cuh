@@ -186,7 +186,7 @@ __device__ __forceinline__ float poolValue(const TreeParams& p, const void* pool
 // Sum of the values in column d that were taken as zero although node i sees them; hi: the first
 // token that every row of the row tile sees.
 template <typename QT, typename KT_>
-__device__ __noinline__ float leftOut(const TreeParams& p, const SeqInfo& s, int b, int kvh, int i, uint32_t hi, int d) {
+__device__ __noinline__ float leftOut(const TreeParams& p, SeqInfo s, int b, int kvh, int i, uint32_t hi, int d) {
     float sum = 0.f;
     for (uint32_t t = firstOf(p, s, i); t < hi; ++t) {
         int64_t blk;
@@ -220,12 +220,16 @@ template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float
 
 // How a request is launched: the kernel, its tiles, the columns of a record, the blocks.
 struct TreePlan {
-    int variant;       // 0: treeGeneralKernel, 1: treeMmaKernel
+    int variant;       // 0: treeGeneralKernel, 1: treeMmaKernel, 2: treeTcKernel
     int rows, keys, dimPad, blocks;
 };
 // tree_mma_kernel.cu: 16-bit and FP8 pools, head_dim up to 128, everything on 16 bytes.
 bool treeMmaApplies(const TreeParams& p);
 TreePlan treeMmaPlan(const TreeParams& p, int smCount);
 cudaError_t launchTreeMma(const TreeParams& p, const TreePlan& plan, cudaStream_t stream);
+// tree_tc_kernel.cu: 16-bit pools, head_dim 128, block sizes that are multiples of 16.
+bool treeTcApplies(const TreeParams& p);
+TreePlan treeTcPlan(const TreeParams& p, int smCount);
+cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t stream);
 
 }  // namespace pam

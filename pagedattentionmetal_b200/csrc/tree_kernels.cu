@@ -332,8 +332,7 @@ cudaError_t allowSmem(K kernel, size_t bytes, std::atomic<unsigned long long>& d
     return e;
 }
 
-TreePlan treePlan(const TreeParams& p, int smCount) {
-    if (treeMmaApplies(p)) return treeMmaPlan(p, smCount);
+TreePlan generalPlan(const TreeParams& p, int smCount) {
     TreePlan t{};
     t.rows = kGenRows;
     t.keys = kGenKeys;
@@ -343,6 +342,16 @@ TreePlan treePlan(const TreeParams& p, int smCount) {
     const int perSm = static_cast<int>(std::min<size_t>(4, std::max<size_t>(1, (227u * 1024) / (smem + 1024))));
     t.blocks = smCount * perSm;
     return t;
+}
+
+TreePlan treePlan(const TreeParams& p, int smCount) {
+    if (treeTcApplies(p) && static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) > 16) return treeTcPlan(p, smCount);
+    if (treeMmaApplies(p)) return treeMmaPlan(p, smCount);
+    return generalPlan(p, smCount);
+}
+
+size_t planBytes(const TreePlan& t) {
+    return headerBytes(t.blocks) + static_cast<size_t>(t.blocks) * 2 * recordFloats(t.rows, t.dimPad) * sizeof(float);
 }
 
 template <typename QT, typename KT_>
@@ -357,7 +366,8 @@ cudaError_t launchGeneral(const TreeParams& p, const TreePlan& plan, cudaStream_
 
 template <typename QT, typename KT_>
 cudaError_t launchOf(const TreeParams& p, const TreePlan& plan, cudaStream_t stream, int* launches) {
-    const cudaError_t e = plan.variant == 1 ? launchTreeMma(p, plan, stream) : launchGeneral<QT, KT_>(p, plan, stream);
+    const cudaError_t e = plan.variant == 2 ? launchTreeTc(p, plan, stream) : plan.variant == 1 ? launchTreeMma(p, plan, stream)
+                                                                            : launchGeneral<QT, KT_>(p, plan, stream);
     *launches += 1;
     return e == cudaSuccess ? launchJoin<QT, KT_>(p, plan, stream, launches) : e;
 }
@@ -371,12 +381,16 @@ int64_t treeTileBound(const TreeParams& p) {
 }
 
 size_t treeWorkspaceBytes(const TreeParams& p, int smCount) {
-    const TreePlan t = treePlan(p, smCount);
-    return tree::headerBytes(t.blocks) + static_cast<size_t>(t.blocks) * 2 * tree::recordFloats(t.rows, t.dimPad) * sizeof(float);
+    // by sizes and types alone: alignment may change between the query and the call (staged copies)
+    size_t n = planBytes(generalPlan(p, smCount));
+    if (p.dtype != kF32 && p.headDim <= 128) n = std::max(n, planBytes(treeMmaPlan(p, smCount)));
+    if (p.dtype != kF32 && p.headDim == 128) n = std::max(n, planBytes(treeTcPlan(p, smCount)));
+    return n;
 }
 
-cudaError_t launchTreeAttention(const TreeParams& p, int smCount, cudaStream_t stream, int* launches) {
+cudaError_t launchTreeAttention(const TreeParams& p, int smCount, cudaStream_t stream, int* launches, bool* bounded) {
     const TreePlan plan = treePlan(p, smCount);
+    *bounded = plan.variant == 2;
     switch (p.dtype) {
         case kF32: return launchOf<float, float>(p, plan, stream, launches);
         case kF16: return launchOf<__half, __half>(p, plan, stream, launches);

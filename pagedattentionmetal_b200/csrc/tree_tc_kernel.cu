@@ -1,0 +1,725 @@
+// Tree attention on the 5th-generation tensor cores: float16 / bfloat16 pools, head_dim 128, block
+// sizes that are multiples of 16.  The products and the softmax are those of the prefill kernel
+// (prefill_tc_kernel.cu): S = Q K^T and O += P V as tcgen05.mma 128 x 128 x 16 with S, P and O in
+// tensor memory, one softmax thread per row, keys and values by TMA straight from the pages.  What
+// differs is the work: few rows (node, query head) against a long cache, so that the keys are
+// what is cut up.  Every block takes an equal piece of the launch's list of key tiles
+// (tree_common.cuh) and leaves the parts of pairs that it shares as records.
+//
+// A pair is a request's up to 256 rows under one KV head.  With more than 128 rows both softmax groups
+// work on every key tile, each on 128 rows, and the tile is fetched once for both (a tile counts as
+// two in the list).  With at most 128 rows the groups take the key tiles in turn, each with its own
+// running maximum, sum and accumulator, and the output warps join the two: the tensor pipe and the
+// loads then work for one group while the other is in its softmax, as with two row tiles.  At 128
+// rows a tile of 64 KB costs about what its fetch costs, below that the kernel is bound by HBM,
+// above it by the chain softmax -> P V -> next S of the two groups.
+//
+//   warps 0-3, 4-7   softmax groups: thread t owns row t of the group's rows.  It also brings its
+//                    query row into shared memory (cp.async into the swizzled layout) and, in tiles
+//                    with keys that are not there or that only some rows see, clears row t of V.
+//   warps 8, 9       TMA producers of K and V (two stages each): eight pages of 16 rows per tile, or
+//                    one box of 128 rows of the step's own keys and values for a tile of the tree.
+//   warp 10          issues the products.  Per group a cursor names its next S product; it is issued
+//                    behind the group's P V product as soon as its tile and queries are there.
+//   warps 12-15      outputs and records: thread t owns row t, out of tensor memory.
+//
+// Every wait is bounded as in the prefill kernel.
+#include <algorithm>
+#include <type_traits>
+
+#include "tc_common.cuh"
+#include "tree_common.cuh"
+
+namespace pam {
+namespace {
+
+using namespace tc;
+using namespace tree;
+
+constexpr int kRows = 128, kKeys = 128, kHd = 128, kPairRows = 256;
+constexpr int kStages = 2;                             // of K and of V
+constexpr int kTileBytes = kKeys * kHd * 2, kHalfBytes = kTileBytes / 2;
+constexpr float kRescaleThreshold = 8.0f;
+constexpr int kShortKeys = 256;                        // bfloat16: fewer visible keys carry the weights as two operands
+constexpr long long kWaitCycles = 400000000LL;
+constexpr int kKProducerWarp = 8, kVProducerWarp = 9, kMmaWarp = 10, kOutputWarp0 = 12;
+constexpr int kThreads = 512;
+
+// The part of a pair that lies in the block's piece: key tiles [first, last) of nT.
+struct Span {
+    SeqInfo s;
+    int b, kvh, rp, first, last, nT, cacheTiles, rows;   // rows: of the request under the KV head
+    int start;                                           // of the pair in the list
+    bool dual;                                           // both groups on every tile
+    __device__ __forceinline__ int step() const { return dual ? 1 : 2; }
+    __device__ __forceinline__ int weight() const { return dual ? 2 : 1; }
+    // tiles of group x
+    __device__ __forceinline__ int tilesOf(int x) const { return dual ? last - first : (last - first + 1 - x) >> 1; }
+    __device__ __forceinline__ int firstRow(int x) const { return rp * kPairRows + (dual ? x * kRows : 0); }
+    __device__ __forceinline__ bool whole() const { return first == 0 && last == nT; }
+    __device__ __forceinline__ bool shortKeys() const { return s.held - s.lo + static_cast<uint32_t>(s.n) < kShortKeys; }
+};
+
+struct Smem {
+    unsigned char q[2][kTileBytes];
+    unsigned char k[kStages][kTileBytes];
+    unsigned char v[kStages][kTileBytes];
+    unsigned long long kFull[kStages], kEmpty[kStages], vFull[kStages], vEmpty[kStages];
+    unsigned long long qFull[2], sFull[2], pFull[2], oFull[2], oEmpty[2];
+    // [span of the group & 1][group][row]: sum and reference of the row, and whether the thread left a
+    // value out.  Written before the weights of the span's last tile are released, read behind the
+    // commit of its last P V product.  Two of each: a group may be in its next span by then, but not
+    // in the one after it, whose first S product comes behind a P V product that waits for the read.
+    float rowL[2][2][kRows], rowM[2][2][kRows];
+    int rowOdd[2][2][kRows];
+    int scratch[kThreads / 32];
+    uint32_t tmemBase;
+    int dead;
+    Span span[kThreads / 32][2];                       // a warp's current and next span (its registers hold a row of scores)
+    int prefix[1];                                     // [batch + 1]
+};
+size_t smemBytes(int batch) { return sizeof(Smem) + static_cast<size_t>(batch) * sizeof(int); }
+static_assert(sizeof(Smem) + kTreeMaxBatch * sizeof(int) <= 227 * 1024, "the block's shared memory must fit the 227 KB a block may opt into");
+
+// The list as one block sees it.
+struct List {
+    const int* prefix;
+    int begin, end, quota;
+    // The first span at or after position `pos` (a pair's start, or the block's begin); moves pos
+    // behind that pair.  False at the end of the piece.
+    __device__ __forceinline__ bool next(const TreeParams& p, int& pos, Span& g) const {
+        const int group = p.heads / p.kvHeads;
+        while (pos < end) {
+            int a = 0, z = p.batch - 1;
+            while (a < z) {
+                const int mid = (a + z + 1) >> 1;
+                if (prefix[mid] <= pos) a = mid; else z = mid - 1;
+            }
+            g.b = a;
+            g.s = SeqInfo(p, a);
+            g.cacheTiles = g.s.cacheTiles<kKeys>();
+            g.nT = g.s.tiles<kKeys>();
+            g.rows = g.s.n * group;
+            const int rowTiles = (g.rows + kRows - 1) / kRows, perHead = rowTiles * g.nT;
+            const int rel = pos - prefix[a];
+            g.kvh = rel / perHead;
+            const int inHead = rel - g.kvh * perHead;
+            g.rp = inHead / (2 * g.nT);
+            g.dual = rowTiles - 2 * g.rp >= 2;
+            g.start = prefix[a] + g.kvh * perHead + g.rp * 2 * g.nT;
+            const int w = g.weight();
+            // the tiles whose place in the list lies in [begin, end)
+            g.first = begin > g.start ? (begin - g.start + w - 1) / w : 0;
+            g.last = min(g.nT, (end - g.start + w - 1) / w);
+            pos = g.start + g.nT * w;
+            if (g.first < g.last) return true;
+        }
+        return false;
+    }
+};
+
+// What the issuer keeps of a place in the stream: tile j of a span, g tiles into the block's piece.
+struct Place {
+    int pos, first, last, j, g;
+    bool valid, dual, lo;
+    __device__ __forceinline__ void take(const Span& s) { first = s.first; last = s.last; dual = s.dual; lo = s.shortKeys(); j = s.first; }
+    __device__ __forceinline__ void init(const TreeParams& p, const List& l) {
+        pos = l.begin;
+        g = 0;
+        Span s;
+        valid = l.next(p, pos, s);
+        if (valid) take(s);
+    }
+    __device__ __forceinline__ void nextTile(const TreeParams& p, const List& l) {
+        ++j;
+        ++g;
+        if (j == last) {
+            Span s;
+            valid = l.next(p, pos, s);
+            if (valid) take(s);
+        }
+    }
+    __device__ __forceinline__ bool takes(int x) const { return dual || ((j - first) & 1) == x; }
+    __device__ __forceinline__ bool firstOf(int x) const { return j == first + (dual ? 0 : x); }
+    __device__ __forceinline__ bool lastOf(int x) const { return j + (dual ? 1 : 2) >= last; }
+    __device__ __forceinline__ void nextOf(const TreeParams& p, const List& l, int x) {
+        do nextTile(p, l);
+        while (valid && !takes(x));
+    }
+    __device__ __forceinline__ void seekOf(const TreeParams& p, const List& l, int x) {
+        while (valid && !takes(x)) nextTile(p, l);
+    }
+};
+
+// Scores of keys that are not visible become -inf: outside [a, b) of the 32, or by bits.
+__device__ __forceinline__ void maskRange(uint32_t (&r)[32], int a, int b) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (i < a || i >= b) r[i] = 0xFF800000u;
+}
+__device__ __forceinline__ void maskBits(uint32_t (&r)[32], uint32_t bits) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (!(bits >> i & 1u)) r[i] = 0xFF800000u;
+}
+__device__ __forceinline__ void tmemLd16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// Whether `v` is set in any of the 128 threads of the output warps (all of them get here).
+__device__ __forceinline__ bool anyOfOutput(bool v) {
+    uint32_t r = v ? 1u : 0u;
+    asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %0, 0;\n\tbarrier.cta.red.or.pred b, 1, 128, a;\n\tselp.u32 %0, 1, 0, b;\n\t}" : "+r"(r)::"memory");
+    return r != 0;
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+             const __grid_constant__ CUtensorMap mapKNew, const __grid_constant__ CUtensorMap mapVNew,
+             const __grid_constant__ TreeParams p, float scaleLog2, int* errFlag, long long waitCycles) {
+    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    extern __shared__ __align__(1024) unsigned char rawSmem[];
+    Smem* s = reinterpret_cast<Smem*>(rawSmem);
+    if ((smemAddr(rawSmem) & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicCAS(errFlag, 0, 40);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.heads / p.kvHeads;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbarInit(&s->qFull[i], kRows);
+            mbarInit(&s->sFull[i], 1);
+            mbarInit(&s->pFull[i], kRows);
+            mbarInit(&s->oFull[i], 1);
+            mbarInit(&s->oEmpty[i], 1);
+        }
+        for (int i = 0; i < kStages; ++i) {
+            mbarInit(&s->kFull[i], 1); mbarInit(&s->kEmpty[i], 1);
+            mbarInit(&s->vFull[i], 1); mbarInit(&s->vEmpty[i], 1);
+        }
+        s->dead = *reinterpret_cast<volatile int*>(errFlag) != 0 ? 1 : 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        Header h{};
+        h.lastBlock = -1;
+        *headerOf(p, blockIdx.x) = h;
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddr(&s->tmemBase)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    buildPrefix<kRows, kKeys, kThreads>(p, s->prefix, s->scratch);
+    tcFenceBefore();
+    __syncthreads();
+    tcFenceAfter();
+    const uint32_t tmem = s->tmemBase;
+    auto tmemS = [&](int x) { return tmem + 128u * static_cast<uint32_t>(x); };
+    auto tmemO = [&](int x) { return tmem + 256u + 128u * static_cast<uint32_t>(x); };
+    const bool live = *reinterpret_cast<volatile int*>(&s->dead) == 0;
+    const long long waitLimit = waitCycles > 0 ? waitCycles : kWaitCycles;
+    List list;
+    {
+        const int total = s->prefix[p.batch];
+        list.prefix = s->prefix;
+        // (at least two, so that every block between a pair's first and last has a tile of it)
+        list.quota = max(2, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+        list.begin = static_cast<int>(min(static_cast<long long>(blockIdx.x) * list.quota, static_cast<long long>(total)));
+        list.end = min(total, list.begin + list.quota);
+    }
+
+    // 512 x 128 registers at launch: 80 for the service warps, 64 for the output warps, 184 for softmax
+    if (warp == kKProducerWarp || warp == kVProducerWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (!live) goto done;
+        const bool isV = warp == kVProducerWarp;
+        const CUtensorMap* pool = isV ? &mapV : &mapK;
+        const CUtensorMap* fresh = isV ? &mapVNew : &mapKNew;
+        unsigned long long *full = isV ? s->vFull : s->kFull, *empty = isV ? s->vEmpty : s->kEmpty;
+        unsigned char(*tiles)[kTileBytes] = isV ? s->v : s->k;
+        const int tilesPerPage = p.blockSize / 16;
+        int pos = list.begin, gt = 0;
+        Span g;
+        bool ok = true;
+        while (ok && list.next(p, pos, g)) {
+            const int32_t* table = p.tables + static_cast<int64_t>(g.b) * p.maxNumBlocks;
+            for (int j = g.first; j < g.last && ok; ++j, ++gt) {
+                const int st = gt % kStages;
+                const bool inTree = j >= g.cacheTiles;
+                int row = 0;
+                if (!inTree && lane < kKeys / 16) {
+                    const int t16 = (static_cast<int>(g.s.lo / kKeys) + j) * (kKeys / 16) + lane;
+                    const int page = min(t16 / tilesPerPage, p.maxNumBlocks - 1);
+                    const int blk = min(max(table[page], 0), p.poolBlocks - 1);
+                    row = (blk * p.kvHeads + g.kvh) * p.blockSize + (t16 % tilesPerPage) * 16;
+                }
+                if (gt >= kStages) ok = mbarWait(&empty[st], ((gt / kStages) - 1) & 1, &s->dead, errFlag, waitLimit, isV ? 42 : 41);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                if (lane == 0) mbarExpectTx(&full[st], kTileBytes);
+                __syncwarp();
+                if (inTree) {
+                    if (lane < 2)
+                        tmaLoad3d(tiles[st] + lane * kHalfBytes, fresh, &full[st], 64 * lane, g.kvh, g.s.start + (j - g.cacheTiles) * kKeys);
+                } else if (lane < kKeys / 16) {
+                    tmaLoad2d(tiles[st] + lane * 2048, pool, &full[st], 0, row);
+                    tmaLoad2d(tiles[st] + kHalfBytes + lane * 2048, pool, &full[st], 64, row);
+                }
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (!live) goto done;
+        const bool leader = electOne();
+        const uint32_t fmt = BF16 ? 1u : 0u;
+        const uint32_t idescS = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+        const uint32_t idescO = idescS | (1u << 16);
+        const uint32_t hiK = descHi(1024);
+        bool ok = true;
+        Place c, n0, n1;                     // the tile at hand; the groups' next S products
+        c.init(p, list);
+        n0 = n1 = c;
+        n1.seekOf(p, list, 1);
+        int steps0 = 0, steps1 = 0;          // P V products of a group: phase of pFull
+        int spans0 = 0, spans1 = 0;          // spans whose S products of a group have begun: phase of qFull
+        int begun0 = 0, begun1 = 0;          // ... whose P V products have: phase of oEmpty
+        int open0 = 0, open1 = 0;            // per key stage: S products still to come on its tile
+        // The group's next S product: when `poll`, only if its tile and queries are there already.
+        // A tile is at most two ahead of the one at hand, so that the phase before the one asked for
+        // is known to be complete (every S product of the tile two before it has been issued).
+        auto issueQK = [&](int x, Place& n, int& spans, bool poll) {
+            const int st = n.g % kStages;
+            const bool begins = n.firstOf(x);
+            if (poll) {
+                bool there = mbarTry(&s->kFull[st], (n.g / kStages) & 1);
+                if (begins) there = there && mbarTry(&s->qFull[x], spans & 1);
+                if (!__all_sync(0xFFFFFFFFu, there)) return;
+            } else {
+                if (begins) ok = mbarWait(&s->qFull[x], spans & 1, &s->dead, errFlag, waitLimit, 43);
+                if (ok) ok = mbarWait(&s->kFull[st], (n.g / kStages) & 1, &s->dead, errFlag, waitLimit, 44);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) return;
+            }
+            tcFenceAfter();
+            const uint32_t qLo = descLo(smemAddr(s->q[x]), 16), kLo = descLo(smemAddr(s->k[st]), 16), dS = tmemS(x);
+            int& open = st ? open1 : open0;
+            if (open == 0) open = n.dual ? 2 : 1;
+            --open;
+            if (leader) {
+#pragma unroll
+                for (int ks = 0; ks < kHd / 16; ++ks) {
+                    const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                    umma(dS, desc64(qLo + off, hiK), desc64(kLo + off, hiK), idescS, ks > 0);
+                }
+                ummaCommit(&s->sFull[x]);
+                if (open == 0) ummaCommit(&s->kEmpty[st]);
+            }
+            __syncwarp();
+            if (begins) ++spans;
+            n.nextOf(p, list, x);
+        };
+        while (c.valid && ok) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                Place& n = x ? n1 : n0;
+                int& spans = x ? spans1 : spans0;
+                if (ok && n.valid && n.g <= c.g) issueQK(x, n, spans, false);
+            }
+            // (a group that takes the next tile need not wait for this one's weights)
+            if (ok && n0.valid && n0.g == c.g + 1 && !c.takes(0)) issueQK(0, n0, spans0, true);
+            if (ok && n1.valid && n1.g == c.g + 1 && !c.takes(1)) issueQK(1, n1, spans1, true);
+            if (!ok) break;
+            const int st = c.g % kStages;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                if (!c.takes(x) || !ok) continue;
+                int &steps = x ? steps1 : steps0, &spans = x ? spans1 : spans0;
+                Place& n = x ? n1 : n0;
+                ok = mbarWait(&s->pFull[x], steps & 1, &s->dead, errFlag, waitLimit, 45);
+                if (ok) ok = mbarWait(&s->vFull[st], (c.g / kStages) & 1, &s->dead, errFlag, waitLimit, 46);
+                // the accumulator is free once the output of the group's span before was read from it
+                const bool begins = c.firstOf(x);
+                int& begun = x ? begun1 : begun0;
+                if (ok && begins && begun >= 1) ok = mbarWait(&s->oEmpty[x], (begun - 1) & 1, &s->dead, errFlag, waitLimit, 47);
+                if (begins) ++begun;
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                tcFenceAfter();
+                const uint32_t vLo = descLo(smemAddr(s->v[st]), kHalfBytes);
+                const uint32_t sCol = tmemS(x), dO = tmemO(x);
+                const bool lastUser = x == 1 || !c.takes(1);
+                if (leader) {
+#pragma unroll
+                    for (int ks = 0; ks < kKeys / 16; ++ks)
+                        ummaTs(dO, sCol + 32u * (ks >> 1) + 8u * (ks & 1), desc64(vLo + ks * 128, hiK), idescO, ks > 0 || !begins ? 1u : 0u);
+                    if (BF16 && c.lo) {
+#pragma unroll
+                        for (int ks = 0; ks < kKeys / 16; ++ks)
+                            ummaTs(dO, sCol + 32u * (ks >> 1) + 8u * (ks & 1) + 16u, desc64(vLo + ks * 128, hiK), idescO, 1u);
+                    }
+                    if (c.lastOf(x)) ummaCommit(&s->oFull[x]);
+                    if (lastUser) ummaCommit(&s->vEmpty[st]);
+                }
+                __syncwarp();
+                ++steps;
+                // the group's next S product, behind the product that read the weights it overwrites
+                if (n.valid && n.g <= c.g + 2) issueQK(x, n, spans, true);
+            }
+            c.nextTile(p, list);
+        }
+    } else if (warp < kOutputWarp0 && warp > kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");          // (the fourth warp of the service warpgroup)
+    } else if (warp >= kOutputWarp0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (!live) goto done;
+        const int t = (warp & 3) * 32 + lane;
+        const uint32_t laneBase = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const bool first = threadIdx.x == kOutputWarp0 * 32;
+        int cnt0 = 0, cnt1 = 0;              // spans of a group written: phase of oFull
+        int pos = list.begin;
+        const Span& g = s->span[warp][0];
+        auto seek = [&]() {
+            Span q;
+            const bool got = list.next(p, pos, q);
+            __syncwarp();
+            if (lane == 0 && got) s->span[warp][0] = q;
+            __syncwarp();
+            return got;
+        };
+        bool ok = true;
+        while (ok && seek()) {
+            const bool has1 = g.tilesOf(1) > 0;
+            ok = mbarWait(&s->oFull[0], cnt0 & 1, &s->dead, errFlag, waitLimit, 49);
+            if (ok && has1) ok = mbarWait(&s->oFull[1], cnt1 & 1, &s->dead, errFlag, waitLimit, 51);
+            // (all four warps decide together, so that none waits for one that gave up)
+            ok = !anyOfOutput(!ok);
+            if (!ok) break;
+            tcFenceAfter();
+            const int p0 = cnt0 & 1, p1 = cnt1 & 1;
+            // values left out anywhere in the span
+            const bool odd = anyOfOutput(s->rowOdd[p0][0][t] != 0 || (has1 && s->rowOdd[p1][1][t] != 0));
+            const bool whole = g.whole();
+            const int which = g.first == 0 ? 1 : 0;
+            if (!whole && first) {
+                Header* h = headerOf(p, blockIdx.x);
+                h->odd[which] = odd ? 1 : 0;
+                if (which == 1) {
+                    h->b = g.b; h->kvh = g.kvh; h->rt = g.rp;
+                    h->lastBlock = (g.start + (g.nT - 1) * g.weight()) / list.quota;
+                }
+            }
+            const uint32_t hi = odd && whole ? lastFirst(p, g.s, g.rp, kPairRows) : 0u;
+            float* rec = whole ? nullptr : recordOf(p, gridDim.x, blockIdx.x, which, kPairRows, kHd);
+#pragma unroll 1
+            for (int x = 0; x < (g.dual ? 2 : 1); ++x) {
+                const int rl = (g.dual ? x * kRows : 0) + t, rr = g.rp * kPairRows + rl;
+                const bool mine = rr < g.rows;
+                float m = s->rowM[x ? p1 : p0][x][t], l = s->rowL[x ? p1 : p0][x][t], a0 = 1.f, a1 = 0.f;
+                if (!g.dual && has1) {
+                    const float m1 = s->rowM[p1][1][t], top = fmaxf(m, m1), base = top == -INFINITY ? 0.f : top;
+                    a0 = ex2Approx(m - base);
+                    a1 = ex2Approx(m1 - base);
+                    l = l * a0 + s->rowL[p1][1][t] * a1;
+                    m = top;
+                }
+                const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+                a0 *= inv;
+                a1 *= inv;
+                T* out = nullptr;
+                if (whole && mine) out = static_cast<T*>(p.out) + (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd;
+#pragma unroll 1
+                for (int c = 0; c < 8; ++c) {           // 16 columns at a time
+                    uint32_t o[16];
+                    float f[16];
+                    tmemLd16(tmemO(x) + laneBase + 16u * c, o);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * a0;
+                    if (!g.dual && has1) {
+                        tmemLd16(tmemO(1) + laneBase + 16u * c, o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) f[i] = fmaf(__uint_as_float(o[i]), a1, f[i]);
+                    }
+                    if (whole && mine) {
+                        if (odd)
+#pragma unroll 1
+                            for (int i = 0; i < 16; ++i) {
+                                const float add = leftOut<T, T>(p, g.s, g.b, g.kvh, rr / group, hi, 16 * c + i);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k)
+                                    if (k == i) f[k] += add;
+                            }
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            *reinterpret_cast<uint4*>(out + 16 * c + 8 * q) =
+                                make_uint4(pack16<BF16>(f[8 * q], f[8 * q + 1]), pack16<BF16>(f[8 * q + 2], f[8 * q + 3]),
+                                           pack16<BF16>(f[8 * q + 4], f[8 * q + 5]), pack16<BF16>(f[8 * q + 6], f[8 * q + 7]));
+                    } else if (mine) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            *reinterpret_cast<float4*>(rec + rl * kHd + 16 * c + 4 * q) = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+                    }
+                    __syncwarp();
+                }
+                if (!whole && mine) {
+                    rec[kPairRows * kHd + rl] = m;
+                    rec[kPairRows * kHd + kPairRows + rl] = l;
+                }
+            }
+            tcFenceBefore();
+            anyOfOutput(false);
+            if (first) {
+                mbarArrive(&s->oEmpty[0]);              // the accumulators and the rows' sums may be overwritten
+                if (has1) mbarArrive(&s->oEmpty[1]);
+            }
+            ++cnt0;
+            if (has1) ++cnt1;
+        }
+    } else {
+        // ------------------------------------------------------------ softmax groups
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        if (!live) goto done;
+        const int x = warp >> 2, t = (warp & 3) * 32 + lane;
+        const uint32_t laneBase = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t sAddr = tmemS(x) + laneBase, oAddr = tmemO(x) + laneBase;
+        bool ok = true;
+        int steps = 0, spans = 0;            // tiles this group has done (phase of sFull), spans
+        int gt = 0;                          // tiles of the piece before the current span
+        int pos = list.begin;
+        // this thread's query row of a span into the group's tile
+        auto fetchQ = [&](const Span& q) {
+            const int rr = q.firstRow(x) + t;
+            const bool there = rr < q.rows;
+            const T* src = static_cast<const T*>(p.q) + (there ? static_cast<int64_t>(q.s.start + rr / group) * p.qStride +
+                                                                     static_cast<int64_t>(q.kvh * group + rr % group) * kHd : 0);
+            const uint32_t dst = smemAddr(s->q[x]) + t * 128;
+            const int n = there ? 16 : 0;
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (c >> 3) * kHalfBytes + (((c & 7) ^ (t & 7)) << 4)), "l"(src + c * 8), "r"(n) : "memory");
+        };
+        auto postQ = [&]() {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbarArrive(&s->qFull[x]);
+        };
+        // the next span with tiles of this group, into the warp's slot `k`; the tiles of spans without
+        // are counted
+        int skipped = 0;
+        auto seek = [&](int k) {
+            Span q;
+            skipped = 0;
+            while (list.next(p, pos, q)) {
+                if (q.tilesOf(x) > 0) {
+                    if (lane == 0) s->span[warp][k & 1] = q;
+                    __syncwarp();
+                    return true;
+                }
+                skipped += q.last - q.first;
+            }
+            return false;
+        };
+        bool have = seek(0);
+        gt = skipped;
+        if (have) {
+            fetchQ(s->span[warp][0]);
+            postQ();
+        }
+        while (have && ok) {
+            const Span& g = s->span[warp][spans & 1];
+            have = seek(spans + 1);
+            const Span& nx = s->span[warp][(spans + 1) & 1];
+            const int rr = g.firstRow(x) + t;
+            const bool mine = rr < g.rows;
+            const int node = mine ? rr / group : 0;
+            const uint32_t from = max(firstOf(p, g.s, node), g.s.lo);
+            const uint32_t hi = lastFirst(p, g.s, g.rp, kPairRows);
+            const bool useLo = BF16 && g.shortKeys();
+            float mUsed = -INFINITY, l = 0.f;
+            int odd = 0;
+            const int j0 = g.first + (g.dual ? 0 : x);
+            for (int j = j0; j < g.last && ok; j += g.step(), ++steps) {
+                const bool inTree = j >= g.cacheTiles;
+                const uint32_t k0 = inTree ? static_cast<uint32_t>(j - g.cacheTiles) * kKeys : (g.s.lo / kKeys + j) * kKeys;
+                const uint32_t keyEnd = inTree ? static_cast<uint32_t>(g.s.n) : g.s.held;
+                const bool edge = inTree || k0 < hi || k0 < g.s.lo || k0 + kKeys > keyEnd;
+                ok = mbarWait(&s->sFull[x], steps & 1, &s->dead, errFlag, waitLimit, 52);
+                if (!ok) break;
+                tcFenceAfter();
+                const bool lastTile = j + g.step() >= g.last;
+                if (lastTile && have) fetchQ(nx);      // S of the span's last tile is there: the query tile is no longer read
+                uint32_t r0[32], r1[32], r2[32], r3[32];
+                tmemLd32NoWait(sAddr, r0);
+                tmemLd32NoWait(sAddr + 32u, r1);
+                tmemLd32NoWait(sAddr + 64u, r2);
+                tmemLd32NoWait(sAddr + 96u, r3);
+                tmemLdWait();
+                if (edge) {
+                    if (inTree) {
+                        const int w = static_cast<int>(k0 / 32);
+                        maskBits(r0, treeBits(p, g.s, node, w));
+                        maskBits(r1, treeBits(p, g.s, node, w + 1));
+                        maskBits(r2, treeBits(p, g.s, node, w + 2));
+                        maskBits(r3, treeBits(p, g.s, node, w + 3));
+                    } else {
+                        const int a = from > k0 ? static_cast<int>(min(from - k0, 128u)) : 0, b = static_cast<int>(min(g.s.held - k0, 128u));
+                        maskRange(r0, a, b);
+                        maskRange(r1, a - 32, b - 32);
+                        maskRange(r2, a - 64, b - 64);
+                        maskRange(r3, a - 96, b - 96);
+                    }
+                }
+                const float tmax = fmaxf(fmaxf(quarterRowMax(r0), quarterRowMax(r1)), fmaxf(quarterRowMax(r2), quarterRowMax(r3))) * scaleLog2;
+                bool raise = false;
+                float corr = 1.f;
+                if (j == j0) mUsed = tmax;
+                else if (tmax > mUsed + kRescaleThreshold) {
+                    raise = true;
+                    corr = ex2Approx(mUsed - tmax);
+                    mUsed = tmax;
+                }
+                if (j > j0 && __any_sync(0xFFFFFFFFu, raise)) {
+                    // (complete up to the group's tile before: this S product was issued behind that P V product)
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        tmemLd32(oAddr + 32u * c, o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                        tmemSt32(oAddr + 32u * c, o);
+                    }
+                    tmemStWait();
+                    l *= corr;
+                }
+                const float negM = mUsed == -INFINITY ? 0.f : -mUsed;
+                {
+                    uint32_t wgt[32];
+                    if (useLo) {
+                        l += weightsRange<BF16, true, 0, 32>(r0, wgt, scaleLog2, negM);
+                        tmemSt32(sAddr, wgt);
+                        l += weightsRange<BF16, true, 0, 32>(r1, wgt, scaleLog2, negM);
+                        tmemSt32(sAddr + 32u, wgt);
+                        l += weightsRange<BF16, true, 0, 32>(r2, wgt, scaleLog2, negM);
+                        tmemSt32(sAddr + 64u, wgt);
+                        l += weightsRange<BF16, true, 0, 32>(r3, wgt, scaleLog2, negM);
+                        tmemSt32(sAddr + 96u, wgt);
+                    } else {
+                        l += weightsRange<BF16, false, 0, 32>(r0, wgt, scaleLog2, negM);
+                        tmemSt16(sAddr, wgt);
+                        l += weightsRange<BF16, false, 0, 32>(r1, wgt, scaleLog2, negM);
+                        tmemSt16(sAddr + 32u, wgt);
+                        l += weightsRange<BF16, false, 0, 32>(r2, wgt, scaleLog2, negM);
+                        tmemSt16(sAddr + 64u, wgt);
+                        l += weightsRange<BF16, false, 0, 32>(r3, wgt, scaleLog2, negM);
+                        tmemSt16(sAddr + 96u, wgt);
+                    }
+                }
+                tmemStWait();
+                if (edge) {
+                    // Row t of V: zeros where there is no such key, finite values where some row may not
+                    // see it.  (Both groups of a dual span may write the same.  The phase asked for is not two
+                    // ahead: this S product was issued after the wait for V of the tile two before.)
+                    const int tile = gt + j - g.first, st = tile % kStages;
+                    ok = mbarWait(&s->vFull[st], (tile / kStages) & 1, &s->dead, errFlag, waitLimit, 53);
+                    if (!ok) break;
+                    const uint32_t key = k0 + static_cast<uint32_t>(t);
+                    const bool there = key < keyEnd && (inTree || key >= g.s.lo);
+                    unsigned char* row = s->v[st] + t * 128;
+                    if (!there) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(row + (c >> 3) * kHalfBytes + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    } else if (inTree || key < hi) {
+                        constexpr uint32_t kExp = BF16 ? 0x7F80u : 0x7C00u;
+#pragma unroll 1
+                        for (int c = 0; c < 64; ++c) {
+                            uint32_t* w = reinterpret_cast<uint32_t*>(row + (c >> 5) * kHalfBytes + (c & 31) * 4);
+                            uint32_t v = *w;
+                            if ((v & kExp) == kExp) v &= 0xFFFF0000u;
+                            if ((v >> 16 & kExp) == kExp) v &= 0x0000FFFFu;
+                            if (v != *w) { *w = v; odd = 1; }
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                if (lastTile) {
+                    s->rowL[spans & 1][x][t] = l;
+                    s->rowM[spans & 1][x][t] = mUsed;
+                    s->rowOdd[spans & 1][x][t] = odd;
+                }
+                tcFenceBefore();
+                mbarArrive(&s->pFull[x]);
+            }
+            if (!ok) break;
+            ++spans;
+            gt += g.last - g.first + skipped;
+            if (have) postQ();
+        }
+    }
+
+done:
+    tcFenceBefore();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tcFenceAfter();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace
+
+bool treeTcApplies(const TreeParams& p) {
+    if ((p.dtype != kF16 && p.dtype != kBF16) || p.headDim != kHd || p.blockSize % 16 != 0) return false;
+    // (rows of the pool are counted in 32 bits)
+    if (p.poolBlocks <= 0 || p.poolBlocks >= (1 << 30) / (p.kvHeads * p.blockSize)) return false;
+    for (int64_t s : {p.qStride, p.kStride, p.vStride})
+        if (s % 8) return false;
+    for (const void* ptr : {p.q, p.kNew, p.vNew, p.kPool, p.vPool, static_cast<const void*>(p.out)})
+        if (reinterpret_cast<uintptr_t>(ptr) & 15) return false;
+    return true;
+}
+
+TreePlan treeTcPlan(const TreeParams&, int smCount) {
+    TreePlan t{};
+    t.variant = 2;
+    t.rows = kPairRows;
+    t.keys = kKeys;
+    t.dimPad = kHd;
+    t.blocks = smCount;
+    return t;
+}
+
+cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t stream) {
+    EncodeFn encode = encodeFn();
+    if (!encode) return cudaErrorNotSupported;
+    const CUtensorMapDataType dt = p.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap pool[2], fresh[2];
+    for (int which = 0; which < 2; ++which) {
+        // pools: [block * kv_head * slot][128]; a box is 64 dims x 16 rows (half of a 16-token piece)
+        const cuuint64_t dims[2] = {kHd, static_cast<cuuint64_t>(p.poolBlocks) * p.kvHeads * p.blockSize};
+        const cuuint64_t strides[1] = {kHd * 2};
+        const cuuint32_t box[2] = {64, 16}, one[2] = {1, 1};
+        if (encode(&pool[which], dt, 2, const_cast<void*>(which ? p.vPool : p.kPool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+        // the step's rows: [row][kv_head][128]; a box is 64 dims x 1 head x 128 rows (rows behind the last: zeros)
+        const cuuint64_t fdims[3] = {kHd, static_cast<cuuint64_t>(p.kvHeads), static_cast<cuuint64_t>(p.numRows)};
+        const cuuint64_t fstrides[2] = {kHd * 2, static_cast<cuuint64_t>(which ? p.vStride : p.kStride) * 2};
+        const cuuint32_t fbox[3] = {64, 1, kKeys}, fone[3] = {1, 1, 1};
+        if (encode(&fresh[which], dt, 3, const_cast<void*>(which ? p.vNew : p.kNew), fdims, fstrides, fbox, fone, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    }
+    const float scaleLog2 = 1.4426950408889634f / sqrtf(static_cast<float>(kHd));
+    const size_t smem = smemBytes(p.batch);
+    auto run = [&](auto kernel) -> cudaError_t {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smemBytes(kTreeMaxBatch)));
+        if (e != cudaSuccess) return e;
+        kernel<<<plan.blocks, kThreads, smem, stream>>>(pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag, p.waitCycles);
+        return cudaGetLastError();
+    };
+    return p.dtype == kBF16 ? run(treeTcKernel<true>) : run(treeTcKernel<false>);
+}
+
+}  // namespace pam
