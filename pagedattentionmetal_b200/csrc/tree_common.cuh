@@ -183,25 +183,6 @@ __device__ __forceinline__ float poolValue(const TreeParams& p, const void* pool
         return valueOf(static_cast<const KT_*>(pool) + at);
 }
 
-// Sum of the values in column d that were taken as zero although node i sees them; hi: the first
-// token that every row of the row tile sees.
-template <typename QT, typename KT_>
-__device__ __noinline__ float leftOut(const TreeParams& p, SeqInfo s, int b, int kvh, int i, uint32_t hi, int d) {
-    float sum = 0.f;
-    for (uint32_t t = firstOf(p, s, i); t < hi; ++t) {
-        int64_t blk;
-        const int64_t at = poolRow(p, b, t, kvh, &blk) + d;
-        const float v = poolValue<KT_>(p, p.vPool, p.vScale, at, blk, kvh);
-        if (isOdd(v)) sum += v;
-    }
-    for (int w = 0; w * 32 < s.n; ++w)
-        for (uint32_t bits = treeBits(p, s, i, w); bits; bits &= bits - 1) {
-            const int j = 32 * w + __ffs(bits) - 1;
-            const float v = valueOf(static_cast<const QT*>(p.vNew) + static_cast<int64_t>(s.start + j) * p.vStride + static_cast<int64_t>(kvh) * p.headDim + d);
-            if (isOdd(v)) sum += v;
-        }
-    return sum;
-}
 // First token that every row of a row tile sees (the largest of the rows' first tokens).
 __device__ __forceinline__ uint32_t lastFirst(const TreeParams& p, const SeqInfo& s, int rt, int mr) {
     if (p.window <= 0) return 0u;
@@ -215,6 +196,27 @@ template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Adds the values that were taken as zero although node i sees them to columns [d0, d1) of its row
+// of the result, which this thread (or its warp, before a __syncwarp) has stored.  hi: the first token
+// that every row of the row tile sees.
+template <typename QT, typename KT_>
+__device__ __noinline__ void addLeftOut(const TreeParams& p, SeqInfo s, int b, int kvh, int i, uint32_t hi, QT* row, int d0, int d1) {
+    for (uint32_t t = firstOf(p, s, i); t < hi; ++t) {
+        int64_t blk;
+        const int64_t at = poolRow(p, b, t, kvh, &blk);
+        for (int d = d0; d < d1; ++d) {
+            const float v = poolValue<KT_>(p, p.vPool, p.vScale, at + d, blk, kvh);
+            if (isOdd(v)) row[d] = narrow<QT>(valueOf(row + d) + v);
+        }
+    }
+    for (int w = 0; w * 32 < s.n; ++w)
+        for (uint32_t bits = treeBits(p, s, i, w); bits; bits &= bits - 1) {
+            const QT* v = static_cast<const QT*>(p.vNew) + static_cast<int64_t>(s.start + 32 * w + __ffs(bits) - 1) * p.vStride + static_cast<int64_t>(kvh) * p.headDim;
+            for (int d = d0; d < d1; ++d)
+                if (isOdd(valueOf(v + d))) row[d] = narrow<QT>(valueOf(row + d) + valueOf(v + d));
+        }
+}
 
 }  // namespace tree
 

@@ -234,14 +234,17 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
                     QT* out = static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + g.kvh * group + rr % group) * D;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (d + e < D) {
-                            float v = acc[h][r][e] * inv;
-                            if (odd) v += leftOut<QT, KT_>(p, s, g.b, g.kvh, rr / group, hi, d + e);
-                            out[d + e] = narrow<QT>(v);
-                        }
+                        if (d + e < D) out[d + e] = narrow<QT>(acc[h][r][e] * inv);
                 } else {
                     *reinterpret_cast<float4*>(rec + rl * dp + d) = make_float4(acc[h][r][0], acc[h][r][1], acc[h][r][2], acc[h][r][3]);
                 }
+            }
+            if (whole && odd) {
+                __syncwarp();
+                if (lane == 0)
+                    addLeftOut<QT, KT_>(p, s, g.b, g.kvh, rr / group, hi,
+                                        static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + g.kvh * group + rr % group) * D, 0, D);
+                __syncwarp();
             }
             if (!whole && lane == 0) {
                 rec[kGenRows * dp + rl] = mr;
@@ -295,19 +298,75 @@ treeJoinKernel(const __grid_constant__ TreeParams p, int blocks, int mr, int dim
         const float inv = l == 0.f ? 0.f : 1.f / l, v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (d + e < p.headDim) {
-                float x = v[e] * inv;
-                if (odd) x += leftOut<QT, KT_>(p, s, h.b, h.kvh, rr / group, hi, d + e);
-                out[d + e] = narrow<QT>(x);
-            }
+            if (d + e < p.headDim) out[d + e] = narrow<QT>(v[e] * inv);
+    }
+    if (odd) {
+        __syncwarp();
+        if (lane == 0) addLeftOut<QT, KT_>(p, s, h.b, h.kvh, rr / group, hi, out, 0, p.headDim);
     }
 }
 
-template <typename QT, typename KT_>
-cudaError_t launchJoin(const TreeParams& p, const TreePlan& plan, cudaStream_t stream, int* launches) {
-    if (plan.blocks < 2) return cudaSuccess;
+// The same for the records of treeTcKernel, whose O is [piece of 4 columns][256 rows]: block (i, y)
+// takes rows 32 y .. + 31, a lane a row and a warp four pieces, so that the reads of a record are
+// whole lines.
+template <typename QT>
+__global__ void __launch_bounds__(256)
+treeJoinColumnsKernel(const __grid_constant__ TreeParams p, int blocks) {
+    constexpr int MR = 256, HD = 128;
+    cudaGridDependencySynchronize();
+    const Header h = *headerOf(p, blockIdx.x);
+    if (h.lastBlock < 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rl = blockIdx.y * 32 + lane;
+    const SeqInfo s(p, h.b);
+    const int group = p.heads / p.kvHeads, rr = h.rt * MR + rl;
+    if (h.rt * MR + static_cast<int>(blockIdx.y) * 32 >= s.n * group) return;
+    const bool mine = rr < s.n * group;
+    const int first = blockIdx.x, count = h.lastBlock - first + 1;
+    auto record = [&](int i) -> const float* { return recordOf(p, blocks, first + i, i == 0 ? 1 : 0, MR, HD); };
+    float top = -INFINITY;
+    bool odd = false;
+    if (mine) {
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) top = fmaxf(top, record(i)[MR * HD + rl]);
+    }
+    for (int i = lane; i < count; i += 32) odd = odd || headerOf(p, first + i)->odd[i == 0 ? 1 : 0] != 0;
+    odd = __any_sync(0xFFFFFFFFu, odd);
+    if (!mine) return;
+    const float base = top == -INFINITY ? 0.f : top;
+    float4 sum[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+        const float* r = record(i);
+        const float f = exp2f(r[MR * HD + rl] - base);
+        l += f * r[MR * HD + MR + rl];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 o = reinterpret_cast<const float4*>(r)[(4 * warp + q) * MR + rl];
+            sum[q].x += f * o.x; sum[q].y += f * o.y; sum[q].z += f * o.z; sum[q].w += f * o.w;
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    QT out[16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const float v[4] = {sum[q].x * inv, sum[q].y * inv, sum[q].z * inv, sum[q].w * inv};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[4 * q + e] = narrow<QT>(v[e]);
+    }
+    QT* to = static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + h.kvh * group + rr % group) * HD;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) reinterpret_cast<uint4*>(to + 16 * warp)[q] = reinterpret_cast<const uint4*>(out)[q];
+    if (odd) addLeftOut<QT, QT>(p, s, h.b, h.kvh, rr / group, lastFirst(p, s, h.rt, MR), to, 16 * warp, 16 * warp + 16);
+}
+
+// The joining kernel may be set up while the attention kernel still runs.
+template <typename... Kernel, typename... Args>
+cudaError_t launchEarly(void (*kernel)(Kernel...), dim3 grid, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(plan.blocks - 1, (plan.rows + 7) / 8);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
@@ -315,8 +374,17 @@ cudaError_t launchJoin(const TreeParams& p, const TreePlan& plan, cudaStream_t s
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename QT, typename KT_>
+cudaError_t launchJoin(const TreeParams& p, const TreePlan& plan, cudaStream_t stream, int* launches) {
+    if (plan.blocks < 2) return cudaSuccess;
     *launches += 1;
-    return cudaLaunchKernelEx(&cfg, treeJoinKernel<QT, KT_>, p, plan.blocks, plan.rows, plan.dimPad);
+    const unsigned blocks = static_cast<unsigned>(plan.blocks - 1);
+    if constexpr (sizeof(QT) == 2 && sizeof(KT_) == 2)
+        if (plan.variant == 2) return launchEarly(treeJoinColumnsKernel<QT>, dim3(blocks, plan.rows / 32), stream, p, plan.blocks);
+    return launchEarly(treeJoinKernel<QT, KT_>, dim3(blocks, (plan.rows + 7) / 8), stream, p, plan.blocks, plan.rows, plan.dimPad);
 }
 
 // Dynamic shared memory above 48 KB has to be allowed once per device and kernel.

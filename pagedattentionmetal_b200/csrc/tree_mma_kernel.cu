@@ -494,12 +494,7 @@ treeMmaKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
                 for (int n = 0; n < HD / 8; ++n) {
                     const int d = 8 * n + 2 * gc;
                     if (d >= D) continue;
-                    float x = o[n][2 * h] * inv, y = o[n][2 * h + 1] * inv;
-                    if (odd) {
-                        x += leftOut<T, std::conditional_t<FP8, uint8_t, T>>(p, g.s, g.b, g.kvh, rr / group, hi, d);
-                        y += leftOut<T, std::conditional_t<FP8, uint8_t, T>>(p, g.s, g.b, g.kvh, rr / group, hi, d + 1);
-                    }
-                    *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(x, y);
+                    *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
                 }
             } else {
 #pragma unroll
@@ -510,6 +505,16 @@ treeMmaKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
                     rec[MR * HD + MR + rl] = l;
                 }
             }
+        }
+        if (whole && odd) {
+            __syncwarp();
+            for (int h = 0; h < 2; ++h) {
+                const int rr = g.rt * MR + 16 * rowGroup + gr + 8 * h;
+                if (gc == 0 && rr < rows)
+                    addLeftOut<T, std::conditional_t<FP8, uint8_t, T>>(p, g.s, g.b, g.kvh, rr / group, hi,
+                        static_cast<T*>(p.out) + (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * D, 0, D);
+            }
+            __syncwarp();
         }
     }
     waitGroups<0>();

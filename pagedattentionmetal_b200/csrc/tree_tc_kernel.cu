@@ -19,6 +19,9 @@
 //                    with keys that are not there or that only some rows see, clears row t of V.
 //   warps 8, 9       TMA producers of K and V (two stages each): eight pages of 16 rows per tile, or
 //                    one box of 128 rows of the step's own keys and values for a tile of the tree.
+//   warp 11          walks the list and leaves the block's spans (its parts of pairs) in a ring in
+//                    shared memory, a few ahead of the warps that work on them: a step of that walk is
+//                    some loads and divisions in a row, a microsecond that nobody else waits for.
 //   warp 10          issues the products.  Per group a cursor names its next S product; it is issued
 //                    behind the group's P V product as soon as its tile and queries are there.
 //   warps 12-15      outputs and records: thread t owns row t, out of tensor memory.
@@ -42,17 +45,19 @@ constexpr int kTileBytes = kKeys * kHd * 2, kHalfBytes = kTileBytes / 2;
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kShortKeys = 256;                        // bfloat16: fewer visible keys carry the weights as two operands
 constexpr long long kWaitCycles = 400000000LL;
-constexpr int kKProducerWarp = 8, kVProducerWarp = 9, kMmaWarp = 10, kOutputWarp0 = 12;
+constexpr int kKProducerWarp = 8, kVProducerWarp = 9, kMmaWarp = 10, kPlanWarp = 11, kOutputWarp0 = 12;
 constexpr int kThreads = 512;
 
 // The part of a pair that lies in the block's piece: key tiles [first, last) of nT.
 struct Span {
     SeqInfo s;
     int b, kvh, rp, first, last, nT, cacheTiles, rows;   // rows: of the request under the KV head
-    int start;                                           // of the pair in the list
-    bool dual;                                           // both groups on every tile
+    int lastBlock;                                       // that shares the pair
+    uint32_t hi;                                         // see lastFirst
+    int tile;                                            // the block's tiles before this span
+    int dual;                                            // both groups on every tile
+    int valid;                                           // 0: the list ends here
     __device__ __forceinline__ int step() const { return dual ? 1 : 2; }
-    __device__ __forceinline__ int weight() const { return dual ? 2 : 1; }
     // tiles of group x
     __device__ __forceinline__ int tilesOf(int x) const { return dual ? last - first : (last - first + 1 - x) >> 1; }
     __device__ __forceinline__ int firstRow(int x) const { return rp * kPairRows + (dual ? x * kRows : 0); }
@@ -60,95 +65,75 @@ struct Span {
     __device__ __forceinline__ bool shortKeys() const { return s.held - s.lo + static_cast<uint32_t>(s.n) < kShortKeys; }
 };
 
+constexpr int kSpans = 8;        // of the ring: no warp is more than six spans ahead of another
+
 struct Smem {
     unsigned char q[2][kTileBytes];
     unsigned char k[kStages][kTileBytes];
     unsigned char v[kStages][kTileBytes];
     unsigned long long kFull[kStages], kEmpty[kStages], vFull[kStages], vEmpty[kStages];
     unsigned long long qFull[2], sFull[2], pFull[2], oFull[2], oEmpty[2];
+    unsigned long long spanFull[kSpans], spanEmpty[kSpans];
     // [span of the group & 1][group][row]: sum and reference of the row, and whether the thread left a
     // value out.  Written before the weights of the span's last tile are released, read behind the
     // commit of its last P V product.  Two of each: a group may be in its next span by then, but not
     // in the one after it, whose first S product comes behind a P V product that waits for the read.
     float rowL[2][2][kRows], rowM[2][2][kRows];
     int rowOdd[2][2][kRows];
+    // what a softmax thread keeps here to have registers for a row of scores: its node, its first cache
+    // token, and in a tree's tile the bits of the nodes that it sees
+    int rowNode[2][kRows];
+    uint32_t rowFrom[2][kRows], rowBits[2][4][kRows];
+    Span span[kSpans];
     int scratch[kThreads / 32];
     uint32_t tmemBase;
     int dead;
-    Span span[kThreads / 32][2];                       // a warp's current and next span (its registers hold a row of scores)
     int prefix[1];                                     // [batch + 1]
 };
 size_t smemBytes(int batch) { return sizeof(Smem) + static_cast<size_t>(batch) * sizeof(int); }
 static_assert(sizeof(Smem) + kTreeMaxBatch * sizeof(int) <= 227 * 1024, "the block's shared memory must fit the 227 KB a block may opt into");
+constexpr int kSpanReaders = 2 + 1 + 4 + 8;            // warps: producers, issuer, output, softmax
 
-// The list as one block sees it.
-struct List {
-    const int* prefix;
-    int begin, end, quota;
-    // The first span at or after position `pos` (a pair's start, or the block's begin); moves pos
-    // behind that pair.  False at the end of the piece.
-    __device__ __forceinline__ bool next(const TreeParams& p, int& pos, Span& g) const {
-        const int group = p.heads / p.kvHeads;
-        while (pos < end) {
-            int a = 0, z = p.batch - 1;
-            while (a < z) {
-                const int mid = (a + z + 1) >> 1;
-                if (prefix[mid] <= pos) a = mid; else z = mid - 1;
-            }
-            g.b = a;
-            g.s = SeqInfo(p, a);
-            g.cacheTiles = g.s.cacheTiles<kKeys>();
-            g.nT = g.s.tiles<kKeys>();
-            g.rows = g.s.n * group;
-            const int rowTiles = (g.rows + kRows - 1) / kRows, perHead = rowTiles * g.nT;
-            const int rel = pos - prefix[a];
-            g.kvh = rel / perHead;
-            const int inHead = rel - g.kvh * perHead;
-            g.rp = inHead / (2 * g.nT);
-            g.dual = rowTiles - 2 * g.rp >= 2;
-            g.start = prefix[a] + g.kvh * perHead + g.rp * 2 * g.nT;
-            const int w = g.weight();
-            // the tiles whose place in the list lies in [begin, end)
-            g.first = begin > g.start ? (begin - g.start + w - 1) / w : 0;
-            g.last = min(g.nT, (end - g.start + w - 1) / w);
-            pos = g.start + g.nT * w;
-            if (g.first < g.last) return true;
+// The block's next span at or after position `pos` of the list (a pair's start, or the block's
+// begin); moves pos behind that pair.  False at the end of the piece.
+__device__ __forceinline__ bool nextSpan(const TreeParams& p, const int* prefix, int begin, int end, int quota, int& pos, Span& g) {
+    const int group = p.heads / p.kvHeads;
+    while (pos < end) {
+        int a = 0, z = p.batch - 1;
+        while (a < z) {
+            const int mid = (a + z + 1) >> 1;
+            if (prefix[mid] <= pos) a = mid; else z = mid - 1;
         }
-        return false;
+        g.b = a;
+        g.s = SeqInfo(p, a);
+        g.cacheTiles = g.s.cacheTiles<kKeys>();
+        g.nT = g.s.tiles<kKeys>();
+        g.rows = g.s.n * group;
+        const int rowTiles = (g.rows + kRows - 1) / kRows, perHead = rowTiles * g.nT;
+        const int rel = pos - prefix[a];
+        g.kvh = rel / perHead;
+        const int inHead = rel - g.kvh * perHead;
+        g.rp = inHead / (2 * g.nT);
+        g.dual = rowTiles - 2 * g.rp >= 2;
+        const int start = prefix[a] + g.kvh * perHead + g.rp * 2 * g.nT, w = g.dual ? 2 : 1;
+        // the tiles whose place in the list lies in [begin, end)
+        g.first = begin > start ? (begin - start + w - 1) / w : 0;
+        g.last = min(g.nT, (end - start + w - 1) / w);
+        g.lastBlock = (start + (g.nT - 1) * w) / quota;
+        pos = start + g.nT * w;
+        if (g.first < g.last) return true;
     }
-};
+    return false;
+}
 
-// What the issuer keeps of a place in the stream: tile j of a span, g tiles into the block's piece.
+// What the issuer keeps of a place in the stream: tile j of the block's span number k, g tiles into
+// its piece.
 struct Place {
-    int pos, first, last, j, g;
+    int k, first, last, j, g;
     bool valid, dual, lo;
-    __device__ __forceinline__ void take(const Span& s) { first = s.first; last = s.last; dual = s.dual; lo = s.shortKeys(); j = s.first; }
-    __device__ __forceinline__ void init(const TreeParams& p, const List& l) {
-        pos = l.begin;
-        g = 0;
-        Span s;
-        valid = l.next(p, pos, s);
-        if (valid) take(s);
-    }
-    __device__ __forceinline__ void nextTile(const TreeParams& p, const List& l) {
-        ++j;
-        ++g;
-        if (j == last) {
-            Span s;
-            valid = l.next(p, pos, s);
-            if (valid) take(s);
-        }
-    }
     __device__ __forceinline__ bool takes(int x) const { return dual || ((j - first) & 1) == x; }
     __device__ __forceinline__ bool firstOf(int x) const { return j == first + (dual ? 0 : x); }
     __device__ __forceinline__ bool lastOf(int x) const { return j + (dual ? 1 : 2) >= last; }
-    __device__ __forceinline__ void nextOf(const TreeParams& p, const List& l, int x) {
-        do nextTile(p, l);
-        while (valid && !takes(x));
-    }
-    __device__ __forceinline__ void seekOf(const TreeParams& p, const List& l, int x) {
-        while (valid && !takes(x)) nextTile(p, l);
-    }
 };
 
 // Scores of keys that are not visible become -inf: outside [a, b) of the 32, or by bits.
@@ -162,11 +147,10 @@ __device__ __forceinline__ void maskBits(uint32_t (&r)[32], uint32_t bits) {
     for (int i = 0; i < 32; ++i)
         if (!(bits >> i & 1u)) r[i] = 0xFF800000u;
 }
-__device__ __forceinline__ void tmemLd16(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmemLd8(uint32_t taddr, uint32_t (&r)[8]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
         : "r"(taddr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -181,7 +165,7 @@ template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
              const __grid_constant__ CUtensorMap mapKNew, const __grid_constant__ CUtensorMap mapVNew,
-             const __grid_constant__ TreeParams p, float scaleLog2, int* errFlag, long long waitCycles) {
+             const __grid_constant__ TreeParams p, float scaleLog2, int* errFlag, long long waitLimit) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     extern __shared__ __align__(1024) unsigned char rawSmem[];
     Smem* s = reinterpret_cast<Smem*>(rawSmem);
@@ -202,6 +186,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
             mbarInit(&s->kFull[i], 1); mbarInit(&s->kEmpty[i], 1);
             mbarInit(&s->vFull[i], 1); mbarInit(&s->vEmpty[i], 1);
         }
+        for (int i = 0; i < kSpans; ++i) { mbarInit(&s->spanFull[i], 1); mbarInit(&s->spanEmpty[i], kSpanReaders); }
         s->dead = *reinterpret_cast<volatile int*>(errFlag) != 0 ? 1 : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         Header h{};
@@ -220,16 +205,16 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
     auto tmemS = [&](int x) { return tmem + 128u * static_cast<uint32_t>(x); };
     auto tmemO = [&](int x) { return tmem + 256u + 128u * static_cast<uint32_t>(x); };
     const bool live = *reinterpret_cast<volatile int*>(&s->dead) == 0;
-    const long long waitLimit = waitCycles > 0 ? waitCycles : kWaitCycles;
-    List list;
-    {
-        const int total = s->prefix[p.batch];
-        list.prefix = s->prefix;
-        // (at least two, so that every block between a pair's first and last has a tile of it)
-        list.quota = max(2, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-        list.begin = static_cast<int>(min(static_cast<long long>(blockIdx.x) * list.quota, static_cast<long long>(total)));
-        list.end = min(total, list.begin + list.quota);
-    }
+    // The block's span number k.  Null when the wait for it ran out.
+    auto spanAt = [&](int k) -> const Span* {
+        bool ok = mbarWait(&s->spanFull[k % kSpans], (k / kSpans) & 1, &s->dead, errFlag, waitLimit, 54);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        return ok ? &s->span[k % kSpans] : nullptr;
+    };
+    auto spanDone = [&](int k) {
+        __syncwarp();
+        if (lane == 0) mbarArrive(&s->spanEmpty[k % kSpans]);
+    };
 
     // 512 x 128 registers at launch: 80 for the service warps, 64 for the output warps, 184 for softmax
     if (warp == kKProducerWarp || warp == kVProducerWarp) {
@@ -241,10 +226,12 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         unsigned long long *full = isV ? s->vFull : s->kFull, *empty = isV ? s->vEmpty : s->kEmpty;
         unsigned char(*tiles)[kTileBytes] = isV ? s->v : s->k;
         const int tilesPerPage = p.blockSize / 16;
-        int pos = list.begin, gt = 0;
-        Span g;
+        int gt = 0;
         bool ok = true;
-        while (ok && list.next(p, pos, g)) {
+        for (int k = 0; ok; ++k) {
+            const Span* at = spanAt(k);
+            if (!at || !at->valid) break;
+            const Span& g = *at;
             const int32_t* table = p.tables + static_cast<int64_t>(g.b) * p.maxNumBlocks;
             for (int j = g.first; j < g.last && ok; ++j, ++gt) {
                 const int st = gt % kStages;
@@ -269,6 +256,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                     tmaLoad2d(tiles[st] + kHalfBytes + lane * 2048, pool, &full[st], 64, row);
                 }
             }
+            spanDone(k);
         }
     } else if (warp == kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -280,9 +268,22 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         const uint32_t hiK = descHi(1024);
         bool ok = true;
         Place c, n0, n1;                     // the tile at hand; the groups' next S products
-        c.init(p, list);
+        auto take = [&](Place& n, int k) {
+            const Span* at = spanAt(k);
+            n.k = k;
+            n.valid = at && at->valid;
+            if (!at) ok = false;
+            if (n.valid) { n.first = n.j = at->first; n.last = at->last; n.dual = at->dual != 0; n.lo = at->shortKeys(); }
+        };
+        auto nextTile = [&](Place& n) {
+            ++n.j;
+            ++n.g;
+            if (n.j == n.last) take(n, n.k + 1);
+        };
+        c.g = 0;
+        take(c, 0);
         n0 = n1 = c;
-        n1.seekOf(p, list, 1);
+        while (n1.valid && !n1.takes(1)) nextTile(n1);
         int steps0 = 0, steps1 = 0;          // P V products of a group: phase of pFull
         int spans0 = 0, spans1 = 0;          // spans whose S products of a group have begun: phase of qFull
         int begun0 = 0, begun1 = 0;          // ... whose P V products have: phase of oEmpty
@@ -319,7 +320,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
             }
             __syncwarp();
             if (begins) ++spans;
-            n.nextOf(p, list, x);
+            do nextTile(n);
+            while (n.valid && !n.takes(x));
         };
         while (c.valid && ok) {
 #pragma unroll
@@ -368,10 +370,39 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 // the group's next S product, behind the product that read the weights it overwrites
                 if (n.valid && n.g <= c.g + 2) issueQK(x, n, spans, true);
             }
-            c.nextTile(p, list);
+            const int k = c.k;
+            nextTile(c);
+            if (c.k != k) spanDone(k);       // (the cursors ahead are in later spans by now)
         }
-    } else if (warp < kOutputWarp0 && warp > kMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");          // (the fourth warp of the service warpgroup)
+    } else if (warp == kPlanWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (!live) goto done;
+        const int total = s->prefix[p.batch];
+        // (a piece of at least two, so that every block between a pair's first and last has a tile of it)
+        const int quota = max(2, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+        const int begin = static_cast<int>(min(static_cast<long long>(blockIdx.x) * quota, static_cast<long long>(total)));
+        const int end = min(total, begin + quota);
+        int pos = begin, tile = 0;
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+            Span g;
+            const bool got = nextSpan(p, s->prefix, begin, end, quota, pos, g);
+            g.valid = got;
+            g.tile = tile;
+            if (got) {
+                g.hi = lastFirst(p, g.s, g.rp, kPairRows);
+                tile += g.last - g.first;
+            }
+            if (k >= kSpans) ok = mbarWait(&s->spanEmpty[k % kSpans], ((k / kSpans) - 1) & 1, &s->dead, errFlag, waitLimit, 55);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            if (lane == 0) {
+                s->span[k % kSpans] = g;
+                mbarArrive(&s->spanFull[k % kSpans]);
+            }
+            __syncwarp();
+            if (!got) break;
+        }
     } else if (warp >= kOutputWarp0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (!live) goto done;
@@ -379,22 +410,15 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         const uint32_t laneBase = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const bool first = threadIdx.x == kOutputWarp0 * 32;
         int cnt0 = 0, cnt1 = 0;              // spans of a group written: phase of oFull
-        int pos = list.begin;
-        const Span& g = s->span[warp][0];
-        auto seek = [&]() {
-            Span q;
-            const bool got = list.next(p, pos, q);
-            __syncwarp();
-            if (lane == 0 && got) s->span[warp][0] = q;
-            __syncwarp();
-            return got;
-        };
         bool ok = true;
-        while (ok && seek()) {
+        for (int k = 0; ok; ++k) {
+            const Span* at = spanAt(k);
+            ok = !anyOfOutput(at == nullptr);          // (all four warps decide together, so that none waits for one that gave up)
+            if (!ok || !at->valid) break;
+            const Span& g = *at;
             const bool has1 = g.tilesOf(1) > 0;
             ok = mbarWait(&s->oFull[0], cnt0 & 1, &s->dead, errFlag, waitLimit, 49);
             if (ok && has1) ok = mbarWait(&s->oFull[1], cnt1 & 1, &s->dead, errFlag, waitLimit, 51);
-            // (all four warps decide together, so that none waits for one that gave up)
             ok = !anyOfOutput(!ok);
             if (!ok) break;
             tcFenceAfter();
@@ -408,10 +432,9 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 h->odd[which] = odd ? 1 : 0;
                 if (which == 1) {
                     h->b = g.b; h->kvh = g.kvh; h->rt = g.rp;
-                    h->lastBlock = (g.start + (g.nT - 1) * g.weight()) / list.quota;
+                    h->lastBlock = g.lastBlock;
                 }
             }
-            const uint32_t hi = odd && whole ? lastFirst(p, g.s, g.rp, kPairRows) : 0u;
             float* rec = whole ? nullptr : recordOf(p, gridDim.x, blockIdx.x, which, kPairRows, kHd);
 #pragma unroll 1
             for (int x = 0; x < (g.dual ? 2 : 1); ++x) {
@@ -428,41 +451,58 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 a0 *= inv;
                 a1 *= inv;
-                T* out = nullptr;
-                if (whole && mine) out = static_cast<T*>(p.out) + (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd;
+                {
+                    // the row's address, and those of the three rows whose pieces this lane stores as well
+                    int64_t at64 = mine ? (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd : -1;
+                    float4* recO = reinterpret_cast<float4*>(rec) + rl;
 #pragma unroll 1
-                for (int c = 0; c < 8; ++c) {           // 16 columns at a time
-                    uint32_t o[16];
-                    float f[16];
-                    tmemLd16(tmemO(x) + laneBase + 16u * c, o);
+                    for (int c = 0; c < 4; ++c) {           // 32 columns at a time
+                        uint32_t o[32];
+                        tmemLd32(tmemO(x) + laneBase + 32u * c, o);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * a0;
-                    if (!g.dual && has1) {
-                        tmemLd16(tmemO(1) + laneBase + 16u * c, o);
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a0);
+                        if (!g.dual && has1) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) f[i] = fmaf(__uint_as_float(o[i]), a1, f[i]);
-                    }
-                    if (whole && mine) {
-                        if (odd)
-#pragma unroll 1
-                            for (int i = 0; i < 16; ++i) {
-                                const float add = leftOut<T, T>(p, g.s, g.b, g.kvh, rr / group, hi, 16 * c + i);
+                            for (int h = 0; h < 4; ++h) {
+                                uint32_t u[8];
+                                tmemLd8(tmemO(1) + laneBase + 32u * c + 8u * h, u);
 #pragma unroll
-                                for (int k = 0; k < 16; ++k)
-                                    if (k == i) f[k] += add;
+                                for (int i = 0; i < 8; ++i) o[8 * h + i] = __float_as_uint(fmaf(__uint_as_float(u[i]), a1, __uint_as_float(o[8 * h + i])));
                             }
+                        }
+                        if (!whole) {
+                            // records are [32 pieces of 4 columns][256 rows]: consecutive lanes, consecutive 16 bytes
+                            if (mine)
 #pragma unroll
-                        for (int q = 0; q < 2; ++q)
-                            *reinterpret_cast<uint4*>(out + 16 * c + 8 * q) =
-                                make_uint4(pack16<BF16>(f[8 * q], f[8 * q + 1]), pack16<BF16>(f[8 * q + 2], f[8 * q + 3]),
-                                           pack16<BF16>(f[8 * q + 4], f[8 * q + 5]), pack16<BF16>(f[8 * q + 6], f[8 * q + 7]));
-                    } else if (mine) {
+                                for (int q = 0; q < 8; ++q)
+                                    recO[(8 * c + q) * kPairRows] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
+                        } else {
+                            // Four lanes trade their rows' four 16-byte pieces so that each store covers
+                            // 64 consecutive bytes of eight rows instead of 16 bytes of 32.
+                            uint32_t w[16];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            *reinterpret_cast<float4*>(rec + rl * kHd + 16 * c + 4 * q) = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+                            for (int i = 0; i < 16; ++i) w[i] = pack16<BF16>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+                            const int me = lane & 3;
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) {
+                                // step d: lane `me` sends piece (me ^ d) to lane me ^ d, which stores it as its own number
+                                const int dest = me ^ d;
+                                uint32_t v[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint32_t lo = dest & 1 ? w[4 + e] : w[e], hi2 = dest & 1 ? w[12 + e] : w[8 + e];
+                                    v[e] = __shfl_xor_sync(0xFFFFFFFFu, dest & 2 ? hi2 : lo, d);
+                                }
+                                const int64_t to = __shfl_xor_sync(0xFFFFFFFFu, at64, d);
+                                if (to >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to + 32 * c + 8 * me) = make_uint4(v[0], v[1], v[2], v[3]);
+                            }
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
+                if (whole && odd && mine)
+                    addLeftOut<T, T>(p, g.s, g.b, g.kvh, rr / group, g.hi, static_cast<T*>(p.out) + (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd, 0, kHd);
+                __syncwarp();
                 if (!whole && mine) {
                     rec[kPairRows * kHd + rl] = m;
                     rec[kPairRows * kHd + kPairRows + rl] = l;
@@ -476,6 +516,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
             }
             ++cnt0;
             if (has1) ++cnt1;
+            spanDone(k);
         }
     } else {
         // ------------------------------------------------------------ softmax groups
@@ -486,8 +527,6 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         const uint32_t sAddr = tmemS(x) + laneBase, oAddr = tmemO(x) + laneBase;
         bool ok = true;
         int steps = 0, spans = 0;            // tiles this group has done (phase of sFull), spans
-        int gt = 0;                          // tiles of the piece before the current span
-        int pos = list.begin;
         // this thread's query row of a span into the group's tile
         auto fetchQ = [&](const Span& q) {
             const int rr = q.firstRow(x) + t;
@@ -505,37 +544,30 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbarArrive(&s->qFull[x]);
         };
-        // the next span with tiles of this group, into the warp's slot `k`; the tiles of spans without
-        // are counted
-        int skipped = 0;
+        // the number of the next span at or after k with tiles of this group, or -1; spans without are
+        // given back
         auto seek = [&](int k) {
-            Span q;
-            skipped = 0;
-            while (list.next(p, pos, q)) {
-                if (q.tilesOf(x) > 0) {
-                    if (lane == 0) s->span[warp][k & 1] = q;
-                    __syncwarp();
-                    return true;
-                }
-                skipped += q.last - q.first;
+            for (;; ++k) {
+                const Span* at = spanAt(k);
+                if (!at) ok = false;
+                if (!at || !at->valid) return -1;
+                if (at->tilesOf(x) > 0) return k;
+                spanDone(k);
             }
-            return false;
         };
-        bool have = seek(0);
-        gt = skipped;
-        if (have) {
-            fetchQ(s->span[warp][0]);
+        int k = seek(0);
+        if (k >= 0) {
+            fetchQ(s->span[k % kSpans]);
             postQ();
         }
-        while (have && ok) {
-            const Span& g = s->span[warp][spans & 1];
-            have = seek(spans + 1);
-            const Span& nx = s->span[warp][(spans + 1) & 1];
-            const int rr = g.firstRow(x) + t;
-            const bool mine = rr < g.rows;
-            const int node = mine ? rr / group : 0;
-            const uint32_t from = max(firstOf(p, g.s, node), g.s.lo);
-            const uint32_t hi = lastFirst(p, g.s, g.rp, kPairRows);
+        while (k >= 0 && ok) {
+            const Span& g = s->span[k % kSpans];
+            int next = -2;                   // looked up at the span's last tile
+            {
+                const int rr = g.firstRow(x) + t, node = rr < g.rows ? rr / group : 0;
+                s->rowNode[x][t] = node;
+                s->rowFrom[x][t] = max(firstOf(p, g.s, node), g.s.lo);
+            }
             const bool useLo = BF16 && g.shortKeys();
             float mUsed = -INFINITY, l = 0.f;
             int odd = 0;
@@ -544,12 +576,16 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 const bool inTree = j >= g.cacheTiles;
                 const uint32_t k0 = inTree ? static_cast<uint32_t>(j - g.cacheTiles) * kKeys : (g.s.lo / kKeys + j) * kKeys;
                 const uint32_t keyEnd = inTree ? static_cast<uint32_t>(g.s.n) : g.s.held;
-                const bool edge = inTree || k0 < hi || k0 < g.s.lo || k0 + kKeys > keyEnd;
-                ok = mbarWait(&s->sFull[x], steps & 1, &s->dead, errFlag, waitLimit, 52);
+                const bool edge = inTree || k0 < g.hi || k0 < g.s.lo || k0 + kKeys > keyEnd;
+                const bool lastTile = j + g.step() >= g.last;
+                if (inTree)                               // (loads that the wait below hides)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s->rowBits[x][i][t] = treeBits(p, g.s, s->rowNode[x][t], static_cast<int>(k0 / 32) + i);
+                if (lastTile) next = seek(k + 1);
+                if (ok) ok = mbarWait(&s->sFull[x], steps & 1, &s->dead, errFlag, waitLimit, 52);
                 if (!ok) break;
                 tcFenceAfter();
-                const bool lastTile = j + g.step() >= g.last;
-                if (lastTile && have) fetchQ(nx);      // S of the span's last tile is there: the query tile is no longer read
+                if (next >= 0) fetchQ(s->span[next % kSpans]);     // S of the span's last tile is there: the query tile is no longer read
                 uint32_t r0[32], r1[32], r2[32], r3[32];
                 tmemLd32NoWait(sAddr, r0);
                 tmemLd32NoWait(sAddr + 32u, r1);
@@ -558,12 +594,12 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 tmemLdWait();
                 if (edge) {
                     if (inTree) {
-                        const int w = static_cast<int>(k0 / 32);
-                        maskBits(r0, treeBits(p, g.s, node, w));
-                        maskBits(r1, treeBits(p, g.s, node, w + 1));
-                        maskBits(r2, treeBits(p, g.s, node, w + 2));
-                        maskBits(r3, treeBits(p, g.s, node, w + 3));
+                        maskBits(r0, s->rowBits[x][0][t]);
+                        maskBits(r1, s->rowBits[x][1][t]);
+                        maskBits(r2, s->rowBits[x][2][t]);
+                        maskBits(r3, s->rowBits[x][3][t]);
                     } else {
+                        const uint32_t from = s->rowFrom[x][t];
                         const int a = from > k0 ? static_cast<int>(min(from - k0, 128u)) : 0, b = static_cast<int>(min(g.s.held - k0, 128u));
                         maskRange(r0, a, b);
                         maskRange(r1, a - 32, b - 32);
@@ -621,24 +657,32 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                     // Row t of V: zeros where there is no such key, finite values where some row may not
                     // see it.  (Both groups of a dual span may write the same.  The phase asked for is not two
                     // ahead: this S product was issued after the wait for V of the tile two before.)
-                    const int tile = gt + j - g.first, st = tile % kStages;
+                    const int tile = g.tile + j - g.first, st = tile % kStages;
                     ok = mbarWait(&s->vFull[st], (tile / kStages) & 1, &s->dead, errFlag, waitLimit, 53);
                     if (!ok) break;
                     const uint32_t key = k0 + static_cast<uint32_t>(t);
                     const bool there = key < keyEnd && (inTree || key >= g.s.lo);
-                    unsigned char* row = s->v[st] + t * 128;
-                    if (!there) {
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(row + (c >> 3) * kHalfBytes + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    } else if (inTree || key < hi) {
+                    if (!there || inTree || key < g.hi) {
                         constexpr uint32_t kExp = BF16 ? 0x7F80u : 0x7C00u;
 #pragma unroll 1
-                        for (int c = 0; c < 64; ++c) {
-                            uint32_t* w = reinterpret_cast<uint32_t*>(row + (c >> 5) * kHalfBytes + (c & 31) * 4);
-                            uint32_t v = *w;
-                            if ((v & kExp) == kExp) v &= 0xFFFF0000u;
-                            if ((v >> 16 & kExp) == kExp) v &= 0x0000FFFFu;
-                            if (v != *w) { *w = v; odd = 1; }
+                        for (int c = 0; c < 16; ++c) {
+                            // (lane by lane another piece of the row first: no two on one bank)
+                            uint4* at = reinterpret_cast<uint4*>(s->v[st] + (c >> 3) * kHalfBytes + t * 128 + (((c ^ t) & 7) << 4));
+                            if (!there) {
+                                *at = make_uint4(0u, 0u, 0u, 0u);
+                                continue;
+                            }
+                            uint4 w = *at;
+                            uint32_t changed = 0;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                uint32_t& u = e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w;
+                                const uint32_t was = u;
+                                if ((u & kExp) == kExp) u &= 0xFFFF0000u;
+                                if ((u >> 16 & kExp) == kExp) u &= 0x0000FFFFu;
+                                changed |= was ^ u;
+                            }
+                            if (changed) { *at = w; odd = 1; }
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -653,8 +697,9 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
             }
             if (!ok) break;
             ++spans;
-            gt += g.last - g.first + skipped;
-            if (have) postQ();
+            if (next >= 0) postQ();
+            spanDone(k);
+            k = next;
         }
     }
 
@@ -716,7 +761,8 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
     auto run = [&](auto kernel) -> cudaError_t {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smemBytes(kTreeMaxBatch)));
         if (e != cudaSuccess) return e;
-        kernel<<<plan.blocks, kThreads, smem, stream>>>(pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag, p.waitCycles);
+        kernel<<<plan.blocks, kThreads, smem, stream>>>(pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag,
+                                                     p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
         return cudaGetLastError();
     };
     return p.dtype == kBF16 ? run(treeTcKernel<true>) : run(treeTcKernel<false>);
