@@ -37,6 +37,18 @@ __device__ __forceinline__ bool mbarTry(unsigned long long* bar, uint32_t parity
         : "memory");
     return ok != 0;
 }
+// Whether the phase is complete, without waiting at all (try_wait may suspend the thread for a while).
+__device__ __forceinline__ bool mbarTest(unsigned long long* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smemAddr(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // The same with a suspend-time hint: the warp sleeps in hardware until the
 // phase completes or about that many nanoseconds have passed, instead of
 // spinning through issue slots that the working warps need.

@@ -14,17 +14,23 @@
 // rows a tile of 64 KB costs about what its fetch costs, below that the kernel is bound by HBM,
 // above it by the chain softmax -> P V -> next S of the two groups.
 //
-//   warps 0-3, 4-7   softmax groups: thread t owns row t of the group's rows.  It also brings its
-//                    query row into shared memory (cp.async into the swizzled layout) and, in tiles
-//                    with keys that are not there or that only some rows see, clears row t of V.
-//   warps 8, 9       TMA producers of K and V (two stages each): eight pages of 16 rows per tile, or
-//                    one box of 128 rows of the step's own keys and values for a tile of the tree.
+//   warps 0-3, 4-7   softmax groups: thread t owns row t of the group's rows.  In tiles with keys
+//                    that are not there or that only some rows see it also clears row t of V.
+//   warps 8, 9       TMA producers of K (tiles) and V (half tiles: a stage is free again after half
+//                    a P V product): pages of 16 rows, or boxes of the step's own keys and values for
+//                    a tile of the tree.
 //   warp 11          walks the list and leaves the block's spans (its parts of pairs) in a ring in
 //                    shared memory, a few ahead of the warps that work on them: a step of that walk is
 //                    some loads and divisions in a row, a microsecond that nobody else waits for.
 //   warp 10          issues the products.  Per group a cursor names its next S product; it is issued
 //                    behind the group's P V product as soon as its tile and queries are there.
-//   warps 12-15      outputs and records: thread t owns row t, out of tensor memory.
+//   warps 12-15      outputs and records: thread t owns row t, out of tensor memory.  Before that they
+//                    bring the queries of the next span into shared memory (cp.async, row t each),
+//                    once the span's last S product is complete.
+//
+// Two forms: when no request of the launch can have more than 128 rows under a KV head there is one
+// query tile and room for three K stages and five half stages of V (measured at 64 requests of 2048
+// tokens and 64 rows each, bound by HBM: LATENCY_FIGURE); else two query tiles, two and four.
 //
 // Every wait is bounded as in the prefill kernel.
 #include <algorithm>
@@ -40,8 +46,8 @@ using namespace tc;
 using namespace tree;
 
 constexpr int kRows = 128, kKeys = 128, kHd = 128, kPairRows = 256;
-constexpr int kStages = 2;                             // of K and of V
-constexpr int kTileBytes = kKeys * kHd * 2, kHalfBytes = kTileBytes / 2;
+constexpr int kTileBytes = kKeys * kHd * 2, kHalfBytes = kTileBytes / 2;      // a 64-dim block of a tile
+constexpr int kVHalfBytes = kTileBytes / 2, kVBlockBytes = kVHalfBytes / 2;   // 64 keys of V, a 64-dim block of them
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kShortKeys = 256;                        // bfloat16: fewer visible keys carry the weights as two operands
 constexpr long long kWaitCycles = 400000000LL;
@@ -65,14 +71,16 @@ struct Span {
     __device__ __forceinline__ bool shortKeys() const { return s.held - s.lo + static_cast<uint32_t>(s.n) < kShortKeys; }
 };
 
-constexpr int kSpans = 8;        // of the ring: no warp is more than six spans ahead of another
+constexpr int kSpans = 8;        // of the ring: no warp needs a span more than five behind the oldest one in use
 
+template <bool WIDE>
 struct Smem {
-    unsigned char q[2][kTileBytes];
-    unsigned char k[kStages][kTileBytes];
-    unsigned char v[kStages][kTileBytes];
-    unsigned long long kFull[kStages], kEmpty[kStages], vFull[kStages], vEmpty[kStages];
-    unsigned long long qFull[2], sFull[2], pFull[2], oFull[2], oEmpty[2];
+    static constexpr int kQTiles = WIDE ? 2 : 1, kKStages = WIDE ? 2 : 3, kVStages = WIDE ? 4 : 5;
+    unsigned char q[kQTiles][kTileBytes];
+    unsigned char k[kKStages][kTileBytes];
+    unsigned char v[kVStages][kVHalfBytes];
+    unsigned long long kFull[kKStages], kEmpty[kKStages], vFull[kVStages], vEmpty[kVStages];
+    unsigned long long qFull, qEmpty, sFull[2], pFull[2], oFull[2], oEmpty[2];
     unsigned long long spanFull[kSpans], spanEmpty[kSpans];
     // [span of the group & 1][group][row]: sum and reference of the row, and whether the thread left a
     // value out.  Written before the weights of the span's last tile are released, read behind the
@@ -90,8 +98,9 @@ struct Smem {
     int dead;
     int prefix[1];                                     // [batch + 1]
 };
-size_t smemBytes(int batch) { return sizeof(Smem) + static_cast<size_t>(batch) * sizeof(int); }
-static_assert(sizeof(Smem) + kTreeMaxBatch * sizeof(int) <= 227 * 1024, "the block's shared memory must fit the 227 KB a block may opt into");
+constexpr size_t kSmemLimit = 227 * 1024;
+template <bool WIDE> constexpr size_t smemBytes(int batch) { return sizeof(Smem<WIDE>) + static_cast<size_t>(batch) * sizeof(int); }
+static_assert(smemBytes<true>(kTreeMaxBatch) <= kSmemLimit, "the block's shared memory must fit the 227 KB a block may opt into");
 constexpr int kSpanReaders = 2 + 1 + 4 + 8;            // warps: producers, issuer, output, softmax
 
 // The block's next span at or after position `pos` of the list (a pair's start, or the block's
@@ -126,33 +135,29 @@ __device__ __forceinline__ bool nextSpan(const TreeParams& p, const int* prefix,
     return false;
 }
 
-// What the issuer keeps of a place in the stream: tile j of the block's span number k, g tiles into
-// its piece.
-struct Place {
-    int k, first, last, j, g;
+// A step of the block's stream: group x on tile j of the span number k, g tiles into the piece.
+struct Step {
+    int k, first, last, j, g, x;
     bool valid, dual, lo;
-    __device__ __forceinline__ bool takes(int x) const { return dual || ((j - first) & 1) == x; }
-    __device__ __forceinline__ bool firstOf(int x) const { return j == first + (dual ? 0 : x); }
-    __device__ __forceinline__ bool lastOf(int x) const { return j + (dual ? 1 : 2) >= last; }
+    __device__ __forceinline__ bool begins() const { return j == first + (dual ? 0 : x); }        // the group's first of the span
+    __device__ __forceinline__ bool ends() const { return j + (dual ? 1 : 2) >= last; }           // ... last
+    __device__ __forceinline__ bool endsTile() const { return !dual || x == 1; }
+    __device__ __forceinline__ bool opensSpan() const { return j == first && x == 0; }
+    __device__ __forceinline__ bool closesSpan() const { return j + 1 == last && endsTile(); }
 };
 
-// Scores of keys that are not visible become -inf: outside [a, b) of the 32, or by bits.
-__device__ __forceinline__ void maskRange(uint32_t (&r)[32], int a, int b) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-        if (i < a || i >= b) r[i] = 0xFF800000u;
-}
+// Scores of keys that are not visible (bit i clear) become -inf.
 __device__ __forceinline__ void maskBits(uint32_t (&r)[32], uint32_t bits) {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
         if (!(bits >> i & 1u)) r[i] = 0xFF800000u;
 }
-__device__ __forceinline__ void tmemLd8(uint32_t taddr, uint32_t (&r)[8]) {
+__device__ __forceinline__ void tmemLd16NoWait(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 // Whether `v` is set in any of the 128 threads of the output warps (all of them get here).
 __device__ __forceinline__ bool anyOfOutput(bool v) {
@@ -161,31 +166,31 @@ __device__ __forceinline__ bool anyOfOutput(bool v) {
     return r != 0;
 }
 
-template <bool BF16>
+template <bool BF16, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1)
 treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
              const __grid_constant__ CUtensorMap mapKNew, const __grid_constant__ CUtensorMap mapVNew,
              const __grid_constant__ TreeParams p, float scaleLog2, int* errFlag, long long waitLimit) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     extern __shared__ __align__(1024) unsigned char rawSmem[];
-    Smem* s = reinterpret_cast<Smem*>(rawSmem);
+    using S = Smem<WIDE>;
+    S* s = reinterpret_cast<S*>(rawSmem);
     if ((smemAddr(rawSmem) & 1023u) != 0) {
         if (threadIdx.x == 0) atomicCAS(errFlag, 0, 40);
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.heads / p.kvHeads;
     if (threadIdx.x == 0) {
+        mbarInit(&s->qFull, kRows);
+        mbarInit(&s->qEmpty, 1);
         for (int i = 0; i < 2; ++i) {
-            mbarInit(&s->qFull[i], kRows);
             mbarInit(&s->sFull[i], 1);
             mbarInit(&s->pFull[i], kRows);
             mbarInit(&s->oFull[i], 1);
             mbarInit(&s->oEmpty[i], 1);
         }
-        for (int i = 0; i < kStages; ++i) {
-            mbarInit(&s->kFull[i], 1); mbarInit(&s->kEmpty[i], 1);
-            mbarInit(&s->vFull[i], 1); mbarInit(&s->vEmpty[i], 1);
-        }
+        for (int i = 0; i < S::kKStages; ++i) { mbarInit(&s->kFull[i], 1); mbarInit(&s->kEmpty[i], 1); }
+        for (int i = 0; i < S::kVStages; ++i) { mbarInit(&s->vFull[i], 1); mbarInit(&s->vEmpty[i], 1); }
         for (int i = 0; i < kSpans; ++i) { mbarInit(&s->spanFull[i], 1); mbarInit(&s->spanEmpty[i], kSpanReaders); }
         s->dead = *reinterpret_cast<volatile int*>(errFlag) != 0 ? 1 : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -223,10 +228,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         const bool isV = warp == kVProducerWarp;
         const CUtensorMap* pool = isV ? &mapV : &mapK;
         const CUtensorMap* fresh = isV ? &mapVNew : &mapKNew;
-        unsigned long long *full = isV ? s->vFull : s->kFull, *empty = isV ? s->vEmpty : s->kEmpty;
-        unsigned char(*tiles)[kTileBytes] = isV ? s->v : s->k;
         const int tilesPerPage = p.blockSize / 16;
-        int gt = 0;
+        int gt = 0;                          // tiles of the block's piece so far
         bool ok = true;
         for (int k = 0; ok; ++k) {
             const Span* at = spanAt(k);
@@ -234,8 +237,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
             const Span& g = *at;
             const int32_t* table = p.tables + static_cast<int64_t>(g.b) * p.maxNumBlocks;
             for (int j = g.first; j < g.last && ok; ++j, ++gt) {
-                const int st = gt % kStages;
                 const bool inTree = j >= g.cacheTiles;
+                const int freshRow = g.s.start + (j - g.cacheTiles) * kKeys;
                 int row = 0;
                 if (!inTree && lane < kKeys / 16) {
                     const int t16 = (static_cast<int>(g.s.lo / kKeys) + j) * (kKeys / 16) + lane;
@@ -243,17 +246,39 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                     const int blk = min(max(table[page], 0), p.poolBlocks - 1);
                     row = (blk * p.kvHeads + g.kvh) * p.blockSize + (t16 % tilesPerPage) * 16;
                 }
-                if (gt >= kStages) ok = mbarWait(&empty[st], ((gt / kStages) - 1) & 1, &s->dead, errFlag, waitLimit, isV ? 42 : 41);
-                ok = __all_sync(0xFFFFFFFFu, ok);
-                if (!ok) break;
-                if (lane == 0) mbarExpectTx(&full[st], kTileBytes);
-                __syncwarp();
-                if (inTree) {
-                    if (lane < 2)
-                        tmaLoad3d(tiles[st] + lane * kHalfBytes, fresh, &full[st], 64 * lane, g.kvh, g.s.start + (j - g.cacheTiles) * kKeys);
-                } else if (lane < kKeys / 16) {
-                    tmaLoad2d(tiles[st] + lane * 2048, pool, &full[st], 0, row);
-                    tmaLoad2d(tiles[st] + kHalfBytes + lane * 2048, pool, &full[st], 64, row);
+                if (!isV) {
+                    const int st = gt % S::kKStages;
+                    if (gt >= S::kKStages) ok = mbarWait(&s->kEmpty[st], ((gt / S::kKStages) - 1) & 1, &s->dead, errFlag, waitLimit, 41);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbarExpectTx(&s->kFull[st], kTileBytes);
+                    __syncwarp();
+                    unsigned char* to = s->k[st];
+                    if (inTree) {
+                        if (lane < 2)
+                            for (int h = 0; h < 2; ++h)        // (a box is 64 rows)
+                                tmaLoad3d(to + lane * kHalfBytes + h * kVBlockBytes, fresh, &s->kFull[st], 64 * lane, g.kvh, freshRow + 64 * h);
+                    } else if (lane < kKeys / 16) {
+                        tmaLoad2d(to + lane * 2048, pool, &s->kFull[st], 0, row);
+                        tmaLoad2d(to + kHalfBytes + lane * 2048, pool, &s->kFull[st], 64, row);
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int n = 2 * gt + h, st = n % S::kVStages;
+                        if (n >= S::kVStages) ok = mbarWait(&s->vEmpty[st], ((n / S::kVStages) - 1) & 1, &s->dead, errFlag, waitLimit, 42);
+                        ok = __all_sync(0xFFFFFFFFu, ok);
+                        if (!ok) break;
+                        if (lane == 0) mbarExpectTx(&s->vFull[st], kVHalfBytes);
+                        __syncwarp();
+                        unsigned char* to = s->v[st];
+                        if (inTree) {
+                            if (lane < 2) tmaLoad3d(to + lane * kVBlockBytes, fresh, &s->vFull[st], 64 * lane, g.kvh, freshRow + 64 * h);
+                        } else if (lane >> 2 == h) {
+                            tmaLoad2d(to + (lane & 3) * 2048, pool, &s->vFull[st], 0, row);
+                            tmaLoad2d(to + kVBlockBytes + (lane & 3) * 2048, pool, &s->vFull[st], 64, row);
+                        }
+                    }
                 }
             }
             spanDone(k);
@@ -267,112 +292,135 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         const uint32_t idescO = idescS | (1u << 16);
         const uint32_t hiK = descHi(1024);
         bool ok = true;
-        Place c, n0, n1;                     // the tile at hand; the groups' next S products
-        auto take = [&](Place& n, int k) {
-            const Span* at = spanAt(k);
-            n.k = k;
-            n.valid = at && at->valid;
-            if (!at) ok = false;
-            if (n.valid) { n.first = n.j = at->first; n.last = at->last; n.dual = at->dual != 0; n.lo = at->shortKeys(); }
+        // The steps of the stream, in order: a tile of a dual span is one step of each group, else tiles
+        // alternate between the groups.  Products of a group come in the order S, P V, S, ..., and of
+        // two steps in a row (nearly always of two groups) the second one's S must not wait for the
+        // first one's weights: c is the next step to have its P V product issued, n the next one to have
+        // its S product issued, up to two steps ahead, where the group's step before is through.
+        Step c, n;
+        auto take = [&](Step& at, int k) {
+            const Span* sp = spanAt(k);
+            at.k = k;
+            at.x = 0;
+            at.valid = sp && sp->valid;
+            if (!sp) ok = false;
+            if (at.valid) { at.first = at.j = sp->first; at.last = sp->last; at.dual = sp->dual != 0; at.lo = sp->shortKeys(); }
         };
-        auto nextTile = [&](Place& n) {
-            ++n.j;
-            ++n.g;
-            if (n.j == n.last) take(n, n.k + 1);
+        auto advance = [&](Step& at) {
+            const bool sameTile = at.dual && at.x == 0;
+            at.x ^= 1;
+            if (sameTile) return;
+            ++at.g;
+            if (++at.j == at.last) take(at, at.k + 1);
         };
         c.g = 0;
         take(c, 0);
-        n0 = n1 = c;
-        while (n1.valid && !n1.takes(1)) nextTile(n1);
-        int steps0 = 0, steps1 = 0;          // P V products of a group: phase of pFull
-        int spans0 = 0, spans1 = 0;          // spans whose S products of a group have begun: phase of qFull
-        int begun0 = 0, begun1 = 0;          // ... whose P V products have: phase of oEmpty
-        int open0 = 0, open1 = 0;            // per key stage: S products still to come on its tile
-        // The group's next S product: when `poll`, only if its tile and queries are there already.
-        // A tile is at most two ahead of the one at hand, so that the phase before the one asked for
-        // is known to be complete (every S product of the tile two before it has been issued).
-        auto issueQK = [&](int x, Place& n, int& spans, bool poll) {
-            const int st = n.g % kStages;
-            const bool begins = n.firstOf(x);
-            if (poll) {
-                bool there = mbarTry(&s->kFull[st], (n.g / kStages) & 1);
-                if (begins) there = there && mbarTry(&s->qFull[x], spans & 1);
-                if (!__all_sync(0xFFFFFFFFu, there)) return;
-            } else {
-                if (begins) ok = mbarWait(&s->qFull[x], spans & 1, &s->dead, errFlag, waitLimit, 43);
-                if (ok) ok = mbarWait(&s->kFull[st], (n.g / kStages) & 1, &s->dead, errFlag, waitLimit, 44);
-                ok = __all_sync(0xFFFFFFFFu, ok);
-                if (!ok) return;
-            }
-            tcFenceAfter();
-            const uint32_t qLo = descLo(smemAddr(s->q[x]), 16), kLo = descLo(smemAddr(s->k[st]), 16), dS = tmemS(x);
-            int& open = st ? open1 : open0;
-            if (open == 0) open = n.dual ? 2 : 1;
-            --open;
-            if (leader) {
-#pragma unroll
-                for (int ks = 0; ks < kHd / 16; ++ks) {
-                    const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
-                    umma(dS, desc64(qLo + off, hiK), desc64(kLo + off, hiK), idescS, ks > 0);
-                }
-                ummaCommit(&s->sFull[x]);
-                if (open == 0) ummaCommit(&s->kEmpty[st]);
-            }
-            __syncwarp();
-            if (begins) ++spans;
-            do nextTile(n);
-            while (n.valid && !n.takes(x));
-        };
+        n = c;
+        int cs = 0, ns = 0;                  // numbers of the two steps
+        int nPrev = -1;                      // group of the step before n
+        uint32_t pParity = 0, oParity = 0, begun = 0;      // bit x: phase of pFull, of oEmpty; group x has begun a span
         while (c.valid && ok) {
+            // ---- S products, while the weights of step c are waited for
+            bool got = false;                // ... they are there
+            long long since = 0;
+            while (ok && !got) {
+                if (n.valid && ns <= cs + 1 && !(ns > cs && n.x == nPrev)) {      // (the group's step before is n - 1, or through)
+                    const int st = n.g % S::kKStages;
+                    const uint32_t kPar = (n.g / S::kKStages) & 1, qPar = n.k & 1;
+                    bool there = true;
+                    if (ns > cs) {
+                        // ahead of need: only if everything is there
+                        there = mbarTest(&s->kFull[st], kPar) && (!n.opensSpan() || mbarTest(&s->qFull, qPar));
+                        there = __all_sync(0xFFFFFFFFu, there);
+                    } else {
+                        if (n.opensSpan()) ok = mbarWait(&s->qFull, qPar, &s->dead, errFlag, waitLimit, 43);
+                        if (ok) ok = mbarWait(&s->kFull[st], kPar, &s->dead, errFlag, waitLimit, 44);
+                        ok = __all_sync(0xFFFFFFFFu, ok);
+                        if (!ok) break;
+                    }
+                    if (there) {
+                        tcFenceAfter();
+                        const uint32_t qLo = descLo(smemAddr(s->q[0]) + (WIDE && n.dual ? n.x * kTileBytes : 0), 16);
+                        const uint32_t kLo = descLo(smemAddr(s->k[0]) + st * kTileBytes, 16), dS = tmemS(n.x);
+                        uint64_t dq[kHd / 16], dk[kHd / 16];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                Place& n = x ? n1 : n0;
-                int& spans = x ? spans1 : spans0;
-                if (ok && n.valid && n.g <= c.g) issueQK(x, n, spans, false);
+                        for (int ks = 0; ks < kHd / 16; ++ks) {
+                            const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                            dq[ks] = desc64(qLo + off, hiK);
+                            dk[ks] = desc64(kLo + off, hiK);
+                        }
+                        if (leader) {
+#pragma unroll
+                            for (int ks = 0; ks < kHd / 16; ++ks) umma(dS, dq[ks], dk[ks], idescS, ks > 0);
+                            ummaCommit(&s->sFull[n.x]);
+                            if (n.endsTile()) ummaCommit(&s->kEmpty[st]);
+                            if (n.closesSpan()) ummaCommit(&s->qEmpty);
+                        }
+                        __syncwarp();
+                        nPrev = n.x;
+                        ++ns;
+                        advance(n);
+                        continue;
+                    }
+                }
+                // (a fifth of a microsecond at most, then the other condition again)
+                got = __all_sync(0xFFFFFFFFu, mbarTrySleep(&s->pFull[c.x], pParity >> c.x & 1, 200u));
+                if (!got) {
+                    if (since == 0) since = clock64();
+                    else if (clock64() - since > waitLimit) {
+                        *reinterpret_cast<volatile int*>(&s->dead) = 1;
+                        atomicCAS(errFlag, 0, 45);
+                    }
+                    if (*reinterpret_cast<volatile int*>(&s->dead)) ok = false;
+                    ok = __all_sync(0xFFFFFFFFu, ok);
+                }
             }
-            // (a group that takes the next tile need not wait for this one's weights)
-            if (ok && n0.valid && n0.g == c.g + 1 && !c.takes(0)) issueQK(0, n0, spans0, true);
-            if (ok && n1.valid && n1.g == c.g + 1 && !c.takes(1)) issueQK(1, n1, spans1, true);
             if (!ok) break;
-            const int st = c.g % kStages;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                if (!c.takes(x) || !ok) continue;
-                int &steps = x ? steps1 : steps0, &spans = x ? spans1 : spans0;
-                Place& n = x ? n1 : n0;
-                ok = mbarWait(&s->pFull[x], steps & 1, &s->dead, errFlag, waitLimit, 45);
-                if (ok) ok = mbarWait(&s->vFull[st], (c.g / kStages) & 1, &s->dead, errFlag, waitLimit, 46);
+            // ---- the P V product of step c
+            const int x = c.x;
+            pParity ^= 1u << x;
+            const bool begins = c.begins();
+            if (begins) {
                 // the accumulator is free once the output of the group's span before was read from it
-                const bool begins = c.firstOf(x);
-                int& begun = x ? begun1 : begun0;
-                if (ok && begins && begun >= 1) ok = mbarWait(&s->oEmpty[x], (begun - 1) & 1, &s->dead, errFlag, waitLimit, 47);
-                if (begins) ++begun;
+                if (ok && (begun >> x & 1)) {
+                    ok = mbarWait(&s->oEmpty[x], oParity >> x & 1, &s->dead, errFlag, waitLimit, 47);
+                    oParity ^= 1u << x;
+                }
+                begun |= 1u << x;
+            }
+            const uint32_t sCol = tmemS(x), dO = tmemO(x);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int v = 2 * c.g + h, st = v % S::kVStages;
+                if (ok) ok = mbarWait(&s->vFull[st], (v / S::kVStages) & 1, &s->dead, errFlag, waitLimit, 46);
                 ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
                 tcFenceAfter();
-                const uint32_t vLo = descLo(smemAddr(s->v[st]), kHalfBytes);
-                const uint32_t sCol = tmemS(x), dO = tmemO(x);
-                const bool lastUser = x == 1 || !c.takes(1);
-                if (leader) {
+                const uint32_t vLo = descLo(smemAddr(s->v[0]) + st * kVHalfBytes, kVBlockBytes);
+                uint64_t dv[4];
 #pragma unroll
-                    for (int ks = 0; ks < kKeys / 16; ++ks)
-                        ummaTs(dO, sCol + 32u * (ks >> 1) + 8u * (ks & 1), desc64(vLo + ks * 128, hiK), idescO, ks > 0 || !begins ? 1u : 0u);
+                for (int ks = 0; ks < 4; ++ks) dv[ks] = desc64(vLo + ks * 128, hiK);
+                if (leader) {
+                    // P of keys 32 i .. 32 i + 31 sits in columns 32 i .. 32 i + 15 of the S buffer (and, with
+                    // two operands, its remainder in columns 32 i + 16 .. 32 i + 31)
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        ummaTs(dO, sCol + 64u * h + 32u * (ks >> 1) + 8u * (ks & 1), dv[ks], idescO, h + ks > 0 || !begins ? 1u : 0u);
                     if (BF16 && c.lo) {
 #pragma unroll
-                        for (int ks = 0; ks < kKeys / 16; ++ks)
-                            ummaTs(dO, sCol + 32u * (ks >> 1) + 8u * (ks & 1) + 16u, desc64(vLo + ks * 128, hiK), idescO, 1u);
+                        for (int ks = 0; ks < 4; ++ks)
+                            ummaTs(dO, sCol + 64u * h + 32u * (ks >> 1) + 8u * (ks & 1) + 16u, dv[ks], idescO, 1u);
                     }
-                    if (c.lastOf(x)) ummaCommit(&s->oFull[x]);
-                    if (lastUser) ummaCommit(&s->vEmpty[st]);
+                    if (h == 1 && c.ends()) ummaCommit(&s->oFull[x]);
+                    if (c.endsTile()) ummaCommit(&s->vEmpty[st]);
                 }
                 __syncwarp();
-                ++steps;
-                // the group's next S product, behind the product that read the weights it overwrites
-                if (n.valid && n.g <= c.g + 2) issueQK(x, n, spans, true);
             }
+            if (!ok) break;
             const int k = c.k;
-            nextTile(c);
-            if (c.k != k) spanDone(k);       // (the cursors ahead are in later spans by now)
+            ++cs;
+            advance(c);
+            if (c.k != k) spanDone(k);       // (n is in a later span by now)
         }
     } else if (warp == kPlanWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -410,14 +458,45 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         const uint32_t laneBase = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const bool first = threadIdx.x == kOutputWarp0 * 32;
         int cnt0 = 0, cnt1 = 0;              // spans of a group written: phase of oFull
+        // row t (and, of a dual span, 128 + t) of a span's queries into the query tiles, zeros where
+        // the request has no such row
+        auto fetchQ = [&](const Span& g) {
+#pragma unroll
+            for (int i = 0; i < S::kQTiles; ++i) {
+                if (i > 0 && !g.dual) break;
+                const int rr = g.rp * kPairRows + i * kRows + t;
+                const bool there = rr < g.rows;
+                const T* src = static_cast<const T*>(p.q) + (there ? static_cast<int64_t>(g.s.start + rr / group) * p.qStride +
+                                                                         static_cast<int64_t>(g.kvh * group + rr % group) * kHd : 0);
+                const uint32_t dst = smemAddr(s->q[i]) + t * 128;
+                const int n = there ? 16 : 0;
+#pragma unroll
+                for (int c = 0; c < 16; ++c)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (c >> 3) * kHalfBytes + (((c & 7) ^ (t & 7)) << 4)), "l"(src + c * 8), "r"(n) : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbarArrive(&s->qFull);
+        };
         bool ok = true;
+        {
+            const Span* at = spanAt(0);
+            if (at && at->valid) fetchQ(*at);
+        }
         for (int k = 0; ok; ++k) {
             const Span* at = spanAt(k);
             ok = !anyOfOutput(at == nullptr);          // (all four warps decide together, so that none waits for one that gave up)
             if (!ok || !at->valid) break;
             const Span& g = *at;
+            const Span* next = spanAt(k + 1);
+            if (next && next->valid) {
+                // the last S product of this span is complete: its queries are no longer read
+                ok = mbarWait(&s->qEmpty, k & 1, &s->dead, errFlag, waitLimit, 48);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (ok) fetchQ(*next);
+            }
             const bool has1 = g.tilesOf(1) > 0;
-            ok = mbarWait(&s->oFull[0], cnt0 & 1, &s->dead, errFlag, waitLimit, 49);
+            if (ok) ok = mbarWait(&s->oFull[0], cnt0 & 1, &s->dead, errFlag, waitLimit, 49);
             if (ok && has1) ok = mbarWait(&s->oFull[1], cnt1 & 1, &s->dead, errFlag, waitLimit, 51);
             ok = !anyOfOutput(!ok);
             if (!ok) break;
@@ -451,54 +530,44 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 a0 *= inv;
                 a1 *= inv;
-                {
-                    // the row's address, and those of the three rows whose pieces this lane stores as well
-                    int64_t at64 = mine ? (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd : -1;
-                    float4* recO = reinterpret_cast<float4*>(rec) + rl;
+                const int64_t at64 = mine ? (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd : -1;
+                float4* recO = reinterpret_cast<float4*>(rec) + rl;
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {           // 32 columns at a time
-                        uint32_t o[32];
-                        tmemLd32(tmemO(x) + laneBase + 32u * c, o);
+                for (int c = 0; c < 8; ++c) {               // 16 columns at a time
+                    uint32_t o[16], u[16];
+                    tmemLd16NoWait(tmemO(x) + laneBase + 16u * c, o);
+                    if (!g.dual && has1) tmemLd16NoWait(tmemO(1) + laneBase + 16u * c, u);
+                    tmemLdWait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a0);
-                        if (!g.dual && has1) {
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a0);
+                    if (!g.dual && has1)
 #pragma unroll
-                            for (int h = 0; h < 4; ++h) {
-                                uint32_t u[8];
-                                tmemLd8(tmemO(1) + laneBase + 32u * c + 8u * h, u);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(u[i]), a1, __uint_as_float(o[i])));
+                    if (!whole) {
+                        // records are [32 pieces of 4 columns][256 rows]: consecutive lanes, consecutive 16 bytes
+                        if (mine)
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) o[8 * h + i] = __float_as_uint(fmaf(__uint_as_float(u[i]), a1, __uint_as_float(o[8 * h + i])));
-                            }
-                        }
-                        if (!whole) {
-                            // records are [32 pieces of 4 columns][256 rows]: consecutive lanes, consecutive 16 bytes
-                            if (mine)
+                            for (int q = 0; q < 4; ++q)
+                                recO[(4 * c + q) * kPairRows] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
+                    } else {
+                        // Two lanes trade a piece of their rows, so that a store covers 32 consecutive
+                        // bytes (a whole sector) of 16 rows: first the even lane's row, then the odd's.
+                        uint32_t w[8];
 #pragma unroll
-                                for (int q = 0; q < 8; ++q)
-                                    recO[(8 * c + q) * kPairRows] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
-                        } else {
-                            // Four lanes trade their rows' four 16-byte pieces so that each store covers
-                            // 64 consecutive bytes of eight rows instead of 16 bytes of 32.
-                            uint32_t w[16];
+                        for (int i = 0; i < 8; ++i) w[i] = pack16<BF16>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+                        const int me = lane & 1;
+                        const int64_t to = __shfl_xor_sync(0xFFFFFFFFu, at64, 1);
+                        uint32_t v[4];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) w[i] = pack16<BF16>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
-                            const int me = lane & 3;
-#pragma unroll
-                            for (int d = 0; d < 4; ++d) {
-                                // step d: lane `me` sends piece (me ^ d) to lane me ^ d, which stores it as its own number
-                                const int dest = me ^ d;
-                                uint32_t v[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const uint32_t lo = dest & 1 ? w[4 + e] : w[e], hi2 = dest & 1 ? w[12 + e] : w[8 + e];
-                                    v[e] = __shfl_xor_sync(0xFFFFFFFFu, dest & 2 ? hi2 : lo, d);
-                                }
-                                const int64_t to = __shfl_xor_sync(0xFFFFFFFFu, at64, d);
-                                if (to >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to + 32 * c + 8 * me) = make_uint4(v[0], v[1], v[2], v[3]);
-                            }
-                        }
-                        __syncwarp();
+                        for (int e = 0; e < 4; ++e) v[e] = __shfl_xor_sync(0xFFFFFFFFu, me ? w[e] : w[4 + e], 1);
+                        const uint4 own = me ? make_uint4(w[4], w[5], w[6], w[7]) : make_uint4(w[0], w[1], w[2], w[3]);
+                        const uint4 got = make_uint4(v[0], v[1], v[2], v[3]);
+                        T* base = static_cast<T*>(p.out) + 16 * c + 8 * me;
+                        const int64_t even = me ? to : at64, oddRow = me ? at64 : to;
+                        if (even >= 0) *reinterpret_cast<uint4*>(base + even) = me ? got : own;
+                        if (oddRow >= 0) *reinterpret_cast<uint4*>(base + oddRow) = me ? own : got;
                     }
+                    __syncwarp();
                 }
                 if (whole && odd && mine)
                     addLeftOut<T, T>(p, g.s, g.b, g.kvh, rr / group, g.hi, static_cast<T*>(p.out) + (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd, 0, kHd);
@@ -527,23 +596,6 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         const uint32_t sAddr = tmemS(x) + laneBase, oAddr = tmemO(x) + laneBase;
         bool ok = true;
         int steps = 0, spans = 0;            // tiles this group has done (phase of sFull), spans
-        // this thread's query row of a span into the group's tile
-        auto fetchQ = [&](const Span& q) {
-            const int rr = q.firstRow(x) + t;
-            const bool there = rr < q.rows;
-            const T* src = static_cast<const T*>(p.q) + (there ? static_cast<int64_t>(q.s.start + rr / group) * p.qStride +
-                                                                     static_cast<int64_t>(q.kvh * group + rr % group) * kHd : 0);
-            const uint32_t dst = smemAddr(s->q[x]) + t * 128;
-            const int n = there ? 16 : 0;
-#pragma unroll
-            for (int c = 0; c < 16; ++c)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (c >> 3) * kHalfBytes + (((c & 7) ^ (t & 7)) << 4)), "l"(src + c * 8), "r"(n) : "memory");
-        };
-        auto postQ = [&]() {
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbarArrive(&s->qFull[x]);
-        };
         // the number of the next span at or after k with tiles of this group, or -1; spans without are
         // given back
         auto seek = [&](int k) {
@@ -556,13 +608,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
             }
         };
         int k = seek(0);
-        if (k >= 0) {
-            fetchQ(s->span[k % kSpans]);
-            postQ();
-        }
         while (k >= 0 && ok) {
             const Span& g = s->span[k % kSpans];
-            int next = -2;                   // looked up at the span's last tile
             {
                 const int rr = g.firstRow(x) + t, node = rr < g.rows ? rr / group : 0;
                 s->rowNode[x][t] = node;
@@ -578,14 +625,24 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 const uint32_t keyEnd = inTree ? static_cast<uint32_t>(g.s.n) : g.s.held;
                 const bool edge = inTree || k0 < g.hi || k0 < g.s.lo || k0 + kKeys > keyEnd;
                 const bool lastTile = j + g.step() >= g.last;
-                if (inTree)                               // (loads that the wait below hides)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s->rowBits[x][i][t] = treeBits(p, g.s, s->rowNode[x][t], static_cast<int>(k0 / 32) + i);
-                if (lastTile) next = seek(k + 1);
-                if (ok) ok = mbarWait(&s->sFull[x], steps & 1, &s->dead, errFlag, waitLimit, 52);
+                if (edge) {
+                    // the keys of the tile that the row sees, as bits (loads that the wait below hides)
+                    const uint32_t first = s->rowFrom[x][t];
+                    const int from = first > k0 ? static_cast<int>(min(first - k0, 128u)) : 0, to = static_cast<int>(min(keyEnd - k0, 128u));
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t bits;
+                        if (inTree) bits = treeBits(p, g.s, s->rowNode[x][t], static_cast<int>(k0 / 32) + i);
+                        else {
+                            const int a = min(max(from - 32 * i, 0), 32), b = min(max(to - 32 * i, 0), 32);
+                            bits = (b < 32 ? (1u << b) - 1u : 0xFFFFFFFFu) & (a < 32 ? 0xFFFFFFFFu << a : 0u);
+                        }
+                        s->rowBits[x][i][t] = bits;
+                    }
+                }
+                ok = mbarWait(&s->sFull[x], steps & 1, &s->dead, errFlag, waitLimit, 52);
                 if (!ok) break;
                 tcFenceAfter();
-                if (next >= 0) fetchQ(s->span[next % kSpans]);     // S of the span's last tile is there: the query tile is no longer read
                 uint32_t r0[32], r1[32], r2[32], r3[32];
                 tmemLd32NoWait(sAddr, r0);
                 tmemLd32NoWait(sAddr + 32u, r1);
@@ -593,19 +650,10 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 tmemLd32NoWait(sAddr + 96u, r3);
                 tmemLdWait();
                 if (edge) {
-                    if (inTree) {
-                        maskBits(r0, s->rowBits[x][0][t]);
-                        maskBits(r1, s->rowBits[x][1][t]);
-                        maskBits(r2, s->rowBits[x][2][t]);
-                        maskBits(r3, s->rowBits[x][3][t]);
-                    } else {
-                        const uint32_t from = s->rowFrom[x][t];
-                        const int a = from > k0 ? static_cast<int>(min(from - k0, 128u)) : 0, b = static_cast<int>(min(g.s.held - k0, 128u));
-                        maskRange(r0, a, b);
-                        maskRange(r1, a - 32, b - 32);
-                        maskRange(r2, a - 64, b - 64);
-                        maskRange(r3, a - 96, b - 96);
-                    }
+                    maskBits(r0, s->rowBits[x][0][t]);
+                    maskBits(r1, s->rowBits[x][1][t]);
+                    maskBits(r2, s->rowBits[x][2][t]);
+                    maskBits(r3, s->rowBits[x][3][t]);
                 }
                 const float tmax = fmaxf(fmaxf(quarterRowMax(r0), quarterRowMax(r1)), fmaxf(quarterRowMax(r2), quarterRowMax(r3))) * scaleLog2;
                 bool raise = false;
@@ -657,8 +705,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                     // Row t of V: zeros where there is no such key, finite values where some row may not
                     // see it.  (Both groups of a dual span may write the same.  The phase asked for is not two
                     // ahead: this S product was issued after the wait for V of the tile two before.)
-                    const int tile = g.tile + j - g.first, st = tile % kStages;
-                    ok = mbarWait(&s->vFull[st], (tile / kStages) & 1, &s->dead, errFlag, waitLimit, 53);
+                    const int half = 2 * (g.tile + j - g.first) + (t >> 6), st = half % S::kVStages;
+                    ok = mbarWait(&s->vFull[st], (half / S::kVStages) & 1, &s->dead, errFlag, waitLimit, 53);
                     if (!ok) break;
                     const uint32_t key = k0 + static_cast<uint32_t>(t);
                     const bool there = key < keyEnd && (inTree || key >= g.s.lo);
@@ -667,7 +715,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
 #pragma unroll 1
                         for (int c = 0; c < 16; ++c) {
                             // (lane by lane another piece of the row first: no two on one bank)
-                            uint4* at = reinterpret_cast<uint4*>(s->v[st] + (c >> 3) * kHalfBytes + t * 128 + (((c ^ t) & 7) << 4));
+                            uint4* at = reinterpret_cast<uint4*>(s->v[st] + (c >> 3) * kVBlockBytes + (t & 63) * 128 + (((c ^ t) & 7) << 4));
                             if (!there) {
                                 *at = make_uint4(0u, 0u, 0u, 0u);
                                 continue;
@@ -697,9 +745,9 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
             }
             if (!ok) break;
             ++spans;
-            if (next >= 0) postQ();
-            spanDone(k);
-            k = next;
+            const int before = k;
+            k = seek(k + 1);
+            spanDone(before);
         }
     }
 
@@ -748,24 +796,25 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
         if (encode(&pool[which], dt, 2, const_cast<void*>(which ? p.vPool : p.kPool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
-        // the step's rows: [row][kv_head][128]; a box is 64 dims x 1 head x 128 rows (rows behind the last: zeros)
+        // the step's rows: [row][kv_head][128]; a box is 64 dims x 1 head x 64 rows (rows behind the last: zeros)
         const cuuint64_t fdims[3] = {kHd, static_cast<cuuint64_t>(p.kvHeads), static_cast<cuuint64_t>(p.numRows)};
         const cuuint64_t fstrides[2] = {kHd * 2, static_cast<cuuint64_t>(which ? p.vStride : p.kStride) * 2};
-        const cuuint32_t fbox[3] = {64, 1, kKeys}, fone[3] = {1, 1, 1};
+        const cuuint32_t fbox[3] = {64, 1, 64}, fone[3] = {1, 1, 1};
         if (encode(&fresh[which], dt, 3, const_cast<void*>(which ? p.vNew : p.kNew), fdims, fstrides, fbox, fone, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
     }
     const float scaleLog2 = 1.4426950408889634f / sqrtf(static_cast<float>(kHd));
-    const size_t smem = smemBytes(p.batch);
-    auto run = [&](auto kernel) -> cudaError_t {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smemBytes(kTreeMaxBatch)));
+    auto run = [&](auto kernel, size_t smem) -> cudaError_t {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
         if (e != cudaSuccess) return e;
         kernel<<<plan.blocks, kThreads, smem, stream>>>(pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag,
-                                                     p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
+                                                         p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
         return cudaGetLastError();
     };
-    return p.dtype == kBF16 ? run(treeTcKernel<true>) : run(treeTcKernel<false>);
+    const bool wide = static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) > kRows || smemBytes<false>(p.batch) > kSmemLimit;
+    if (wide) return p.dtype == kBF16 ? run(treeTcKernel<true, true>, smemBytes<true>(p.batch)) : run(treeTcKernel<false, true>, smemBytes<true>(p.batch));
+    return p.dtype == kBF16 ? run(treeTcKernel<true, false>, smemBytes<false>(p.batch)) : run(treeTcKernel<false, false>, smemBytes<false>(p.batch));
 }
 
 }  // namespace pam

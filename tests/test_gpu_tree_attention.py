@@ -174,6 +174,14 @@ def test_matches_float64(engine, dtype, name):
     TreeCase(31, dtype=dtype, **SHAPES[name]).check(engine)
 
 
+@pytest.mark.parametrize("dtype", [DT.float16, DT.float8, DT.float32], ids=lambda d: d.name)
+def test_very_many_short_requests(engine, dtype):
+    """Hundreds of pairs in every block's piece, most of one key tile, some of none of the cache."""
+    lens = [0 if i % 3 else 5 + i % 40 for i in range(900)]
+    TreeCase(44, lens, [5 + i % 2 for i in range(900)], heads=8, kv_heads=2, dtype=dtype).check(engine)
+    TreeCase(45, [0] * 1500, [17] + [0, 1] * 749 + [3], heads=8, kv_heads=2, dtype=dtype).check(engine)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=lambda d: d.name)
 @pytest.mark.parametrize("window", [1, 5, 64, 200])
 @pytest.mark.parametrize("masks", [True, False])
