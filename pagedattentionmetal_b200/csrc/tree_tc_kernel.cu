@@ -320,61 +320,53 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         int nPrev = -1;                      // group of the step before n
         uint32_t pParity = 0, oParity = 0, begun = 0;      // bit x: phase of pFull, of oEmpty; group x has begun a span
         while (c.valid && ok) {
-            // ---- S products, while the weights of step c are waited for
-            bool got = false;                // ... they are there
+            // ---- S products; while one is held up by its keys or queries, the weights of step c may come
+            // first (test_wait: try_wait would sleep through the other condition)
+            bool got = false;                // the weights of step c are there
             long long since = 0;
             while (ok && !got) {
-                if (n.valid && ns <= cs + 1 && !(ns > cs && n.x == nPrev)) {      // (the group's step before is n - 1, or through)
-                    const int st = n.g % S::kKStages;
-                    const uint32_t kPar = (n.g / S::kKStages) & 1, qPar = n.k & 1;
-                    bool there = true;
-                    if (ns > cs) {
-                        // ahead of need: only if everything is there
-                        there = mbarTest(&s->kFull[st], kPar) && (!n.opensSpan() || mbarTest(&s->qFull, qPar));
-                        there = __all_sync(0xFFFFFFFFu, there);
-                    } else {
-                        if (n.opensSpan()) ok = mbarWait(&s->qFull, qPar, &s->dead, errFlag, waitLimit, 43);
-                        if (ok) ok = mbarWait(&s->kFull[st], kPar, &s->dead, errFlag, waitLimit, 44);
-                        ok = __all_sync(0xFFFFFFFFu, ok);
-                        if (!ok) break;
-                    }
-                    if (there) {
-                        tcFenceAfter();
-                        const uint32_t qLo = descLo(smemAddr(s->q[0]) + (WIDE && n.dual ? n.x * kTileBytes : 0), 16);
-                        const uint32_t kLo = descLo(smemAddr(s->k[0]) + st * kTileBytes, 16), dS = tmemS(n.x);
-                        uint64_t dq[kHd / 16], dk[kHd / 16];
-#pragma unroll
-                        for (int ks = 0; ks < kHd / 16; ++ks) {
-                            const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
-                            dq[ks] = desc64(qLo + off, hiK);
-                            dk[ks] = desc64(kLo + off, hiK);
-                        }
-                        if (leader) {
-#pragma unroll
-                            for (int ks = 0; ks < kHd / 16; ++ks) umma(dS, dq[ks], dk[ks], idescS, ks > 0);
-                            ummaCommit(&s->sFull[n.x]);
-                            if (n.endsTile()) ummaCommit(&s->kEmpty[st]);
-                            if (n.closesSpan()) ummaCommit(&s->qEmpty);
-                        }
-                        __syncwarp();
-                        nPrev = n.x;
-                        ++ns;
-                        advance(n);
-                        continue;
-                    }
-                }
-                // (a fifth of a microsecond at most, then the other condition again)
-                got = __all_sync(0xFFFFFFFFu, mbarTrySleep(&s->pFull[c.x], pParity >> c.x & 1, 200u));
-                if (!got) {
+                // (the group's step before is n - 1 at the earliest; it is through if that is another group's)
+                if (!n.valid || ns > cs + 1 || (ns > cs && n.x == nPrev)) break;
+                const int st = n.g % S::kKStages;
+                const uint32_t kPar = (n.g / S::kKStages) & 1, qPar = n.k & 1;
+                bool there = mbarTest(&s->kFull[st], kPar) && (!n.opensSpan() || mbarTest(&s->qFull, qPar));
+                there = __all_sync(0xFFFFFFFFu, there);
+                if (!there) {
+                    if (ns > cs) got = __all_sync(0xFFFFFFFFu, mbarTest(&s->pFull[c.x], pParity >> c.x & 1));
                     if (since == 0) since = clock64();
                     else if (clock64() - since > waitLimit) {
                         *reinterpret_cast<volatile int*>(&s->dead) = 1;
-                        atomicCAS(errFlag, 0, 45);
+                        atomicCAS(errFlag, 0, 44);
                     }
                     if (*reinterpret_cast<volatile int*>(&s->dead)) ok = false;
                     ok = __all_sync(0xFFFFFFFFu, ok);
+                    continue;
                 }
+                since = 0;
+                tcFenceAfter();
+                const uint32_t qLo = descLo(smemAddr(s->q[0]) + (WIDE && n.dual ? n.x * kTileBytes : 0), 16);
+                const uint32_t kLo = descLo(smemAddr(s->k[0]) + st * kTileBytes, 16), dS = tmemS(n.x);
+                uint64_t dq[kHd / 16], dk[kHd / 16];
+#pragma unroll
+                for (int ks = 0; ks < kHd / 16; ++ks) {
+                    const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                    dq[ks] = desc64(qLo + off, hiK);
+                    dk[ks] = desc64(kLo + off, hiK);
+                }
+                if (leader) {
+#pragma unroll
+                    for (int ks = 0; ks < kHd / 16; ++ks) umma(dS, dq[ks], dk[ks], idescS, ks > 0);
+                    ummaCommit(&s->sFull[n.x]);
+                    if (n.endsTile()) ummaCommit(&s->kEmpty[st]);
+                    if (n.closesSpan()) ummaCommit(&s->qEmpty);
+                }
+                __syncwarp();
+                nPrev = n.x;
+                ++ns;
+                advance(n);
             }
+            if (ok && !got) ok = mbarWait(&s->pFull[c.x], pParity >> c.x & 1, &s->dead, errFlag, waitLimit, 45);
+            ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             // ---- the P V product of step c
             const int x = c.x;
@@ -458,21 +450,24 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         const uint32_t laneBase = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const bool first = threadIdx.x == kOutputWarp0 * 32;
         int cnt0 = 0, cnt1 = 0;              // spans of a group written: phase of oFull
-        // row t (and, of a dual span, 128 + t) of a span's queries into the query tiles, zeros where
-        // the request has no such row
+        // a span's queries into the query tile (a dual span's: tiles), zeros where the request has no
+        // such row
         auto fetchQ = [&](const Span& g) {
 #pragma unroll
             for (int i = 0; i < S::kQTiles; ++i) {
                 if (i > 0 && !g.dual) break;
+                // every lane looks its row up; half a warp then copies a row, 16 bytes a lane
                 const int rr = g.rp * kPairRows + i * kRows + t;
-                const bool there = rr < g.rows;
-                const T* src = static_cast<const T*>(p.q) + (there ? static_cast<int64_t>(g.s.start + rr / group) * p.qStride +
-                                                                         static_cast<int64_t>(g.kvh * group + rr % group) * kHd : 0);
-                const uint32_t dst = smemAddr(s->q[i]) + t * 128;
-                const int n = there ? 16 : 0;
-#pragma unroll
-                for (int c = 0; c < 16; ++c)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (c >> 3) * kHalfBytes + (((c & 7) ^ (t & 7)) << 4)), "l"(src + c * 8), "r"(n) : "memory");
+                const int64_t off = rr < g.rows ? static_cast<int64_t>(g.s.start + rr / group) * p.qStride + static_cast<int64_t>(g.kvh * group + rr % group) * kHd : -1;
+                const int c = lane & 15;
+#pragma unroll 4
+                for (int r = 0; r < 16; ++r) {
+                    const int in = 2 * r + (lane >> 4), row = (warp & 3) * 32 + in;
+                    const int64_t at = __shfl_sync(0xFFFFFFFFu, off, in);
+                    const uint32_t dst = smemAddr(s->q[i]) + row * 128 + (c >> 3) * kHalfBytes + (((c & 7) ^ (row & 7)) << 4);
+                    const int n = at >= 0 ? 16 : 0;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(static_cast<const T*>(p.q) + (at >= 0 ? at + c * 8 : 0)), "r"(n) : "memory");
+                }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -702,8 +697,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 }
                 tmemStWait();
                 if (edge) {
-                    // Row t of V: zeros where there is no such key, finite values where some row may not
-                    // see it.  (Both groups of a dual span may write the same.  The phase asked for is not two
+                    // Row t of V: finite values where there is no such key, or some row may not see it.  (Both groups of a dual span may write the same.  The phase asked for is not two
                     // ahead: this S product was issued after the wait for V of the tile two before.)
                     const int half = 2 * (g.tile + j - g.first) + (t >> 6), st = half % S::kVStages;
                     ok = mbarWait(&s->vFull[st], (half / S::kVStages) & 1, &s->dead, errFlag, waitLimit, 53);
@@ -711,26 +705,23 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                     const uint32_t key = k0 + static_cast<uint32_t>(t);
                     const bool there = key < keyEnd && (inTree || key >= g.s.lo);
                     if (!there || inTree || key < g.hi) {
-                        constexpr uint32_t kExp = BF16 ? 0x7F80u : 0x7C00u;
-#pragma unroll 1
+                        // A weight of zero removes what a row does not see, unless it is infinite or NaN: an
+                        // exponent of ones, which carries out of its field when one is added at its end.
+                        constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
+                        uint32_t carry = 0;
+#pragma unroll 4
                         for (int c = 0; c < 16; ++c) {
                             // (lane by lane another piece of the row first: no two on one bank)
-                            uint4* at = reinterpret_cast<uint4*>(s->v[st] + (c >> 3) * kVBlockBytes + (t & 63) * 128 + (((c ^ t) & 7) << 4));
-                            if (!there) {
-                                *at = make_uint4(0u, 0u, 0u, 0u);
-                                continue;
+                            const uint4 w = *reinterpret_cast<const uint4*>(s->v[st] + (c >> 3) * kVBlockBytes + (t & 63) * 128 + (((c ^ t) & 7) << 4));
+                            carry |= ((w.x & kExp) + kOne) | ((w.y & kExp) + kOne) | ((w.z & kExp) + kOne) | ((w.w & kExp) + kOne);
+                        }
+                        if (carry & 0x80008000u) {
+#pragma unroll 1
+                            for (int c = 0; c < 128; ++c) {
+                                unsigned short* at = reinterpret_cast<unsigned short*>(s->v[st] + (c >> 6) * kVBlockBytes + (t & 63) * 128 + (c & 63) * 2);
+                                if ((*at & kExp & 0xFFFFu) == (kExp & 0xFFFFu)) *at = 0;
                             }
-                            uint4 w = *at;
-                            uint32_t changed = 0;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                uint32_t& u = e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w;
-                                const uint32_t was = u;
-                                if ((u & kExp) == kExp) u &= 0xFFFF0000u;
-                                if ((u >> 16 & kExp) == kExp) u &= 0x0000FFFFu;
-                                changed |= was ^ u;
-                            }
-                            if (changed) { *at = w; odd = 1; }
+                            if (there) odd = 1;
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
