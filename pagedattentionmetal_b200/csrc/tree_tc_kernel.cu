@@ -168,7 +168,7 @@ __device__ __forceinline__ bool anyOfOutput(bool v) {
 
 template <bool BF16, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1)
-treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
              const __grid_constant__ CUtensorMap mapKNew, const __grid_constant__ CUtensorMap mapVNew,
              const __grid_constant__ TreeParams p, float scaleLog2, int* errFlag, long long waitLimit) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
@@ -181,7 +181,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.heads / p.kvHeads;
     if (threadIdx.x == 0) {
-        mbarInit(&s->qFull, kRows);
+        mbarInit(&s->qFull, kRows % group == 0 ? 1 : kRows);
         mbarInit(&s->qEmpty, 1);
         for (int i = 0; i < 2; ++i) {
             mbarInit(&s->sFull[i], 1);
@@ -453,7 +453,19 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
         // a span's queries into the query tile (a dual span's: tiles), zeros where the request has no
         // such row
         auto fetchQ = [&](const Span& g) {
-#pragma unroll
+            if (kRows % group == 0) {
+                // a tile of whole nodes: one box of (64 dims, the KV head's query heads, 128 / group nodes)
+                // for each half (rows behind the request's belong to others and are not used)
+                if (first) {
+                    const int node = g.rp * (kPairRows / group), tiles = WIDE && g.dual ? 2 : 1;
+                    mbarExpectTx(&s->qFull, tiles * kTileBytes);
+                    for (int i = 0; i < 2 * tiles; ++i)
+                        tmaLoad3d(s->q[i >> 1] + (i & 1) * kHalfBytes, &mapQ, &s->qFull, 64 * (i & 1), g.kvh * group,
+                                  g.s.start + node + (i >> 1) * (kRows / group));
+                }
+                return;
+            }
+#pragma unroll 1
             for (int i = 0; i < S::kQTiles; ++i) {
                 if (i > 0 && !g.dual) break;
                 // every lane looks its row up; half a warp then copies a row, 16 bytes a lane
@@ -525,47 +537,49 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ C
                 const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 a0 *= inv;
                 a1 *= inv;
-                const int64_t at64 = mine ? (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd : -1;
+                T* out = static_cast<T*>(p.out) + (mine ? (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd : 0);
                 float4* recO = reinterpret_cast<float4*>(rec) + rl;
+                const bool both = !g.dual && has1;
+                const unsigned long long scale0 = pack2(a0, a0), scale1 = pack2(a1, a1);
+                // 16 columns at a time.  (What counts here are instructions: one warp on each scheduler,
+                // whose fetches compete with the softmax warps' long loop.  Trading pieces among lanes for
+                // wider segments of a row made the loop longer and 1.5 times slower.)
 #pragma unroll 1
-                for (int c = 0; c < 8; ++c) {               // 16 columns at a time
+                for (int c = 0; c < 8; ++c) {
                     uint32_t o[16], u[16];
                     tmemLd16NoWait(tmemO(x) + laneBase + 16u * c, o);
-                    if (!g.dual && has1) tmemLd16NoWait(tmemO(1) + laneBase + 16u * c, u);
+                    if (both) tmemLd16NoWait(tmemO(1) + laneBase + 16u * c, u);
                     tmemLdWait();
+                    unsigned long long f[8];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a0);
-                    if (!g.dual && has1)
+                    for (int i = 0; i < 8; ++i) f[i] = mul2(pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), scale0);
+                    if (both)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(u[i]), a1, __uint_as_float(o[i])));
-                    if (!whole) {
-                        // records are [32 pieces of 4 columns][256 rows]: consecutive lanes, consecutive 16 bytes
-                        if (mine)
+                        for (int i = 0; i < 8; ++i) f[i] = fma2(pack2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), scale1, f[i]);
+                    if (mine) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float lo, hi;
+                            unpack2(f[i], lo, hi);
+                            o[2 * i] = __float_as_uint(lo);
+                            o[2 * i + 1] = __float_as_uint(hi);
+                        }
+                        if (whole) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) o[i] = pack16<BF16>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+                            *reinterpret_cast<uint4*>(out + 16 * c) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(out + 16 * c + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+                        } else {
+                            // records are [32 pieces of 4 columns][256 rows]: consecutive lanes, consecutive 16 bytes
 #pragma unroll
                             for (int q = 0; q < 4; ++q)
                                 recO[(4 * c + q) * kPairRows] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
-                    } else {
-                        // Two lanes trade a piece of their rows, so that a store covers 32 consecutive
-                        // bytes (a whole sector) of 16 rows: first the even lane's row, then the odd's.
-                        uint32_t w[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i] = pack16<BF16>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
-                        const int me = lane & 1;
-                        const int64_t to = __shfl_xor_sync(0xFFFFFFFFu, at64, 1);
-                        uint32_t v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = __shfl_xor_sync(0xFFFFFFFFu, me ? w[e] : w[4 + e], 1);
-                        const uint4 own = me ? make_uint4(w[4], w[5], w[6], w[7]) : make_uint4(w[0], w[1], w[2], w[3]);
-                        const uint4 got = make_uint4(v[0], v[1], v[2], v[3]);
-                        T* base = static_cast<T*>(p.out) + 16 * c + 8 * me;
-                        const int64_t even = me ? to : at64, oddRow = me ? at64 : to;
-                        if (even >= 0) *reinterpret_cast<uint4*>(base + even) = me ? got : own;
-                        if (oddRow >= 0) *reinterpret_cast<uint4*>(base + oddRow) = me ? own : got;
+                        }
                     }
                     __syncwarp();
                 }
                 if (whole && odd && mine)
-                    addLeftOut<T, T>(p, g.s, g.b, g.kvh, rr / group, g.hi, static_cast<T*>(p.out) + (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd, 0, kHd);
+                    addLeftOut<T, T>(p, g.s, g.b, g.kvh, rr / group, g.hi, out, 0, kHd);
                 __syncwarp();
                 if (!whole && mine) {
                     rec[kPairRows * kHd + rl] = m;
@@ -778,7 +792,18 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
     EncodeFn encode = encodeFn();
     if (!encode) return cudaErrorNotSupported;
     const CUtensorMapDataType dt = p.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    CUtensorMap pool[2], fresh[2];
+    CUtensorMap queries, pool[2], fresh[2];
+    {
+        // queries: [row][head][128]; a box is 64 dims x the heads of a KV head x 128 rows' worth of nodes
+        // (used when the group divides 128; else any valid box)
+        const int group = p.heads / p.kvHeads, nodes = kRows % group == 0 ? kRows / group : 1, heads = kRows % group == 0 ? group : 1;
+        const cuuint64_t dims[3] = {kHd, static_cast<cuuint64_t>(p.heads), static_cast<cuuint64_t>(p.numRows)};
+        const cuuint64_t strides[2] = {kHd * 2, static_cast<cuuint64_t>(p.qStride) * 2};
+        const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(heads), static_cast<cuuint32_t>(nodes)}, one[3] = {1, 1, 1};
+        if (encode(&queries, dt, 3, const_cast<void*>(p.q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    }
     for (int which = 0; which < 2; ++which) {
         // pools: [block * kv_head * slot][128]; a box is 64 dims x 16 rows (half of a 16-token piece)
         const cuuint64_t dims[2] = {kHd, static_cast<cuuint64_t>(p.poolBlocks) * p.kvHeads * p.blockSize};
@@ -799,7 +824,7 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
     auto run = [&](auto kernel, size_t smem) -> cudaError_t {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
         if (e != cudaSuccess) return e;
-        kernel<<<plan.blocks, kThreads, smem, stream>>>(pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag,
+        kernel<<<plan.blocks, kThreads, smem, stream>>>(queries, pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag,
                                                          p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
         return cudaGetLastError();
     };
