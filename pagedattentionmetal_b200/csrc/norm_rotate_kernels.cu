@@ -19,11 +19,27 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
+#include "tc_common.cuh"
 
 namespace pam {
 namespace {
+
+// Two float32 in one register pair: the passes are close to the issue rate, and a packed product or
+// sum is one instruction.
+using F2 = unsigned long long;
+using tc::add2;
+using tc::fma2;
+using tc::mul2;
+using tc::pack2;
+using tc::unpack2;
+__device__ __forceinline__ float sumOf(F2 v) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    return lo + hi;
+}
 
 __device__ __forceinline__ float toFloat(float v) { return v; }
 __device__ __forceinline__ float toFloat(__half v) { return __half2float(v); }
@@ -42,22 +58,51 @@ __device__ __forceinline__ float2 turnOf(int position, float freq) {
     return cs;
 }
 
-// E elements of 16 bytes: 8 of a 16-bit type, 4 of float32.
-template <typename T>
+// BYTES (8 or 16) of a row: E elements.
+template <typename T, int BYTES>
 struct Piece {
-    static constexpr int E = 16 / sizeof(T);
-    uint4 raw;
-    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = raw; }
-    __device__ __forceinline__ void unpack(float (&f)[E]) const {
-        const T* t = reinterpret_cast<const T*>(&raw);
+    static constexpr int E = BYTES / sizeof(T);
+    using Vec = std::conditional_t<BYTES == 16, uint4, uint2>;
+    union {
+        Vec raw;
+        uint32_t word[BYTES / 4];
+    };
+    __device__ __forceinline__ Piece() {
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = toFloat(t[e]);
+        for (int i = 0; i < BYTES / 4; ++i) word[i] = 0u;
     }
-    __device__ __forceinline__ void pack(const float (&f)[E]) {
-        T* t = reinterpret_cast<T*>(&raw);
+    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const Vec*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Vec*>(p) = raw; }
+    // The compiler may not keep what was unpacked before: unpacking again costs less than the registers
+    // that hold it (more rows in flight).
+    __device__ __forceinline__ void forget() {
 #pragma unroll
-        for (int e = 0; e < E; ++e) t[e] = fromFloat<T>(f[e]);
+        for (int i = 0; i < BYTES / 4; ++i) asm volatile("" : "+r"(word[i]));
+    }
+    __device__ __forceinline__ void unpack(F2 (&f)[E / 2]) const {
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+            if constexpr (sizeof(T) == 4) f[e] = pack2(__uint_as_float(word[2 * e]), __uint_as_float(word[2 * e + 1]));
+            else if constexpr (std::is_same_v<T, __half>) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&word[e]));
+                f[e] = pack2(v.x, v.y);
+            } else f[e] = pack2(__uint_as_float(word[e] << 16), __uint_as_float(word[e] & 0xFFFF0000u));
+        }
+    }
+    __device__ __forceinline__ void pack(const F2 (&f)[E / 2]) {
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+            float lo, hi;
+            unpack2(f[e], lo, hi);
+            if constexpr (sizeof(T) == 4) { word[2 * e] = __float_as_uint(lo); word[2 * e + 1] = __float_as_uint(hi); }
+            else if constexpr (std::is_same_v<T, __half>) {
+                const __half2 v = __floats2half2_rn(lo, hi);
+                word[e] = *reinterpret_cast<const uint32_t*>(&v);
+            } else {
+                const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+                word[e] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+        }
     }
 };
 
@@ -75,9 +120,8 @@ struct Layout {
     }
 };
 
-template <typename T>
+template <int E>
 Layout layoutOf(int headDim, int rotaryDim, int interleaved) {
-    constexpr int E = Piece<T>::E;
     Layout l{};
     l.pieces = headDim / E;
     l.pairs = interleaved ? (rotaryDim / E + 1) / 2 : rotaryDim / (2 * E);
@@ -87,26 +131,189 @@ Layout layoutOf(int headDim, int rotaryDim, int interleaved) {
     return l;
 }
 
-// Elements [first, first + E) of a piece and their index in the head: the turn of element d.
-// `cs` holds (cos, sin) of the row's rotaryDim / 2 angles.
+// The turn of the pieces' pairs by the angles that `cs` (cosines, and sines `half` behind them) holds
+// from the piece's first one on: sign * angle.
 template <int E>
-__device__ __forceinline__ void rotateHalves(float (&x)[E], float (&y)[E], const float2* cs, float sign) {
+__device__ __forceinline__ void rotateHalves(F2 (&x)[E / 2], F2 (&y)[E / 2], const float* cs, int half, float sign) {
+    const F2 s2 = pack2(sign, sign), minus = pack2(-sign, -sign);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float2 t = cs[e];
-        const float s = sign * t.y, a = x[e], b = y[e];
-        x[e] = a * t.x - b * s;
-        y[e] = b * t.x + a * s;
+    for (int q = 0; q < E / 4; ++q) {
+        const float4 c = *reinterpret_cast<const float4*>(cs + 4 * q), s = *reinterpret_cast<const float4*>(cs + half + 4 * q);
+        const F2 cc[2] = {pack2(c.x, c.y), pack2(c.z, c.w)}, ss[2] = {pack2(s.x, s.y), pack2(s.z, s.w)};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const F2 a = x[2 * q + e], b = y[2 * q + e];
+            x[2 * q + e] = fma2(mul2(b, ss[e]), minus, mul2(a, cc[e]));
+            y[2 * q + e] = fma2(mul2(a, ss[e]), s2, mul2(b, cc[e]));
+        }
     }
 }
 template <int E>
-__device__ __forceinline__ void rotatePairs(float (&x)[E], const float2* cs, float sign) {
+__device__ __forceinline__ void rotatePairs(F2 (&x)[E / 2], const float* cs, int half, float sign) {
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-        const float2 t = cs[e / 2];
-        const float s = sign * t.y, a = x[e], b = x[e + 1];
-        x[e] = a * t.x - b * s;
-        x[e + 1] = b * t.x + a * s;
+    for (int e = 0; e < E / 2; ++e) {
+        const float c = cs[e], s = sign * cs[half + e];
+        float a, b;
+        unpack2(x[e], a, b);
+        x[e] = pack2(a * c - b * s, b * c + a * s);
+    }
+}
+
+// Where a slot's row starts in a pool [block][kvHeads][blockSize][dim], head 0: element offset, or -1
+// outside the pool.  (One division per row of the launch, not per head.)
+__device__ __forceinline__ int64_t poolBase(int64_t slot, int64_t numSlots, int kvHeads, int blockSize, int dim) {
+    if (slot < 0 || slot >= numSlots) return -1;
+    int64_t blk;
+    int off;
+    if ((blockSize & (blockSize - 1)) == 0) {
+        blk = slot >> (__ffs(blockSize) - 1);
+        off = static_cast<int>(slot & (blockSize - 1));
+    } else {
+        blk = slot / blockSize;
+        off = static_cast<int>(slot - blk * blockSize);
+    }
+    return (blk * kvHeads * blockSize + off) * dim;
+}
+
+// What a block looks up of its rows before it works on them.
+struct RowInfo {
+    int64_t pool;      // poolBase of the row's slot
+    int position;      // negative: skipped
+};
+
+// Positions, slots and turns of rows [row0, row0 + n) into shared memory.
+__device__ __forceinline__ void lookRowsUp(RowInfo* info, float* turns, int64_t row0, int n, const int32_t* positions, const int64_t* slots,
+                                           int64_t numSlots, const float* invFreq, int half, int kvHeads, int blockSize, int dim) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        info[i].position = positions[row0 + i];
+        info[i].pool = slots ? poolBase(slots[row0 + i], numSlots, kvHeads, blockSize, dim) : -1;
+    }
+    for (int i = threadIdx.x; i < n * half; i += blockDim.x) {
+        const int r = i / half, pos = positions[row0 + r];
+        if (pos >= 0) {
+            const float2 cs = turnOf(pos, invFreq[i - r * half]);
+            turns[r * half + i] = cs.x;              // a row's cosines, then its sines
+            turns[r * half + i + half] = cs.y;
+        }
+    }
+    __syncthreads();
+}
+
+template <int E>
+__device__ __forceinline__ void turnPieces(F2 (&fa)[E / 2], F2 (&fb)[E / 2], const Layout& l, int lane, int pa, int pb, int rotaryDim,
+                                           const float* cs, float sign) {
+    const int half = rotaryDim / 2;
+    if (l.half) {
+        if (lane < l.pairs) rotateHalves<E>(fa, fb, cs + pa * E, half, sign);
+    } else {
+        if (pa * E < rotaryDim) rotatePairs<E>(fa, cs + pa * E / 2, half, sign);
+        if (pb * E < rotaryDim) rotatePairs<E>(fb, cs + pb * E / 2, half, sign);
+    }
+}
+
+// ---- forward ----------------------------------------------------------------
+
+// A block takes `rowsPer` rows.  A group of l.lanes lanes keeps one head of them (of the queries,
+// keys and values of a row, one after the other), so that its weights stay in registers and nothing
+// is divided inside the loop; the next row's loads are under way while a row is worked on.
+// Measured at 32768 rows of 32 + 8 + 8 heads of 128, float16 (806 MB): 155 us = 5.2 TB/s, 0.79 of the
+// copy rate; one row a block with a division per head 277 us; 8-byte pieces 242 us (twice the
+// instructions per byte); 64 registers 161 us, 48 with spills 181 us.
+template <typename T, int BYTES>
+__global__ void __maxnreg__(56)
+normRotateKernel(const __grid_constant__ NormRotateParams p, const Layout l, int rowsPer) {
+    using P = Piece<T, BYTES>;
+    constexpr int E = P::E;
+    extern __shared__ __align__(16) unsigned char rowSmem[];
+    RowInfo* info = reinterpret_cast<RowInfo*>(rowSmem);                  // [rowsPer]
+    float* turns = reinterpret_cast<float*>(info + rowsPer);              // [rowsPer][rotaryDim]
+    const int tid = threadIdx.x, half = p.rotaryDim / 2;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rowsPer;
+    const int n = static_cast<int>(min(static_cast<int64_t>(rowsPer), p.numRows - row0));
+    lookRowsUp(info, turns, row0, n, p.positions, p.slots, p.numSlots, p.invFreq, half, p.kvHeads, p.blockSize, p.headDim);
+    if (p.slotsOut && blockIdx.y == 0)
+        for (int i = tid; i < n; i += blockDim.x) p.slotsOut[row0 + i] = info[i].position >= 0 ? p.slots[row0 + i] : -1;
+    const int lane = tid & (l.lanes - 1), group = tid / l.lanes, groups = blockDim.x / l.lanes;
+    const int perRow = p.heads + 2 * p.kvHeads;       // queries, keys, values
+    int pa, pb;
+    l.lane(lane, pa, pb);
+    const bool hasA = pa < l.pieces, hasB = pb < l.pieces;
+    const float invDim = 1.f / static_cast<float>(p.headDim);
+    // (whole warps stay in the loops for the shuffles)
+    {
+        const int h = static_cast<int>(blockIdx.y) * groups + group;
+        const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads;
+        const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
+        const bool wanted = h < perRow && !(isV && !p.vPool && !p.vOut);
+        const T* src = isQ ? static_cast<const T*>(p.q) + static_cast<int64_t>(h) * p.headDim
+                     : isV ? static_cast<const T*>(p.v) + static_cast<int64_t>(kvh) * p.headDim
+                           : static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * p.headDim;
+        const int64_t stride = isQ ? p.qStride : isV ? p.vStride : p.kStride;
+        T* rows = static_cast<T*>(isQ ? p.qOut : isV ? p.vOut : p.kOut);
+        const int64_t rowsStride = isQ ? p.qOutStride : isV ? p.vOutStride : p.kOutStride;
+        if (rows) rows += static_cast<int64_t>(isQ ? h : kvh) * p.headDim;
+        T* pool = isQ ? nullptr : static_cast<T*>(isV ? p.vPool : p.kPool);
+        if (pool) pool += static_cast<int64_t>(kvh) * p.blockSize * p.headDim;
+        P wa, wb;
+        if (wanted && !isV && hasA) {
+            const T* weight = static_cast<const T*>(isQ ? p.qWeight : p.kWeight);
+            wa.load(weight + pa * E);
+            if (hasB) wb.load(weight + pb * E);
+        }
+        auto load = [&](int r, P& a, P& b) {
+            a = b = P();
+            if (!wanted || !hasA || r >= n || info[r].position < 0) return;
+            const T* at = src + (row0 + r) * stride;
+            a.load(at + pa * E);
+            if (hasB) b.load(at + pb * E);
+        };
+        P a, b;
+        load(0, a, b);
+        for (int r = 0; r < n; ++r) {
+            P na, nb;
+            load(r + 1, na, nb);
+            F2 sq = 0ull;
+            {
+                F2 fa[E / 2], fb[E / 2];
+                a.unpack(fa);
+                b.unpack(fb);
+#pragma unroll
+                for (int e = 0; e < E / 2; ++e) sq = fma2(fb[e], fb[e], fma2(fa[e], fa[e], sq));
+            }
+            float sum = sumOf(sq);
+            for (int o = l.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            a.forget(); b.forget(); wa.forget(); wb.forget();
+            if (wanted && hasA && info[r].position >= 0) {
+                if (!isV) {
+                    F2 fa[E / 2], fb[E / 2], ga[E / 2], gb[E / 2];
+                    a.unpack(fa);
+                    b.unpack(fb);
+                    wa.unpack(ga);
+                    wb.unpack(gb);
+                    const float root = rsqrtf(sum * invDim + p.eps);
+                    const F2 scale = pack2(root, root);
+#pragma unroll
+                    for (int e = 0; e < E / 2; ++e) {
+                        fa[e] = mul2(mul2(fa[e], scale), ga[e]);
+                        fb[e] = mul2(mul2(fb[e], scale), gb[e]);
+                    }
+                    turnPieces<E>(fa, fb, l, lane, pa, pb, p.rotaryDim, turns + r * 2 * half, 1.f);
+                    a.pack(fa);
+                    b.pack(fb);
+                }
+                const int64_t row = row0 + r, at = info[r].pool;
+                if (rows) {
+                    a.store(rows + row * rowsStride + pa * E);
+                    if (hasB) b.store(rows + row * rowsStride + pb * E);
+                }
+                if (pool && at >= 0) {
+                    a.store(pool + at + pa * E);
+                    if (hasB) b.store(pool + at + pb * E);
+                }
+            }
+            a = na;
+            b = nb;
+        }
     }
 }
 
@@ -116,105 +323,14 @@ __device__ __forceinline__ int64_t poolOffset(int64_t slot, int kvh, int kvHeads
     return ((blk * kvHeads + kvh) * blockSize + off) * static_cast<int64_t>(dim);
 }
 
-// ---- forward ----------------------------------------------------------------
-
-// A block takes `rowsPer` rows: first the turns of the rows' angles into shared memory, then
-// every group of l.lanes lanes takes one (row, head) of queries, keys and values after the other.
-template <typename T>
-__global__ void __launch_bounds__(512)
-normRotateKernel(const NormRotateParams p, const Layout l, int rowsPer) {
-    constexpr int E = Piece<T>::E;
-    extern __shared__ float2 turns[];                 // [rowsPer][rotaryDim / 2]
-    const int tid = threadIdx.x, half = p.rotaryDim / 2;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rowsPer;
-    for (int i = tid; i < rowsPer * half; i += blockDim.x) {
-        const int64_t row = row0 + i / half;
-        const int pos = row < p.numRows ? p.positions[row] : -1;
-        if (pos >= 0) turns[i] = turnOf(pos, p.invFreq[i % half]);
-    }
-    if (p.slotsOut && tid < rowsPer && row0 + tid < p.numRows)
-        p.slotsOut[row0 + tid] = p.positions[row0 + tid] >= 0 ? p.slots[row0 + tid] : -1;
-    __syncthreads();
-    const int lane = tid % l.lanes, group = tid / l.lanes, groups = blockDim.x / l.lanes;
-    const int perRow = p.heads + 2 * p.kvHeads;       // queries, keys, values
-    int pa, pb;
-    l.lane(lane, pa, pb);
-    const bool hasA = pa < l.pieces, hasB = pb < l.pieces;
-    // whole warps stay in the loop for the shuffles
-    const int total = rowsPer * perRow, rounds = (total + groups - 1) / groups;
-    for (int it = 0; it < rounds; ++it) {
-        const int w = it * groups + group;
-        const int64_t row = row0 + w / perRow;
-        const int h = w % perRow;
-        const bool live = w < total && row < p.numRows && p.positions[row] >= 0;
-        const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads;
-        const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
-        const T* src = nullptr;
-        if (live) {
-            if (isQ) src = static_cast<const T*>(p.q) + row * p.qStride + static_cast<int64_t>(h) * p.headDim;
-            else if (!isV) src = static_cast<const T*>(p.k) + row * p.kStride + static_cast<int64_t>(kvh) * p.headDim;
-            else if (p.vPool || p.vOut) src = static_cast<const T*>(p.v) + row * p.vStride + static_cast<int64_t>(kvh) * p.headDim;
-        }
-        Piece<T> a{}, b{};
-        if (src && hasA) a.load(src + pa * E);
-        if (src && hasB) b.load(src + pb * E);
-        float fa[E], fb[E];
-        a.unpack(fa);
-        b.unpack(fb);
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum += fa[e] * fa[e] + fb[e] * fb[e];
-        for (int o = l.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        if (!src || !hasA) continue;                  // (no shuffle below)
-        if (!isV) {
-            const float r = rsqrtf(sum / static_cast<float>(p.headDim) + p.eps);
-            const T* weight = static_cast<const T*>(isQ ? p.qWeight : p.kWeight);
-            Piece<T> wa{}, wb{};
-            wa.load(weight + pa * E);
-            if (hasB) wb.load(weight + pb * E);
-            float ga[E], gb[E];
-            wa.unpack(ga);
-            wb.unpack(gb);
-#pragma unroll
-            for (int e = 0; e < E; ++e) { fa[e] *= r * ga[e]; fb[e] *= r * gb[e]; }
-            const float2* cs = turns + (w / perRow) * half;
-            if (l.half) {
-                if (lane < l.pairs) rotateHalves<E>(fa, fb, cs + pa * E, 1.f);
-            } else {
-                if (pa * E < p.rotaryDim) rotatePairs<E>(fa, cs + pa * E / 2, 1.f);
-                if (pb * E < p.rotaryDim) rotatePairs<E>(fb, cs + pb * E / 2, 1.f);
-            }
-            a.pack(fa);
-            b.pack(fb);
-        }
-        T* dst[2] = {nullptr, nullptr};
-        if (isQ) dst[0] = static_cast<T*>(p.qOut) + row * p.qOutStride + static_cast<int64_t>(h) * p.headDim;
-        else {
-            void* rows = isV ? p.vOut : p.kOut;
-            void* pool = isV ? p.vPool : p.kPool;
-            if (rows) dst[0] = static_cast<T*>(rows) + row * (isV ? p.vOutStride : p.kOutStride) + static_cast<int64_t>(kvh) * p.headDim;
-            if (pool) {
-                const int64_t slot = p.slots[row];
-                if (slot >= 0 && slot < p.numSlots)
-                    dst[1] = static_cast<T*>(pool) + poolOffset(slot, kvh, p.kvHeads, p.blockSize, p.headDim);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (!dst[i]) continue;
-            a.store(dst[i] + pa * E);
-            if (hasB) b.store(dst[i] + pb * E);
-        }
-    }
-}
-
+constexpr int kForwardRows = 16;
 constexpr int kMaxDim = 256;
 
 // Any head_dim, rotaryDim and alignment: one warp per (row, head), element by element, the row
 // in shared memory so that outputs may lie over the inputs.
 template <typename T>
 __global__ void __launch_bounds__(128)
-normRotateAnyKernel(const NormRotateParams p) {
+normRotateAnyKernel(const __grid_constant__ NormRotateParams p) {
     __shared__ float xs[4][kMaxDim];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rotaryDim / 2;
     const int perRow = p.heads + 2 * p.kvHeads;
@@ -276,18 +392,27 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // The 16-byte pieces need every address and stride on 16 bytes, no pair cut by a piece's end,
 // and a head within a warp.
-template <typename T>
+template <int E>
 bool piecesApply(int headDim, int rotaryDim, int interleaved) {
-    constexpr int E = Piece<T>::E;
     if (headDim % E || headDim / E > 64) return false;
     return interleaved ? rotaryDim % E == 0 : rotaryDim % (2 * E) == 0;
 }
 
+// Heads of a row that one block takes, and its threads: chunks of equal size, about kThreadsWanted
+// threads each.
+constexpr int kThreadsWanted = 512;
+inline void headChunks(int perRow, int lanes, int* chunks, int* threads) {
+    *chunks = std::max(1, (perRow * lanes + kThreadsWanted - 1) / kThreadsWanted);
+    const int heads = (perRow + *chunks - 1) / *chunks;
+    *threads = (heads * lanes + 31) / 32 * 32;
+    *chunks = (perRow * lanes + *threads - 1) / *threads;
+}
+
 template <typename T>
 cudaError_t normRotateOf(const NormRotateParams& p, cudaStream_t stream, int* launches) {
-    constexpr int E = Piece<T>::E;
+    constexpr int BYTES = 16, E = BYTES / sizeof(T);
     const void* ptrs[] = {p.q, p.k, p.v, p.qWeight, p.kWeight, p.qOut, p.kOut, p.vOut, p.kPool, p.vPool};
-    bool pieces = piecesApply<T>(p.headDim, p.rotaryDim, p.interleaved);
+    bool pieces = piecesApply<E>(p.headDim, p.rotaryDim, p.interleaved);
     for (const void* ptr : ptrs) pieces = pieces && aligned16(ptr);
     for (int64_t s : {p.qStride, p.kStride, p.vStride, p.qOutStride, p.kOutStride, p.vOutStride}) pieces = pieces && s % E == 0;
     const int perRow = p.heads + 2 * p.kvHeads;
@@ -295,15 +420,14 @@ cudaError_t normRotateOf(const NormRotateParams& p, cudaStream_t stream, int* la
         const int64_t warps = static_cast<int64_t>(p.numRows) * perRow;
         normRotateAnyKernel<T><<<static_cast<unsigned>(std::min<int64_t>((warps + 3) / 4, 148 * 16)), 128, 0, stream>>>(p);
     } else {
-        const Layout l = layoutOf<T>(p.headDim, p.rotaryDim, p.interleaved);
-        const int rowLanes = perRow * l.lanes;
-        const int threads = std::min(512, (rowLanes + 31) / 32 * 32);
-        // short rows share a block, as far as their angles fit
-        const int rowsPer = std::max(1, std::min(256 / std::max(rowLanes, 1), 64));
-        const int block = rowsPer > 1 ? 256 : threads;
-        const size_t smem = static_cast<size_t>(rowsPer) * (p.rotaryDim / 2) * sizeof(float2);
-        const int64_t grid = (static_cast<int64_t>(p.numRows) + rowsPer - 1) / rowsPer;
-        normRotateKernel<T><<<static_cast<unsigned>(grid), block, smem, stream>>>(p, l, rowsPer);
+        const Layout l = layoutOf<E>(p.headDim, p.rotaryDim, p.interleaved);
+        int chunks, threads;
+        headChunks(perRow, l.lanes, &chunks, &threads);
+        // enough blocks for every SM first, then rows to share the look-ups and the weights
+        const int rowsPer = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kForwardRows, p.numRows / (148 * 4))));
+        const size_t smem = static_cast<size_t>(rowsPer) * (sizeof(RowInfo) + (p.rotaryDim / 2) * sizeof(float2));
+        const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.numRows) + rowsPer - 1) / rowsPer), chunks);
+        normRotateKernel<T, BYTES><<<grid, threads, smem, stream>>>(p, l, rowsPer);
     }
     *launches += 1;
     return cudaGetLastError();
@@ -311,129 +435,154 @@ cudaError_t normRotateOf(const NormRotateParams& p, cudaStream_t stream, int* la
 
 // ---- backward ---------------------------------------------------------------
 
-constexpr int kBackwardThreads = 256;
+constexpr int kBackwardRows = 8;         // rows that a block looks up at a time
 
-// The rows are dealt to the blocks round robin.  A thread always holds the same pieces of a head,
-// so that its share of the weight gradients stays in registers over all its rows; at the end the
-// block's groups are summed through shared memory in a fixed order and the block writes its
-// [2][dim] partial sums: no atomics, the same bits for the same grid.
-template <typename T>
-__global__ void __launch_bounds__(kBackwardThreads)
-normRotateBackwardKernel(const NormRotateBackwardParams p, const Layout l) {
-    constexpr int E = Piece<T>::E;
-    extern __shared__ float2 turns[];                 // [rotaryDim / 2], then floats [groups][2 E lanes]
-    const int tid = threadIdx.x, half = p.rotaryDim / 2;
-    const int lane = tid % l.lanes, group = tid / l.lanes, groups = kBackwardThreads / l.lanes;
+// As the forward kernel, every block with an equal share of the rows.  A group of lanes keeps one head
+// of a row and each lane its pieces of it, so that its share of the weight gradients stays in
+// registers over all its rows; then the groups of the queries and those of the keys are summed through
+// shared memory in a fixed order and the block writes its [2][dim] partial sums: no atomics, the same
+// bits for the same grid.  Measured at 8192 rows of 32 + 8 heads of 128, bfloat16 (252 MB): 76 us =
+// 3.3 TB/s, 0.51 of the copy rate: bound by the issue of some 250 instructions per 16 elements and by
+// the registers that hold the next row (96, two blocks on an SM); four blocks 91 us, 8-byte pieces
+// 128 us, a row at a time 137 us.
+template <typename T, int BYTES>
+__global__ void __maxnreg__(96)
+normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, const Layout l, int share) {
+    using P = Piece<T, BYTES>;
+    constexpr int E = P::E;
+    extern __shared__ __align__(16) unsigned char rowSmem[];
+    const int tid = threadIdx.x, half = p.rotaryDim / 2, threads = blockDim.x;
+    float* sums = reinterpret_cast<float*>(rowSmem);                      // [threads][2 E]
+    RowInfo* info = reinterpret_cast<RowInfo*>(sums + (p.partials ? threads * 2 * E : 0));                // [kBackwardRows]
+    float* turns = reinterpret_cast<float*>(info + kBackwardRows);        // [kBackwardRows][rotaryDim]
+    const int lane = tid & (l.lanes - 1), group = tid / l.lanes, groups = threads / l.lanes;
     const int perRow = p.heads + p.kvHeads + (p.dV ? p.kvHeads : 0);
-    const int rounds = (perRow + groups - 1) / groups;
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * share, end = min(begin + share, static_cast<int64_t>(p.numRows));
     int pa, pb;
     l.lane(lane, pa, pb);
     const bool hasA = pa < l.pieces, hasB = pb < l.pieces;
-    float accQ[2 * E], accK[2 * E];
-#pragma unroll
-    for (int e = 0; e < 2 * E; ++e) accQ[e] = accK[e] = 0.f;
     const float invDim = 1.f / static_cast<float>(p.headDim);
-    for (int64_t row = blockIdx.x; row < p.numRows; row += gridDim.x) {
-        const int pos = p.positions[row];
-        if (pos < 0) continue;                        // the same for the whole block
-        __syncthreads();
-        for (int i = tid; i < half; i += kBackwardThreads) turns[i] = turnOf(pos, p.invFreq[i]);
-        __syncthreads();
-        const int64_t slot = p.slots ? p.slots[row] : -1;
-        const bool inPool = slot >= 0 && slot < p.numSlots;
-        for (int it = 0; it < rounds; ++it) {
-            const int h = it * groups + group;
-            const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads, live = h < perRow;
-            const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
-            const T *x = nullptr, *dy = nullptr;
-            T* dst = nullptr;
-            if (live && isQ) {
-                x = static_cast<const T*>(p.q) + row * p.qStride + static_cast<int64_t>(h) * p.headDim;
-                dy = static_cast<const T*>(p.dQOut) + (row * p.heads + h) * static_cast<int64_t>(p.headDim);
-                dst = static_cast<T*>(p.dQ) + row * p.dQStride + static_cast<int64_t>(h) * p.headDim;
-            } else if (live && !isV) {
-                x = static_cast<const T*>(p.k) + row * p.kStride + static_cast<int64_t>(kvh) * p.headDim;
-                if (p.dKOut) dy = static_cast<const T*>(p.dKOut) + (row * p.kvHeads + kvh) * static_cast<int64_t>(p.headDim);
-                else if (inPool) dy = static_cast<const T*>(p.dKPool) + poolOffset(slot, kvh, p.kvHeads, p.blockSize, p.headDim);
-                dst = static_cast<T*>(p.dK) + row * p.dKStride + static_cast<int64_t>(kvh) * p.headDim;
-            } else if (live) {
-                if (inPool) dy = static_cast<const T*>(p.dVPool) + poolOffset(slot, kvh, p.kvHeads, p.blockSize, p.headDim);
-                dst = static_cast<T*>(p.dV) + row * p.dVStride + static_cast<int64_t>(kvh) * p.headDim;
-            }
-            Piece<T> xa{}, xb{}, ya{}, yb{};
-            if (x && hasA) xa.load(x + pa * E);
-            if (x && hasB) xb.load(x + pb * E);
-            if (dy && hasA) ya.load(dy + pa * E);
-            if (dy && hasB) yb.load(dy + pb * E);
-            if (isV) {                                // (a group's lanes agree; the shuffles below name them alone)
-                if (dst && hasA) ya.store(dst + pa * E);
-                if (dst && hasB) yb.store(dst + pb * E);
-            }
-            float fa[E], fb[E], ga[E], gb[E];
-            xa.unpack(fa); xb.unpack(fb);
-            ya.unpack(ga); yb.unpack(gb);
-            if (l.half) {
-                if (lane < l.pairs) rotateHalves<E>(ga, gb, turns + pa * E, -1.f);
-            } else {
-                if (pa * E < p.rotaryDim) rotatePairs<E>(ga, turns + pa * E / 2, -1.f);
-                if (pb * E < p.rotaryDim) rotatePairs<E>(gb, turns + pb * E / 2, -1.f);
-            }
+    {
+        const int h0 = static_cast<int>(blockIdx.y) * groups, h = h0 + group;
+        const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads, wanted = h < perRow;
+        const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
+        const T* src = isQ ? static_cast<const T*>(p.q) + static_cast<int64_t>(h) * p.headDim : static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * p.headDim;
+        const int64_t srcStride = isQ ? p.qStride : p.kStride;
+        // the gradient with respect to the rotated row: rows, or (keys and values) pages
+        const T* up = isQ ? static_cast<const T*>(p.dQOut) + static_cast<int64_t>(h) * p.headDim
+                    : !isV && p.dKOut ? static_cast<const T*>(p.dKOut) + static_cast<int64_t>(kvh) * p.headDim
+                    : static_cast<const T*>(isV ? p.dVPool : p.dKPool) + static_cast<int64_t>(kvh) * p.blockSize * p.headDim;
+        const int64_t upStride = static_cast<int64_t>(isQ ? p.heads : p.kvHeads) * p.headDim;
+        const bool fromPool = !isQ && (isV || !p.dKOut);
+        T* dst = static_cast<T*>(isQ ? p.dQ : isV ? p.dV : p.dK) + static_cast<int64_t>(isQ ? h : kvh) * p.headDim;
+        const int64_t dstStride = isQ ? p.dQStride : isV ? p.dVStride : p.dKStride;
+        P wa, wb;
+        if (wanted && !isV && hasA) {
             const T* weight = static_cast<const T*>(isQ ? p.qWeight : p.kWeight);
-            Piece<T> wa{}, wb{};
-            if (hasA) wa.load(weight + pa * E);
+            wa.load(weight + pa * E);
             if (hasB) wb.load(weight + pb * E);
-            float va[E], vb[E];
-            wa.unpack(va); wb.unpack(vb);
-            float sum = 0.f, dot = 0.f;               // of x^2, and of x * g
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                sum += fa[e] * fa[e] + fb[e] * fb[e];
-                dot += fa[e] * ga[e] * va[e] + fb[e] * gb[e] * vb[e];
-            }
-            for (int o = l.lanes >> 1; o > 0; o >>= 1) {
-                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-                dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
-            }
-            if (!live || isV || !hasA) continue;      // (no shuffle below)
-            const float r = rsqrtf(sum * invDim + p.eps);
-            const float mean = dot * r * invDim;      // of xhat * g
-            float ha[E], hb[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float xa_ = fa[e] * r, xb_ = fb[e] * r;
-                ha[e] = r * (ga[e] * va[e] - xa_ * mean);
-                hb[e] = r * (gb[e] * vb[e] - xb_ * mean);
-                if (isQ) {
-                    accQ[e] += ga[e] * xa_;
-                    accQ[E + e] += gb[e] * xb_;
-                } else {
-                    accK[e] += ga[e] * xa_;
-                    accK[E + e] += gb[e] * xb_;
-                }
-            }
-            xa.pack(ha);
-            xb.pack(hb);
-            xa.store(dst + pa * E);
-            if (hasB) xb.store(dst + pb * E);
         }
-    }
-    if (!p.partials) return;
-    float* sums = reinterpret_cast<float*>(turns + half + (half & 1));
-    const int width = 2 * E * l.lanes;                // floats of a group
+        F2 accA[E / 2], accB[E / 2];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
+        for (int e = 0; e < E / 2; ++e) accA[e] = accB[e] = 0ull;
+        for (int64_t row0 = begin; row0 < end; row0 += kBackwardRows) {
+            const int n = static_cast<int>(min(static_cast<int64_t>(kBackwardRows), end - row0));
+            __syncthreads();
+            lookRowsUp(info, turns, row0, n, p.positions, p.slots, p.numSlots, p.invFreq, half, p.kvHeads, p.blockSize, p.headDim);
+            struct Row { P xa, xb, ya, yb; };
+            auto load = [&](int r) {
+                Row w;
+                if (!wanted || !hasA || r >= n || info[r].position < 0) return w;
+                if (!isV) {
+                    const T* at = src + (row0 + r) * srcStride;
+                    w.xa.load(at + pa * E);
+                    if (hasB) w.xb.load(at + pb * E);
+                }
+                const int64_t slot = info[r].pool;
+                const T* from = fromPool ? up + (slot >= 0 ? slot : 0) : up + (row0 + r) * upStride;
+                if (!fromPool || slot >= 0) {
+                    w.ya.load(from + pa * E);
+                    if (hasB) w.yb.load(from + pb * E);
+                }
+                return w;
+            };
+            Row w = load(0);
+#pragma unroll 1
+            for (int r = 0; r < n; ++r) {
+                const Row next = load(r + 1);         // on its way while this row is worked on
+                const bool live = wanted && hasA && info[r].position >= 0;
+                T* to = dst + (row0 + r) * dstStride;
+                if (live && isV) {
+                    w.ya.store(to + pa * E);
+                    if (hasB) w.yb.store(to + pb * E);
+                }
+                F2 ga[E / 2], gb[E / 2], sq = 0ull, xg = 0ull;                // sums of x^2, and of x * g
+                w.ya.unpack(ga); w.yb.unpack(gb);
+                turnPieces<E>(ga, gb, l, lane, pa, pb, p.rotaryDim, turns + r * 2 * half, -1.f);
+                {
+                    F2 fa[E / 2], fb[E / 2], va[E / 2], vb[E / 2];
+                    w.xa.unpack(fa); w.xb.unpack(fb);
+                    wa.unpack(va); wb.unpack(vb);
+#pragma unroll
+                    for (int e = 0; e < E / 2; ++e) {
+                        sq = fma2(fb[e], fb[e], fma2(fa[e], fa[e], sq));
+                        xg = fma2(fb[e], mul2(gb[e], vb[e]), fma2(fa[e], mul2(ga[e], va[e]), xg));
+                    }
+                }
+                w.xa.forget(); w.xb.forget(); wa.forget(); wb.forget();
+                float sum = sumOf(sq), dot = sumOf(xg);
+                for (int o = l.lanes >> 1; o > 0; o >>= 1) {
+                    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+                    dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+                }
+                if (live && !isV) {
+                    const float root = rsqrtf(sum * invDim + p.eps);
+                    const float mean = dot * root * invDim;               // of xhat * g
+                    const F2 scale = pack2(root, root), minusMean = pack2(-mean, -mean);
+                    F2 fa[E / 2], fb[E / 2], va[E / 2], vb[E / 2], ha[E / 2], hb[E / 2];
+                    w.xa.unpack(fa); w.xb.unpack(fb);
+                    wa.unpack(va); wb.unpack(vb);
+#pragma unroll
+                    for (int e = 0; e < E / 2; ++e) {
+                        const F2 ua = mul2(fa[e], scale), ub = mul2(fb[e], scale);        // xhat
+                        ha[e] = mul2(scale, fma2(ua, minusMean, mul2(ga[e], va[e])));
+                        hb[e] = mul2(scale, fma2(ub, minusMean, mul2(gb[e], vb[e])));
+                        accA[e] = fma2(ga[e], ua, accA[e]);
+                        accB[e] = fma2(gb[e], ub, accB[e]);
+                    }
+                    P out;
+                    out.pack(ha);
+                    out.store(to + pa * E);
+                    if (hasB) {
+                        out.pack(hb);
+                        out.store(to + pb * E);
+                    }
+                }
+                w = next;
+            }
+        }
+        if (!p.partials) return;
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 2 * E; ++e) sums[group * width + lane * 2 * E + e] = which ? accK[e] : accQ[e];
+        for (int e = 0; e < E / 2; ++e) {
+            *reinterpret_cast<F2*>(sums + tid * 2 * E + 2 * e) = accA[e];
+            *reinterpret_cast<F2*>(sums + tid * 2 * E + E + 2 * e) = accB[e];
+        }
         __syncthreads();
-        for (int i = tid; i < width; i += kBackwardThreads) {
+        // element i of a head: the lane and place that hold it, its groups in order, queries and keys apart
+        for (int i = tid; i < l.lanes * 2 * E; i += threads) {
             int a, b;
             l.lane(i / (2 * E), a, b);
             const int e = i % (2 * E), piece = e < E ? a : b;
             if (piece >= l.pieces) continue;
-            float total = 0.f;
-            for (int g = 0; g < groups; ++g) total += sums[g * width + i];
-            p.partials[(static_cast<int64_t>(blockIdx.x) * 2 + which) * p.headDim + piece * E + e % E] = total;
+            const int d = piece * E + e % E, queries = min(max(p.heads - h0, 0), groups);
+            const int both = min(max(p.heads + p.kvHeads - h0, 0), groups);
+            float q = 0.f, k = 0.f;
+            for (int g = 0; g < queries; ++g) q += sums[g * l.lanes * 2 * E + i];
+            for (int g = queries; g < both; ++g) k += sums[g * l.lanes * 2 * E + i];
+            float* out = p.partials + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 2 * p.headDim;
+            out[d] = q;
+            out[p.headDim + d] = k;
         }
     }
 }
@@ -442,7 +591,7 @@ normRotateBackwardKernel(const NormRotateBackwardParams p, const Layout l) {
 // gradients is added up in shared memory, each element by the lane that owns it.
 template <typename T>
 __global__ void __launch_bounds__(128)
-normRotateBackwardAnyKernel(const NormRotateBackwardParams p) {
+normRotateBackwardAnyKernel(const __grid_constant__ NormRotateBackwardParams p) {
     extern __shared__ float smemAny[];                // per warp: x, g (dn), accQ, accK, [dim] each
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rotaryDim / 2, D = p.headDim;
     float *x = smemAny + static_cast<size_t>(warp) * 4 * D, *g = x + D, *accQ = g + D, *accK = accQ + D;
@@ -529,30 +678,46 @@ weightGradientKernel(const float* __restrict__ partials, int blocks, int dim, fl
     }
 }
 
+// Blocks that share the rows: two for every SM, each with at least one look-up's worth of rows.
 int backwardBlocks(const NormRotateBackwardParams& p, int smCount) {
-    return static_cast<int>(std::min<int64_t>(p.numRows, static_cast<int64_t>(smCount) * 4));
+    return static_cast<int>(std::min<int64_t>((static_cast<int64_t>(p.numRows) + kBackwardRows - 1) / kBackwardRows, static_cast<int64_t>(smCount) * 2));
+}
+template <typename T> constexpr int backwardBytes() { return 16; }
+// Lanes and threads of the launch that the pieces allow (chunks 1, threads 0: the other kernel runs).
+template <typename T>
+int backwardChunks(const NormRotateBackwardParams& p, Layout* l, int* threads) {
+    constexpr int E = backwardBytes<T>() / sizeof(T);
+    *threads = 0;
+    if (!piecesApply<E>(p.headDim, p.rotaryDim, p.interleaved)) return 1;
+    *l = layoutOf<E>(p.headDim, p.rotaryDim, p.interleaved);
+    int chunks;
+    headChunks(p.heads + (p.dV ? 2 : 1) * p.kvHeads, l->lanes, &chunks, threads);
+    return chunks;
 }
 
 template <typename T>
 cudaError_t normRotateBackwardOf(const NormRotateBackwardParams& p, int smCount, cudaStream_t stream, int* launches) {
-    constexpr int E = Piece<T>::E;
+    constexpr int BYTES = backwardBytes<T>(), E = BYTES / sizeof(T);
     const void* ptrs[] = {p.q, p.k, p.qWeight, p.kWeight, p.dQOut, p.dKOut, p.dKPool, p.dVPool, p.dQ, p.dK, p.dV};
-    bool pieces = piecesApply<T>(p.headDim, p.rotaryDim, p.interleaved);
+    Layout l{};
+    int threads, chunks = backwardChunks<T>(p, &l, &threads);
+    bool pieces = threads > 0;
     for (const void* ptr : ptrs) pieces = pieces && aligned16(ptr);
     for (int64_t s : {p.qStride, p.kStride, p.dQStride, p.dKStride, p.dVStride}) pieces = pieces && s % E == 0;
     const int blocks = backwardBlocks(p, smCount);
     if (pieces) {
-        const Layout l = layoutOf<T>(p.headDim, p.rotaryDim, p.interleaved);
-        const int half = p.rotaryDim / 2;
-        const size_t smem = (half + (half & 1)) * sizeof(float2) + (p.partials ? kBackwardThreads * 2 * E * sizeof(float) : 0);
-        normRotateBackwardKernel<T><<<blocks, kBackwardThreads, smem, stream>>>(p, l);
+        const int share = static_cast<int>((static_cast<int64_t>(p.numRows) + blocks - 1) / blocks);
+        const size_t smem = (p.partials ? static_cast<size_t>(threads) * 2 * E * sizeof(float) : 0) +
+                            kBackwardRows * (sizeof(RowInfo) + (p.rotaryDim / 2) * sizeof(float2));
+        normRotateBackwardKernel<T, BYTES><<<dim3(blocks, chunks), threads, smem, stream>>>(p, l, share);
     } else {
+        chunks = 1;
         normRotateBackwardAnyKernel<T><<<blocks, 128, static_cast<size_t>(16) * p.headDim * sizeof(float), stream>>>(p);
     }
     *launches += 1;
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess && p.partials) {
-        weightGradientKernel<<<dim3((p.headDim + 31) / 32, 2), 256, 0, stream>>>(p.partials, blocks, p.headDim, p.dQWeight, p.dKWeight);
+        weightGradientKernel<<<dim3((p.headDim + 31) / 32, 2), 256, 0, stream>>>(p.partials, blocks * chunks, p.headDim, p.dQWeight, p.dKWeight);
         *launches += 1;
         e = cudaGetLastError();
     }
@@ -571,7 +736,10 @@ cudaError_t launchNormRotate(const NormRotateParams& p, cudaStream_t stream, int
 
 size_t normRotateBackwardWorkspaceBytes(const NormRotateBackwardParams& p, int smCount) {
     if (!p.dQWeight && !p.dKWeight) return 0;
-    return static_cast<size_t>(backwardBlocks(p, smCount)) * 2 * p.headDim * sizeof(float);
+    Layout l{};
+    int threads;
+    const int chunks = p.ioType == kF32 ? backwardChunks<float>(p, &l, &threads) : backwardChunks<__half>(p, &l, &threads);
+    return static_cast<size_t>(backwardBlocks(p, smCount)) * chunks * 2 * p.headDim * sizeof(float);
 }
 
 cudaError_t launchNormRotateBackward(const NormRotateBackwardParams& p, int smCount, cudaStream_t stream, int* launches) {

@@ -375,6 +375,7 @@ static void normBackwardSizes(const PamNormRotateBackwardRequest& rq, pam::NormR
     p->numRows = rq.num_rows; p->heads = rq.layer.num_heads; p->kvHeads = rq.layer.num_kv_heads; p->headDim = rq.layer.head_dim;
     p->blockSize = rq.layer.block_size; p->rotaryDim = rq.rotary_dim; p->interleaved = rq.interleaved != 0; p->ioType = rq.layer.data_type;
     p->eps = rq.epsilon;
+    p->dV = rq.d_v.ptr;
     p->dQWeight = static_cast<float*>(rq.d_q_weight.ptr);
     p->dKWeight = static_cast<float*>(rq.d_k_weight.ptr);
 }
