@@ -306,13 +306,13 @@ treeJoinKernel(const __grid_constant__ TreeParams p, int blocks, int mr, int dim
     }
 }
 
-// The same for the records of treeTcKernel, whose O is [piece of 4 columns][256 rows]: block (i, y)
+// The same for the records of treeTcKernel, whose O is [piece of 4 columns][MR rows]: block (i, y)
 // takes rows 32 y .. + 31, a lane a row and a warp four pieces, so that the reads of a record are
 // whole lines.
-template <typename QT>
+template <typename QT, typename KT_, int MR>
 __global__ void __launch_bounds__(256)
 treeJoinColumnsKernel(const __grid_constant__ TreeParams p, int blocks) {
-    constexpr int MR = 256, HD = 128;
+    constexpr int HD = 128;
     cudaGridDependencySynchronize();
     const Header h = *headerOf(p, blockIdx.x);
     if (h.lastBlock < 0) return;
@@ -359,7 +359,7 @@ treeJoinColumnsKernel(const __grid_constant__ TreeParams p, int blocks) {
     QT* to = static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + h.kvh * group + rr % group) * HD;
 #pragma unroll
     for (int q = 0; q < 2; ++q) reinterpret_cast<uint4*>(to + 16 * warp)[q] = reinterpret_cast<const uint4*>(out)[q];
-    if (odd) addLeftOut<QT, QT>(p, s, h.b, h.kvh, rr / group, lastFirst(p, s, h.rt, MR), to, 16 * warp, 16 * warp + 16);
+    if (odd) addLeftOut<QT, KT_>(p, s, h.b, h.kvh, rr / group, lastFirst(p, s, h.rt, MR), to, 16 * warp, 16 * warp + 16);
 }
 
 // The joining kernel may be set up while the attention kernel still runs.
@@ -382,8 +382,10 @@ cudaError_t launchJoin(const TreeParams& p, const TreePlan& plan, cudaStream_t s
     if (plan.blocks < 2) return cudaSuccess;
     *launches += 1;
     const unsigned blocks = static_cast<unsigned>(plan.blocks - 1);
-    if constexpr (sizeof(QT) == 2 && sizeof(KT_) == 2)
-        if (plan.variant == 2) return launchEarly(treeJoinColumnsKernel<QT>, dim3(blocks, plan.rows / 32), stream, p, plan.blocks);
+    if constexpr (sizeof(QT) == 2)
+        if (plan.variant == 2)
+            return plan.rows == 256 ? launchEarly(treeJoinColumnsKernel<QT, KT_, 256>, dim3(blocks, 8), stream, p, plan.blocks)
+                                    : launchEarly(treeJoinColumnsKernel<QT, KT_, 128>, dim3(blocks, 4), stream, p, plan.blocks);
     return launchEarly(treeJoinKernel<QT, KT_>, dim3(blocks, (plan.rows + 7) / 8), stream, p, plan.blocks, plan.rows, plan.dimPad);
 }
 
@@ -413,7 +415,7 @@ TreePlan generalPlan(const TreeParams& p, int smCount) {
 }
 
 TreePlan treePlan(const TreeParams& p, int smCount) {
-    if (treeTcApplies(p) && static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) > 16) return treeTcPlan(p, smCount);
+    if (treeTcApplies(p)) return treeTcPlan(p, smCount);
     if (treeMmaApplies(p)) return treeMmaPlan(p, smCount);
     return generalPlan(p, smCount);
 }

@@ -45,14 +45,15 @@ namespace {
 using namespace tc;
 using namespace tree;
 
-constexpr int kRows = 128, kKeys = 128, kHd = 128, kPairRows = 256;
+constexpr int kRows = 128, kKeys = 128, kHd = 128;
 constexpr int kTileBytes = kKeys * kHd * 2, kHalfBytes = kTileBytes / 2;      // a 64-dim block of a tile
 constexpr int kVHalfBytes = kTileBytes / 2, kVBlockBytes = kVHalfBytes / 2;   // 64 keys of V, a 64-dim block of them
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kShortKeys = 256;                        // bfloat16: fewer visible keys carry the weights as two operands
 constexpr long long kWaitCycles = 400000000LL;
 constexpr int kKProducerWarp = 8, kVProducerWarp = 9, kMmaWarp = 10, kPlanWarp = 11, kOutputWarp0 = 12;
-constexpr int kThreads = 512;
+constexpr int kConvertWarp0 = 16;                      // FP8: four more warps
+template <bool FP8> constexpr int kThreads = FP8 ? 640 : 512;
 
 // The part of a pair that lies in the block's piece: key tiles [first, last) of nT.
 struct Span {
@@ -66,19 +67,30 @@ struct Span {
     __device__ __forceinline__ int step() const { return dual ? 1 : 2; }
     // tiles of group x
     __device__ __forceinline__ int tilesOf(int x) const { return dual ? last - first : (last - first + 1 - x) >> 1; }
-    __device__ __forceinline__ int firstRow(int x) const { return rp * kPairRows + (dual ? x * kRows : 0); }
     __device__ __forceinline__ bool whole() const { return first == 0 && last == nT; }
     __device__ __forceinline__ bool shortKeys() const { return s.held - s.lo + static_cast<uint32_t>(s.n) < kShortKeys; }
 };
 
 constexpr int kSpans = 8;        // of the ring: no warp needs a span more than five behind the oldest one in use
 
-template <bool WIDE>
+// FP8, of a key tile: per 16 keys (a page holds a multiple of them) the key scale times log2(e) /
+// sqrt(dim), the logarithm of the value scale, and one over it; negative where the value scale is zero.
+struct PageScales {
+    float4 key[2], valueLog[2], valueInv[2];
+};
+
+// WIDE: pairs of up to 256 rows (two query tiles), else of 128.
+template <bool WIDE, bool FP8>
 struct Smem {
-    static constexpr int kQTiles = WIDE ? 2 : 1, kKStages = WIDE ? 2 : 3, kVStages = WIDE ? 4 : 5;
+    static constexpr int kPairRows = WIDE ? 256 : 128;
+    static constexpr int kQTiles = WIDE ? 2 : 1, kKStages = WIDE || FP8 ? 2 : 3, kVStages = WIDE || FP8 ? 4 : 5;
+    static constexpr int kRawStages = FP8 ? 3 : 1, kScaleStages = FP8 ? 8 : 1;
     unsigned char q[kQTiles][kTileBytes];
     unsigned char k[kKStages][kTileBytes];
     unsigned char v[kVStages][kVHalfBytes];
+    unsigned char raw[kRawStages][FP8 ? kKeys * kHd : 16];                // FP8: codes of a tile's keys or values as they arrive
+    unsigned long long rawFull[kRawStages], rawEmpty[kRawStages];
+    PageScales scales[kScaleStages];         // [tile of the block % stages]
     unsigned long long kFull[kKStages], kEmpty[kKStages], vFull[kVStages], vEmpty[kVStages];
     unsigned long long qFull, qEmpty, sFull[2], pFull[2], oFull[2], oEmpty[2];
     unsigned long long spanFull[kSpans], spanEmpty[kSpans];
@@ -93,18 +105,20 @@ struct Smem {
     int rowNode[2][kRows];
     uint32_t rowFrom[2][kRows], rowBits[2][4][kRows];
     Span span[kSpans];
-    int scratch[kThreads / 32];
+    int scratch[32];
     uint32_t tmemBase;
     int dead;
     int prefix[1];                                     // [batch + 1]
 };
 constexpr size_t kSmemLimit = 227 * 1024;
-template <bool WIDE> constexpr size_t smemBytes(int batch) { return sizeof(Smem<WIDE>) + static_cast<size_t>(batch) * sizeof(int); }
-static_assert(smemBytes<true>(kTreeMaxBatch) <= kSmemLimit, "the block's shared memory must fit the 227 KB a block may opt into");
-constexpr int kSpanReaders = 2 + 1 + 4 + 8;            // warps: producers, issuer, output, softmax
+template <bool WIDE, bool FP8> constexpr size_t smemBytes(int batch) { return sizeof(Smem<WIDE, FP8>) + static_cast<size_t>(batch) * sizeof(int); }
+static_assert(smemBytes<true, false>(kTreeMaxBatch) <= kSmemLimit, "the block's shared memory must fit the 227 KB a block may opt into");
+// warps that read the spans: producers, issuer, output, softmax; FP8: one producer, and the converters
+template <bool FP8> constexpr int kSpanReaders = FP8 ? 1 + 1 + 4 + 8 + 4 : 2 + 1 + 4 + 8;
 
 // The block's next span at or after position `pos` of the list (a pair's start, or the block's
 // begin); moves pos behind that pair.  False at the end of the piece.
+template <bool WIDE>
 __device__ __forceinline__ bool nextSpan(const TreeParams& p, const int* prefix, int begin, int end, int quota, int& pos, Span& g) {
     const int group = p.heads / p.kvHeads;
     while (pos < end) {
@@ -122,9 +136,10 @@ __device__ __forceinline__ bool nextSpan(const TreeParams& p, const int* prefix,
         const int rel = pos - prefix[a];
         g.kvh = rel / perHead;
         const int inHead = rel - g.kvh * perHead;
-        g.rp = inHead / (2 * g.nT);
-        g.dual = rowTiles - 2 * g.rp >= 2;
-        const int start = prefix[a] + g.kvh * perHead + g.rp * 2 * g.nT, w = g.dual ? 2 : 1;
+        constexpr int kTiles = WIDE ? 2 : 1;            // row tiles of a pair
+        g.rp = inHead / (kTiles * g.nT);
+        g.dual = WIDE && rowTiles - 2 * g.rp >= 2;
+        const int start = prefix[a] + g.kvh * perHead + g.rp * kTiles * g.nT, w = g.dual ? 2 : 1;
         // the tiles whose place in the list lies in [begin, end)
         g.first = begin > start ? (begin - start + w - 1) / w : 0;
         g.last = min(g.nT, (end - start + w - 1) / w);
@@ -159,6 +174,37 @@ __device__ __forceinline__ void tmemLd16NoWait(uint32_t taddr, uint32_t (&r)[16]
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
+// FP8: the largest of 16 raw scores, and the weights of 16 keys with their page's scales (the sum
+// without the value scale is returned).
+template <int BEGIN>
+__device__ __forceinline__ float rowMax16(const uint32_t (&r)[32]) {
+    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        m0 = max3(m0, __uint_as_float(r[BEGIN + i]), __uint_as_float(r[BEGIN + i + 1]));
+        m1 = max3(m1, __uint_as_float(r[BEGIN + i + 2]), __uint_as_float(r[BEGIN + i + 3]));
+    }
+    return fmaxf(m0, m1);
+}
+template <int BEGIN>
+__device__ __forceinline__ float pageWeights(const uint32_t (&r)[32], uint32_t (&w)[32], float key, float valueLog, float inv, float negM) {
+    const float sum = weightsRange<false, false, BEGIN, BEGIN + 16>(r, w, key, negM + valueLog);
+    if (inv > 0.f) return sum * inv;
+    // a value scale of zero: the keys count, their values are zero
+#pragma unroll
+    for (int i = BEGIN / 2; i < BEGIN / 2 + 8; ++i) w[i] = 0u;
+    return sum;
+}
+// Two codes to two float16 values.
+__device__ __forceinline__ uint32_t widen(uint32_t codes) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<unsigned short>(codes)));
+    return r;
+}
+__device__ __forceinline__ void bulkLoad(void* dst, const void* src, uint32_t bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smemAddr(dst)), "l"(src), "r"(bytes), "r"(smemAddr(bar)) : "memory");
+}
 // Whether `v` is set in any of the 128 threads of the output warps (all of them get here).
 __device__ __forceinline__ bool anyOfOutput(bool v) {
     uint32_t r = v ? 1u : 0u;
@@ -166,14 +212,16 @@ __device__ __forceinline__ bool anyOfOutput(bool v) {
     return r != 0;
 }
 
-template <bool BF16, bool WIDE>
-__global__ void __launch_bounds__(kThreads, 1)
+template <bool BF16, bool WIDE, bool FP8>
+__global__ void __launch_bounds__(kThreads<FP8>, 1)
 treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
              const __grid_constant__ CUtensorMap mapKNew, const __grid_constant__ CUtensorMap mapVNew,
              const __grid_constant__ TreeParams p, float scaleLog2, int* errFlag, long long waitLimit) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     extern __shared__ __align__(1024) unsigned char rawSmem[];
-    using S = Smem<WIDE>;
+    using S = Smem<WIDE, FP8>;
+    using PoolT = typename std::conditional<FP8, uint8_t, T>::type;
+    constexpr int kPairRows = S::kPairRows;
     S* s = reinterpret_cast<S*>(rawSmem);
     if ((smemAddr(rawSmem) & 1023u) != 0) {
         if (threadIdx.x == 0) atomicCAS(errFlag, 0, 40);
@@ -189,9 +237,10 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             mbarInit(&s->oFull[i], 1);
             mbarInit(&s->oEmpty[i], 1);
         }
-        for (int i = 0; i < S::kKStages; ++i) { mbarInit(&s->kFull[i], 1); mbarInit(&s->kEmpty[i], 1); }
-        for (int i = 0; i < S::kVStages; ++i) { mbarInit(&s->vFull[i], 1); mbarInit(&s->vEmpty[i], 1); }
-        for (int i = 0; i < kSpans; ++i) { mbarInit(&s->spanFull[i], 1); mbarInit(&s->spanEmpty[i], kSpanReaders); }
+        for (int i = 0; i < S::kKStages; ++i) { mbarInit(&s->kFull[i], FP8 ? kRows : 1); mbarInit(&s->kEmpty[i], 1); }
+        for (int i = 0; i < S::kVStages; ++i) { mbarInit(&s->vFull[i], FP8 ? kRows / 2 : 1); mbarInit(&s->vEmpty[i], 1); }
+        for (int i = 0; i < S::kRawStages; ++i) { mbarInit(&s->rawFull[i], 1); mbarInit(&s->rawEmpty[i], kRows); }
+        for (int i = 0; i < kSpans; ++i) { mbarInit(&s->spanFull[i], 1); mbarInit(&s->spanEmpty[i], kSpanReaders<FP8>); }
         s->dead = *reinterpret_cast<volatile int*>(errFlag) != 0 ? 1 : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         Header h{};
@@ -202,7 +251,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddr(&s->tmemBase)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    buildPrefix<kRows, kKeys, kThreads>(p, s->prefix, s->scratch);
+    buildPrefix<kRows, kKeys, kThreads<FP8>>(p, s->prefix, s->scratch);
     tcFenceBefore();
     __syncthreads();
     tcFenceAfter();
@@ -221,9 +270,10 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         if (lane == 0) mbarArrive(&s->spanEmpty[k % kSpans]);
     };
 
-    // 512 x 128 registers at launch: 96 for the service warps, 96 for the output warps, 160 for softmax
+    // 512 x 128 registers at launch: 96 for the service warps, 96 for the output warps, 160 for softmax;
+    // FP8 640 x 96: 80, 80, 120, and 80 for the converting warps
     if (warp == kKProducerWarp || warp == kVProducerWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (!live) goto done;
         const bool isV = warp == kVProducerWarp;
         const CUtensorMap* pool = isV ? &mapV : &mapK;
@@ -231,7 +281,74 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         const int tilesPerPage = p.blockSize / 16;
         int gt = 0;                          // tiles of the block's piece so far
         bool ok = true;
-        for (int k = 0; ok; ++k) {
+        if constexpr (FP8) {
+            // One warp for keys and values: pages of 16 rows, 2 KB of codes each, keys before values in
+            // one ring, and the tile's scales, which the ring of eight keeps until the softmax is through:
+            // behind the ring of codes this warp is at most five tiles ahead of it.  (The rows of a tree are
+            // fetched by the converting warps; their tiles take part in the ring, empty.)  Lane i has page
+            // piece i; its entry of the block table is looked up two tiles ahead, its scales one.
+            auto entry = [&](const Span& g, const int32_t* table, int j) {
+                const int t16 = (static_cast<int>(g.s.lo / kKeys) + j) * (kKeys / 16) + (lane & 7);
+                return table[min(t16 / tilesPerPage, p.maxNumBlocks - 1)];
+            };
+            auto pairOf = [&](const Span& g, int blk) {
+                return static_cast<int64_t>(min(max(blk, 0), p.poolBlocks - 1)) * p.kvHeads + g.kvh;
+            };
+            const __half* kScale = static_cast<const __half*>(p.kScale);
+            const __half* vScale = static_cast<const __half*>(p.vScale);
+            int raw = 0;
+            for (int k = 0; ok && !isV; ++k) {
+                const Span* at = spanAt(k);
+                if (!at || !at->valid) break;
+                const Span& g = *at;
+                const int32_t* table = p.tables + static_cast<int64_t>(g.b) * p.maxNumBlocks;
+                const int end = min(g.last, g.cacheTiles);           // of the tiles of the cache
+                int nextBlk = 0;
+                int64_t pair = 0;
+                __half ksNext = __float2half(0.f), vsNext = ksNext;
+                if (g.first < end) {
+                    pair = pairOf(g, entry(g, table, g.first));
+                    ksNext = kScale[pair];
+                    vsNext = vScale[pair];
+                    if (g.first + 1 < end) nextBlk = entry(g, table, g.first + 1);
+                }
+                for (int j = g.first; j < g.last && ok; ++j, ++gt) {
+                    const bool inTree = j >= g.cacheTiles;
+                    const int t16 = (static_cast<int>(g.s.lo / kKeys) + j) * (kKeys / 16) + (lane & 7);
+                    const int64_t from = (pair * p.blockSize + (t16 % tilesPerPage) * 16) * kHd;
+                    const float ks = __half2float(ksNext), vs = __half2float(vsNext);
+                    if (j + 1 < end) {
+                        pair = pairOf(g, nextBlk);
+                        ksNext = kScale[pair];
+                        vsNext = vScale[pair];
+                        if (j + 2 < end) nextBlk = entry(g, table, j + 2);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h, ++raw) {
+                        const int st = raw % S::kRawStages;
+                        if (raw >= S::kRawStages) ok = mbarWait(&s->rawEmpty[st], ((raw / S::kRawStages) - 1) & 1, &s->dead, errFlag, waitLimit, 56);
+                        ok = __all_sync(0xFFFFFFFFu, ok);
+                        if (!ok) break;
+                        if (h == 0 && lane < kKeys / 16) {
+                            PageScales& sc = s->scales[gt % S::kScaleStages];
+                            reinterpret_cast<float*>(sc.key)[lane] = inTree ? scaleLog2 : fmaxf(ks * scaleLog2, 1e-30f);          // (zero times a masked score would be NaN)
+                            reinterpret_cast<float*>(sc.valueLog)[lane] = inTree || !(vs > 0.f) ? 0.f : log2f(vs);
+                            reinterpret_cast<float*>(sc.valueInv)[lane] = inTree ? 1.f : vs > 0.f ? 1.f / vs : -1.f;
+                        }
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (inTree) mbarArrive(&s->rawFull[st]);
+                            else mbarExpectTx(&s->rawFull[st], kKeys * kHd);
+                        }
+                        __syncwarp();
+                        if (!inTree && lane < kKeys / 16)
+                            bulkLoad(s->raw[st] + lane * 2048, static_cast<const unsigned char*>(h ? p.vPool : p.kPool) + from, 2048, &s->rawFull[st]);
+                    }
+                }
+                spanDone(k);
+            }
+        }
+        for (int k = 0; ok && !FP8; ++k) {
             const Span* at = spanAt(k);
             if (!at || !at->valid) break;
             const Span& g = *at;
@@ -284,7 +401,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             spanDone(k);
         }
     } else if (warp == kMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (!live) goto done;
         const bool leader = electOne();
         const uint32_t fmt = BF16 ? 1u : 0u;
@@ -415,7 +532,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             if (c.k != k) spanDone(k);       // (n is in a later span by now)
         }
     } else if (warp == kPlanWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (!live) goto done;
         const int total = s->prefix[p.batch];
         // (a piece of at least two, so that every block between a pair's first and last has a tile of it)
@@ -426,7 +543,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         bool ok = true;
         for (int k = 0; ok; ++k) {
             Span g;
-            const bool got = nextSpan(p, s->prefix, begin, end, quota, pos, g);
+            const bool got = nextSpan<WIDE>(p, s->prefix, begin, end, quota, pos, g);
             g.valid = got;
             g.tile = tile;
             if (got) {
@@ -443,8 +560,80 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             __syncwarp();
             if (!got) break;
         }
+    } else if (FP8 && warp >= kConvertWarp0) {
+        // ------------------------------------------------------------ converting warps
+        // They turn the rows of every tile from codes into float16 (exactly) in the swizzled layout of
+        // the products' operands.  A tile of the tree comes as float16 already, by TMA.
+        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (!live) goto done;
+        const int t = (warp & 3) * 32 + lane, half = t >> 6;
+        int gt = 0, raw = 0;
+        bool ok = true;
+        // The warp's 32 rows of codes into the 64-dim blocks of a tile, `block` bytes apart: a lane takes 16
+        // codes of a row at a time.  Eight lanes read eight pieces, of row r left of the middle and of row
+        // r ^ 1 right of it: their writes then fall on eight different bank groups too.
+        const int piece = lane & 7, rowIn = (lane >> 3) ^ (piece >> 2);
+        const unsigned rawAt = static_cast<unsigned>((warp & 3) * 4096 + rowIn * 128 + piece * 16);
+        const unsigned outAt = static_cast<unsigned>(rowIn * 128 + ((((2 * piece) & 7) ^ rowIn) << 4));
+        auto convert = [&](const unsigned char* from, unsigned char* to, int block) {
+            from += rawAt;
+            to += (piece >> 2) * block;
+#pragma unroll
+            for (int i0 = 0; i0 < 8; i0 += 4) {
+                uint4 w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(from + (i0 + i) * 512);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    unsigned char* row = to + (i0 + i) * 512;
+                    const unsigned at = outAt ^ (i & 1 ? 64u : 0u);
+                    *reinterpret_cast<uint4*>(row + at) = make_uint4(widen(w[i].x), widen(w[i].x >> 16), widen(w[i].y), widen(w[i].y >> 16));
+                    *reinterpret_cast<uint4*>(row + (at ^ 16u)) = make_uint4(widen(w[i].z), widen(w[i].z >> 16), widen(w[i].w), widen(w[i].w >> 16));
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        for (int k = 0; ok; ++k) {
+            const Span* sp = spanAt(k);
+            if (!sp || !sp->valid) break;
+            const Span& g = *sp;
+            for (int j = g.first; j < g.last && ok; ++j, ++gt) {
+                const bool inTree = j >= g.cacheTiles;
+                const int freshRow = g.s.start + (j - g.cacheTiles) * kKeys;
+                const int ks = gt % S::kKStages, n = 2 * gt + half, vs = n % S::kVStages;
+                int st = raw % S::kRawStages;
+                ok = mbarWait(&s->rawFull[st], (raw / S::kRawStages) & 1, &s->dead, errFlag, waitLimit, 58);
+                if (ok && gt >= S::kKStages) ok = mbarWait(&s->kEmpty[ks], ((gt / S::kKStages) - 1) & 1, &s->dead, errFlag, waitLimit, 57);
+                if (!ok) break;
+                if (!inTree) convert(s->raw[st], s->k[ks] + (warp & 3) * 4096, kHalfBytes);
+                mbarArrive(&s->rawEmpty[st]);
+                if (inTree && t == 0) {
+                    mbarExpectTx(&s->kFull[ks], kTileBytes);
+                    for (int i = 0; i < 4; ++i)      // (a box is 64 rows of 64 dims)
+                        tmaLoad3d(s->k[ks] + (i >> 1) * kHalfBytes + (i & 1) * kVBlockBytes, &mapKNew, &s->kFull[ks], 64 * (i >> 1), g.kvh, freshRow + 64 * (i & 1));
+                } else {
+                    mbarArrive(&s->kFull[ks]);
+                }
+                st = ++raw % S::kRawStages;
+                ok = mbarWait(&s->rawFull[st], (raw / S::kRawStages) & 1, &s->dead, errFlag, waitLimit, 60);
+                if (ok && n >= S::kVStages) ok = mbarWait(&s->vEmpty[vs], ((n / S::kVStages) - 1) & 1, &s->dead, errFlag, waitLimit, 59);
+                if (!ok) break;
+                if (!inTree) convert(s->raw[st], s->v[vs] + (warp & 1) * 4096, kVBlockBytes);
+                mbarArrive(&s->rawEmpty[st]);
+                if (inTree && (t & 63) == 0) {
+                    mbarExpectTx(&s->vFull[vs], kVHalfBytes);
+                    for (int i = 0; i < 2; ++i)
+                        tmaLoad3d(s->v[vs] + i * kVBlockBytes, &mapVNew, &s->vFull[vs], 64 * i, g.kvh, freshRow + 64 * half);
+                } else {
+                    mbarArrive(&s->vFull[vs]);
+                }
+                ++raw;
+            }
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            spanDone(k);
+        }
     } else if (warp >= kOutputWarp0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (!live) goto done;
         const int t = (warp & 3) * 32 + lane;
         const uint32_t laneBase = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -579,7 +768,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                     __syncwarp();
                 }
                 if (whole && odd && mine)
-                    addLeftOut<T, T>(p, g.s, g.b, g.kvh, rr / group, g.hi, out, 0, kHd);
+                    addLeftOut<T, PoolT>(p, g.s, g.b, g.kvh, rr / group, g.hi, out, 0, kHd);
                 __syncwarp();
                 if (!whole && mine) {
                     rec[kPairRows * kHd + rl] = m;
@@ -598,7 +787,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         }
     } else {
         // ------------------------------------------------------------ softmax groups
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 120;"); else asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
         if (!live) goto done;
         const int x = warp >> 2, t = (warp & 3) * 32 + lane;
         const uint32_t laneBase = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -620,7 +809,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         while (k >= 0 && ok) {
             const Span& g = s->span[k % kSpans];
             {
-                const int rr = g.firstRow(x) + t, node = rr < g.rows ? rr / group : 0;
+                const int rr = g.rp * kPairRows + (g.dual ? x * kRows : 0) + t, node = rr < g.rows ? rr / group : 0;
                 s->rowNode[x][t] = node;
                 s->rowFrom[x][t] = max(firstOf(p, g.s, node), g.s.lo);
             }
@@ -655,10 +844,15 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 // Two passes over the row, half of it at a time: the maximum, then the weights.  (All 128
                 // scores in registers, read once, make a loop whose code does not stay in the instruction
                 // caches next to the other roles': 129 against 119 us at 64 requests of 2048 tokens.)
+                // FP8: per 16 keys, score times key scale plus the logarithm of the value scale, so that the weights
+                // come out times the value scale, near 1 whatever the scales are; the sum takes it out again.
+                const PageScales& sc = s->scales[(g.tile + j - g.first) % S::kScaleStages];
                 float tmax = -INFINITY;
 #pragma unroll 1
                 for (int c = 0; c < 4; c += 2) {
                     uint32_t r0[32], r1[32];
+                    float4 key, add;
+                    if constexpr (FP8) { key = sc.key[c >> 1]; add = sc.valueLog[c >> 1]; }
                     tmemLd32NoWait(sAddr + 32u * c, r0);
                     tmemLd32NoWait(sAddr + 32u * c + 32u, r1);
                     tmemLdWait();
@@ -666,9 +860,14 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         maskBits(r0, s->rowBits[x][c][t]);
                         maskBits(r1, s->rowBits[x][c + 1][t]);
                     }
-                    tmax = fmaxf(tmax, fmaxf(quarterRowMax(r0), quarterRowMax(r1)));
+                    if constexpr (FP8) {
+                        tmax = fmaxf(max3(tmax, fmaf(rowMax16<0>(r0), key.x, add.x), fmaf(rowMax16<16>(r0), key.y, add.y)),
+                                     fmaxf(fmaf(rowMax16<0>(r1), key.z, add.z), fmaf(rowMax16<16>(r1), key.w, add.w)));
+                    } else {
+                        tmax = fmaxf(tmax, fmaxf(quarterRowMax(r0), quarterRowMax(r1)));
+                    }
                 }
-                tmax *= scaleLog2;
+                if (!FP8) tmax *= scaleLog2;
                 bool raise = false;
                 float corr = 1.f;
                 if (j == j0) mUsed = tmax;
@@ -694,6 +893,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
 #pragma unroll 1
                 for (int c = 0; c < 4; c += 2) {
                     uint32_t r0[32], r1[32], wgt[32];
+                    float4 key, add, inv;
+                    if constexpr (FP8) { key = sc.key[c >> 1]; add = sc.valueLog[c >> 1]; inv = sc.valueInv[c >> 1]; }
                     tmemLd32NoWait(sAddr + 32u * c, r0);
                     tmemLd32NoWait(sAddr + 32u * c + 32u, r1);
                     tmemLdWait();
@@ -701,7 +902,14 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         maskBits(r0, s->rowBits[x][c][t]);
                         maskBits(r1, s->rowBits[x][c + 1][t]);
                     }
-                    if (useLo) {
+                    if constexpr (FP8) {
+                        l += pageWeights<0>(r0, wgt, key.x, add.x, inv.x, negM);
+                        l += pageWeights<16>(r0, wgt, key.y, add.y, inv.y, negM);
+                        tmemSt16(sAddr + 32u * c, wgt);
+                        l += pageWeights<0>(r1, wgt, key.z, add.z, inv.z, negM);
+                        l += pageWeights<16>(r1, wgt, key.w, add.w, inv.w, negM);
+                        tmemSt16(sAddr + 32u * c + 32u, wgt);
+                    } else if (useLo) {
                         l += weightsRange<BF16, true, 0, 32>(r0, wgt, scaleLog2, negM);
                         tmemSt32(sAddr + 32u * c, wgt);
                         l += weightsRange<BF16, true, 0, 32>(r1, wgt, scaleLog2, negM);
@@ -772,7 +980,8 @@ done:
 }  // namespace
 
 bool treeTcApplies(const TreeParams& p) {
-    if ((p.dtype != kF16 && p.dtype != kBF16) || p.headDim != kHd || p.blockSize % 16 != 0) return false;
+    if (p.dtype == kF32 || p.headDim != kHd || p.blockSize % 16 != 0) return false;
+    if (p.dtype == kFP8 && smemBytes<false, true>(p.batch) > kSmemLimit) return false;
     // (rows of the pool are counted in 32 bits)
     if (p.poolBlocks <= 0 || p.poolBlocks >= (1 << 30) / (p.kvHeads * p.blockSize)) return false;
     for (int64_t s : {p.qStride, p.kStride, p.vStride})
@@ -782,10 +991,17 @@ bool treeTcApplies(const TreeParams& p) {
     return true;
 }
 
-TreePlan treeTcPlan(const TreeParams&, int smCount) {
+// Two query tiles: when a request can have more than 128 rows under a KV head (FP8 takes its row tiles
+// one after the other: the codes' ring leaves no room for two), or the batch's list does not fit beside
+// the longer rings.
+static bool takesWide(const TreeParams& p) {
+    return p.dtype != kFP8 && (static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) > kRows || smemBytes<false, false>(p.batch) > kSmemLimit);
+}
+
+TreePlan treeTcPlan(const TreeParams& p, int smCount) {
     TreePlan t{};
     t.variant = 2;
-    t.rows = kPairRows;
+    t.rows = takesWide(p) ? 256 : 128;
     t.keys = kKeys;
     t.dimPad = kHd;
     t.blocks = smCount;
@@ -809,6 +1025,7 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
             return cudaErrorInvalidValue;
     }
     for (int which = 0; which < 2; ++which) {
+        if (p.dtype != kFP8) {
         // pools: [block * kv_head * slot][128]; a box is 64 dims x 16 rows (half of a 16-token piece)
         const cuuint64_t dims[2] = {kHd, static_cast<cuuint64_t>(p.poolBlocks) * p.kvHeads * p.blockSize};
         const cuuint64_t strides[1] = {kHd * 2};
@@ -816,6 +1033,7 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
         if (encode(&pool[which], dt, 2, const_cast<void*>(which ? p.vPool : p.kPool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
+        }
         // the step's rows: [row][kv_head][128]; a box is 64 dims x 1 head x 64 rows (rows behind the last: zeros)
         const cuuint64_t fdims[3] = {kHd, static_cast<cuuint64_t>(p.kvHeads), static_cast<cuuint64_t>(p.numRows)};
         const cuuint64_t fstrides[2] = {kHd * 2, static_cast<cuuint64_t>(which ? p.vStride : p.kStride) * 2};
@@ -825,16 +1043,23 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
             return cudaErrorInvalidValue;
     }
     const float scaleLog2 = 1.4426950408889634f / sqrtf(static_cast<float>(kHd));
-    auto run = [&](auto kernel, size_t smem) -> cudaError_t {
+    auto run = [&](auto kernel, int threads, size_t smem) -> cudaError_t {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
         if (e != cudaSuccess) return e;
-        kernel<<<plan.blocks, kThreads, smem, stream>>>(queries, pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag,
-                                                         p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
+        kernel<<<plan.blocks, threads, smem, stream>>>(queries, pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag,
+                                                        p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
         return cudaGetLastError();
     };
-    const bool wide = static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) > kRows || smemBytes<false>(p.batch) > kSmemLimit;
-    if (wide) return p.dtype == kBF16 ? run(treeTcKernel<true, true>, smemBytes<true>(p.batch)) : run(treeTcKernel<false, true>, smemBytes<true>(p.batch));
-    return p.dtype == kBF16 ? run(treeTcKernel<true, false>, smemBytes<false>(p.batch)) : run(treeTcKernel<false, false>, smemBytes<false>(p.batch));
+    if (p.dtype == kFP8) {
+        pool[0] = pool[1] = queries;                   // (not read)
+        return run(treeTcKernel<false, false, true>, kThreads<true>, smemBytes<false, true>(p.batch));
+    }
+    if (takesWide(p)) {
+        const size_t smem = smemBytes<true, false>(p.batch);
+        return p.dtype == kBF16 ? run(treeTcKernel<true, true, false>, kThreads<false>, smem) : run(treeTcKernel<false, true, false>, kThreads<false>, smem);
+    }
+    const size_t smem = smemBytes<false, false>(p.batch);
+    return p.dtype == kBF16 ? run(treeTcKernel<true, false, false>, kThreads<false>, smem) : run(treeTcKernel<false, false, false>, kThreads<false>, smem);
 }
 
 }  // namespace pam
