@@ -192,6 +192,15 @@ __device__ __forceinline__ uint32_t lastFirst(const TreeParams& p, const SeqInfo
     return hi;
 }
 
+// The same by a whole warp.
+__device__ __forceinline__ uint32_t lastFirstOfWarp(const TreeParams& p, const SeqInfo& s, int rt, int mr) {
+    if (p.window <= 0) return 0u;
+    const int group = p.heads / p.kvHeads, rows = s.n * group;
+    uint32_t hi = 0u;
+    for (int i = rt * mr / group + static_cast<int>(threadIdx.x & 31); i < s.n && i * group < min(rows, (rt + 1) * mr); i += 32) hi = max(hi, firstOf(p, s, i));
+    return __reduce_max_sync(0xFFFFFFFFu, hi);
+}
+
 template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }

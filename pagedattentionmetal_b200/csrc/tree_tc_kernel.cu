@@ -241,15 +241,20 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         for (int i = 0; i < S::kVStages; ++i) { mbarInit(&s->vFull[i], FP8 ? kRows / 2 : 1); mbarInit(&s->vEmpty[i], 1); }
         for (int i = 0; i < S::kRawStages; ++i) { mbarInit(&s->rawFull[i], 1); mbarInit(&s->rawEmpty[i], kRows); }
         for (int i = 0; i < kSpans; ++i) { mbarInit(&s->spanFull[i], 1); mbarInit(&s->spanEmpty[i], kSpanReaders<FP8>); }
-        s->dead = *reinterpret_cast<volatile int*>(errFlag) != 0 ? 1 : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        Header h{};
-        h.lastBlock = -1;
-        *headerOf(p, blockIdx.x) = h;
+        for (const CUtensorMap* m : {&mapQ, &mapK, &mapV, &mapKNew, &mapVNew}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddr(&s->tmemBase)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // What came before the launch on its stream is done from here on.
+    cudaGridDependencySynchronize();
+    if (threadIdx.x == 0) {
+        s->dead = *reinterpret_cast<volatile int*>(errFlag) != 0 ? 1 : 0;
+        Header h{};
+        h.lastBlock = -1;
+        *headerOf(p, blockIdx.x) = h;
     }
     buildPrefix<kRows, kKeys, kThreads<FP8>>(p, s->prefix, s->scratch);
     tcFenceBefore();
@@ -547,7 +552,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             g.valid = got;
             g.tile = tile;
             if (got) {
-                g.hi = lastFirst(p, g.s, g.rp, kPairRows);
+                g.hi = lastFirstOfWarp(p, g.s, g.rp, kPairRows);
                 tile += g.last - g.first;
             }
             if (k >= kSpans) ok = mbarWait(&s->spanEmpty[k % kSpans], ((k / kSpans) - 1) & 1, &s->dead, errFlag, waitLimit, 55);
@@ -1046,9 +1051,19 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
     auto run = [&](auto kernel, int threads, size_t smem) -> cudaError_t {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
         if (e != cudaSuccess) return e;
-        kernel<<<plan.blocks, threads, smem, stream>>>(queries, pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag,
-                                                        p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
-        return cudaGetLastError();
+        // set up while the kernel before it on the stream still runs
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(plan.blocks);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kernel, queries, pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag,
+                                  p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
     };
     if (p.dtype == kFP8) {
         pool[0] = pool[1] = queries;                   // (not read)
