@@ -306,60 +306,73 @@ treeJoinKernel(const __grid_constant__ TreeParams p, int blocks, int mr, int dim
     }
 }
 
-// The same for the records of treeTcKernel, whose O is [piece of 4 columns][MR rows]: block (i, y)
-// takes rows 32 y .. + 31, a lane a row and a warp four pieces, so that the reads of a record are
-// whole lines.
+// The same for the records of treeTcKernel, whose O is [piece of 4 columns][MR rows]: block (i, y, z)
+// takes rows 32 y .. + 31 and columns 64 z .. + 63, a lane a row and a warp two pieces, so that the
+// reads of a record are whole lines.  One request of 8192 tokens leaves 18 records of each pair and
+// eight blocks with work: what counts is how many reads in a row a block waits for, so that the records
+// are read eight at a time, maxima, sums and O together, under a running maximum.
 template <typename QT, typename KT_, int MR>
 __global__ void __launch_bounds__(256)
 treeJoinColumnsKernel(const __grid_constant__ TreeParams p, int blocks) {
-    constexpr int HD = 128;
+    constexpr int HD = 128, CHUNK = 8;
     cudaGridDependencySynchronize();
     const Header h = *headerOf(p, blockIdx.x);
     if (h.lastBlock < 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rl = blockIdx.y * 32 + lane;
+    const int lane = threadIdx.x & 31, d0 = blockIdx.z * 64 + (threadIdx.x >> 5) * 8, rl = blockIdx.y * 32 + lane;
     const SeqInfo s(p, h.b);
     const int group = p.heads / p.kvHeads, rr = h.rt * MR + rl;
     if (h.rt * MR + static_cast<int>(blockIdx.y) * 32 >= s.n * group) return;
     const bool mine = rr < s.n * group;
     const int first = blockIdx.x, count = h.lastBlock - first + 1;
-    auto record = [&](int i) -> const float* { return recordOf(p, blocks, first + i, i == 0 ? 1 : 0, MR, HD); };
-    float top = -INFINITY;
     bool odd = false;
-    if (mine) {
-#pragma unroll 4
-        for (int i = 0; i < count; ++i) top = fmaxf(top, record(i)[MR * HD + rl]);
-    }
     for (int i = lane; i < count; i += 32) odd = odd || headerOf(p, first + i)->odd[i == 0 ? 1 : 0] != 0;
+    float top = -INFINITY, l = 0.f;
+    float sum[8] = {};
+    if (mine)
+        for (int i0 = 0; i0 < count; i0 += CHUNK) {
+            float m[CHUNK], part[CHUNK];
+            float4 o[CHUNK][2];
+#pragma unroll
+            for (int e = 0; e < CHUNK; ++e) {
+                m[e] = -INFINITY;
+                part[e] = 0.f;
+                o[e][0] = o[e][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i0 + e < count) {
+                    const float* r = recordOf(p, blocks, first + i0 + e, i0 + e == 0 ? 1 : 0, MR, HD);
+                    m[e] = r[MR * HD + rl];
+                    part[e] = r[MR * HD + MR + rl];
+                    for (int q = 0; q < 2; ++q) o[e][q] = reinterpret_cast<const float4*>(r)[(d0 / 4 + q) * MR + rl];
+                }
+            }
+            const float before = top;
+#pragma unroll
+            for (int e = 0; e < CHUNK; ++e) top = fmaxf(top, m[e]);
+            const float base = top == -INFINITY ? 0.f : top, keep = exp2f(before - base);
+            l *= keep;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) sum[c] *= keep;
+#pragma unroll
+            for (int e = 0; e < CHUNK; ++e) {
+                const float f = exp2f(m[e] - base);
+                l += f * part[e];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    sum[4 * q] += f * o[e][q].x;
+                    sum[4 * q + 1] += f * o[e][q].y;
+                    sum[4 * q + 2] += f * o[e][q].z;
+                    sum[4 * q + 3] += f * o[e][q].w;
+                }
+            }
+        }
     odd = __any_sync(0xFFFFFFFFu, odd);
     if (!mine) return;
-    const float base = top == -INFINITY ? 0.f : top;
-    float4 sum[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) sum[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-        const float* r = record(i);
-        const float f = exp2f(r[MR * HD + rl] - base);
-        l += f * r[MR * HD + MR + rl];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float4 o = reinterpret_cast<const float4*>(r)[(4 * warp + q) * MR + rl];
-            sum[q].x += f * o.x; sum[q].y += f * o.y; sum[q].z += f * o.z; sum[q].w += f * o.w;
-        }
-    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    QT out[16];
+    alignas(16) QT out[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const float v[4] = {sum[q].x * inv, sum[q].y * inv, sum[q].z * inv, sum[q].w * inv};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[4 * q + e] = narrow<QT>(v[e]);
-    }
+    for (int c = 0; c < 8; ++c) out[c] = narrow<QT>(sum[c] * inv);
     QT* to = static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + h.kvh * group + rr % group) * HD;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) reinterpret_cast<uint4*>(to + 16 * warp)[q] = reinterpret_cast<const uint4*>(out)[q];
-    if (odd) addLeftOut<QT, KT_>(p, s, h.b, h.kvh, rr / group, lastFirst(p, s, h.rt, MR), to, 16 * warp, 16 * warp + 16);
+    *reinterpret_cast<uint4*>(to + d0) = *reinterpret_cast<const uint4*>(out);
+    if (odd) addLeftOut<QT, KT_>(p, s, h.b, h.kvh, rr / group, lastFirst(p, s, h.rt, MR), to, d0, d0 + 8);
 }
 
 // The joining kernel may be set up while the attention kernel still runs.
@@ -383,9 +396,13 @@ cudaError_t launchJoin(const TreeParams& p, const TreePlan& plan, cudaStream_t s
     *launches += 1;
     const unsigned blocks = static_cast<unsigned>(plan.blocks - 1);
     if constexpr (sizeof(QT) == 2)
-        if (plan.variant == 2)
-            return plan.rows == 256 ? launchEarly(treeJoinColumnsKernel<QT, KT_, 256>, dim3(blocks, 8), stream, p, plan.blocks)
-                                    : launchEarly(treeJoinColumnsKernel<QT, KT_, 128>, dim3(blocks, 4), stream, p, plan.blocks);
+        if (plan.variant == 2) {
+            // (slices of rows that some request can have)
+            const int64_t rows = std::min<int64_t>(plan.rows, static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads));
+            const dim3 grid(blocks, static_cast<unsigned>((rows + 31) / 32), 2);
+            return plan.rows == 256 ? launchEarly(treeJoinColumnsKernel<QT, KT_, 256>, grid, stream, p, plan.blocks)
+                                    : launchEarly(treeJoinColumnsKernel<QT, KT_, 128>, grid, stream, p, plan.blocks);
+        }
     return launchEarly(treeJoinKernel<QT, KT_>, dim3(blocks, (plan.rows + 7) / 8), stream, p, plan.blocks, plan.rows, plan.dimPad);
 }
 
