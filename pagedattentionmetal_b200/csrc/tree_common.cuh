@@ -229,6 +229,23 @@ __device__ __noinline__ void addLeftOut(const TreeParams& p, SeqInfo s, int b, i
 
 }  // namespace tree
 
+// A launch whose blocks may be set up while the kernel before it on the stream still runs: the kernel
+// calls cudaGridDependencySynchronize() before it reads or writes anything.
+template <typename... Params, typename... Args>
+cudaError_t launchEarly(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // How a request is launched: the kernel, its tiles, the columns of a record, the blocks.
 struct TreePlan {
     int variant;       // 0: treeGeneralKernel, 1: treeMmaKernel, 2: treeTcKernel

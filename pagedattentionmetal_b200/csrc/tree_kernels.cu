@@ -36,9 +36,25 @@ struct GeneralSmem {
     }
 };
 
+// Four elements in a row, as float32.
+__device__ __forceinline__ float4 fourOf(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <typename T>
+__device__ __forceinline__ float4 fourOf(const T* p) {
+    if constexpr (sizeof(T) == 2) {
+        alignas(8) T e[4];
+        *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
+        return make_float4(valueOf(e), valueOf(e + 1), valueOf(e + 2), valueOf(e + 3));
+    } else {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+        auto one = [&](int i) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(w >> (8 * i)), __NV_E4M3))); };
+        return make_float4(one(0), one(1), one(2), one(3));
+    }
+}
+
+// wide: rows are multiples of four elements, on boundaries of four elements.
 template <typename QT, typename KT_>
 __global__ void __launch_bounds__(kGenThreads)
-treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
+treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2, bool wide) {
     extern __shared__ __align__(16) unsigned char raw[];
     const int D = p.headDim, dp = GeneralSmem::pad(D), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float* sq = reinterpret_cast<float*>(raw);             // [16][dp]
@@ -50,6 +66,7 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
     long long* blkAt = vAt + kGenKeys;                     // FP8: the block, for its scales
     int* scratch = reinterpret_cast<int*>(blkAt + 2 * kGenKeys);
     int* prefix = scratch + kGenThreads / 32 + 4;
+    cudaGridDependencySynchronize();                   // launched early, as treeTcKernel
     buildPrefix<kGenRows, kGenKeys, kGenThreads>(p, prefix, scratch);
     const int blocks = gridDim.x, me = blockIdx.x, total = prefix[p.batch];
     const int quota = (total + blocks - 1) / blocks;
@@ -66,6 +83,18 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
         const int cacheTiles = s.cacheTiles<kGenKeys>(), rows = s.n * group;
         const uint32_t hi = lastFirst(p, s, g.rt, kGenRows);
         __syncthreads();
+        const int pieces = dp / 4;
+        if (wide) {
+#pragma unroll 4
+            for (int i = tid; i < kGenRows * pieces; i += kGenThreads) {
+                const int r = i / pieces, d = 4 * (i - r * pieces), rr = g.rt * kGenRows + r;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (rr < rows && d < D)
+                    v = fourOf(static_cast<const QT*>(p.q) + static_cast<int64_t>(s.start + rr / group) * p.qStride +
+                               static_cast<int64_t>(g.kvh * group + rr % group) * D + d);
+                *reinterpret_cast<float4*>(sq + r * dp + d) = make_float4(v.x * scaleLog2, v.y * scaleLog2, v.z * scaleLog2, v.w * scaleLog2);
+            }
+        } else
         for (int i = tid; i < kGenRows * dp; i += kGenThreads) {
             const int r = i / dp, d = i - r * dp, rr = g.rt * kGenRows + r;
             float v = 0.f;
@@ -106,6 +135,47 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
                 }
             }
             __syncthreads();
+            if (wide) {
+                // Four pieces of keys and values each are on their way together: an element at a time, as
+                // below, a call of seven short requests spent most of its time on one load after another
+                // (dim 80, float32: 38.5 us, now GENERAL_FIGURE).
+                constexpr int kAhead = 4;
+                for (int i0 = tid; i0 < kGenKeys * pieces; i0 += kAhead * kGenThreads) {
+                    float4 kv[kAhead], vv[kAhead];
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) {
+                        const int i = i0 + u * kGenThreads, r = min(i / pieces, kGenKeys - 1), d = 4 * (i - r * pieces);
+                        kv[u] = vv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (i < kGenKeys * pieces && kAt[r] >= 0 && d < D) {
+                            if (inTree) {
+                                kv[u] = fourOf(static_cast<const QT*>(p.kNew) + kAt[r] + d);
+                                vv[u] = fourOf(static_cast<const QT*>(p.vNew) + vAt[r] + d);
+                            } else {
+                                kv[u] = fourOf(static_cast<const KT_*>(p.kPool) + kAt[r] + d);
+                                vv[u] = fourOf(static_cast<const KT_*>(p.vPool) + vAt[r] + d);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) {
+                        const int i = i0 + u * kGenThreads, r = i / pieces, d = 4 * (i - r * pieces);
+                        if (i >= kGenKeys * pieces) break;
+                        float ks = 1.f, vs = 1.f;
+                        if (sizeof(KT_) == 1 && !inTree && kAt[r] >= 0) {
+                            ks = __half2float(static_cast<const __half*>(p.kScale)[blkAt[r] * p.kvHeads + g.kvh]);
+                            vs = __half2float(static_cast<const __half*>(p.vScale)[blkAt[r] * p.kvHeads + g.kvh]);
+                        }
+                        float e[4] = {vv[u].x * vs, vv[u].y * vs, vv[u].z * vs, vv[u].w * vs};
+                        if (inTree || k0 + r < hi) {               // (some row may not see the key)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                if (isOdd(e[c])) { e[c] = 0.f; odd = true; }
+                        }
+                        *reinterpret_cast<float4*>(sk + r * (dp + 4) + d) = make_float4(kv[u].x * ks, kv[u].y * ks, kv[u].z * ks, kv[u].w * ks);
+                        *reinterpret_cast<float4*>(sv + r * dp + d) = make_float4(e[0], e[1], e[2], e[3]);
+                    }
+                }
+            } else
             for (int i = tid; i < kGenKeys * dp; i += kGenThreads) {
                 const int r = i / dp, d = i - r * dp;
                 float kv = 0.f, vv = 0.f;
@@ -272,28 +342,43 @@ treeJoinKernel(const __grid_constant__ TreeParams p, int blocks, int mr, int dim
     if (rl >= mr || rr >= s.n * group) return;
     const int first = blockIdx.x, count = h.lastBlock - first + 1;
     auto record = [&](int i) -> const float* { return recordOf(p, blocks, first + i, i == 0 ? 1 : 0, mr, dimPad); };
-    float top = -INFINITY;
     bool odd = false;
-    for (int i = lane; i < count; i += 32) {
-        top = fmaxf(top, record(i)[mr * dimPad + rl]);
-        odd = odd || headerOf(p, first + i)->odd[i == 0 ? 1 : 0] != 0;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    for (int i = lane; i < count; i += 32) odd = odd || headerOf(p, first + i)->odd[i == 0 ? 1 : 0] != 0;
     odd = __any_sync(0xFFFFFFFFu, odd);
-    const float base = top == -INFINITY ? 0.f : top;
     const uint32_t hi = odd ? lastFirst(p, s, h.rt, mr) : 0u;
     QT* out = static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + h.kvh * group + rr % group) * p.headDim;
     for (int d = 4 * lane; d < p.headDim; d += 128) {
+        // eight records at a time, maxima, sums and O together: a read is a long wait, and few warps share it
+        constexpr int CHUNK = 8;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-#pragma unroll 4
-        for (int i = 0; i < count; ++i) {
-            const float* r = record(i);
-            const float f = exp2f(r[mr * dimPad + rl] - base);
-            const float4 o = *reinterpret_cast<const float4*>(r + rl * dimPad + d);
-            l += f * r[mr * dimPad + mr + rl];
-            sum.x += f * o.x; sum.y += f * o.y; sum.z += f * o.z; sum.w += f * o.w;
+        float top = -INFINITY, l = 0.f;
+        for (int i0 = 0; i0 < count; i0 += CHUNK) {
+            float m[CHUNK], part[CHUNK];
+            float4 o[CHUNK];
+#pragma unroll
+            for (int e = 0; e < CHUNK; ++e) {
+                m[e] = -INFINITY;
+                part[e] = 0.f;
+                o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i0 + e < count) {
+                    const float* r = record(i0 + e);
+                    m[e] = r[mr * dimPad + rl];
+                    part[e] = r[mr * dimPad + mr + rl];
+                    o[e] = *reinterpret_cast<const float4*>(r + rl * dimPad + d);
+                }
+            }
+            const float before = top;
+#pragma unroll
+            for (int e = 0; e < CHUNK; ++e) top = fmaxf(top, m[e]);
+            const float base = top == -INFINITY ? 0.f : top, keep = exp2f(before - base);
+            l *= keep;
+            sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
+#pragma unroll
+            for (int e = 0; e < CHUNK; ++e) {
+                const float f = exp2f(m[e] - base);
+                l += f * part[e];
+                sum.x += f * o[e].x; sum.y += f * o[e].y; sum.z += f * o[e].z; sum.w += f * o[e].w;
+            }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l, v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
@@ -310,11 +395,14 @@ treeJoinKernel(const __grid_constant__ TreeParams p, int blocks, int mr, int dim
 // takes rows 32 y .. + 31 and columns 64 z .. + 63, a lane a row and a warp two pieces, so that the
 // reads of a record are whole lines.  One request of 8192 tokens leaves 18 records of each pair and
 // eight blocks with work: what counts is how many reads in a row a block waits for, so that the records
-// are read eight at a time, maxima, sums and O together, under a running maximum.
+// are read several at a time, maxima, sums and O together, under a running maximum.
 template <typename QT, typename KT_, int MR>
 __global__ void __launch_bounds__(256)
 treeJoinColumnsKernel(const __grid_constant__ TreeParams p, int blocks) {
-    constexpr int HD = 128, CHUNK = 8;
+    // (pairs of up to 256 rows fill the GPU with work by themselves: there fewer registers and more blocks
+    // win, 61.6 against 65.2 us with 8 requests of 4096 tokens and 256 rows; one request of 8192 tokens
+    // and 4 rows: 22.7 against 26.5 us)
+    constexpr int HD = 128, CHUNK = MR == 256 ? 4 : 8;
     cudaGridDependencySynchronize();
     const Header h = *headerOf(p, blockIdx.x);
     if (h.lastBlock < 0) return;
@@ -375,21 +463,6 @@ treeJoinColumnsKernel(const __grid_constant__ TreeParams p, int blocks) {
     if (odd) addLeftOut<QT, KT_>(p, s, h.b, h.kvh, rr / group, lastFirst(p, s, h.rt, MR), to, d0, d0 + 8);
 }
 
-// The joining kernel may be set up while the attention kernel still runs.
-template <typename... Kernel, typename... Args>
-cudaError_t launchEarly(void (*kernel)(Kernel...), dim3 grid, cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename QT, typename KT_>
 cudaError_t launchJoin(const TreeParams& p, const TreePlan& plan, cudaStream_t stream, int* launches) {
     if (plan.blocks < 2) return cudaSuccess;
@@ -400,10 +473,10 @@ cudaError_t launchJoin(const TreeParams& p, const TreePlan& plan, cudaStream_t s
             // (slices of rows that some request can have)
             const int64_t rows = std::min<int64_t>(plan.rows, static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads));
             const dim3 grid(blocks, static_cast<unsigned>((rows + 31) / 32), 2);
-            return plan.rows == 256 ? launchEarly(treeJoinColumnsKernel<QT, KT_, 256>, grid, stream, p, plan.blocks)
-                                    : launchEarly(treeJoinColumnsKernel<QT, KT_, 128>, grid, stream, p, plan.blocks);
+            return plan.rows == 256 ? launchEarly(treeJoinColumnsKernel<QT, KT_, 256>, grid, 256, 0, stream, p, plan.blocks)
+                                    : launchEarly(treeJoinColumnsKernel<QT, KT_, 128>, grid, 256, 0, stream, p, plan.blocks);
         }
-    return launchEarly(treeJoinKernel<QT, KT_>, dim3(blocks, (plan.rows + 7) / 8), stream, p, plan.blocks, plan.rows, plan.dimPad);
+    return launchEarly(treeJoinKernel<QT, KT_>, dim3(blocks, (plan.rows + 7) / 8), 256, 0, stream, p, plan.blocks, plan.rows, plan.dimPad);
 }
 
 // Dynamic shared memory above 48 KB has to be allowed once per device and kernel.
@@ -447,8 +520,10 @@ cudaError_t launchGeneral(const TreeParams& p, const TreePlan& plan, cudaStream_
     cudaError_t e = allowSmem(treeGeneralKernel<QT, KT_>, 227 * 1024, done);
     if (e != cudaSuccess) return e;
     const float scaleLog2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.headDim));
-    treeGeneralKernel<QT, KT_><<<plan.blocks, kGenThreads, GeneralSmem::bytes(p.headDim, p.batch), stream>>>(p, scaleLog2);
-    return cudaGetLastError();
+    bool wide = p.headDim % 4 == 0 && p.qStride % 4 == 0 && p.kStride % 4 == 0 && p.vStride % 4 == 0;
+    for (const void* rows : {p.q, p.kNew, p.vNew}) wide = wide && reinterpret_cast<uintptr_t>(rows) % (4 * sizeof(QT)) == 0;
+    for (const void* pool : {p.kPool, p.vPool}) wide = wide && reinterpret_cast<uintptr_t>(pool) % (4 * sizeof(KT_)) == 0;
+    return launchEarly(treeGeneralKernel<QT, KT_>, dim3(plan.blocks), kGenThreads, GeneralSmem::bytes(p.headDim, p.batch), stream, p, scaleLog2, wide);
 }
 
 template <typename QT, typename KT_>

@@ -120,6 +120,7 @@ treeMmaKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rowGroup = warp % S::kRowGroups, keyGroup = warp / S::kRowGroups;
     const int gr = lane >> 2, gc = lane & 3;
+    cudaGridDependencySynchronize();                      // launched early, as treeTcKernel
     buildPrefix<MR, kKeys, kThreads>(p, prefix, scratch);
     const int blocks = gridDim.x, me = blockIdx.x, total = prefix[p.batch];
     const int quota = (total + blocks - 1) / blocks;
@@ -533,8 +534,7 @@ cudaError_t launchOne(const TreeParams& p, int blocks, float scaleLog2, cudaStre
         if (e != cudaSuccess) return e;
         done.fetch_or(bit, std::memory_order_relaxed);
     }
-    treeMmaKernel<T, HD, MR, FP8><<<blocks, kThreads, S::bytes(p.batch), stream>>>(p, scaleLog2);
-    return cudaGetLastError();
+    return launchEarly(treeMmaKernel<T, HD, MR, FP8>, dim3(blocks), kThreads, S::bytes(p.batch), stream, p, scaleLog2);
 }
 
 template <typename T, bool FP8>

@@ -1051,19 +1051,8 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
     auto run = [&](auto kernel, int threads, size_t smem) -> cudaError_t {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
         if (e != cudaSuccess) return e;
-        // set up while the kernel before it on the stream still runs
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(plan.blocks);
-        cfg.blockDim = dim3(threads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = stream;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, kernel, queries, pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2, p.errFlag,
-                                  p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
+        return launchEarly(kernel, dim3(plan.blocks), threads, smem, stream, queries, pool[0], pool[1], fresh[0], fresh[1], p, scaleLog2,
+                           p.errFlag, p.waitCycles > 0 ? p.waitCycles : kWaitCycles);
     };
     if (p.dtype == kFP8) {
         pool[0] = pool[1] = queries;                   // (not read)
