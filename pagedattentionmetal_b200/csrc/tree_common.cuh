@@ -251,11 +251,15 @@ struct TreePlan {
     int variant;       // 0: treeGeneralKernel, 1: treeMmaKernel, 2: treeTcKernel
     int rows, keys, dimPad, blocks;
 };
+// Each of the two: whether it takes such sizes and types at all (its workspace is counted then), and
+// whether it takes the request, buffers and strides included.
 // tree_mma_kernel.cu: 16-bit and FP8 pools, head_dim up to 128, everything on 16 bytes.
+bool treeMmaSizes(const TreeParams& p);
 bool treeMmaApplies(const TreeParams& p);
 TreePlan treeMmaPlan(const TreeParams& p, int smCount);
 cudaError_t launchTreeMma(const TreeParams& p, const TreePlan& plan, cudaStream_t stream);
-// tree_tc_kernel.cu: 16-bit pools, head_dim 128, block sizes that are multiples of 16.
+// tree_tc_kernel.cu: 16-bit and FP8 pools, head_dim 64, 80, ... 128, block sizes that are multiples of 16.
+bool treeTcSizes(const TreeParams& p);
 bool treeTcApplies(const TreeParams& p);
 TreePlan treeTcPlan(const TreeParams& p, int smCount);
 cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t stream);

@@ -410,6 +410,7 @@ treeJoinColumnsKernel(const __grid_constant__ TreeParams p, int blocks) {
     const SeqInfo s(p, h.b);
     const int group = p.heads / p.kvHeads, rr = h.rt * MR + rl;
     if (h.rt * MR + static_cast<int>(blockIdx.y) * 32 >= s.n * group) return;
+    if (d0 >= p.headDim) return;
     const bool mine = rr < s.n * group;
     const int first = blockIdx.x, count = h.lastBlock - first + 1;
     bool odd = false;
@@ -458,7 +459,7 @@ treeJoinColumnsKernel(const __grid_constant__ TreeParams p, int blocks) {
     alignas(16) QT out[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c) out[c] = narrow<QT>(sum[c] * inv);
-    QT* to = static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + h.kvh * group + rr % group) * HD;
+    QT* to = static_cast<QT*>(p.out) + (static_cast<int64_t>(s.start + rr / group) * p.heads + h.kvh * group + rr % group) * p.headDim;
     *reinterpret_cast<uint4*>(to + d0) = *reinterpret_cast<const uint4*>(out);
     if (odd) addLeftOut<QT, KT_>(p, s, h.b, h.kvh, rr / group, lastFirst(p, s, h.rt, MR), to, d0, d0 + 8);
 }
@@ -504,8 +505,17 @@ TreePlan generalPlan(const TreeParams& p, int smCount) {
     return t;
 }
 
+// The tcgen05 kernel wherever it applies: at 32 requests of 4096 tokens (head_dim 128) and 4, 64 and 256
+// rows under a KV head 100, 110 and 185 us against 134, 237 and 867 us of the mma kernel, on short lists too, with one request of 8192
+// tokens, 23, 23 and 34 against 23, 34 and 68.  But a call that cannot have work for every block, and few rows, is over
+// sooner in the kernel with the shorter way from start to end (1024 tokens, 4 rows: 12.6 against 15.9 us).
+bool shortCall(const TreeParams& p, int smCount) {
+    const int64_t tiles = static_cast<int64_t>(p.batch) * p.kvHeads * ((static_cast<int64_t>(p.maxNumBlocks) * p.blockSize + 127) / 128 + 1);
+    return static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) <= 16 && tiles <= smCount;
+}
+
 TreePlan treePlan(const TreeParams& p, int smCount) {
-    if (treeTcApplies(p)) return treeTcPlan(p, smCount);
+    if (treeTcApplies(p) && !(shortCall(p, smCount) && treeMmaApplies(p))) return treeTcPlan(p, smCount);
     if (treeMmaApplies(p)) return treeMmaPlan(p, smCount);
     return generalPlan(p, smCount);
 }
@@ -545,8 +555,8 @@ int64_t treeTileBound(const TreeParams& p) {
 size_t treeWorkspaceBytes(const TreeParams& p, int smCount) {
     // by sizes and types alone: alignment may change between the query and the call (staged copies)
     size_t n = planBytes(generalPlan(p, smCount));
-    if (p.dtype != kF32 && p.headDim <= 128) n = std::max(n, planBytes(treeMmaPlan(p, smCount)));
-    if (p.dtype != kF32 && p.headDim == 128) n = std::max(n, planBytes(treeTcPlan(p, smCount)));
+    if (treeMmaSizes(p)) n = std::max(n, planBytes(treeMmaPlan(p, smCount)));
+    if (treeTcSizes(p)) n = std::max(n, planBytes(treeTcPlan(p, smCount)));
     return n;
 }
 

@@ -551,10 +551,13 @@ cudaError_t launchShape(const TreeParams& p, const TreePlan& plan, float scaleLo
 
 }  // namespace
 
-bool treeMmaApplies(const TreeParams& p) {
-    if (p.dtype == kF32 || p.headDim > 128) return false;
+bool treeMmaSizes(const TreeParams& p) {
     // 16-byte pieces: of codes 16 dims, of 16-bit values 8
-    if (p.headDim % (p.dtype == kFP8 ? 16 : 8)) return false;
+    return p.dtype != kF32 && p.headDim <= 128 && p.headDim % (p.dtype == kFP8 ? 16 : 8) == 0;
+}
+
+bool treeMmaApplies(const TreeParams& p) {
+    if (!treeMmaSizes(p)) return false;
     for (int64_t s : {p.qStride, p.kStride, p.vStride})
         if (s % 8) return false;
     for (const void* ptr : {p.q, p.kNew, p.vNew, p.kPool, p.vPool, static_cast<const void*>(p.out)})

@@ -228,6 +228,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.heads / p.kvHeads;
+    const int D = p.headDim, dimBlocks = D > 64 ? 2 : 1;     // blocks of 64 dims; the second one's end is filled with zeros
     if (threadIdx.x == 0) {
         mbarInit(&s->qFull, kRows % group == 0 ? 1 : kRows);
         mbarInit(&s->qEmpty, 1);
@@ -287,7 +288,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         int gt = 0;                          // tiles of the block's piece so far
         bool ok = true;
         if constexpr (FP8) {
-            // One warp for keys and values: pages of 16 rows, 2 KB of codes each, keys before values in
+            // One warp for keys and values: pages of 16 rows, 2 KB of codes each (head_dim 128), keys before values in
             // one ring, and the tile's scales, which the ring of eight keeps until the softmax is through:
             // behind the ring of codes this warp is at most five tiles ahead of it.  (The rows of a tree are
             // fetched by the converting warps; their tiles take part in the ring, empty.)  Lane i has page
@@ -320,7 +321,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 for (int j = g.first; j < g.last && ok; ++j, ++gt) {
                     const bool inTree = j >= g.cacheTiles;
                     const int t16 = (static_cast<int>(g.s.lo / kKeys) + j) * (kKeys / 16) + (lane & 7);
-                    const int64_t from = (pair * p.blockSize + (t16 % tilesPerPage) * 16) * kHd;
+                    const int64_t from = (pair * p.blockSize + (t16 % tilesPerPage) * 16) * D;
                     const float ks = __half2float(ksNext), vs = __half2float(vsNext);
                     if (j + 1 < end) {
                         pair = pairOf(g, nextBlk);
@@ -343,11 +344,11 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         __syncwarp();
                         if (lane == 0) {
                             if (inTree) mbarArrive(&s->rawFull[st]);
-                            else mbarExpectTx(&s->rawFull[st], kKeys * kHd);
+                            else mbarExpectTx(&s->rawFull[st], kKeys * D);
                         }
                         __syncwarp();
                         if (!inTree && lane < kKeys / 16)
-                            bulkLoad(s->raw[st] + lane * 2048, static_cast<const unsigned char*>(h ? p.vPool : p.kPool) + from, 2048, &s->rawFull[st]);
+                            bulkLoad(s->raw[st] + lane * 16 * D, static_cast<const unsigned char*>(h ? p.vPool : p.kPool) + from, 16 * D, &s->rawFull[st]);
                     }
                 }
                 spanDone(k);
@@ -373,16 +374,16 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                     if (gt >= S::kKStages) ok = mbarWait(&s->kEmpty[st], ((gt / S::kKStages) - 1) & 1, &s->dead, errFlag, waitLimit, 41);
                     ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) break;
-                    if (lane == 0) mbarExpectTx(&s->kFull[st], kTileBytes);
+                    if (lane == 0) mbarExpectTx(&s->kFull[st], dimBlocks * kHalfBytes);
                     __syncwarp();
                     unsigned char* to = s->k[st];
                     if (inTree) {
-                        if (lane < 2)
+                        if (lane < dimBlocks)
                             for (int h = 0; h < 2; ++h)        // (a box is 64 rows)
                                 tmaLoad3d(to + lane * kHalfBytes + h * kVBlockBytes, fresh, &s->kFull[st], 64 * lane, g.kvh, freshRow + 64 * h);
                     } else if (lane < kKeys / 16) {
                         tmaLoad2d(to + lane * 2048, pool, &s->kFull[st], 0, row);
-                        tmaLoad2d(to + kHalfBytes + lane * 2048, pool, &s->kFull[st], 64, row);
+                        if (dimBlocks == 2) tmaLoad2d(to + kHalfBytes + lane * 2048, pool, &s->kFull[st], 64, row);
                     }
                 } else {
 #pragma unroll
@@ -391,14 +392,14 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         if (n >= S::kVStages) ok = mbarWait(&s->vEmpty[st], ((n / S::kVStages) - 1) & 1, &s->dead, errFlag, waitLimit, 42);
                         ok = __all_sync(0xFFFFFFFFu, ok);
                         if (!ok) break;
-                        if (lane == 0) mbarExpectTx(&s->vFull[st], kVHalfBytes);
+                        if (lane == 0) mbarExpectTx(&s->vFull[st], dimBlocks * kVBlockBytes);
                         __syncwarp();
                         unsigned char* to = s->v[st];
                         if (inTree) {
-                            if (lane < 2) tmaLoad3d(to + lane * kVBlockBytes, fresh, &s->vFull[st], 64 * lane, g.kvh, freshRow + 64 * h);
+                            if (lane < dimBlocks) tmaLoad3d(to + lane * kVBlockBytes, fresh, &s->vFull[st], 64 * lane, g.kvh, freshRow + 64 * h);
                         } else if (lane >> 2 == h) {
                             tmaLoad2d(to + (lane & 3) * 2048, pool, &s->vFull[st], 0, row);
-                            tmaLoad2d(to + kVBlockBytes + (lane & 3) * 2048, pool, &s->vFull[st], 64, row);
+                            if (dimBlocks == 2) tmaLoad2d(to + kVBlockBytes + (lane & 3) * 2048, pool, &s->vFull[st], 64, row);
                         }
                     }
                 }
@@ -411,7 +412,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         const bool leader = electOne();
         const uint32_t fmt = BF16 ? 1u : 0u;
         const uint32_t idescS = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-        const uint32_t idescO = idescS | (1u << 16);
+        // (of one block of dims: N = 64)
+        const uint32_t idescO = ((1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(dimBlocks * 64 / 8) << 17) | ((128u >> 4) << 24)) | (1u << 16);
         const uint32_t hiK = descHi(1024);
         bool ok = true;
         // The steps of the stream, in order: a tile of a dual span is one step of each group, else tiles
@@ -477,7 +479,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 }
                 if (leader) {
 #pragma unroll
-                    for (int ks = 0; ks < kHd / 16; ++ks) umma(dS, dq[ks], dk[ks], idescS, ks > 0);
+                    for (int ks = 0; ks < kHd / 16; ++ks)
+                        if (ks < 4 || dimBlocks == 2) umma(dS, dq[ks], dk[ks], idescS, ks > 0);
                     ummaCommit(&s->sFull[n.x]);
                     if (n.endsTile()) ummaCommit(&s->kEmpty[st]);
                     if (n.closesSpan()) ummaCommit(&s->qEmpty);
@@ -578,16 +581,18 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         // codes of a row at a time.  Eight lanes read eight pieces, of row r left of the middle and of row
         // r ^ 1 right of it: their writes then fall on eight different bank groups too.
         const int piece = lane & 7, rowIn = (lane >> 3) ^ (piece >> 2);
-        const unsigned rawAt = static_cast<unsigned>((warp & 3) * 4096 + rowIn * 128 + piece * 16);
+        const unsigned rawAt = static_cast<unsigned>(((warp & 3) * 32 + rowIn) * D + piece * 16);
         const unsigned outAt = static_cast<unsigned>(rowIn * 128 + ((((2 * piece) & 7) ^ rowIn) << 4));
         auto convert = [&](const unsigned char* from, unsigned char* to, int block) {
+            if (piece >= 4 * dimBlocks) return;
+            const bool there = piece * 16 < D;
             from += rawAt;
             to += (piece >> 2) * block;
 #pragma unroll
             for (int i0 = 0; i0 < 8; i0 += 4) {
                 uint4 w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(from + (i0 + i) * 512);
+                for (int i = 0; i < 4; ++i) w[i] = there ? *reinterpret_cast<const uint4*>(from + (i0 + i) * 4 * D) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     unsigned char* row = to + (i0 + i) * 512;
@@ -613,8 +618,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 if (!inTree) convert(s->raw[st], s->k[ks] + (warp & 3) * 4096, kHalfBytes);
                 mbarArrive(&s->rawEmpty[st]);
                 if (inTree && t == 0) {
-                    mbarExpectTx(&s->kFull[ks], kTileBytes);
-                    for (int i = 0; i < 4; ++i)      // (a box is 64 rows of 64 dims)
+                    mbarExpectTx(&s->kFull[ks], dimBlocks * kHalfBytes);
+                    for (int i = 0; i < 2 * dimBlocks; ++i)      // (a box is 64 rows of 64 dims)
                         tmaLoad3d(s->k[ks] + (i >> 1) * kHalfBytes + (i & 1) * kVBlockBytes, &mapKNew, &s->kFull[ks], 64 * (i >> 1), g.kvh, freshRow + 64 * (i & 1));
                 } else {
                     mbarArrive(&s->kFull[ks]);
@@ -626,8 +631,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 if (!inTree) convert(s->raw[st], s->v[vs] + (warp & 1) * 4096, kVBlockBytes);
                 mbarArrive(&s->rawEmpty[st]);
                 if (inTree && (t & 63) == 0) {
-                    mbarExpectTx(&s->vFull[vs], kVHalfBytes);
-                    for (int i = 0; i < 2; ++i)
+                    mbarExpectTx(&s->vFull[vs], dimBlocks * kVBlockBytes);
+                    for (int i = 0; i < dimBlocks; ++i)
                         tmaLoad3d(s->v[vs] + i * kVBlockBytes, &mapVNew, &s->vFull[vs], 64 * i, g.kvh, freshRow + 64 * half);
                 } else {
                     mbarArrive(&s->vFull[vs]);
@@ -652,9 +657,9 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 // for each half (rows behind the request's belong to others and are not used)
                 if (first) {
                     const int node = g.rp * (kPairRows / group), tiles = WIDE && g.dual ? 2 : 1;
-                    mbarExpectTx(&s->qFull, tiles * kTileBytes);
+                    mbarExpectTx(&s->qFull, tiles * dimBlocks * kHalfBytes);
                     for (int i = 0; i < 2 * tiles; ++i)
-                        tmaLoad3d(s->q[i >> 1] + (i & 1) * kHalfBytes, &mapQ, &s->qFull, 64 * (i & 1), g.kvh * group,
+                        if (dimBlocks == 2 || !(i & 1)) tmaLoad3d(s->q[i >> 1] + (i & 1) * kHalfBytes, &mapQ, &s->qFull, 64 * (i & 1), g.kvh * group,
                                   g.s.start + node + (i >> 1) * (kRows / group));
                 }
                 return;
@@ -664,12 +669,13 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 if (i > 0 && !g.dual) break;
                 // every lane looks its row up; half a warp then copies a row, 16 bytes a lane
                 const int rr = g.rp * kPairRows + i * kRows + t;
-                const int64_t off = rr < g.rows ? static_cast<int64_t>(g.s.start + rr / group) * p.qStride + static_cast<int64_t>(g.kvh * group + rr % group) * kHd : -1;
+                const int64_t off = rr < g.rows ? static_cast<int64_t>(g.s.start + rr / group) * p.qStride + static_cast<int64_t>(g.kvh * group + rr % group) * D : -1;
                 const int c = lane & 15;
 #pragma unroll 4
                 for (int r = 0; r < 16; ++r) {
                     const int in = 2 * r + (lane >> 4), row = (warp & 3) * 32 + in;
-                    const int64_t at = __shfl_sync(0xFFFFFFFFu, off, in);
+                    int64_t at = __shfl_sync(0xFFFFFFFFu, off, in);
+                    if (c * 8 >= D) at = -1;
                     const uint32_t dst = smemAddr(s->q[i]) + row * 128 + (c >> 3) * kHalfBytes + (((c & 7) ^ (row & 7)) << 4);
                     const int n = at >= 0 ? 16 : 0;
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(static_cast<const T*>(p.q) + (at >= 0 ? at + c * 8 : 0)), "r"(n) : "memory");
@@ -731,7 +737,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 a0 *= inv;
                 a1 *= inv;
-                T* out = static_cast<T*>(p.out) + (mine ? (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * kHd : 0);
+                T* out = static_cast<T*>(p.out) + (mine ? (static_cast<int64_t>(g.s.start + rr / group) * p.heads + g.kvh * group + rr % group) * D : 0);
                 float4* recO = reinterpret_cast<float4*>(rec) + rl;
                 const bool both = !g.dual && has1;
                 const unsigned long long scale0 = pack2(a0, a0), scale1 = pack2(a1, a1);
@@ -739,7 +745,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 // whose fetches compete with the softmax warps' long loop.  Trading pieces among lanes for
                 // wider segments of a row made the loop longer and 1.5 times slower.)
 #pragma unroll 1
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < D / 16; ++c) {
                     uint32_t o[16], u[16];
                     tmemLd16NoWait(tmemO(x) + laneBase + 16u * c, o);
                     if (both) tmemLd16NoWait(tmemO(1) + laneBase + 16u * c, u);
@@ -773,7 +779,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                     __syncwarp();
                 }
                 if (whole && odd && mine)
-                    addLeftOut<T, PoolT>(p, g.s, g.b, g.kvh, rr / group, g.hi, out, 0, kHd);
+                    addLeftOut<T, PoolT>(p, g.s, g.b, g.kvh, rr / group, g.hi, out, 0, D);
                 __syncwarp();
                 if (!whole && mine) {
                     rec[kPairRows * kHd + rl] = m;
@@ -941,14 +947,14 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
                         uint32_t carry = 0;
 #pragma unroll 4
-                        for (int c = 0; c < 16; ++c) {
+                        for (int c = 0; c < 8 * dimBlocks; ++c) {
                             // (lane by lane another piece of the row first: no two on one bank)
                             const uint4 w = *reinterpret_cast<const uint4*>(s->v[st] + (c >> 3) * kVBlockBytes + (t & 63) * 128 + (((c ^ t) & 7) << 4));
                             carry |= ((w.x & kExp) + kOne) | ((w.y & kExp) + kOne) | ((w.z & kExp) + kOne) | ((w.w & kExp) + kOne);
                         }
                         if (carry & 0x80008000u) {
 #pragma unroll 1
-                            for (int c = 0; c < 128; ++c) {
+                            for (int c = 0; c < 64 * dimBlocks; ++c) {
                                 unsigned short* at = reinterpret_cast<unsigned short*>(s->v[st] + (c >> 6) * kVBlockBytes + (t & 63) * 128 + (c & 63) * 2);
                                 if ((*at & kExp & 0xFFFFu) == (kExp & 0xFFFFu)) *at = 0;
                             }
@@ -984,8 +990,12 @@ done:
 
 }  // namespace
 
+bool treeTcSizes(const TreeParams& p) {
+    return p.dtype != kF32 && p.headDim >= 64 && p.headDim <= kHd && p.headDim % 16 == 0 && p.blockSize % 16 == 0;
+}
+
 bool treeTcApplies(const TreeParams& p) {
-    if (p.dtype == kF32 || p.headDim != kHd || p.blockSize % 16 != 0) return false;
+    if (!treeTcSizes(p)) return false;
     if (p.dtype == kFP8 && smemBytes<false, true>(p.batch) > kSmemLimit) return false;
     // (rows of the pool are counted in 32 bits)
     if (p.poolBlocks <= 0 || p.poolBlocks >= (1 << 30) / (p.kvHeads * p.blockSize)) return false;
@@ -1017,13 +1027,14 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
     EncodeFn encode = encodeFn();
     if (!encode) return cudaErrorNotSupported;
     const CUtensorMapDataType dt = p.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint64_t D = p.headDim;
     CUtensorMap queries, pool[2], fresh[2];
     {
         // queries: [row][head][128]; a box is 64 dims x the heads of a KV head x 128 rows' worth of nodes
         // (used when the group divides 128; else any valid box)
         const int group = p.heads / p.kvHeads, nodes = kRows % group == 0 ? kRows / group : 1, heads = kRows % group == 0 ? group : 1;
-        const cuuint64_t dims[3] = {kHd, static_cast<cuuint64_t>(p.heads), static_cast<cuuint64_t>(p.numRows)};
-        const cuuint64_t strides[2] = {kHd * 2, static_cast<cuuint64_t>(p.qStride) * 2};
+        const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(p.heads), static_cast<cuuint64_t>(p.numRows)};
+        const cuuint64_t strides[2] = {D * 2, static_cast<cuuint64_t>(p.qStride) * 2};
         const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(heads), static_cast<cuuint32_t>(nodes)}, one[3] = {1, 1, 1};
         if (encode(&queries, dt, 3, const_cast<void*>(p.q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
@@ -1032,22 +1043,22 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
     for (int which = 0; which < 2; ++which) {
         if (p.dtype != kFP8) {
         // pools: [block * kv_head * slot][128]; a box is 64 dims x 16 rows (half of a 16-token piece)
-        const cuuint64_t dims[2] = {kHd, static_cast<cuuint64_t>(p.poolBlocks) * p.kvHeads * p.blockSize};
-        const cuuint64_t strides[1] = {kHd * 2};
+        const cuuint64_t dims[2] = {D, static_cast<cuuint64_t>(p.poolBlocks) * p.kvHeads * p.blockSize};
+        const cuuint64_t strides[1] = {D * 2};
         const cuuint32_t box[2] = {64, 16}, one[2] = {1, 1};
         if (encode(&pool[which], dt, 2, const_cast<void*>(which ? p.vPool : p.kPool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
         }
         // the step's rows: [row][kv_head][128]; a box is 64 dims x 1 head x 64 rows (rows behind the last: zeros)
-        const cuuint64_t fdims[3] = {kHd, static_cast<cuuint64_t>(p.kvHeads), static_cast<cuuint64_t>(p.numRows)};
-        const cuuint64_t fstrides[2] = {kHd * 2, static_cast<cuuint64_t>(which ? p.vStride : p.kStride) * 2};
+        const cuuint64_t fdims[3] = {D, static_cast<cuuint64_t>(p.kvHeads), static_cast<cuuint64_t>(p.numRows)};
+        const cuuint64_t fstrides[2] = {D * 2, static_cast<cuuint64_t>(which ? p.vStride : p.kStride) * 2};
         const cuuint32_t fbox[3] = {64, 1, 64}, fone[3] = {1, 1, 1};
         if (encode(&fresh[which], dt, 3, const_cast<void*>(which ? p.vNew : p.kNew), fdims, fstrides, fbox, fone, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
     }
-    const float scaleLog2 = 1.4426950408889634f / sqrtf(static_cast<float>(kHd));
+    const float scaleLog2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.headDim));
     auto run = [&](auto kernel, int threads, size_t smem) -> cudaError_t {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
         if (e != cudaSuccess) return e;

@@ -150,6 +150,10 @@ SHAPES = {
     "no groups": dict(lens=[70, 300], sizes=[9, 33], heads=4, kv_heads=4),
     "dim 64": dict(lens=[70, 300], sizes=[9, 33], dim=64),
     "dim 80": dict(lens=[70, 300], sizes=[9, 3], dim=80),
+    "dim 64, long": dict(lens=[2100, 300, 0], sizes=[40, 9, 65], dim=64),
+    "dim 80, seven heads a group": dict(lens=[270, 900], sizes=[9, 30], dim=80, heads=14, kv_heads=2),
+    "dim 96": dict(lens=[270, 1000, 17], sizes=[33, 5, 40], dim=96),
+    "dim 112, strided": dict(lens=[270, 1000, 17], sizes=[33, 5, 64], dim=112, strided=True),
     "dim 33": dict(lens=[70, 20], sizes=[9, 3], dim=33),
     "dim 256": dict(lens=[70, 200], sizes=[9, 3], dim=256),
     "blocks of 8": dict(lens=[70, 300], sizes=[9, 20], block=8),
@@ -216,9 +220,10 @@ def test_masks_that_leave_rows_empty(engine, dtype):
 @pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("window", [0, 90])
 @pytest.mark.parametrize("lens", [[100, 0], [3000, 64]])
-def test_values_a_row_does_not_see_do_not_reach_it(engine, dtype, what, window, lens):
+@pytest.mark.parametrize("dim", [128, 80, 64])
+def test_values_a_row_does_not_see_do_not_reach_it(engine, dtype, what, window, lens, dim):
     """A node's values that are not finite reach the rows that see it and no others; so at the edge of a window."""
-    case = TreeCase(36, lens, [40, 70], dtype=dtype, window=window)
+    case = TreeCase(36, lens, [40, 70], dtype=dtype, window=window, dim=dim)
     bad = to_storage(np.full(1, what, np.float32), dtype)[0]
     case.v[case.starts[0] + 7, :, 3::5] = bad
     case.v[case.starts[1] + 30, 1, :] = bad
@@ -228,6 +233,30 @@ def test_values_a_row_does_not_see_do_not_reach_it(engine, dtype, what, window, 
             case.v_pool[case.tables[0, t // 16], 0, t % 16, ::7] = bad
     out = case.check(engine, finite=False)
     assert np.isfinite(out[case.starts[0]:case.starts[2]]).any() and not np.isfinite(out[case.starts[2] - 1]).any()
+
+
+@pytest.mark.parametrize("dim", [128, 80, 64])
+@pytest.mark.parametrize("window", [0, 90])
+def test_values_a_row_does_not_see_behind_float8_pages(engine, dim, window):
+    """The same for float16 rows behind a float8 cache, whose codes know NaN (0x7f) as well."""
+    lens = [300, 64]
+    case = TreeCase(46, lens, [40, 70], dtype=DT.float8, window=window, dim=dim)
+    bad = to_storage(np.full(1, np.inf, np.float32), DT.float16)[0]
+    case.v[case.starts[0] + 7, :, 3::5] = bad
+    case.v[case.starts[1] + 69] = bad
+    if window:
+        for t in range(lens[0] + 1 - window, lens[0] + 3 - window):
+            case.v_pool[case.tables[0, t // 16], 0, t % 16, ::7] = 0x7F
+    out = case.check(engine, finite=False)
+    assert np.isfinite(out[case.starts[0]:case.starts[2]]).any() and not np.isfinite(out[case.starts[2] - 1]).any()
+
+
+def test_float8_scales_of_zero(engine):
+    """Pages whose scale is zero: keys that all score alike, values that are zero."""
+    case = TreeCase(47, [300, 64], [40, 9], dtype=DT.float8)
+    case.k_scale[::3] = 0
+    case.v_scale[1::3] = 0
+    case.check(engine)
 
 
 @pytest.mark.parametrize("dtype", [DT.float32, DT.float16, DT.bfloat16], ids=lambda d: d.name)
@@ -303,6 +332,22 @@ def test_host_buffers_and_workspace(engine):
     request.kPool = case.k_pool
     with pytest.raises(pam.PagedAttentionError, match="device memory"):
         engine.treeAttention(request)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda d: d.name)
+@pytest.mark.parametrize("dim", [33, 64, 80, 96, 128, 256])
+@pytest.mark.parametrize("size", [1, 12, 40, 70])
+def test_workspace_is_as_large_as_it_says(engine, dtype, dim, size):
+    """The bytes behind the workspace stay as they are.  (They are there: a kernel that wrote them would harm nobody.)"""
+    case = TreeCase(48, [2100, 40, 3], [size, 1, size], dtype=dtype, dim=dim)
+    out = engine.makeBufferFrom(np.zeros(case.q.shape, case.q.dtype))
+    request = case.request(engine, out)
+    need, behind = engine.treeAttentionWorkspace(request), 32 << 20
+    memory = engine.makeBufferFrom(np.full(need + behind, 0x5A, np.uint8))
+    from pagedattentionmetal_b200 import _cabi
+    request.workspace = _cabi.PamBuffer(memory.ptr, need)
+    engine.treeAttention(request)
+    assert (memory.download(np.uint8, (behind,), need) == 0x5A).all()
 
 
 def test_failed_launches_degrade_like_a_decode(engine):
