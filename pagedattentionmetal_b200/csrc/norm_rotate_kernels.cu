@@ -435,16 +435,24 @@ cudaError_t normRotateOf(const NormRotateParams& p, cudaStream_t stream, int* la
 
 // ---- backward ---------------------------------------------------------------
 
-constexpr int kBackwardRows = 8;         // rows that a block looks up at a time
+constexpr int kBackwardRows = 32;        // rows that a block looks up at a time
+constexpr int kBackwardShare = 4;        // rows that a block has at least
+constexpr int kBackwardStages = 3;       // rows in shared memory or on their way there
+
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void copyAhead(void* to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
 
 // As the forward kernel, every block with an equal share of the rows.  A group of lanes keeps one head
 // of a row and each lane its pieces of it, so that its share of the weight gradients stays in
 // registers over all its rows; then the groups of the queries and those of the keys are summed through
 // shared memory in a fixed order and the block writes its [2][dim] partial sums: no atomics, the same
-// bits for the same grid.  Measured at 8192 rows of 32 + 8 heads of 128, bfloat16 (252 MB): 76 us =
-// 3.3 TB/s, 0.51 of the copy rate: bound by the issue of some 250 instructions per 16 elements and by
-// the registers that hold the next row (96, two blocks on an SM); four blocks 91 us, 8-byte pieces
-// 128 us, a row at a time 137 us.
+// bits for the same grid.  Rows come to shared memory by asynchronous copies, two ahead, each thread its
+// own pieces, so that no registers wait for them and no barrier stands in the loop.  Measured at 8192
+// rows of 32 + 8 heads of 128, bfloat16 (252 MB): 55.5 us = 4.5 TB/s, 0.69 of the copy rate, bound by the
+// issue of some 250 instructions per 16 elements; one row ahead in registers, with look-ups for 8 rows at
+// a time, 76 us; three rows ahead 55.5 us; 80 registers, with spills, 61 us; four blocks on an SM 59 us.
 template <typename T, int BYTES>
 __global__ void __maxnreg__(96)
 normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, const Layout l, int share) {
@@ -452,8 +460,10 @@ normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, con
     constexpr int E = P::E;
     extern __shared__ __align__(16) unsigned char rowSmem[];
     const int tid = threadIdx.x, half = p.rotaryDim / 2, threads = blockDim.x;
-    float* sums = reinterpret_cast<float*>(rowSmem);                      // [threads][2 E]
-    RowInfo* info = reinterpret_cast<RowInfo*>(sums + (p.partials ? threads * 2 * E : 0));                // [kBackwardRows]
+    unsigned char* ring = rowSmem;                                        // [kBackwardStages][4][threads][16]
+    float* sums = reinterpret_cast<float*>(rowSmem);                      // [threads][2 E], behind the loop
+    static_assert(2 * E * sizeof(float) <= kBackwardStages * 4 * 16, "the sums take the place of the rows");
+    RowInfo* info = reinterpret_cast<RowInfo*>(ring + kBackwardStages * 4 * 16 * threads);                // [kBackwardRows]
     float* turns = reinterpret_cast<float*>(info + kBackwardRows);        // [kBackwardRows][rotaryDim]
     const int lane = tid & (l.lanes - 1), group = tid / l.lanes, groups = threads / l.lanes;
     const int perRow = p.heads + p.kvHeads + (p.dV ? p.kvHeads : 0);
@@ -489,27 +499,36 @@ normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, con
             const int n = static_cast<int>(min(static_cast<int64_t>(kBackwardRows), end - row0));
             __syncthreads();
             lookRowsUp(info, turns, row0, n, p.positions, p.slots, p.numSlots, p.invFreq, half, p.kvHeads, p.blockSize, p.headDim);
-            struct Row { P xa, xb, ya, yb; };
-            auto load = [&](int r) {
-                Row w;
-                if (!wanted || !hasA || r >= n || info[r].position < 0) return w;
-                if (!isV) {
-                    const T* at = src + (row0 + r) * srcStride;
-                    w.xa.load(at + pa * E);
-                    if (hasB) w.xb.load(at + pb * E);
+            // A thread copies what it will read itself, two rows ahead; nobody waits for anybody.
+            auto place = [&](int r, int which) { return ring + static_cast<size_t>(((r % kBackwardStages) * 4 + which) * threads + tid) * 16; };
+            auto fetch = [&](int r) {
+                if (wanted && hasA && r < n && info[r].position >= 0) {
+                    if (!isV) {
+                        const T* at = src + (row0 + r) * srcStride;
+                        copyAhead(place(r, 0), at + pa * E, true);
+                        copyAhead(place(r, 1), at + (hasB ? pb : pa) * E, hasB);
+                    }
+                    const int64_t slot = info[r].pool;
+                    const T* from = fromPool ? up + (slot >= 0 ? slot : 0) : up + (row0 + r) * upStride;
+                    const bool there = !fromPool || slot >= 0;
+                    copyAhead(place(r, 2), from + pa * E, there);
+                    copyAhead(place(r, 3), from + (hasB ? pb : pa) * E, there && hasB);
                 }
-                const int64_t slot = info[r].pool;
-                const T* from = fromPool ? up + (slot >= 0 ? slot : 0) : up + (row0 + r) * upStride;
-                if (!fromPool || slot >= 0) {
-                    w.ya.load(from + pa * E);
-                    if (hasB) w.yb.load(from + pb * E);
-                }
-                return w;
+                asm volatile("cp.async.commit_group;" ::: "memory");
             };
-            Row w = load(0);
+#pragma unroll
+            for (int r = 0; r < kBackwardStages - 1; ++r) fetch(r);
 #pragma unroll 1
             for (int r = 0; r < n; ++r) {
-                const Row next = load(r + 1);         // on its way while this row is worked on
+                asm volatile("cp.async.wait_group %0;" ::"n"(kBackwardStages - 2) : "memory");
+                struct { P xa, xb, ya, yb; } w;
+                if (hasA) {                           // (lanes without a piece add zeros)
+                    w.xa.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 0));
+                    w.xb.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 1));
+                    w.ya.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 2));
+                    w.yb.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 3));
+                }
+                fetch(r + kBackwardStages - 1);       // (where the row before this one was)
                 const bool live = wanted && hasA && info[r].position >= 0;
                 T* to = dst + (row0 + r) * dstStride;
                 if (live && isV) {
@@ -558,10 +577,10 @@ normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, con
                         out.store(to + pb * E);
                     }
                 }
-                w = next;
             }
         }
         if (!p.partials) return;
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < E / 2; ++e) {
@@ -661,26 +680,28 @@ normRotateBackwardAnyKernel(const __grid_constant__ NormRotateBackwardParams p) 
 
 // dw = the blocks' partial sums added up in block order (float64: the sum of up to a few
 // thousand terms costs nothing here and adds no error of its own).
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 weightGradientKernel(const float* __restrict__ partials, int blocks, int dim, float* dQWeight, float* dKWeight) {
-    __shared__ double part[8][32];
+    __shared__ double part[32][32];
+    cudaGridDependencySynchronize();                  // launched early; the partial sums are there from here on
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
     const int d = blockIdx.x * 32 + lane, which = blockIdx.y;
     double sum = 0.0;
     if (d < dim)
-        for (int b = slice; b < blocks; b += 8) sum += partials[(static_cast<int64_t>(b) * 2 + which) * dim + d];
+#pragma unroll 4
+        for (int b = slice; b < blocks; b += 32) sum += partials[(static_cast<int64_t>(b) * 2 + which) * dim + d];
     part[slice][lane] = sum;
     __syncthreads();
     if (slice == 0 && d < dim) {
-        for (int s = 1; s < 8; ++s) sum += part[s][lane];
+        for (int s = 1; s < 32; ++s) sum += part[s][lane];
         float* out = which ? dKWeight : dQWeight;
         if (out) out[d] = static_cast<float>(sum);
     }
 }
 
-// Blocks that share the rows: two for every SM, each with at least one look-up's worth of rows.
+// Blocks that share the rows: two for every SM, each with a few rows at least.
 int backwardBlocks(const NormRotateBackwardParams& p, int smCount) {
-    return static_cast<int>(std::min<int64_t>((static_cast<int64_t>(p.numRows) + kBackwardRows - 1) / kBackwardRows, static_cast<int64_t>(smCount) * 2));
+    return static_cast<int>(std::min<int64_t>((static_cast<int64_t>(p.numRows) + kBackwardShare - 1) / kBackwardShare, static_cast<int64_t>(smCount) * 2));
 }
 template <typename T> constexpr int backwardBytes() { return 16; }
 // Lanes and threads of the launch that the pieces allow (chunks 1, threads 0: the other kernel runs).
@@ -707,8 +728,11 @@ cudaError_t normRotateBackwardOf(const NormRotateBackwardParams& p, int smCount,
     const int blocks = backwardBlocks(p, smCount);
     if (pieces) {
         const int share = static_cast<int>((static_cast<int64_t>(p.numRows) + blocks - 1) / blocks);
-        const size_t smem = (p.partials ? static_cast<size_t>(threads) * 2 * E * sizeof(float) : 0) +
+        const size_t smem = static_cast<size_t>(threads) * kBackwardStages * 4 * 16 +
                             kBackwardRows * (sizeof(RowInfo) + (p.rotaryDim / 2) * sizeof(float2));
+        // (at most 512 threads, 96 KB of rows, and 32 KB of turns)
+        const cudaError_t allowed = cudaFuncSetAttribute(normRotateBackwardKernel<T, BYTES>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        if (allowed != cudaSuccess) return allowed;
         normRotateBackwardKernel<T, BYTES><<<dim3(blocks, chunks), threads, smem, stream>>>(p, l, share);
     } else {
         chunks = 1;
@@ -717,9 +741,17 @@ cudaError_t normRotateBackwardOf(const NormRotateBackwardParams& p, int smCount,
     *launches += 1;
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess && p.partials) {
-        weightGradientKernel<<<dim3((p.headDim + 31) / 32, 2), 256, 0, stream>>>(p.partials, blocks * chunks, p.headDim, p.dQWeight, p.dKWeight);
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((p.headDim + 31) / 32, 2);
+        cfg.blockDim = dim3(1024);
+        cfg.stream = stream;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, weightGradientKernel, static_cast<const float*>(p.partials), blocks * chunks, p.headDim, p.dQWeight, p.dKWeight);
         *launches += 1;
-        e = cudaGetLastError();
     }
     return e;
 }
