@@ -258,7 +258,7 @@ bool treeMmaSizes(const TreeParams& p);
 bool treeMmaApplies(const TreeParams& p);
 TreePlan treeMmaPlan(const TreeParams& p, int smCount);
 cudaError_t launchTreeMma(const TreeParams& p, const TreePlan& plan, cudaStream_t stream);
-// tree_tc_kernel.cu: 16-bit and FP8 pools, head_dim 64, 80, ... 128, block sizes that are multiples of 16.
+// tree_tc_kernel.cu: 16-bit and FP8 pools, head_dim 64, 80, ... 128, block sizes that are multiples of 8 (FP8: 16).
 bool treeTcSizes(const TreeParams& p);
 bool treeTcApplies(const TreeParams& p);
 TreePlan treeTcPlan(const TreeParams& p, int smCount);

@@ -1,5 +1,5 @@
-// Tree attention on the 5th-generation tensor cores: float16 / bfloat16 pools, head_dim 128, block
-// sizes that are multiples of 16.  The products and the softmax are those of the prefill kernel
+// Tree attention on the 5th-generation tensor cores: float16, bfloat16 and FP8 pools, head_dim 64, 80,
+// ... 128, block sizes that are multiples of 8 (FP8: 16).  The products and the softmax are those of the prefill kernel
 // (prefill_tc_kernel.cu): S = Q K^T and O += P V as tcgen05.mma 128 x 128 x 16 with S, P and O in
 // tensor memory, one softmax thread per row, keys and values by TMA straight from the pages.  What
 // differs is the work: few rows (node, query head) against a long cache, so that the keys are
@@ -286,6 +286,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         const CUtensorMap* pool = isV ? &mapV : &mapK;
         const CUtensorMap* fresh = isV ? &mapVNew : &mapKNew;
         const int tilesPerPage = p.blockSize / 16;
+        // 16-bit pages come in pieces of 16 rows, or of 8 (an atom of the swizzle) where 16 does not divide them
+        const int pieceRows = p.blockSize % 16 == 0 ? 16 : 8, pieces = kKeys / pieceRows, piecesPerPage = p.blockSize / pieceRows, pieceBytes = pieceRows * 128;
         int gt = 0;                          // tiles of the block's piece so far
         bool ok = true;
         if constexpr (FP8) {
@@ -364,11 +366,11 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 const bool inTree = j >= g.cacheTiles;
                 const int freshRow = g.s.start + (j - g.cacheTiles) * kKeys;
                 int row = 0;
-                if (!inTree && lane < kKeys / 16) {
-                    const int t16 = (static_cast<int>(g.s.lo / kKeys) + j) * (kKeys / 16) + lane;
-                    const int page = min(t16 / tilesPerPage, p.maxNumBlocks - 1);
+                if (!inTree && lane < pieces) {
+                    const int at = (static_cast<int>(g.s.lo / kKeys) + j) * pieces + lane;
+                    const int page = min(at / piecesPerPage, p.maxNumBlocks - 1);
                     const int blk = min(max(table[page], 0), p.poolBlocks - 1);
-                    row = (blk * p.kvHeads + g.kvh) * p.blockSize + (t16 % tilesPerPage) * 16;
+                    row = (blk * p.kvHeads + g.kvh) * p.blockSize + (at % piecesPerPage) * pieceRows;
                 }
                 if (!isV) {
                     const int st = gt % S::kKStages;
@@ -382,9 +384,9 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         if (lane < dimBlocks)
                             for (int h = 0; h < 2; ++h)        // (a box is 64 rows)
                                 tmaLoad3d(to + lane * kHalfBytes + h * kVBlockBytes, fresh, &s->kFull[st], 64 * lane, g.kvh, freshRow + 64 * h);
-                    } else if (lane < kKeys / 16) {
-                        tmaLoad2d(to + lane * 2048, pool, &s->kFull[st], 0, row);
-                        if (dimBlocks == 2) tmaLoad2d(to + kHalfBytes + lane * 2048, pool, &s->kFull[st], 64, row);
+                    } else if (lane < pieces) {
+                        tmaLoad2d(to + lane * pieceBytes, pool, &s->kFull[st], 0, row);
+                        if (dimBlocks == 2) tmaLoad2d(to + kHalfBytes + lane * pieceBytes, pool, &s->kFull[st], 64, row);
                     }
                 } else {
 #pragma unroll
@@ -398,9 +400,10 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         unsigned char* to = s->v[st];
                         if (inTree) {
                             if (lane < dimBlocks) tmaLoad3d(to + lane * kVBlockBytes, fresh, &s->vFull[st], 64 * lane, g.kvh, freshRow + 64 * h);
-                        } else if (lane >> 2 == h) {
-                            tmaLoad2d(to + (lane & 3) * 2048, pool, &s->vFull[st], 0, row);
-                            if (dimBlocks == 2) tmaLoad2d(to + kVBlockBytes + (lane & 3) * 2048, pool, &s->vFull[st], 64, row);
+                        } else if (lane < pieces && (lane >= pieces / 2) == (h == 1)) {
+                            const int in = (lane - h * (pieces / 2)) * pieceBytes;
+                            tmaLoad2d(to + in, pool, &s->vFull[st], 0, row);
+                            if (dimBlocks == 2) tmaLoad2d(to + kVBlockBytes + in, pool, &s->vFull[st], 64, row);
                         }
                     }
                 }
@@ -992,7 +995,7 @@ done:
 }  // namespace
 
 bool treeTcSizes(const TreeParams& p) {
-    return p.dtype != kF32 && p.headDim >= 64 && p.headDim <= kHd && p.headDim % 16 == 0 && p.blockSize % 16 == 0;
+    return p.dtype != kF32 && p.headDim >= 64 && p.headDim <= kHd && p.headDim % 16 == 0 && p.blockSize % (p.dtype == kFP8 ? 16 : 8) == 0;
 }
 
 bool treeTcApplies(const TreeParams& p) {
@@ -1043,10 +1046,10 @@ cudaError_t launchTreeTc(const TreeParams& p, const TreePlan& plan, cudaStream_t
     }
     for (int which = 0; which < 2; ++which) {
         if (p.dtype != kFP8) {
-        // pools: [block * kv_head * slot][128]; a box is 64 dims x 16 rows (half of a 16-token piece)
+        // pools: [block * kv_head * slot][128]; a box is 64 dims x 16 or 8 rows
         const cuuint64_t dims[2] = {D, static_cast<cuuint64_t>(p.poolBlocks) * p.kvHeads * p.blockSize};
         const cuuint64_t strides[1] = {D * 2};
-        const cuuint32_t box[2] = {64, 16}, one[2] = {1, 1};
+        const cuuint32_t box[2] = {64, p.blockSize % 16 == 0 ? 16u : 8u}, one[2] = {1, 1};
         if (encode(&pool[which], dt, 2, const_cast<void*>(which ? p.vPool : p.kPool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;

@@ -158,6 +158,8 @@ SHAPES = {
     "dim 256": dict(lens=[70, 200], sizes=[9, 3], dim=256),
     "blocks of 8": dict(lens=[70, 300], sizes=[9, 20], block=8),
     "blocks of 24": dict(lens=[70, 300], sizes=[9, 20], block=24),
+    "blocks of 8, long": dict(lens=[700, 129, 2000], sizes=[40, 9, 64], block=8),
+    "blocks of 24, long": dict(lens=[700, 129, 2000], sizes=[40, 9, 64], block=24, dim=64),
     "blocks of 32": dict(lens=[70, 300], sizes=[9, 20], block=32),
     "blocks of 128": dict(lens=[70, 300], sizes=[9, 20], block=128),
     "chain": dict(lens=[70, 300], sizes=[40, 64], kind="chain"),
