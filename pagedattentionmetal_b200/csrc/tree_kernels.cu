@@ -20,18 +20,21 @@ using namespace tree;
 // ---- general kernel -----------------------------------------------------------
 
 // Any type, any head_dim up to 256, any strides: float32 products on the CUDA cores out of
-// shared memory.  16 rows (node, head) against 32 keys at a time, 128 threads; warp w owns rows
-// 4 w .. 4 w + 3 from the scores to the result, so that the only block-wide waits are around
-// the tile loads.  Lane (c, z) = (lane / 4, lane % 4) sums the 4 x 4 scores of its warp's rows and
-// keys 4 c .. 4 c + 3 over every fourth 4-element piece of the dimension (8 loads of 16 bytes for
-// 64 products) and, after a sum over z, keeps row z's four.
-constexpr int kGenRows = 16, kGenKeys = 32, kGenThreads = 128;
+// shared memory.  4 RW rows (node, head) against 32 keys at a time, 128 threads; warp w owns rows
+// RW w .. RW w + RW - 1 from the scores to the result, so that the only block-wide waits are around
+// the tile loads.  Lane (c, z) = (lane / 4, lane % 4) sums the RW x 4 scores of its warp's rows and
+// keys 4 c .. 4 c + 3 over every fourth 4-element piece of the dimension and, after a sum over z, keeps
+// those of rows z and z + 4.  RW 8 takes 12 loads of 16 bytes for 128 products where RW 4 takes 8 for
+// 64, and half the fetches of keys and values: chosen when a request can have more than 16 rows (32
+// float32 requests of 4096 tokens, 64 rows: 1.40 against 1.66 ms; half of the instructions are products).
+// HALVES: blocks of 128 dims.
+constexpr int kGenKeys = 32, kGenThreads = 128;
 
 struct GeneralSmem {
     static __host__ __device__ int pad(int dim) { return (dim + 15) / 16 * 16; }
-    static __host__ __device__ size_t bytes(int dim, int batch) {
+    static __host__ __device__ size_t bytes(int dim, int batch, int rows) {
         const size_t dp = pad(dim);
-        return (kGenRows * dp + kGenKeys * (dp + 4) + kGenKeys * dp + kGenKeys * kGenRows) * sizeof(float) +
+        return (rows * dp + kGenKeys * (dp + 4) + kGenKeys * dp + kGenKeys * rows) * sizeof(float) +
                2 * kGenKeys * sizeof(long long) * 2 + (kGenThreads / 32 + 4) * sizeof(int) + (static_cast<size_t>(batch) + 1) * sizeof(int);
     }
 };
@@ -52,15 +55,16 @@ __device__ __forceinline__ float4 fourOf(const T* p) {
 }
 
 // wide: rows are multiples of four elements, on boundaries of four elements.
-template <typename QT, typename KT_>
-__global__ void __launch_bounds__(kGenThreads)
+template <typename QT, typename KT_, int RW, int HALVES>
+__global__ void __launch_bounds__(kGenThreads, 4)
 treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2, bool wide) {
+    constexpr int kGenRows = 4 * RW, kOwn = RW / 4;        // rows of a tile; rows whose softmax a lane keeps
     extern __shared__ __align__(16) unsigned char raw[];
     const int D = p.headDim, dp = GeneralSmem::pad(D), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float* sq = reinterpret_cast<float*>(raw);             // [16][dp]
+    float* sq = reinterpret_cast<float*>(raw);             // [rows][dp]
     float* sk = sq + kGenRows * dp;                        // [32][dp + 4]
     float* sv = sk + kGenKeys * (dp + 4);                  // [32][dp]
-    float* sp = sv + kGenKeys * dp;                        // [32][16]
+    float* sp = sv + kGenKeys * dp;                        // [32][rows]
     long long* kAt = reinterpret_cast<long long*>(sp + kGenKeys * kGenRows);   // [32] element offsets, -1: no key
     long long* vAt = kAt + kGenKeys;
     long long* blkAt = vAt + kGenKeys;                     // FP8: the block, for its scales
@@ -103,15 +107,25 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2, bool wi
                             static_cast<int64_t>(g.kvh * group + rr % group) * D + d) * scaleLog2;
             sq[i] = v;
         }
-        // the row whose softmax this lane keeps
-        const int row = g.rt * kGenRows + 4 * warp + z, node = min(row / group, s.n - 1);
-        const uint32_t first = firstOf(p, s, node);
-        float m = -INFINITY, l = 0.f;
-        float acc[2][4][4];                                // [dims lane * 4 (+ 128)][row][dim]
+        // the rows whose softmax this lane keeps
+        int node[kOwn];
+        uint32_t first[kOwn];
+        float m[kOwn], l[kOwn];
+        bool there[kOwn];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < kOwn; ++i) {
+            const int row = g.rt * kGenRows + RW * warp + z + 4 * i;
+            there[i] = row < rows;
+            node[i] = min(row / group, s.n - 1);
+            first[i] = firstOf(p, s, node[i]);
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+        }
+        float acc[HALVES][RW][4];                          // [dims lane * 4 (+ 128)][row][dim]
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int r = 0; r < RW; ++r)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[h][r][e] = 0.f;
         bool odd = false;
@@ -138,7 +152,7 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2, bool wi
             if (wide) {
                 // Four pieces of keys and values each are on their way together: an element at a time, as
                 // below, a call of seven short requests spent most of its time on one load after another
-                // (dim 80, float32: 38.5 us, now GENERAL_FIGURE).
+                // (dim 80, float32: 38.5 us, now 22).
                 constexpr int kAhead = 4;
                 for (int i0 = tid; i0 < kGenKeys * pieces; i0 += kAhead * kGenThreads) {
                     float4 kv[kAhead], vv[kAhead];
@@ -193,84 +207,92 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2, bool wi
                 sv[i] = vv;
             }
             __syncthreads();
-            float dot[4][4];
+            float dot[RW][4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < RW; ++r)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) dot[r][k] = 0.f;
             for (int d = 4 * z; d < dp; d += 16) {
-                float4 a[4], b[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4*>(sq + (4 * warp + r) * dp + d);
+                float4 b[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) b[k] = *reinterpret_cast<const float4*>(sk + (4 * c + k) * (dp + 4) + d);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
+                for (int r = 0; r < RW; ++r) {
+                    const float4 a = *reinterpret_cast<const float4*>(sq + (RW * warp + r) * dp + d);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        dot[r][k] += a[r].x * b[k].x + a[r].y * b[k].y + a[r].z * b[k].z + a[r].w * b[k].w;
+                        dot[r][k] += a.x * b[k].x + a.y * b[k].y + a.z * b[k].z + a.w * b[k].w;
+                }
             }
-            float x[4] = {0.f, 0.f, 0.f, 0.f};             // row z's scores of keys 4 c .. 4 c + 3
+            float x[kOwn][4];                              // the lane's rows: scores of keys 4 c .. 4 c + 3
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < RW; ++r)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float v = dot[r][k];
                     v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
                     v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
-                    if (r == z) x[k] = v;
+                    if ((r & 3) == z) x[r >> 2][k] = v;
                 }
-            uint32_t bits = 0u;
-            if (row < rows) {
-                if (inTree) bits = treeBits(p, s, node, static_cast<int>(k0 / 32));
-                else
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t key = k0 + 4 * c + k;
-                        if (key >= first && key < s.held) bits |= 1u << (4 * c + k);
-                    }
+            float corr[kOwn];
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                uint32_t bits = 0u;
+                if (there[i]) {
+                    if (inTree) bits = treeBits(p, s, node[i], static_cast<int>(k0 / 32));
+                    else
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t key = k0 + 4 * c + k;
+                            if (key >= first[i] && key < s.held) bits |= 1u << (4 * c + k);
+                        }
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (!(bits >> (4 * c + k) & 1u)) x[i][k] = -INFINITY;
+                    top = fmaxf(top, x[i][k]);
+                }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                const float mNew = fmaxf(m[i], top), base = mNew == -INFINITY ? 0.f : mNew;
+                corr[i] = exp2f(m[i] - base);
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[i][k] = exp2f(x[i][k] - base);
+                    sum += x[i][k];
+                    sp[(4 * c + k) * kGenRows + RW * warp + z + 4 * i] = x[i][k];
+                }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+                l[i] = l[i] * corr[i] + sum;
+                m[i] = mNew;
             }
-            float top = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (!(bits >> (4 * c + k) & 1u)) x[k] = -INFINITY;
-                top = fmaxf(top, x[k]);
-            }
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-            const float mNew = fmaxf(m, top), base = mNew == -INFINITY ? 0.f : mNew;
-            const float corr = exp2f(m - base);
-            float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                x[k] = exp2f(x[k] - base);
-                sum += x[k];
-                sp[(4 * c + k) * kGenRows + 4 * warp + z] = x[k];
-            }
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-            l = l * corr + sum;
-            m = mNew;
             __syncwarp();
-            float f[4];
+            float f[RW];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) f[r] = __shfl_sync(0xFFFFFFFFu, corr, r);
+            for (int r = 0; r < RW; ++r) f[r] = __shfl_sync(0xFFFFFFFFu, corr[r >> 2], r & 3);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < HALVES; ++h) {
                 const int d = 4 * lane + 128 * h;
                 if (d >= dp) break;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
+                for (int r = 0; r < RW; ++r)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[h][r][e] *= f[r];
 #pragma unroll 8
                 for (int k = 0; k < kGenKeys; ++k) {
-                    const float4 w = *reinterpret_cast<const float4*>(sp + k * kGenRows + 4 * warp);
                     const float4 v = *reinterpret_cast<const float4*>(sv + k * dp + d);
-                    const float ww[4] = {w.x, w.y, w.z, w.w}, vv[4] = {v.x, v.y, v.z, v.w};
+                    const float vv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+                    for (int q = 0; q < kOwn; ++q) {
+                        const float4 w = *reinterpret_cast<const float4*>(sp + k * kGenRows + RW * warp + 4 * q);
+                        const float ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[h][r][e] += ww[r] * vv[e];
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[h][4 * q + r][e] += ww[r] * vv[e];
+                    }
                 }
             }
             __syncwarp();
@@ -291,12 +313,12 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2, bool wi
             }
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float lr = __shfl_sync(0xFFFFFFFFu, l, r), mr = __shfl_sync(0xFFFFFFFFu, m, r);
-            const int rl = 4 * warp + r, rr = g.rt * kGenRows + rl;
+        for (int r = 0; r < RW; ++r) {
+            const float lr = __shfl_sync(0xFFFFFFFFu, l[r >> 2], r & 3), mr = __shfl_sync(0xFFFFFFFFu, m[r >> 2], r & 3);
+            const int rl = RW * warp + r, rr = g.rt * kGenRows + rl;
             if (rr >= rows) continue;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < HALVES; ++h) {
                 const int d = 4 * lane + 128 * h;
                 if (d >= dp) break;
                 if (whole) {
@@ -495,11 +517,11 @@ cudaError_t allowSmem(K kernel, size_t bytes, std::atomic<unsigned long long>& d
 
 TreePlan generalPlan(const TreeParams& p, int smCount) {
     TreePlan t{};
-    t.rows = kGenRows;
+    t.rows = p.headDim <= 128 && static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) > 16 ? 32 : 16;
     t.keys = kGenKeys;
     t.dimPad = GeneralSmem::pad(p.headDim);
     // as many blocks as an SM's shared memory holds, four at most
-    const size_t smem = GeneralSmem::bytes(p.headDim, p.batch);
+    const size_t smem = GeneralSmem::bytes(p.headDim, p.batch, t.rows);
     const int perSm = static_cast<int>(std::min<size_t>(4, std::max<size_t>(1, (227u * 1024) / (smem + 1024))));
     t.blocks = smCount * perSm;
     return t;
@@ -524,16 +546,23 @@ size_t planBytes(const TreePlan& t) {
     return headerBytes(t.blocks) + static_cast<size_t>(t.blocks) * 2 * recordFloats(t.rows, t.dimPad) * sizeof(float);
 }
 
-template <typename QT, typename KT_>
-cudaError_t launchGeneral(const TreeParams& p, const TreePlan& plan, cudaStream_t stream) {
+template <typename QT, typename KT_, int RW, int HALVES>
+cudaError_t launchGeneralShape(const TreeParams& p, const TreePlan& plan, cudaStream_t stream) {
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = allowSmem(treeGeneralKernel<QT, KT_>, 227 * 1024, done);
+    cudaError_t e = allowSmem(treeGeneralKernel<QT, KT_, RW, HALVES>, 227 * 1024, done);
     if (e != cudaSuccess) return e;
     const float scaleLog2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.headDim));
     bool wide = p.headDim % 4 == 0 && p.qStride % 4 == 0 && p.kStride % 4 == 0 && p.vStride % 4 == 0;
     for (const void* rows : {p.q, p.kNew, p.vNew}) wide = wide && reinterpret_cast<uintptr_t>(rows) % (4 * sizeof(QT)) == 0;
     for (const void* pool : {p.kPool, p.vPool}) wide = wide && reinterpret_cast<uintptr_t>(pool) % (4 * sizeof(KT_)) == 0;
-    return launchEarly(treeGeneralKernel<QT, KT_>, dim3(plan.blocks), kGenThreads, GeneralSmem::bytes(p.headDim, p.batch), stream, p, scaleLog2, wide);
+    return launchEarly(treeGeneralKernel<QT, KT_, RW, HALVES>, dim3(plan.blocks), kGenThreads, GeneralSmem::bytes(p.headDim, p.batch, plan.rows),
+                       stream, p, scaleLog2, wide);
+}
+
+template <typename QT, typename KT_>
+cudaError_t launchGeneral(const TreeParams& p, const TreePlan& plan, cudaStream_t stream) {
+    if (p.headDim > 128) return launchGeneralShape<QT, KT_, 4, 2>(p, plan, stream);
+    return plan.rows == 32 ? launchGeneralShape<QT, KT_, 8, 1>(p, plan, stream) : launchGeneralShape<QT, KT_, 4, 1>(p, plan, stream);
 }
 
 template <typename QT, typename KT_>
@@ -547,7 +576,8 @@ cudaError_t launchOf(const TreeParams& p, const TreePlan& plan, cudaStream_t str
 }  // namespace
 
 int64_t treeTileBound(const TreeParams& p) {
-    const int64_t rowTiles = (static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) + kGenRows - 1) / kGenRows;
+    constexpr int kFewestRows = 16;                    // of a tile of any kernel
+    const int64_t rowTiles = (static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) + kFewestRows - 1) / kFewestRows;
     const int64_t keyTiles = static_cast<int64_t>(p.maxNumBlocks) * p.blockSize / kGenKeys + 2 + p.maxNew / kGenKeys + 1;
     return static_cast<int64_t>(p.batch) * p.kvHeads * rowTiles * keyTiles;
 }
