@@ -74,9 +74,11 @@ struct Span {
 constexpr int kSpans = 8;        // of the ring: no warp needs a span more than five behind the oldest one in use
 
 // FP8, of a key tile: per 16 keys (a page holds a multiple of them) the key scale times log2(e) /
-// sqrt(dim), the logarithm of the value scale, and one over it; negative where the value scale is zero.
-struct PageScales {
-    float4 key[2], valueLog[2], valueInv[2];
+// sqrt(dim), the logarithm of the value scale, and one over it.  Where the value scale is zero the bit
+// in `zeros` is set, the values are converted to zeros and the scale counts as one.
+struct alignas(16) PageScales {
+    float key[8], valueLog[8], valueInv[8];
+    uint32_t zeros;
 };
 
 // WIDE: pairs of up to 256 rows (two query tiles), else of 128.
@@ -188,12 +190,7 @@ __device__ __forceinline__ float rowMax16(const uint32_t (&r)[32]) {
 }
 template <int BEGIN>
 __device__ __forceinline__ float pageWeights(const uint32_t (&r)[32], uint32_t (&w)[32], float key, float valueLog, float inv, float negM) {
-    const float sum = weightsRange<false, false, BEGIN, BEGIN + 16>(r, w, key, negM + valueLog);
-    if (inv > 0.f) return sum * inv;
-    // a value scale of zero: the keys count, their values are zero
-#pragma unroll
-    for (int i = BEGIN / 2; i < BEGIN / 2 + 8; ++i) w[i] = 0u;
-    return sum;
+    return inv * weightsRange<false, false, BEGIN, BEGIN + 16>(r, w, key, negM + valueLog);
 }
 // Two codes to two float16 values.
 __device__ __forceinline__ uint32_t widen(uint32_t codes) {
@@ -338,11 +335,16 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         if (raw >= S::kRawStages) ok = mbarWait(&s->rawEmpty[st], ((raw / S::kRawStages) - 1) & 1, &s->dead, errFlag, waitLimit, 56);
                         ok = __all_sync(0xFFFFFFFFu, ok);
                         if (!ok) break;
-                        if (h == 0 && lane < kKeys / 16) {
+                        if (h == 0) {
                             PageScales& sc = s->scales[gt % S::kScaleStages];
-                            reinterpret_cast<float*>(sc.key)[lane] = inTree ? scaleLog2 : fmaxf(ks * scaleLog2, 1e-30f);          // (zero times a masked score would be NaN)
-                            reinterpret_cast<float*>(sc.valueLog)[lane] = inTree || !(vs > 0.f) ? 0.f : log2f(vs);
-                            reinterpret_cast<float*>(sc.valueInv)[lane] = inTree ? 1.f : vs > 0.f ? 1.f / vs : -1.f;
+                            const bool zero = !inTree && !(vs > 0.f);
+                            if (lane < kKeys / 16) {
+                                sc.key[lane] = inTree ? scaleLog2 : fmaxf(ks * scaleLog2, 1e-30f);          // (zero times a masked score would be NaN)
+                                sc.valueLog[lane] = inTree || zero ? 0.f : log2f(vs);
+                                sc.valueInv[lane] = inTree || zero ? 1.f : 1.f / vs;
+                            }
+                            const uint32_t zeros = __ballot_sync(0xFFFFFFFFu, zero);
+                            if (lane == 0) sc.zeros = zeros & 0xFFu;
                         }
                         __syncwarp();
                         if (lane == 0) {
@@ -587,7 +589,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         const int piece = lane & 7, rowIn = (lane >> 3) ^ (piece >> 2);
         const unsigned rawAt = static_cast<unsigned>(((warp & 3) * 32 + rowIn) * D + piece * 16);
         const unsigned outAt = static_cast<unsigned>(rowIn * 128 + ((((2 * piece) & 7) ^ rowIn) << 4));
-        auto convert = [&](const unsigned char* from, unsigned char* to, int block) {
+        auto convert = [&](const unsigned char* from, unsigned char* to, int block, uint32_t zeros) {
             if (piece >= 4 * dimBlocks) return;
             const bool there = piece * 16 < D;
             from += rawAt;
@@ -596,7 +598,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             for (int i0 = 0; i0 < 8; i0 += 4) {
                 uint4 w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = there ? *reinterpret_cast<const uint4*>(from + (i0 + i) * 4 * D) : make_uint4(0u, 0u, 0u, 0u);
+                for (int i = 0; i < 4; ++i) w[i] = there && !(zeros >> (i0 >> 2) & 1u) ? *reinterpret_cast<const uint4*>(from + (i0 + i) * 4 * D) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     unsigned char* row = to + (i0 + i) * 512;
@@ -619,7 +621,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 ok = mbarWait(&s->rawFull[st], (raw / S::kRawStages) & 1, &s->dead, errFlag, waitLimit, 58);
                 if (ok && gt >= S::kKStages) ok = mbarWait(&s->kEmpty[ks], ((gt / S::kKStages) - 1) & 1, &s->dead, errFlag, waitLimit, 57);
                 if (!ok) break;
-                if (!inTree) convert(s->raw[st], s->k[ks] + (warp & 3) * 4096, kHalfBytes);
+                if (!inTree) convert(s->raw[st], s->k[ks] + (warp & 3) * 4096, kHalfBytes, 0u);
                 mbarArrive(&s->rawEmpty[st]);
                 if (inTree && t == 0) {
                     mbarExpectTx(&s->kFull[ks], dimBlocks * kHalfBytes);
@@ -632,7 +634,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 ok = mbarWait(&s->rawFull[st], (raw / S::kRawStages) & 1, &s->dead, errFlag, waitLimit, 60);
                 if (ok && n >= S::kVStages) ok = mbarWait(&s->vEmpty[vs], ((n / S::kVStages) - 1) & 1, &s->dead, errFlag, waitLimit, 59);
                 if (!ok) break;
-                if (!inTree) convert(s->raw[st], s->v[vs] + (warp & 1) * 4096, kVBlockBytes);
+                if (!inTree) convert(s->raw[st], s->v[vs] + (warp & 1) * 4096, kVBlockBytes, s->scales[gt % S::kScaleStages].zeros >> (2 * (warp & 3)));
                 mbarArrive(&s->rawEmpty[st]);
                 if (inTree && (t & 63) == 0) {
                     mbarExpectTx(&s->vFull[vs], dimBlocks * kVBlockBytes);
@@ -867,7 +869,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 for (int c = 0; c < 4; c += 2) {
                     uint32_t r0[32], r1[32];
                     float4 key, add;
-                    if constexpr (FP8) { key = sc.key[c >> 1]; add = sc.valueLog[c >> 1]; }
+                    if constexpr (FP8) { key = reinterpret_cast<const float4*>(sc.key)[c >> 1]; add = reinterpret_cast<const float4*>(sc.valueLog)[c >> 1]; }
                     tmemLd32NoWait(sAddr + 32u * c, r0);
                     tmemLd32NoWait(sAddr + 32u * c + 32u, r1);
                     tmemLdWait();
@@ -905,11 +907,24 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                     l *= corr;
                 }
                 const float negM = mUsed == -INFINITY ? 0.f : -mUsed;
+                if constexpr (FP8) {
+                    // (a quarter at a time: there are fewer registers)
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t r[32], wgt[32];
+                        const float2 key = reinterpret_cast<const float2*>(sc.key)[c], add = reinterpret_cast<const float2*>(sc.valueLog)[c];
+                        const float2 inv = reinterpret_cast<const float2*>(sc.valueInv)[c];
+                        tmemLd32NoWait(sAddr + 32u * c, r);
+                        tmemLdWait();
+                        if (edge) maskBits(r, s->rowBits[x][c][t]);
+                        l += pageWeights<0>(r, wgt, key.x, add.x, inv.x, negM);
+                        l += pageWeights<16>(r, wgt, key.y, add.y, inv.y, negM);
+                        tmemSt16(sAddr + 32u * c, wgt);
+                    }
+                } else
 #pragma unroll 1
                 for (int c = 0; c < 4; c += 2) {
                     uint32_t r0[32], r1[32], wgt[32];
-                    float4 key, add, inv;
-                    if constexpr (FP8) { key = sc.key[c >> 1]; add = sc.valueLog[c >> 1]; inv = sc.valueInv[c >> 1]; }
                     tmemLd32NoWait(sAddr + 32u * c, r0);
                     tmemLd32NoWait(sAddr + 32u * c + 32u, r1);
                     tmemLdWait();
@@ -917,14 +932,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         maskBits(r0, s->rowBits[x][c][t]);
                         maskBits(r1, s->rowBits[x][c + 1][t]);
                     }
-                    if constexpr (FP8) {
-                        l += pageWeights<0>(r0, wgt, key.x, add.x, inv.x, negM);
-                        l += pageWeights<16>(r0, wgt, key.y, add.y, inv.y, negM);
-                        tmemSt16(sAddr + 32u * c, wgt);
-                        l += pageWeights<0>(r1, wgt, key.z, add.z, inv.z, negM);
-                        l += pageWeights<16>(r1, wgt, key.w, add.w, inv.w, negM);
-                        tmemSt16(sAddr + 32u * c + 32u, wgt);
-                    } else if (useLo) {
+                    if (useLo) {
                         l += weightsRange<BF16, true, 0, 32>(r0, wgt, scaleLog2, negM);
                         tmemSt32(sAddr + 32u * c, wgt);
                         l += weightsRange<BF16, true, 0, 32>(r1, wgt, scaleLog2, negM);
@@ -938,7 +946,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 }
                 tmemStWait();
                 if (edge) {
-                    // Row t of V: finite values where there is no such key, or some row may not see it.  (Both groups of a dual span may write the same.  The phase asked for is not two
+                    // Row t of V: finite values where there is no such key, or some row may not see it.
+                    // (Both groups of a dual span may write the same.  The phase asked for is not two
                     // ahead: this S product was issued after the wait for V of the tile two before.)
                     const int half = 2 * (g.tile + j - g.first) + (t >> 6), st = half % S::kVStages;
                     ok = mbarWait(&s->vFull[st], (half / S::kVStages) & 1, &s->dead, errFlag, waitLimit, 53);
@@ -1010,9 +1019,11 @@ bool treeTcApplies(const TreeParams& p) {
     return true;
 }
 
-// Two query tiles: when a request can have more than 128 rows under a KV head (FP8 takes its row tiles
-// one after the other: the codes' ring leaves no room for two), or the batch's list does not fit beside
-// the longer rings.
+// Two query tiles: when a request can have more than 128 rows under a KV head, or the batch's list does
+// not fit beside the longer rings.  Over FP8 pages row tiles are taken one after the other: the ring of
+// codes leaves room for two query tiles and one tile of V, which then waits for the products of the
+// tile before (32 requests of 4096 tokens, 256 rows: 201 us, against 207; one of 8192 tokens 37
+// against 31).
 static bool takesWide(const TreeParams& p) {
     return p.dtype != kFP8 && (static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) > kRows || smemBytes<false, false>(p.batch) > kSmemLimit);
 }

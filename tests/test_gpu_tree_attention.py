@@ -186,6 +186,8 @@ def test_very_many_short_requests(engine, dtype):
     lens = [0 if i % 3 else 5 + i % 40 for i in range(900)]
     TreeCase(44, lens, [5 + i % 2 for i in range(900)], heads=8, kv_heads=2, dtype=dtype).check(engine)
     TreeCase(45, [0] * 1500, [17] + [0, 1] * 749 + [3], heads=8, kv_heads=2, dtype=dtype).check(engine)
+    # small ones beside one with more than 128 rows under a KV head, and beside its second row tile
+    TreeCase(49, lens[:300] + [500, 30], [5 + i % 2 for i in range(300)] + [40, 70], heads=8, kv_heads=2, dtype=dtype).check(engine)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=lambda d: d.name)
