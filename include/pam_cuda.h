@@ -577,7 +577,7 @@ typedef struct PamTreeAttentionRequest {
     PamBuffer masks;              /* uint32 [num_rows][mask_words], optional */
     PamBuffer positions;          /* int32 [num_rows], optional */
     PamBuffer output;             /* [num_rows][heads][head_dim] */
-    PamBuffer k_scale, v_scale;   /* FP8 only */
+    PamBuffer k_scale, v_scale;   /* FP8 only; not negative */
     PamBuffer workspace;          /* optional, see pamc_tree_attention_workspace */
     int64_t q_stride, k_stride, v_stride; /* elements, 0: back to back */
     int32_t batch_size, max_num_blocks, num_rows, max_new_tokens, mask_words;

@@ -1,36 +1,43 @@
 // Tree attention on the 5th-generation tensor cores: float16, bfloat16 and FP8 pools, head_dim 64, 80,
-// ... 128, block sizes that are multiples of 8 (FP8: 16).  The products and the softmax are those of the prefill kernel
-// (prefill_tc_kernel.cu): S = Q K^T and O += P V as tcgen05.mma 128 x 128 x 16 with S, P and O in
-// tensor memory, one softmax thread per row, keys and values by TMA straight from the pages.  What
-// differs is the work: few rows (node, query head) against a long cache, so that the keys are
-// what is cut up.  Every block takes an equal piece of the launch's list of key tiles
+// ... 128, block sizes that are multiples of 8 (FP8: 16).  S = Q K^T and O += P V as tcgen05.mma
+// 128 x 128 x 16 with S, P and O in tensor memory, one softmax thread per row, keys and values by TMA
+// straight from the pages.  The work is few rows (node, query head) against a long cache, so that the
+// keys are what is cut up: every block takes an equal piece of the launch's list of key tiles
 // (tree_common.cuh) and leaves the parts of pairs that it shares as records.
 //
 // A pair is a request's up to 256 rows under one KV head.  With more than 128 rows both softmax groups
 // work on every key tile, each on 128 rows, and the tile is fetched once for both (a tile counts as
 // two in the list).  With at most 128 rows the groups take the key tiles in turn, each with its own
 // running maximum, sum and accumulator, and the output warps join the two: the tensor pipe and the
-// loads then work for one group while the other is in its softmax, as with two row tiles.  At 128
-// rows a tile of 64 KB costs about what its fetch costs, below that the kernel is bound by HBM,
-// above it by the chain softmax -> P V -> next S of the two groups.
+// loads then work for one group while the other is in its softmax, as with two row tiles.
 //
 //   warps 0-3, 4-7   softmax groups: thread t owns row t of the group's rows.  In tiles with keys
 //                    that are not there or that only some rows see it also clears row t of V.
 //   warps 8, 9       TMA producers of K (tiles) and V (half tiles: a stage is free again after half
-//                    a P V product): pages of 16 rows, or boxes of the step's own keys and values for
-//                    a tile of the tree.
+//                    a P V product): pages in pieces of 16 or 8 rows, or boxes of the step's own keys and
+//                    values for a tile of the tree.  FP8: warp 8 alone, codes by bulk copies.
 //   warp 11          walks the list and leaves the block's spans (its parts of pairs) in a ring in
 //                    shared memory, a few ahead of the warps that work on them: a step of that walk is
 //                    some loads and divisions in a row, a microsecond that nobody else waits for.
-//   warp 10          issues the products.  Per group a cursor names its next S product; it is issued
-//                    behind the group's P V product as soon as its tile and queries are there.
+//   warp 10          issues the products, S products up to two steps ahead of the P V product that waits
+//                    for its weights.
 //   warps 12-15      outputs and records: thread t owns row t, out of tensor memory.  Before that they
-//                    bring the queries of the next span into shared memory (cp.async, row t each),
-//                    once the span's last S product is complete.
+//                    bring the queries of the next span into shared memory, once the span's last S product
+//                    is complete: boxes where the group divides 128, else row by row.
+//   warps 16-19      FP8 only: codes to float16, which holds every e4m3 value, in the swizzled layout of
+//                    the operands.  The key scale multiplies the scores; the value scale the weights, with
+//                    the running maximum over score plus logarithm of the value scale, so that the weights
+//                    that go into the second product as float16 stay near 1 however small the scales are.
 //
 // Two forms: when no request of the launch can have more than 128 rows under a KV head there is one
-// query tile and room for three K stages and five half stages of V (measured at 64 requests of 2048
-// tokens and 64 rows each, bound by HBM: LATENCY_FIGURE); else two query tiles, two and four.
+// query tile and room for three K stages and five half stages of V; else two query tiles, two and four.
+//
+// What bounds it, measured with 32 requests of 4096 tokens, 8 KV heads of 128, pages of 16: 4 rows,
+// bfloat16, 101 us = 0.81 of the copy rate, 64 rows 108 us = 0.77: HBM.  256 rows (dual) 177 us, 0.94 us a tile and
+// group: the chain S -> softmax -> P V of each group (some 3000 cycles), whose instructions come from
+// caches that six kinds of warps share; half of the tensor pipe's rate.  FP8 64 rows 110 us, the same
+// chain with scales in it, where the codes would take 38 us.  One request of 1024 tokens 16 us: 9 us of
+// a block's way from start to end, 5 us of the join, launches.
 //
 // Every wait is bounded as in the prefill kernel.
 #include <algorithm>

@@ -36,10 +36,14 @@ class _Request:
         missing = [x for x in self._required if x not in values]
         if missing:
             raise TypeError(f"{type(self).__name__} needs {', '.join(missing)}")
+        unknown = [x for x in values if x not in self._fields]
+        if unknown:
+            raise TypeError(f"{type(self).__name__} has no field {', '.join(unknown)}")
         for name, (field, default) in self._fields.items():
-            setattr(self, name, values.pop(name, default))
-        if values:
-            raise TypeError(f"{type(self).__name__} has no field {', '.join(values)}")
+            if name in values or default:            # (a new struct is all zeros, as most fields are to begin with)
+                setattr(self, name, values.get(name, default))
+            else:
+                self._values[name] = default
 
     def __setattr__(self, name, value):
         if name not in self._fields:
