@@ -148,7 +148,7 @@ void *pamc_create_host_context(void);
 /* Class of the last error on this context (PAM_ERR_*), PAM_OK if none. */
 int32_t pamc_last_error_code(void *ctx);
 /* Run on a caller-owned CUDA stream (a cudaStream_t); NULL restores the
- * context's own stream. */
+ * context's own stream, which is in order with the device's default stream. */
 int32_t pamc_set_stream(void *ctx, void *cuda_stream);
 /* 1: operations return after enqueueing; 0 (default): they wait for the GPU
  * like the reference's commitAndWait (PagedAttentionEngine.swift:2008-2015). */

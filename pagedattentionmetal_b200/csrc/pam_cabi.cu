@@ -904,7 +904,9 @@ void* pamc_create_context_on(int32_t device) {
     c->device = device;
     cudaDeviceProp prop{};
     if (cudaGetDeviceProperties(&prop, device) == cudaSuccess) c->smCount = prop.multiProcessorCount;
-    if (cudaStreamCreateWithFlags(&c->ownStream, cudaStreamNonBlocking) != cudaSuccess) {
+    // A stream in order with the default stream: buffers that a caller filled there a moment ago (torch's
+    // tensors, unless the caller works on streams of its own) are complete when a call reads them.
+    if (cudaStreamCreateWithFlags(&c->ownStream, cudaStreamDefault) != cudaSuccess) {
         cudaGetLastError();
         delete c;
         return nullptr;
