@@ -33,13 +33,14 @@
 // query tile and room for three K stages and five half stages of V; else two query tiles, two and four.
 //
 // What bounds it, measured with 32 requests of 4096 tokens, 8 KV heads of 128, pages of 16: 4 rows,
-// bfloat16, 101 us = 0.81 of the copy rate, 64 rows 108 us = 0.77: HBM.  256 rows (dual) 177 us, 0.94 us a tile and
-// group: the chain S -> softmax -> P V of each group (some 3000 cycles), whose instructions come from
-// caches that six kinds of warps share; half of the tensor pipe's rate.  FP8 64 rows 110 us, the same
+// bfloat16, 101 us = 0.81 of the copy rate, 64 rows 109 us = 0.76: HBM.  256 rows (dual) 180 us, 0.95 us a tile
+// and group: the chain S -> softmax -> P V of each group (some 3000 cycles), whose instructions come from
+// caches that six kinds of warps share; half of the tensor pipe's rate.  FP8 64 rows 114 us, the same
 // chain with scales in it, where the codes would take 38 us.  One request of 1024 tokens 16 us: 9 us of
 // a block's way from start to end, 5 us of the join, launches.
 //
-// Every wait is bounded as in the prefill kernel.
+// Every wait is bounded as in the prefill kernel; a block that gives up waits for the copies and products
+// that it has under way before it ends.
 #include <algorithm>
 #include <type_traits>
 
@@ -58,6 +59,7 @@ constexpr int kVHalfBytes = kTileBytes / 2, kVBlockBytes = kVHalfBytes / 2;   //
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kShortKeys = 256;                        // bfloat16: fewer visible keys carry the weights as two operands
 constexpr long long kWaitCycles = 400000000LL;
+constexpr long long kDrainCycles = 4000000LL;          // for the copies in flight when a wait ran out
 constexpr int kKProducerWarp = 8, kVProducerWarp = 9, kMmaWarp = 10, kPlanWarp = 11, kOutputWarp0 = 12;
 constexpr int kConvertWarp0 = 16;                      // FP8: four more warps
 template <bool FP8> constexpr int kThreads = FP8 ? 640 : 512;
@@ -117,6 +119,8 @@ struct Smem {
     int scratch[32];
     uint32_t tmemBase;
     int dead;
+    int issuedK, issuedV, issuedRaw, issuedQ;          // key tiles, value half tiles, tiles of codes, query tiles asked for
+    unsigned long long drained;
     int prefix[1];                                     // [batch + 1]
 };
 constexpr size_t kSmemLimit = 227 * 1024;
@@ -237,6 +241,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
     if (threadIdx.x == 0) {
         mbarInit(&s->qFull, kRows % group == 0 ? 1 : kRows);
         mbarInit(&s->qEmpty, 1);
+        mbarInit(&s->drained, 1);
+        s->issuedK = s->issuedV = s->issuedRaw = s->issuedQ = 0;
         for (int i = 0; i < 2; ++i) {
             mbarInit(&s->sFull[i], 1);
             mbarInit(&s->pFull[i], kRows);
@@ -365,7 +371,9 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 }
                 spanDone(k);
             }
+            if (!isV && lane == 0) s->issuedRaw = raw;
         }
+        int issued = 0;
         for (int k = 0; ok && !FP8; ++k) {
             const Span* at = spanAt(k);
             if (!at || !at->valid) break;
@@ -388,6 +396,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                     if (!ok) break;
                     if (lane == 0) mbarExpectTx(&s->kFull[st], dimBlocks * kHalfBytes);
                     __syncwarp();
+                    ++issued;
                     unsigned char* to = s->k[st];
                     if (inTree) {
                         if (lane < dimBlocks)
@@ -406,6 +415,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         if (!ok) break;
                         if (lane == 0) mbarExpectTx(&s->vFull[st], dimBlocks * kVBlockBytes);
                         __syncwarp();
+                        ++issued;
                         unsigned char* to = s->v[st];
                         if (inTree) {
                             if (lane < dimBlocks) tmaLoad3d(to + lane * kVBlockBytes, fresh, &s->vFull[st], 64 * lane, g.kvh, freshRow + 64 * h);
@@ -419,6 +429,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             }
             spanDone(k);
         }
+        if (!FP8 && lane == 0) (isV ? s->issuedV : s->issuedK) = issued;
     } else if (warp == kMmaWarp) {
         if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (!live) goto done;
@@ -655,6 +666,12 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             ok = __all_sync(0xFFFFFFFFu, ok);
             spanDone(k);
         }
+        if (t == 0) {
+            // (only tiles of a tree are copies, and the thread that asks for half of V may be a tile ahead: what
+            // counts too much costs the error exit a wait)
+            s->issuedK = gt + 1;
+            s->issuedV = 2 * gt + 4;
+        }
     } else if (warp >= kOutputWarp0) {
         if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (!live) goto done;
@@ -662,9 +679,11 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
         const uint32_t laneBase = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const bool first = threadIdx.x == kOutputWarp0 * 32;
         int cnt0 = 0, cnt1 = 0;              // spans of a group written: phase of oFull
+        int asked = 0;
         // a span's queries into the query tile (a dual span's: tiles), zeros where the request has no
         // such row
         auto fetchQ = [&](const Span& g) {
+            ++asked;
             if (kRows % group == 0) {
                 // a tile of whole nodes: one box of (64 dims, the KV head's query heads, 128 / group nodes)
                 // for each half (rows behind the request's belong to others and are not used)
@@ -809,6 +828,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             if (has1) ++cnt1;
             spanDone(k);
         }
+        if (first) s->issuedQ = asked;
     } else {
         // ------------------------------------------------------------ softmax groups
         if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 120;"); else asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
@@ -863,6 +883,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                     }
                 }
                 ok = mbarWait(&s->sFull[x], steps & 1, &s->dead, errFlag, waitLimit, 52);
+                ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
                 tcFenceAfter();
                 // Two passes over the row, half of it at a time: the maximum, then the weights.  (All 128
@@ -958,6 +979,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                     // ahead: this S product was issued after the wait for V of the tile two before.)
                     const int half = 2 * (g.tile + j - g.first) + (t >> 6), st = half % S::kVStages;
                     ok = mbarWait(&s->vFull[st], (half / S::kVStages) & 1, &s->dead, errFlag, waitLimit, 53);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) break;
                     const uint32_t key = k0 + static_cast<uint32_t>(t);
                     const bool there = key < keyEnd && (inTree || key >= g.s.lo);
@@ -1002,6 +1024,28 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
 done:
     tcFenceBefore();
     __syncthreads();
+    if (*reinterpret_cast<volatile int*>(&s->dead)) {
+        // A wait ran out: neither the copies nor the products that are under way may outlive the block.
+        auto drain = [&](unsigned long long* bar, uint32_t parity) {
+            const long long t0 = clock64();
+            while (!mbarTest(bar, parity) && clock64() - t0 < kDrainCycles) {}
+        };
+        if (threadIdx.x == 0) {
+            constexpr int kRounds = FP8 ? 2 : 1;
+            for (int i = max(0, s->issuedK - kRounds * S::kKStages); i < s->issuedK; ++i) drain(&s->kFull[i % S::kKStages], (i / S::kKStages) & 1);
+            for (int i = max(0, s->issuedV - kRounds * S::kVStages); i < s->issuedV; ++i) drain(&s->vFull[i % S::kVStages], (i / S::kVStages) & 1);
+            for (int i = max(0, s->issuedRaw - S::kRawStages); i < s->issuedRaw; ++i) drain(&s->rawFull[i % S::kRawStages], (i / S::kRawStages) & 1);
+            if (s->issuedQ > 0) drain(&s->qFull, (s->issuedQ - 1) & 1);
+        }
+        if (warp == kMmaWarp && live) {
+            if (electOne()) {
+                ummaCommit(&s->drained);
+                drain(&s->drained, 0);
+            }
+            __syncwarp();
+        }
+        __syncthreads();
+    }
     if (warp == kMmaWarp) {
         tcFenceAfter();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");

@@ -338,6 +338,27 @@ def test_host_buffers_and_workspace(engine):
         engine.treeAttention(request)
 
 
+@pytest.mark.parametrize("dtype", [DT.float16, DT.bfloat16, DT.float8], ids=lambda d: d.name)
+@pytest.mark.parametrize("sizes", [[9, 20, 17], [40, 64, 3]])
+def test_waits_that_run_out_leave_the_context_usable(dtype, sizes):
+    """With a limit of one cycle the wait for the first key tile runs out while the copies are on their way: the
+    kernel waits for those, returns, and the call fails like any failed launch."""
+    engine = pam.PagedAttentionEngine()
+    case = TreeCase(50, [3000, 500, 70], sizes, dtype=dtype)
+    out = engine.makeBufferFrom(np.full(case.q.shape, 7, case.q.dtype))
+    request = case.request(engine, out)
+    engine.setWaitLimit(1)
+    engine.enableGracefulDegradation = False
+    with pytest.raises(pam.PagedAttentionError, match="bounded wait ran out"):
+        engine.treeAttention(request)
+    engine.enableGracefulDegradation = True
+    engine.treeAttention(request)
+    assert (from_io(out.download(io_numpy_dtype(dtype), case.q.shape), dtype) == 0).all()
+    engine.setWaitLimit(0)
+    case.check(engine)
+    engine.close()
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=lambda d: d.name)
 @pytest.mark.parametrize("dim", [33, 64, 80, 96, 128, 256])
 @pytest.mark.parametrize("size", [1, 12, 40, 70])
