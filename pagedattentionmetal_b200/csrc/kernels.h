@@ -3,6 +3,8 @@
 // synchronising.
 #pragma once
 
+#include <atomic>
+
 #include <cuda_runtime.h>
 
 #include <cstddef>
@@ -10,6 +12,19 @@
 #include <string>
 
 namespace pam {
+
+// Dynamic shared memory above 48 KB has to be allowed once per device and kernel.
+template <typename K>
+cudaError_t allowSmem(K kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 enum DType { kF32 = 0, kF16 = 1, kFP8 = 2, kBF16 = 3 };
 

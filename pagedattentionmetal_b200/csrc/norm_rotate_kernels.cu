@@ -213,19 +213,27 @@ __device__ __forceinline__ void turnPieces(F2 (&fa)[E / 2], F2 (&fb)[E / 2], con
 
 // ---- forward ----------------------------------------------------------------
 
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void copyAhead(void* to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+constexpr int kForwardStages = 4;        // rows in shared memory or on their way there
+
 // A block takes `rowsPer` rows.  A group of l.lanes lanes keeps one head of them (of the queries,
 // keys and values of a row, one after the other), so that its weights stay in registers and nothing
-// is divided inside the loop; the next row's loads are under way while a row is worked on.
-// Measured at 32768 rows of 32 + 8 + 8 heads of 128, float16 (806 MB): 155 us = 5.2 TB/s, 0.79 of the
-// copy rate; one row a block with a division per head 277 us; 8-byte pieces 242 us (twice the
-// instructions per byte); 64 registers 161 us, 48 with spills 181 us.
+// is divided inside the loop; rows come to shared memory by asynchronous copies, three ahead, each
+// thread its own pieces.  Measured at 32768 rows of 32 + 8 + 8 heads of 128, float16 (806 MB): 139 us =
+// 5.8 TB/s, 0.89 of the copy rate; two rows ahead 142 us, 96 registers (one block less on an SM) 195 us, 56
+// 154 us; one row ahead in registers 155 us; one row a block with a division per head 277 us; 8-byte
+// pieces 242 us (twice the instructions per byte).
 template <typename T, int BYTES>
-__global__ void __maxnreg__(56)
+__global__ void __maxnreg__(80)
 normRotateKernel(const __grid_constant__ NormRotateParams p, const Layout l, int rowsPer) {
     using P = Piece<T, BYTES>;
     constexpr int E = P::E;
     extern __shared__ __align__(16) unsigned char rowSmem[];
-    RowInfo* info = reinterpret_cast<RowInfo*>(rowSmem);                  // [rowsPer]
+    unsigned char* ring = rowSmem;                                        // [kForwardStages][2][threads][16]
+    RowInfo* info = reinterpret_cast<RowInfo*>(ring + kForwardStages * 2 * 16 * blockDim.x);              // [rowsPer]
     float* turns = reinterpret_cast<float*>(info + rowsPer);              // [rowsPer][rotaryDim]
     const int tid = threadIdx.x, half = p.rotaryDim / 2;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rowsPer;
@@ -260,18 +268,26 @@ normRotateKernel(const __grid_constant__ NormRotateParams p, const Layout l, int
             wa.load(weight + pa * E);
             if (hasB) wb.load(weight + pb * E);
         }
-        auto load = [&](int r, P& a, P& b) {
-            a = b = P();
-            if (!wanted || !hasA || r >= n || info[r].position < 0) return;
-            const T* at = src + (row0 + r) * stride;
-            a.load(at + pa * E);
-            if (hasB) b.load(at + pb * E);
+        auto place = [&](int r, int which) { return ring + static_cast<size_t>(((r % kForwardStages) * 2 + which) * blockDim.x + tid) * 16; };
+        auto fetch = [&](int r) {
+            if (wanted && hasA && r < n && info[r].position >= 0) {
+                const T* at = src + (row0 + r) * stride;
+                copyAhead(place(r, 0), at + pa * E, true);
+                copyAhead(place(r, 1), at + (hasB ? pb : pa) * E, hasB);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        P a, b;
-        load(0, a, b);
+#pragma unroll
+        for (int r = 0; r < kForwardStages - 1; ++r) fetch(r);
+#pragma unroll 1
         for (int r = 0; r < n; ++r) {
-            P na, nb;
-            load(r + 1, na, nb);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kForwardStages - 2) : "memory");
+            P a, b;
+            if (hasA) {                               // (lanes without a piece add zeros)
+                a.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 0));
+                b.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 1));
+            }
+            fetch(r + kForwardStages - 1);            // (where the row before this one was)
             F2 sq = 0ull;
             {
                 F2 fa[E / 2], fb[E / 2];
@@ -311,8 +327,6 @@ normRotateKernel(const __grid_constant__ NormRotateParams p, const Layout l, int
                     if (hasB) b.store(pool + at + pb * E);
                 }
             }
-            a = na;
-            b = nb;
         }
     }
 }
@@ -425,7 +439,11 @@ cudaError_t normRotateOf(const NormRotateParams& p, cudaStream_t stream, int* la
         headChunks(perRow, l.lanes, &chunks, &threads);
         // enough blocks for every SM first, then rows to share the look-ups and the weights
         const int rowsPer = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kForwardRows, p.numRows / (148 * 4))));
-        const size_t smem = static_cast<size_t>(rowsPer) * (sizeof(RowInfo) + (p.rotaryDim / 2) * sizeof(float2));
+        const size_t smem = static_cast<size_t>(threads) * kForwardStages * 2 * 16 + static_cast<size_t>(rowsPer) * (sizeof(RowInfo) + (p.rotaryDim / 2) * sizeof(float2));
+        // (at most 544 threads, 68 KB of rows, and 16 KB of turns)
+        static std::atomic<unsigned long long> done{0};
+        const cudaError_t allowed = allowSmem(normRotateKernel<T, BYTES>, 100 * 1024, done);
+        if (allowed != cudaSuccess) return allowed;
         const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.numRows) + rowsPer - 1) / rowsPer), chunks);
         normRotateKernel<T, BYTES><<<grid, threads, smem, stream>>>(p, l, rowsPer);
     }
@@ -439,10 +457,6 @@ constexpr int kBackwardRows = 32;        // rows that a block looks up at a time
 constexpr int kBackwardShare = 4;        // rows that a block has at least
 constexpr int kBackwardStages = 3;       // rows in shared memory or on their way there
 
-// 16 bytes to shared memory, or zeros.
-__device__ __forceinline__ void copyAhead(void* to, const void* from, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
 
 // As the forward kernel, every block with an equal share of the rows.  A group of lanes keeps one head
 // of a row and each lane its pieces of it, so that its share of the weight gradients stays in
@@ -730,8 +744,9 @@ cudaError_t normRotateBackwardOf(const NormRotateBackwardParams& p, int smCount,
         const int share = static_cast<int>((static_cast<int64_t>(p.numRows) + blocks - 1) / blocks);
         const size_t smem = static_cast<size_t>(threads) * kBackwardStages * 4 * 16 +
                             kBackwardRows * (sizeof(RowInfo) + (p.rotaryDim / 2) * sizeof(float2));
-        // (at most 512 threads, 96 KB of rows, and 32 KB of turns)
-        const cudaError_t allowed = cudaFuncSetAttribute(normRotateBackwardKernel<T, BYTES>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        // (at most 544 threads, 102 KB of rows, and 33 KB of turns)
+        static std::atomic<unsigned long long> done{0};
+        const cudaError_t allowed = allowSmem(normRotateBackwardKernel<T, BYTES>, 160 * 1024, done);
         if (allowed != cudaSuccess) return allowed;
         normRotateBackwardKernel<T, BYTES><<<dim3(blocks, chunks), threads, smem, stream>>>(p, l, share);
     } else {

@@ -502,19 +502,6 @@ cudaError_t launchJoin(const TreeParams& p, const TreePlan& plan, cudaStream_t s
     return launchEarly(treeJoinKernel<QT, KT_>, dim3(blocks, (plan.rows + 7) / 8), 256, 0, stream, p, plan.blocks, plan.rows, plan.dimPad);
 }
 
-// Dynamic shared memory above 48 KB has to be allowed once per device and kernel.
-template <typename K>
-cudaError_t allowSmem(K kernel, size_t bytes, std::atomic<unsigned long long>& done) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
-    return e;
-}
-
 TreePlan generalPlan(const TreeParams& p, int smCount) {
     TreePlan t{};
     t.rows = p.headDim <= 128 && static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) > 16 ? 32 : 16;

@@ -528,15 +528,8 @@ template <typename T, int HD, int MR, bool FP8>
 cudaError_t launchOne(const TreeParams& p, int blocks, float scaleLog2, cudaStream_t stream) {
     static std::atomic<unsigned long long> done{0};
     using S = Shape<HD, MR, FP8>;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    const cudaError_t e = allowSmem(treeMmaKernel<T, HD, MR, FP8>, S::bytes(kTreeMaxBatch), done);
     if (e != cudaSuccess) return e;
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (!(done.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(treeMmaKernel<T, HD, MR, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::bytes(kTreeMaxBatch)));
-        if (e != cudaSuccess) return e;
-        done.fetch_or(bit, std::memory_order_relaxed);
-    }
     return launchEarly(treeMmaKernel<T, HD, MR, FP8>, dim3(blocks), kThreads, S::bytes(p.batch), stream, p, scaleLog2);
 }
 
