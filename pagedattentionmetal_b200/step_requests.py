@@ -17,10 +17,12 @@ def _span(x) -> _cabi.PamBuffer:
     """A buffer argument with its length; a strided torch view reaches from its first to its last element."""
     if x is None:
         return _cabi.PamBuffer(None, 0)
-    if hasattr(x, "is_contiguous") and x.numel() and not x.is_contiguous():
-        last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
-        return _cabi.PamBuffer(x.data_ptr(), (last + 1) * x.element_size())
-    return _cabi.buffer(x)
+    if not hasattr(x, "is_contiguous"):
+        return _cabi.buffer(x)
+    elements = x.numel()
+    if elements and not x.is_contiguous():
+        elements = 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return _cabi.PamBuffer(x.data_ptr(), elements * x.element_size())
 
 
 class _Request:
@@ -49,13 +51,13 @@ class _Request:
         if name not in self._fields:
             raise AttributeError(f"{type(self).__name__} has no field {name}")
         field, default = self._fields[name]
-        if isinstance(value, PagedLayerSpec):
+        if default is None:
+            c = _span(value)
+        elif isinstance(value, PagedLayerSpec):
             c = _cabi.PamLayerSpec(value.headDim, value.numHeads, value.numKVHeads, value.blockSize,
                                    int(value.dataType), value.windowSize)
         elif isinstance(default, float):
             c = float(value)
-        elif default is None:
-            c = _span(value)
         else:
             c = int(value)
         setattr(self._c, field, c)
