@@ -338,6 +338,62 @@ def test_host_buffers_and_workspace(engine):
         engine.treeAttention(request)
 
 
+@pytest.mark.parametrize("recorded", [False, True])
+@pytest.mark.parametrize("dtype", [DT.float32, DT.float16], ids=lambda d: d.name)
+@pytest.mark.parametrize("dim", [128, 40])
+def test_inputs_from_copies_and_other_streams_are_complete(engine, dtype, dim, recorded):
+    """The kernels are set up early, but read nothing before what precedes them: a copy on their stream, and a
+    stream that theirs waits for, which writes the queries at the end of a long queue."""
+    torch = pytest.importorskip("torch")
+    case = TreeCase(51, [3000, 500, 70], [9, 20, 17], dtype=dtype, dim=dim)
+    out = engine.makeBufferFrom(np.zeros(case.q.shape, case.q.dtype))
+    request = case.request(engine, out)
+    engine.treeAttention(request)
+    want = out.download(io_numpy_dtype(dtype), case.q.shape)
+    q, v = (torch.from_numpy(x.view(np.uint8).reshape(-1).copy()).pin_memory() for x in (case.q, case.v))
+    device = [torch.zeros_like(x, device="cuda") for x in (q, v)]
+    ready = q.cuda()
+    request.q, request.v = device
+    request.workspace = engine.makeBuffer(engine.treeAttentionWorkspace(request))
+    mine, other = torch.cuda.Stream(), torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device="cuda")
+
+    def work():
+        other.wait_stream(mine)
+        with torch.cuda.stream(other):
+            x = busy
+            for _ in range(10):
+                x = x @ busy
+            device[0].copy_(ready)
+        mine.wait_stream(other)
+        device[1].copy_(v, non_blocking=True)
+        engine.treeAttention(request)
+
+    engine.setAsync(True)
+    engine.setStream(mine.cuda_stream)
+    try:
+        torch.cuda.synchronize()
+        with torch.cuda.stream(mine):
+            work()
+        torch.cuda.synchronize()
+        if recorded:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=mine):
+                work()
+            for _ in range(3):
+                for t in device:
+                    t.zero_()
+                out.upload(np.zeros(case.q.shape, case.q.dtype))
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+            del graph
+    finally:
+        engine.setStream(None)
+        engine.setAsync(False)
+    assert np.array_equal(out.download(io_numpy_dtype(dtype), case.q.shape), want)
+
+
 @pytest.mark.parametrize("dtype", [DT.float16, DT.bfloat16, DT.float8], ids=lambda d: d.name)
 @pytest.mark.parametrize("sizes", [[9, 20, 17], [40, 64, 3]])
 def test_waits_that_run_out_leave_the_context_usable(dtype, sizes):
