@@ -233,12 +233,13 @@ struct NormRotateParams {
     const void *qWeight, *kWeight;   // [dim], io type
     const float* invFreq;         // [rotaryDim / 2]
     const int32_t* positions;     // [numRows]; negative: the row is skipped
-    void *qOut, *kOut, *vOut;     // rows; kOut and vOut may be null
+    void *qOut, *kOut;            // rows; kOut may be null
     void *kPool, *vPool;          // pages, or null; with them slots
     const int64_t* slots;         // [numRows]; a slot outside [0, numSlots) is not written
-    int64_t* slotsOut;            // or null: the slots again, -1 for rows that are skipped
+    int64_t* slotsOut;            // or null: the slots again, -1 for rows that are skipped; kPool and vPool are then
+                                  // back-to-back rows (or null), written whatever the slots are
     int64_t numSlots;
-    int64_t qStride, kStride, vStride, qOutStride, kOutStride, vOutStride;   // elements
+    int64_t qStride, kStride, vStride, qOutStride, kOutStride;   // elements
     int numRows, heads, kvHeads, headDim, blockSize, rotaryDim, interleaved, ioType;
     float eps;
 };

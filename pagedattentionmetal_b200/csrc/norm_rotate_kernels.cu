@@ -181,12 +181,13 @@ struct RowInfo {
     int position;      // negative: skipped
 };
 
-// Positions, slots and turns of rows [row0, row0 + n) into shared memory.
+// Positions, slots and turns of rows [row0, row0 + n) into shared memory.  rowPools: the pools are rows back to
+// back, row r at place r.
 __device__ __forceinline__ void lookRowsUp(RowInfo* info, float* turns, int64_t row0, int n, const int32_t* positions, const int64_t* slots,
-                                           int64_t numSlots, const float* invFreq, int half, int kvHeads, int blockSize, int dim) {
+                                           int64_t numSlots, const float* invFreq, int half, int kvHeads, int blockSize, int dim, bool rowPools) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         info[i].position = positions[row0 + i];
-        info[i].pool = slots ? poolBase(slots[row0 + i], numSlots, kvHeads, blockSize, dim) : -1;
+        info[i].pool = rowPools ? (row0 + i) * kvHeads * dim : slots ? poolBase(slots[row0 + i], numSlots, kvHeads, blockSize, dim) : -1;
     }
     for (int i = threadIdx.x; i < n * half; i += blockDim.x) {
         const int r = i / half, pos = positions[row0 + r];
@@ -238,7 +239,7 @@ normRotateKernel(const __grid_constant__ NormRotateParams p, const Layout l, int
     const int tid = threadIdx.x, half = p.rotaryDim / 2;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rowsPer;
     const int n = static_cast<int>(min(static_cast<int64_t>(rowsPer), p.numRows - row0));
-    lookRowsUp(info, turns, row0, n, p.positions, p.slots, p.numSlots, p.invFreq, half, p.kvHeads, p.blockSize, p.headDim);
+    lookRowsUp(info, turns, row0, n, p.positions, p.slots, p.numSlots, p.invFreq, half, p.kvHeads, p.blockSize, p.headDim, p.slotsOut != nullptr);
     if (p.slotsOut && blockIdx.y == 0)
         for (int i = tid; i < n; i += blockDim.x) p.slotsOut[row0 + i] = info[i].position >= 0 ? p.slots[row0 + i] : -1;
     const int lane = tid & (l.lanes - 1), group = tid / l.lanes, groups = blockDim.x / l.lanes;
@@ -252,16 +253,16 @@ normRotateKernel(const __grid_constant__ NormRotateParams p, const Layout l, int
         const int h = static_cast<int>(blockIdx.y) * groups + group;
         const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads;
         const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
-        const bool wanted = h < perRow && !(isV && !p.vPool && !p.vOut);
+        const bool wanted = h < perRow && !(isV && !p.vPool);
         const T* src = isQ ? static_cast<const T*>(p.q) + static_cast<int64_t>(h) * p.headDim
                      : isV ? static_cast<const T*>(p.v) + static_cast<int64_t>(kvh) * p.headDim
                            : static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * p.headDim;
         const int64_t stride = isQ ? p.qStride : isV ? p.vStride : p.kStride;
-        T* rows = static_cast<T*>(isQ ? p.qOut : isV ? p.vOut : p.kOut);
-        const int64_t rowsStride = isQ ? p.qOutStride : isV ? p.vOutStride : p.kOutStride;
+        T* rows = static_cast<T*>(isQ ? p.qOut : isV ? nullptr : p.kOut);
+        const int64_t rowsStride = isQ ? p.qOutStride : p.kOutStride;
         if (rows) rows += static_cast<int64_t>(isQ ? h : kvh) * p.headDim;
         T* pool = isQ ? nullptr : static_cast<T*>(isV ? p.vPool : p.kPool);
-        if (pool) pool += static_cast<int64_t>(kvh) * p.blockSize * p.headDim;
+        if (pool) pool += static_cast<int64_t>(kvh) * (p.slotsOut ? 1 : p.blockSize) * p.headDim;
         P wa, wb;
         if (wanted && !isV && hasA) {
             const T* weight = static_cast<const T*>(isQ ? p.qWeight : p.kWeight);
@@ -356,7 +357,7 @@ normRotateAnyKernel(const __grid_constant__ NormRotateParams p) {
         if (p.slotsOut && h == 0 && lane == 0) p.slotsOut[row] = pos >= 0 ? p.slots[row] : -1;
         if (pos < 0) continue;
         const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads;
-        if (isV && !p.vPool && !p.vOut) continue;
+        if (isV && !p.vPool) continue;
         const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
         const T* src = isQ ? static_cast<const T*>(p.q) + row * p.qStride + static_cast<int64_t>(h) * p.headDim
                      : isV ? static_cast<const T*>(p.v) + row * p.vStride + static_cast<int64_t>(kvh) * p.headDim
@@ -373,12 +374,12 @@ normRotateAnyKernel(const __grid_constant__ NormRotateParams p) {
         T* dst[2] = {nullptr, nullptr};
         if (isQ) dst[0] = static_cast<T*>(p.qOut) + row * p.qOutStride + static_cast<int64_t>(h) * p.headDim;
         else {
-            void* rows = isV ? p.vOut : p.kOut;
             void* pool = isV ? p.vPool : p.kPool;
-            if (rows) dst[0] = static_cast<T*>(rows) + row * (isV ? p.vOutStride : p.kOutStride) + static_cast<int64_t>(kvh) * p.headDim;
+            if (!isV && p.kOut) dst[0] = static_cast<T*>(p.kOut) + row * p.kOutStride + static_cast<int64_t>(kvh) * p.headDim;
             if (pool) {
                 const int64_t slot = p.slots[row];
-                if (slot >= 0 && slot < p.numSlots)
+                if (p.slotsOut) dst[1] = static_cast<T*>(pool) + (row * p.kvHeads + kvh) * p.headDim;
+                else if (slot >= 0 && slot < p.numSlots)
                     dst[1] = static_cast<T*>(pool) + poolOffset(slot, kvh, p.kvHeads, p.blockSize, p.headDim);
             }
         }
@@ -425,10 +426,10 @@ inline void headChunks(int perRow, int lanes, int* chunks, int* threads) {
 template <typename T>
 cudaError_t normRotateOf(const NormRotateParams& p, cudaStream_t stream, int* launches) {
     constexpr int BYTES = 16, E = BYTES / sizeof(T);
-    const void* ptrs[] = {p.q, p.k, p.v, p.qWeight, p.kWeight, p.qOut, p.kOut, p.vOut, p.kPool, p.vPool};
+    const void* ptrs[] = {p.q, p.k, p.v, p.qWeight, p.kWeight, p.qOut, p.kOut, p.kPool, p.vPool};
     bool pieces = piecesApply<E>(p.headDim, p.rotaryDim, p.interleaved);
     for (const void* ptr : ptrs) pieces = pieces && aligned16(ptr);
-    for (int64_t s : {p.qStride, p.kStride, p.vStride, p.qOutStride, p.kOutStride, p.vOutStride}) pieces = pieces && s % E == 0;
+    for (int64_t s : {p.qStride, p.kStride, p.vStride, p.qOutStride, p.kOutStride}) pieces = pieces && s % E == 0;
     const int perRow = p.heads + 2 * p.kvHeads;
     if (!pieces) {
         const int64_t warps = static_cast<int64_t>(p.numRows) * perRow;
@@ -512,7 +513,7 @@ normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, con
         for (int64_t row0 = begin; row0 < end; row0 += kBackwardRows) {
             const int n = static_cast<int>(min(static_cast<int64_t>(kBackwardRows), end - row0));
             __syncthreads();
-            lookRowsUp(info, turns, row0, n, p.positions, p.slots, p.numSlots, p.invFreq, half, p.kvHeads, p.blockSize, p.headDim);
+            lookRowsUp(info, turns, row0, n, p.positions, p.slots, p.numSlots, p.invFreq, half, p.kvHeads, p.blockSize, p.headDim, false);
             // A thread copies what it will read itself, two rows ahead; nobody waits for anybody.
             auto place = [&](int r, int which) { return ring + static_cast<size_t>(((r % kBackwardStages) * 4 + which) * threads + tid) * 16; };
             auto fetch = [&](int r) {

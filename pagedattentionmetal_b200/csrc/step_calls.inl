@@ -329,7 +329,7 @@ int32_t pamc_norm_rotate(void* ctx, const PamNormRotateRequest* request, void* c
         p.positions = static_cast<const int32_t*>(args[6].device);
         p.qOut = args[7].device; p.kOut = args[8].device;
         p.slots = static_cast<const int64_t*>(args[11].device);
-        p.qStride = qs; p.kStride = ks; p.vStride = vs; p.qOutStride = qo; p.kOutStride = ko; p.vOutStride = kWide;
+        p.qStride = qs; p.kStride = ks; p.vStride = vs; p.qOutStride = qo; p.kOutStride = ko;
         p.numRows = rq.num_rows; p.heads = l.num_heads; p.kvHeads = l.num_kv_heads; p.headDim = l.head_dim;
         p.blockSize = l.block_size; p.rotaryDim = rq.rotary_dim; p.interleaved = rq.interleaved != 0;
         p.ioType = fp8 ? PAM_DTYPE_F16 : l.data_type;
@@ -339,30 +339,23 @@ int32_t pamc_norm_rotate(void* ctx, const PamNormRotateRequest* request, void* c
             p.kPool = args[9].device; p.vPool = args[10].device;
             return pam::launchNormRotate(p, c->stream, launches);
         }
-        // FP8: the scale of a block needs every new row of it first, so the rows are finished in
-        // scratch and go through the append kernels; skipped rows lose their slot.
+        // FP8: the scale of a block needs every new row of it first, so the rows go through the append
+        // kernels, which take them back to back: from kOut and V where they are, else from scratch that the
+        // same launch writes beside kOut (one launch, since the outputs may lie over the inputs).  Skipped
+        // rows lose their slot.
         const size_t bytes = static_cast<size_t>(R) * kWide * io;
-        if (!p.kOut || ko != kWide) {
-            // (a strided kOut is written by a launch of its own)
-            if (p.kOut) {
-                pam::NormRotateParams only = p;
-                cudaError_t e = pam::launchNormRotate(only, c->stream, launches);
-                if (e != cudaSuccess) return e;
-            }
-            p.kOut = c->arena.take(bytes);
-            p.kOutStride = kWide;
-        }
-        const void* values = p.v;
-        if (vs != kWide) values = p.vOut = c->arena.take(bytes);
+        const void *keys = p.kOut, *values = p.v;
+        if (!p.kOut || ko != kWide) keys = p.kPool = c->arena.take(bytes);
+        if (vs != kWide) values = p.vPool = c->arena.take(bytes);
         p.slotsOut = static_cast<int64_t*>(c->arena.take(static_cast<size_t>(R) * 8));
-        if (!p.kOut || !values || !p.slotsOut) return cudaErrorMemoryAllocation;
+        if (!keys || !values || !p.slotsOut) return cudaErrorMemoryAllocation;
         cudaError_t e = nextAbsmaxEpoch(k, c->stream);
         if (e == cudaSuccess) e = pam::launchNormRotate(p, c->stream, launches);
         if (e != cudaSuccess) return e;
         pam::SlotSource src;
         src.slots = p.slotsOut;
         src.numSlots = static_cast<int64_t>(k->maxBlocks) * k->blockSize;
-        return pam::launchReshapeAndCacheFp8(p.kOut, values, k->kPool, k->vPool, k->kScale, k->vScale, src, rq.num_rows, l.num_kv_heads,
+        return pam::launchReshapeAndCacheFp8(keys, values, k->kPool, k->vPool, k->kScale, k->vScale, src, rq.num_rows, l.num_kv_heads,
                                              l.block_size, l.head_dim, k->amax, k->epoch, c->stream, launches);
     });
     if (rc != 0) return rc;

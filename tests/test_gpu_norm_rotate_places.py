@@ -1,0 +1,48 @@
+"""normRotate and normRotateBackward where their buffers may lie: outputs over the inputs, columns of one array of
+the host, addresses off the 16-byte grid.  The same call with every buffer on its own is held against float64 by
+test_gpu_norm_rotate.py; here its bits are the reference."""
+import numpy as np
+import pytest
+
+import pagedattentionmetal_b200 as pam
+from gpu_helpers import DT
+from test_gpu_norm_rotate import NormCase, pam_buffer
+
+pytestmark = pytest.mark.gpu
+
+
+def pools_equal(one, two):
+    for a, b in zip(one.readPools(), two.readPools()):
+        assert (a is None) == (b is None)
+        if a is not None:
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+
+
+@pytest.mark.parametrize("shape", [dict(heads=8, kv_heads=2, dim=64), dict(heads=32, kv_heads=8, dim=128, interleaved=True),
+                                   dict(heads=4, kv_heads=2, dim=33, rotary=32)], ids=lambda s: f"dim{s['dim']}")
+@pytest.mark.parametrize("dtype", [DT.float8, DT.float16, DT.bfloat16], ids=lambda d: d.name)
+@pytest.mark.parametrize("over", ["q", "k", "both"])
+def test_in_place_with_an_append(engine, dtype, shape, over):
+    """Queries and keys over the projection's own rows while the keys and values go to the pages."""
+    case = NormCase(61, rows=50, dtype=dtype, **shape)
+    one, two = (pam.KVCacheManager(engine, case.blocks, case.block, case.D, case.KVH, dtype) for _ in range(2))
+    slots = engine.makeBufferFrom(case.slots)
+    apart, keep = case.inputs(engine)
+    q, k = (engine.makeBufferFrom(np.zeros((case.R, n, case.D), np.uint16)) for n in (case.H, case.KVH))
+    engine.normRotate(pam.PagedNormRotateRequest(**apart, **case.common(engine), qOut=q, kOut=k, slots=slots), two)
+    q, k = q.download(np.uint16, (case.R, case.H * case.D)), k.download(np.uint16, (case.R, case.KVH * case.D))
+    inputs, base = case.inputs(engine)
+    side = engine.makeBufferFrom(np.zeros((case.R, case.wide), np.uint16))
+    part = lambda b, i: pam_buffer(b, case.at[i] * 2, b.nbytes - case.at[i] * 2)
+    q_base, k_base = (base if over in (x, "both") else side for x in "qk")
+    engine.normRotate(pam.PagedNormRotateRequest(**inputs, **case.common(engine), qOut=part(q_base, 0), qOutStride=case.wide,
+                                                 kOut=part(k_base, 1), kOutStride=case.wide, slots=slots), one)
+    pools_equal(one, two)
+    want = case.qkv.view(np.uint16).copy()
+    rest = np.zeros_like(want)
+    for i, (rows, target) in enumerate(((q, want if q_base is base else rest), (k, want if k_base is base else rest))):
+        target[case.live, case.at[i]:case.at[i + 1]] = rows[case.live]
+    assert np.array_equal(base.download(np.uint16, want.shape), want)
+    assert np.array_equal(side.download(np.uint16, want.shape), rest)
+    one.close()
+    two.close()
