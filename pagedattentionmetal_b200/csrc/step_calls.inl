@@ -3,7 +3,13 @@
 
 namespace {
 
-// One buffer of a call: what it must hold, which way it goes, and the address the kernels use.
+// Rows of `width` bytes that start `pitch` bytes apart.
+struct StepRows {
+    size_t count, width, pitch;
+};
+
+// One buffer of a call: what it must hold, which way it goes, the address the kernels use, and for rows that
+// may be strided (count > 0) what of it is the call's.
 struct StepArg {
     const char* name;
     const PamBuffer* buffer;
@@ -11,6 +17,7 @@ struct StepArg {
     bool output, optional;
     bool onDevice;
     void* device;
+    StepRows rows;
 };
 
 bool stepSizes(Context* c, StepArg* args, int n) {
@@ -50,6 +57,14 @@ bool stepPlaces(Context* c, StepArg* args, int n, bool capturing) {
     return true;
 }
 
+// What lies between strided rows belongs to somebody else (often another output of the same call), so that
+// only the rows themselves are copied.
+cudaError_t stepCopy(Context* c, const StepArg& a, void* to, const void* from, cudaMemcpyKind kind) {
+    const StepRows& r = a.rows;
+    if (r.count < 2 || r.width == r.pitch) return cudaMemcpyAsync(to, from, a.need, kind, c->stream);
+    return cudaMemcpy2DAsync(to, r.pitch, from, r.pitch, r.width, r.count, kind, c->stream);
+}
+
 // Host buffers go through the arena.  A host output goes up as well: the kernels leave parts of
 // it as they were.
 cudaError_t stepStage(Context* c, StepArg* args, int n) {
@@ -58,7 +73,7 @@ cudaError_t stepStage(Context* c, StepArg* args, int n) {
         if (a.onDevice || !a.buffer->ptr || a.need == 0) continue;
         a.device = c->arena.take(a.need);
         if (!a.device) return cudaErrorMemoryAllocation;
-        cudaError_t e = cudaMemcpyAsync(a.device, a.buffer->ptr, a.need, cudaMemcpyHostToDevice, c->stream);
+        cudaError_t e = stepCopy(c, a, a.device, a.buffer->ptr, cudaMemcpyHostToDevice);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -67,7 +82,7 @@ cudaError_t stepBack(Context* c, StepArg* args, int n) {
     for (int i = 0; i < n; ++i) {
         StepArg& a = args[i];
         if (a.onDevice || !a.buffer->ptr || !a.output || a.need == 0) continue;
-        cudaError_t e = cudaMemcpyAsync(a.buffer->ptr, a.device, a.need, cudaMemcpyDeviceToHost, c->stream);
+        cudaError_t e = stepCopy(c, a, a.buffer->ptr, a.device, cudaMemcpyDeviceToHost);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -122,6 +137,9 @@ int32_t badStep(Context* c, const std::string& m) { return c->fail(PAM_ERR_INVAL
 // Bytes from the first element of a strided array of rows to its last.
 size_t rowSpan(int64_t rows, int64_t stride, int64_t width, int elem) {
     return static_cast<size_t>((rows - 1) * stride + width) * elem;
+}
+StepRows stridedRows(int64_t rows, int64_t stride, int64_t width, int elem) {
+    return {static_cast<size_t>(rows), static_cast<size_t>(width) * elem, static_cast<size_t>(stride) * elem};
 }
 bool rowStride(Context* c, int64_t given, int64_t width, const char* name, int64_t* out) {
     *out = given == 0 ? width : given;
@@ -297,15 +315,15 @@ int32_t pamc_norm_rotate(void* ctx, const PamNormRotateRequest* request, void* c
     const size_t poolNeed = pages ? static_cast<size_t>(l.block_size) * kvBytesPerToken(l) : 0;
     static const PamBuffer none{nullptr, 0};
     StepArg args[] = {
-        {"Q", &rq.q, rowSpan(R, qs, qWide, io), false, false, false, nullptr},
-        {"K", &rq.k, rowSpan(R, ks, kWide, io), false, false, false, nullptr},
-        {"V", pages ? &rq.v : &none, rowSpan(R, vs, kWide, io), false, !pages, false, nullptr},
+        {"Q", &rq.q, rowSpan(R, qs, qWide, io), false, false, false, nullptr, stridedRows(R, qs, qWide, io)},
+        {"K", &rq.k, rowSpan(R, ks, kWide, io), false, false, false, nullptr, stridedRows(R, ks, kWide, io)},
+        {"V", pages ? &rq.v : &none, rowSpan(R, vs, kWide, io), false, !pages, false, nullptr, stridedRows(R, vs, kWide, io)},
         {"qWeight", &rq.q_weight, static_cast<size_t>(l.head_dim) * io, false, false, false, nullptr},
         {"kWeight", &rq.k_weight, static_cast<size_t>(l.head_dim) * io, false, false, false, nullptr},
         {"invFreq", &rq.inv_freq, static_cast<size_t>(rq.rotary_dim / 2) * 4, false, rq.rotary_dim == 0, false, nullptr},
         {"positions", &rq.positions, static_cast<size_t>(R) * 4, false, false, false, nullptr},
-        {"qOut", &rq.q_out, rowSpan(R, qo, qWide, io), true, false, false, nullptr},
-        {"kOut", &rq.k_out, rowSpan(R, ko, kWide, io), true, true, false, nullptr},
+        {"qOut", &rq.q_out, rowSpan(R, qo, qWide, io), true, false, false, nullptr, stridedRows(R, qo, qWide, io)},
+        {"kOut", &rq.k_out, rowSpan(R, ko, kWide, io), true, true, false, nullptr, stridedRows(R, ko, kWide, io)},
         {"K pool", &kPool, poolNeed, true, true, false, nullptr},
         {"V pool", &vPool, poolNeed, true, true, false, nullptr},
         {"slots", pages ? &rq.slots : &none, static_cast<size_t>(R) * 8, false, !pages, false, nullptr},
@@ -404,8 +422,8 @@ int32_t pamc_norm_rotate_backward(void* ctx, const PamNormRotateBackwardRequest*
     static const PamBuffer none{nullptr, 0};
     const bool wantV = rq.d_v.ptr != nullptr;
     StepArg args[] = {
-        {"Q", &rq.q, rowSpan(R, qs, qWide, io), false, false, false, nullptr},
-        {"K", &rq.k, rowSpan(R, ks, kWide, io), false, false, false, nullptr},
+        {"Q", &rq.q, rowSpan(R, qs, qWide, io), false, false, false, nullptr, stridedRows(R, qs, qWide, io)},
+        {"K", &rq.k, rowSpan(R, ks, kWide, io), false, false, false, nullptr, stridedRows(R, ks, kWide, io)},
         {"qWeight", &rq.q_weight, weight, false, false, false, nullptr},
         {"kWeight", &rq.k_weight, weight, false, false, false, nullptr},
         {"invFreq", &rq.inv_freq, static_cast<size_t>(rq.rotary_dim / 2) * 4, false, rq.rotary_dim == 0, false, nullptr},
@@ -415,9 +433,9 @@ int32_t pamc_norm_rotate_backward(void* ctx, const PamNormRotateBackwardRequest*
         {"dK pool", &rq.d_k_pool, poolNeed, false, true, false, nullptr},
         {"dV pool", wantV ? &rq.d_v_pool : &none, poolNeed, false, !wantV, false, nullptr},
         {"slots", pages ? &rq.slots : &none, static_cast<size_t>(R) * 8, false, !pages, false, nullptr},
-        {"dQ", &rq.d_q, rowSpan(R, dq, qWide, io), true, false, false, nullptr},
-        {"dK", &rq.d_k, rowSpan(R, dk, kWide, io), true, false, false, nullptr},
-        {"dV", &rq.d_v, rowSpan(R, dv, kWide, io), true, true, false, nullptr},
+        {"dQ", &rq.d_q, rowSpan(R, dq, qWide, io), true, false, false, nullptr, stridedRows(R, dq, qWide, io)},
+        {"dK", &rq.d_k, rowSpan(R, dk, kWide, io), true, false, false, nullptr, stridedRows(R, dk, kWide, io)},
+        {"dV", &rq.d_v, rowSpan(R, dv, kWide, io), true, true, false, nullptr, stridedRows(R, dv, kWide, io)},
         {"dQWeight", &rq.d_q_weight, static_cast<size_t>(l.head_dim) * 4, true, true, false, nullptr},
         {"dKWeight", &rq.d_k_weight, static_cast<size_t>(l.head_dim) * 4, true, true, false, nullptr},
         {"workspace", &rq.workspace, 0, true, true, false, nullptr},
@@ -512,9 +530,9 @@ int32_t pamc_tree_attention(void* ctx, const PamTreeAttentionRequest* request) {
     const size_t outBytes = static_cast<size_t>(R) * qWide * io, scaleNeed = static_cast<size_t>(l.num_kv_heads) * 2;
     static const PamBuffer none{nullptr, 0};
     StepArg args[] = {
-        {"Q", &rq.q, rowSpan(R, p.qStride, qWide, io), false, false, false, nullptr},
-        {"K", &rq.k, rowSpan(R, p.kStride, kWide, io), false, false, false, nullptr},
-        {"V", &rq.v, rowSpan(R, p.vStride, kWide, io), false, false, false, nullptr},
+        {"Q", &rq.q, rowSpan(R, p.qStride, qWide, io), false, false, false, nullptr, stridedRows(R, p.qStride, qWide, io)},
+        {"K", &rq.k, rowSpan(R, p.kStride, kWide, io), false, false, false, nullptr, stridedRows(R, p.kStride, kWide, io)},
+        {"V", &rq.v, rowSpan(R, p.vStride, kWide, io), false, false, false, nullptr, stridedRows(R, p.vStride, kWide, io)},
         {"K pool", &rq.k_pool, poolNeed, false, false, false, nullptr},
         {"V pool", &rq.v_pool, poolNeed, false, false, false, nullptr},
         {"blockTables", &rq.block_tables, B * rq.max_num_blocks * 4, false, false, false, nullptr},

@@ -46,3 +46,60 @@ def test_in_place_with_an_append(engine, dtype, shape, over):
     assert np.array_equal(side.download(np.uint16, want.shape), rest)
     one.close()
     two.close()
+
+
+def host_columns(case, values, dtype=None):
+    """One array of the host and its columns: queries, keys, values."""
+    torch = pytest.importorskip("torch")
+    wide = torch.from_numpy(values.copy())
+    return wide, [wide[:, a:b] for a, b in zip(case.at, case.at[1:])]
+
+
+@pytest.mark.parametrize("dtype", [DT.float32, DT.float16], ids=lambda d: d.name)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_forward_into_columns_of_one_host_array(engine, dtype, in_place):
+    case = NormCase(62, 13, 4, 2, 64, dtype=dtype, offset=8)
+    inputs, keep = case.inputs(engine)
+    q, k = (engine.makeBufferFrom(np.zeros((case.R, n, case.D), case.io)) for n in (case.H, case.KVH))
+    engine.normRotate(pam.PagedNormRotateRequest(**inputs, **case.common(engine), qOut=q, kOut=k))
+    want = case.qkv.copy() if in_place else np.full_like(case.qkv, 7)
+    for i, (rows, n) in enumerate(((q, case.H), (k, case.KVH))):
+        want[case.live, case.at[i]:case.at[i + 1]] = rows.download(case.io, (case.R, n * case.D))[case.live]
+    source, columns = host_columns(case, case.qkv)
+    target, outs = (source, columns) if in_place else host_columns(case, np.full_like(case.qkv, 7))
+    common = case.common(engine)
+    engine.normRotate(pam.PagedNormRotateRequest(q=columns[0], k=columns[1], qStride=case.wide, kStride=case.wide, **common,
+                                                 qOut=outs[0], qOutStride=case.wide, kOut=outs[1], kOutStride=case.wide))
+    assert np.array_equal(target.numpy(), want)
+    if not in_place:
+        assert np.array_equal(source.numpy(), case.qkv)
+
+
+@pytest.mark.parametrize("dtype", [DT.float32, DT.float16], ids=lambda d: d.name)
+@pytest.mark.parametrize("pages", [False, True])
+def test_gradient_into_columns_of_one_host_array(engine, dtype, pages):
+    case = NormCase(63, 13, 4, 2, 64, dtype=dtype, offset=8)
+    rng = np.random.default_rng(64)
+    up, rnd = engine.makeBufferFrom, lambda *s: rng.standard_normal(s, dtype=np.float32).astype(case.io)
+    dq_out, pool = rnd(case.R, case.H, case.D), (case.blocks, case.KVH, case.block, case.D)
+    keys = dict(dKPool=up(rnd(*pool)), dVPool=up(rnd(*pool)), slots=up(case.slots)) if pages else dict(dKOut=up(rnd(case.R, case.KVH, case.D)))
+    inputs, keep = case.inputs(engine)
+    inputs = {x: y for x, y in inputs.items() if x not in ("v", "vStride")}
+    strides = dict(dQStride=case.wide, dKStride=case.wide, **(dict(dVStride=case.wide) if pages else {}))
+
+    def run(target, weights):
+        dv = dict(dV=target[2]) if pages else {}
+        engine.normRotateBackward(pam.PagedNormRotateBackwardRequest(
+            **inputs, **case.common(engine), dQOut=up(dq_out), **keys, **strides, dQ=target[0], dK=target[1], **dv,
+            dQWeight=weights[0], dKWeight=weights[1]))
+
+    fill = np.full_like(case.qkv, 7)
+    base, es = up(fill), fill.itemsize
+    weights = [up(np.zeros(case.D, np.float32)) for _ in range(2)]
+    run([pam_buffer(base, a * es, base.nbytes - a * es) for a in case.at[:3]], weights)
+    host, columns = host_columns(case, fill)
+    host_weights = [np.zeros(case.D, np.float32) for _ in range(2)]
+    run(columns, host_weights)
+    assert np.array_equal(host.numpy(), base.download(case.io, fill.shape))
+    for a, b in zip(weights, host_weights):
+        assert np.array_equal(a.download(np.float32, (case.D,)), b)
