@@ -566,8 +566,9 @@ int64_t pamc_norm_rotate_backward_workspace(void *ctx, const PamNormRotateBackwa
  * With a window W (layer.window_size, else the engine's default) a row at position p sees
  * only keys at positions > p - W, in the cache and in the tree; with masks that needs positions (a
  * position below the cache length counts as the cache length; without masks and positions row i
- * stands at cache_lengths[b] + i).  A row that sees nothing is written as zero; values a row
- * does not see do not reach it, whatever they hold; rows outside every request stay as they
+ * stands at cache_lengths[b] + i).  A row that sees nothing is written as zero; values and (FP8)
+ * scales a row does not see do not reach it, whatever they hold; a key scale that is not a finite
+ * number makes the rows that see its page NaN.  Rows outside every request stay as they
  * were.  Requests beyond max_new_tokens rows are cut off there. */
 typedef struct PamTreeAttentionRequest {
     PamBuffer q, k, v, k_pool, v_pool;

@@ -173,6 +173,14 @@ __device__ __forceinline__ int64_t poolRow(const TreeParams& p, int b, uint32_t 
     return ((blk * p.kvHeads + kvh) * p.blockSize + (token - page * p.blockSize)) * static_cast<int64_t>(p.headDim);
 }
 
+// The key scale of a page.  One that is not a finite number makes the scores of the rows that see the page NaN
+// (infinity times a code may be NaN or an infinity of either sign, by the code: kernels that scale the score
+// instead of the codes could not tell).
+__device__ __forceinline__ float keyScaleOf(__half scale) {
+    const float s = __half2float(scale);
+    return isOdd(s) ? __int_as_float(0x7FFFFFFF) : s;
+}
+
 // A pool's element; FP8: code times scale, in float32.
 template <typename KT_>
 __device__ __forceinline__ float poolValue(const TreeParams& p, const void* pool, const void* scale, int64_t at, int64_t blk, int kvh) {
@@ -208,16 +216,34 @@ template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float
 
 // Adds the values that were taken as zero although node i sees them to columns [d0, d1) of its row
 // of the result, which this thread (or its warp, before a __syncwarp) has stored.  hi: the first token
-// that every row of the row tile sees.
+// that every row of the row tile sees.  Behind it only FP8 pages are left out, those whose value scale is not a
+// finite number.  A key scale that is not (see keyScaleOf) makes the row NaN here, whatever the kernel took it for.
 template <typename QT, typename KT_>
 __device__ __noinline__ void addLeftOut(const TreeParams& p, SeqInfo s, int b, int kvh, int i, uint32_t hi, QT* row, int d0, int d1) {
-    for (uint32_t t = firstOf(p, s, i); t < hi; ++t) {
+    auto addToken = [&](uint32_t t) {
         int64_t blk;
         const int64_t at = poolRow(p, b, t, kvh, &blk);
         for (int d = d0; d < d1; ++d) {
             const float v = poolValue<KT_>(p, p.vPool, p.vScale, at + d, blk, kvh);
             if (isOdd(v)) row[d] = narrow<QT>(valueOf(row + d) + v);
         }
+    };
+    const uint32_t from = firstOf(p, s, i);
+    if constexpr (sizeof(KT_) == 1) {
+        for (uint32_t t = from; t < s.held;) {
+            const unsigned long long pageEnd = (static_cast<unsigned long long>(t / p.blockSize) + 1) * p.blockSize;
+            const uint32_t end = static_cast<uint32_t>(min(pageEnd, static_cast<unsigned long long>(s.held)));
+            int64_t blk;
+            poolRow(p, b, t, kvh, &blk);
+            const int64_t pair = blk * p.kvHeads + kvh;
+            const bool odd = isOdd(__half2float(static_cast<const __half*>(p.vScale)[pair]));
+            if (isOdd(__half2float(static_cast<const __half*>(p.kScale)[pair])))
+                for (int d = d0; d < d1; ++d) row[d] = narrow<QT>(__int_as_float(0x7FFFFFFF));
+            for (; t < (odd ? end : min(end, hi)); ++t) addToken(t);
+            t = end;
+        }
+    } else {
+        for (uint32_t t = from; t < hi; ++t) addToken(t);
     }
     for (int w = 0; w * 32 < s.n; ++w)
         for (uint32_t bits = treeBits(p, s, i, w); bits; bits &= bits - 1) {

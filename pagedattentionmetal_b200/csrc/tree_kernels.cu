@@ -176,7 +176,7 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2, bool wi
                         if (i >= kGenKeys * pieces) break;
                         float ks = 1.f, vs = 1.f;
                         if (sizeof(KT_) == 1 && !inTree && kAt[r] >= 0) {
-                            ks = __half2float(static_cast<const __half*>(p.kScale)[blkAt[r] * p.kvHeads + g.kvh]);
+                            ks = keyScaleOf(static_cast<const __half*>(p.kScale)[blkAt[r] * p.kvHeads + g.kvh]);
                             vs = __half2float(static_cast<const __half*>(p.vScale)[blkAt[r] * p.kvHeads + g.kvh]);
                         }
                         float e[4] = {vv[u].x * vs, vv[u].y * vs, vv[u].z * vs, vv[u].w * vs};
@@ -199,6 +199,7 @@ treeGeneralKernel(const __grid_constant__ TreeParams p, float scaleLog2, bool wi
                         vv = valueOf(static_cast<const QT*>(p.vNew) + vAt[r] + d);
                     } else {
                         kv = poolValue<KT_>(p, p.kPool, p.kScale, kAt[r] + d, blkAt[r], g.kvh);
+                        if (sizeof(KT_) == 1 && isOdd(kv)) kv = __int_as_float(0x7FFFFFFF);            // (see keyScaleOf; a code may be NaN itself)
                         vv = poolValue<KT_>(p, p.vPool, p.vScale, vAt[r] + d, blkAt[r], g.kvh);
                     }
                     if ((inTree || k0 + r < hi) && isOdd(vv)) { vv = 0.f; odd = true; }   // (some row may not see the key)

@@ -82,10 +82,12 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there
 __device__ __forceinline__ void commitGroup() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void waitGroups() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Where the rows of one tile come from (0: nowhere), and for FP8 their scales.
+// Where the rows of one tile come from (0: nowhere), and for FP8 their scales.  Values whose scale is not a finite
+// number come from nowhere, and `odd` says so for either half of the rows (see addLeftOut).
 struct RowSource {
     unsigned long long k[kKeys], v[kKeys];
     float kScale[kKeys], vScale[kKeys], vExp[kKeys];
+    int odd[2];
 };
 
 template <int HD, int MR, bool FP8>
@@ -146,6 +148,7 @@ treeMmaKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
         const int cacheTiles = ahead.s.cacheTiles<kKeys>(), i = tid & 63;
         const bool isV = tid >= 64, inTree = aheadJ >= cacheTiles;
         unsigned long long at = 0;
+        bool leftOut = false;
         if (inTree) {
             const int node = (aheadJ - cacheTiles) * kKeys + i;
             if (node < ahead.s.n)
@@ -164,14 +167,20 @@ treeMmaKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
                 at = reinterpret_cast<unsigned long long>(static_cast<const unsigned char*>(isV ? p.vPool : p.kPool) + row * (FP8 ? 1 : 2));
             }
             if (FP8) {
-                const float s = at ? __half2float(static_cast<const __half*>(isV ? p.vScale : p.kScale)[blk * p.kvHeads + ahead.kvh]) : 1.f;
+                const __half scale = at ? static_cast<const __half*>(isV ? p.vScale : p.kScale)[blk * p.kvHeads + ahead.kvh] : __float2half_rn(1.f);
                 if (isV) {
+                    float s = __half2float(scale);
+                    if (isOdd(s)) { s = 1.f; at = 0; leftOut = true; }
                     r.vScale[i] = s;
                     r.vExp[i] = s > 0.f ? static_cast<float>(ilogbf(s) + 1) : -25.f;
                 } else {
-                    r.kScale[i] = s;
+                    r.kScale[i] = keyScaleOf(scale);
                 }
             }
+        }
+        if (FP8 && isV) {
+            leftOut = __any_sync(0xFFFFFFFFu, leftOut);
+            if (lane == 0) r.odd[warp & 1] = leftOut ? 1 : 0;
         }
         (isV ? r.v : r.k)[i] = at;
         ++aheadT;
@@ -316,6 +325,7 @@ treeMmaKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
             }
             odd = __syncthreads_or(found) || odd;
         }
+        if (FP8) odd = odd || src.odd[0] != 0 || src.odd[1] != 0;
         // ---- scores of this warp's rows and keys
         float s[NB][4];
 #pragma unroll

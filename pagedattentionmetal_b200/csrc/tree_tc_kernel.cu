@@ -83,8 +83,10 @@ struct Span {
 constexpr int kSpans = 8;        // of the ring: no warp needs a span more than five behind the oldest one in use
 
 // FP8, of a key tile: per 16 keys (a page holds a multiple of them) the key scale times log2(e) /
-// sqrt(dim), the logarithm of the value scale, and one over it.  Where the value scale is zero the bit
-// in `zeros` is set, the values are converted to zeros and the scale counts as one.
+// sqrt(dim), the logarithm of the value scale, and one over it.  Pages with other than positive finite scales
+// are rare and prepared apart (preparePages): where the value scale is zero or not a finite number the bit in
+// `zeros` is set, the values are converted to zeros and the scale counts as one; a key scale that is not a
+// finite number counts as one.  Smem::spanOdd notes the latter two for addLeftOut.
 struct alignas(16) PageScales {
     float key[8], valueLog[8], valueInv[8];
     uint32_t zeros;
@@ -116,6 +118,7 @@ struct Smem {
     int rowNode[2][kRows];
     uint32_t rowFrom[2][kRows], rowBits[2][4][kRows];
     Span span[kSpans];
+    int spanOdd[kSpans];                               // FP8: a page of the span has a scale that is not finite
     int scratch[32];
     uint32_t tmemBase;
     int dead;
@@ -208,6 +211,20 @@ __device__ __forceinline__ uint32_t widen(uint32_t codes) {
     uint32_t r;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<unsigned short>(codes)));
     return r;
+}
+// The entries of a tile with pages whose scales are not positive finite numbers; lane i has page i (mod 8).  A
+// page of which the request holds nothing counts as one of zeros.
+__device__ __forceinline__ void preparePages(PageScales& sc, int* odd, float ks, float vs, bool held, float scaleLog2) {
+    const int lane = threadIdx.x & 31;
+    const bool zero = !held || isOdd(vs) || !(vs > 0.f);
+    if (lane < kKeys / 16) {
+        sc.key[lane] = !held || isOdd(ks) ? scaleLog2 : fmaxf(ks * scaleLog2, 1e-30f);
+        sc.valueLog[lane] = zero ? 0.f : log2f(vs);
+        sc.valueInv[lane] = zero ? 1.f : 1.f / vs;
+    }
+    const uint32_t zeros = __ballot_sync(0xFFFFFFFFu, zero);
+    if (lane == 0) sc.zeros = zeros & 0xFFu;
+    if (held && (isOdd(ks) || isOdd(vs))) *odd = 1;
 }
 __device__ __forceinline__ void bulkLoad(void* dst, const void* src, uint32_t bytes, unsigned long long* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -322,6 +339,8 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 const Span& g = *at;
                 const int32_t* table = p.tables + static_cast<int64_t>(g.b) * p.maxNumBlocks;
                 const int end = min(g.last, g.cacheTiles);           // of the tiles of the cache
+                if (lane == 0) s->spanOdd[k % kSpans] = 0;
+                __syncwarp();
                 int nextBlk = 0;
                 int64_t pair = 0;
                 __half ksNext = __float2half(0.f), vsNext = ksNext;
@@ -350,14 +369,17 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                         if (!ok) break;
                         if (h == 0) {
                             PageScales& sc = s->scales[gt % S::kScaleStages];
-                            const bool zero = !inTree && !(vs > 0.f);
-                            if (lane < kKeys / 16) {
-                                sc.key[lane] = inTree ? scaleLog2 : fmaxf(ks * scaleLog2, 1e-30f);          // (zero times a masked score would be NaN)
-                                sc.valueLog[lane] = inTree || zero ? 0.f : log2f(vs);
-                                sc.valueInv[lane] = inTree || zero ? 1.f : 1.f / vs;
+                            if (__all_sync(0xFFFFFFFFu, inTree || (vs > 0.f && !isOdd(vs) && !isOdd(ks)))) {
+                                if (lane < kKeys / 16) {
+                                    sc.key[lane] = inTree ? scaleLog2 : fmaxf(ks * scaleLog2, 1e-30f);      // (zero times a masked score would be NaN)
+                                    sc.valueLog[lane] = inTree ? 0.f : log2f(vs);
+                                    sc.valueInv[lane] = inTree ? 1.f : 1.f / vs;
+                                }
+                                if (lane == 0) sc.zeros = 0u;
+                            } else {
+                                const uint32_t piece = static_cast<uint32_t>(t16);
+                                preparePages(sc, &s->spanOdd[k % kSpans], ks, vs, piece >= g.s.lo / 16u && piece <= (g.s.held - 1u) / 16u, scaleLog2);
                             }
-                            const uint32_t zeros = __ballot_sync(0xFFFFFFFFu, zero);
-                            if (lane == 0) sc.zeros = zeros & 0xFFu;
                         }
                         __syncwarp();
                         if (lane == 0) {
@@ -742,7 +764,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             tcFenceAfter();
             const int p0 = cnt0 & 1, p1 = cnt1 & 1;
             // values left out anywhere in the span
-            const bool odd = anyOfOutput(s->rowOdd[p0][0][t] != 0 || (has1 && s->rowOdd[p1][1][t] != 0));
+            const bool odd = anyOfOutput(s->rowOdd[p0][0][t] != 0 || (has1 && s->rowOdd[p1][1][t] != 0) || (FP8 && s->spanOdd[k % kSpans] != 0));
             const bool whole = g.whole();
             const int which = g.first == 0 ? 1 : 0;
             if (!whole && first) {
