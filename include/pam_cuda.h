@@ -153,7 +153,12 @@ int32_t pamc_set_stream(void *ctx, void *cuda_stream);
 /* 1: operations return after enqueueing; 0 (default): they wait for the GPU
  * like the reference's commitAndWait (PagedAttentionEngine.swift:2008-2015). */
 int32_t pamc_set_async(void *ctx, int32_t enabled);
-/* Wait for everything enqueued on the context's stream. */
+/* Wait for everything enqueued on the context's stream.  Fails with "a kernel's bounded wait ran out" (see
+ * pamc_set_wait_limit) when that befell an asynchronous call or a replay of a recorded one since the last
+ * pamc_synchronize: whatever such calls wrote since then is not to be used.  Replays are therefore followed by a
+ * pamc_synchronize (those on a stream that is not the context's are waited for first); until it has reported the
+ * failure, further replays return without doing their work.  Calls that wait for the GPU report and retry their own
+ * waits only. */
 int32_t pamc_synchronize(void *ctx);
 /* Engine properties (PagedAttentionEngine.swift:116-129). */
 int32_t pamc_set_max_retries(void *ctx, int32_t n);            /* maxRetries, default 3 */
@@ -179,9 +184,11 @@ int32_t pamc_set_prefill_exact_weights(void *ctx, int32_t mode);
 int32_t pamc_inject_launch_failures(void *ctx, int32_t n);
 /* Number of this library's kernels launched on the context since creation. */
 int64_t pamc_kernel_launches(void *ctx);
-/* Every wait inside the tensor-core prefill kernel is bounded; a wait that runs out makes
- * the kernel return early and the call fail with "a kernel's bounded wait ran out (site n)"
- * (retried and degraded like any failed launch, PagedAttentionEngine.swift:375-414).
+/* Every wait inside the tensor-core kernels (prefill, tree attention) is bounded; a wait that
+ * runs out makes the kernel return early and the call fail with "a kernel's bounded wait ran
+ * out (site n)" (retried and degraded like any failed launch, PagedAttentionEngine.swift:375-414;
+ * reported by pamc_synchronize for asynchronous calls and replays).  A recorded call keeps the
+ * bound it was recorded with.
  * sm_cycles is that bound in SM clock cycles; 0 restores the default (about 0.2 s). */
 int32_t pamc_set_wait_limit(void *ctx, int64_t sm_cycles);
 /* Test switch for that path: in each of the next `launches` tensor-core prefill launches

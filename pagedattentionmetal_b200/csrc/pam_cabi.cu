@@ -92,7 +92,10 @@ struct Context {
     Arena arena;
     int* devErr = nullptr;    // set by a kernel whose bounded wait ran out
     int* hostErr = nullptr;   // pinned copy, read after the stream has been synchronised
-    bool errPending = false;
+    bool errPending = false;  // a kernel with bounded waits was launched and *devErr not fetched since
+    bool errRecorded = false; // one was recorded into a graph: its replays may set *devErr at any time
+    bool errFetched = false;  // the attempt of withRetry that is under way fetches *devErr behind its kernel
+    int earlierSite = 0;      // a wait of an earlier launch that ran out, not reported yet (see pamc_synchronize)
     bool forceGeneralPrefill = false;
     int exactWeights = 1;
     void* pinned = nullptr;   // page-locked scratch for host arrays the library builds itself (batch tables)
@@ -353,6 +356,48 @@ private:
     bool ok_ = true;
 };
 
+bool isCapturing(Context* c) {
+    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(c->stream, &s) != cudaSuccess) { cudaGetLastError(); return false; }
+    return s != cudaStreamCaptureStatusNone;
+}
+
+// The word that a kernel sets when one of its bounded waits runs out.  A launch that waits for the GPU fetches it
+// and is tried again; of asynchronous and recorded launches pamc_synchronize reports it.
+
+cudaError_t fetchWaitWord(Context* c) { return cudaMemcpyAsync(c->hostErr, c->devErr, sizeof(int), cudaMemcpyDeviceToHost, c->stream); }
+
+// What was fetched: the site of the wait, 0 for none.  Clears the word.
+int takeWaitWord(Context* c) {
+    const int site = *c->hostErr;
+    c->errPending = false;
+    if (site != 0) {
+        *c->hostErr = 0;
+        cudaMemsetAsync(c->devErr, 0, sizeof(int), c->stream);
+    }
+    return site;
+}
+
+// Before a kernel with bounded waits: a word that an earlier launch has set would keep it from starting, and is
+// kept for pamc_synchronize to report.
+cudaError_t beforeBounded(Context* c, bool capturing) {
+    if (c->async || capturing || !(c->errPending || c->errRecorded)) return cudaSuccess;
+    cudaError_t e = fetchWaitWord(c);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+    if (e != cudaSuccess) return e;
+    if (const int site = takeWaitWord(c)) c->earlierSite = site;
+    return cudaSuccess;
+}
+
+// Behind it.
+cudaError_t afterBounded(Context* c, bool capturing) {
+    if (capturing) { c->errRecorded = true; return cudaSuccess; }
+    c->errPending = true;
+    if (c->async) return cudaSuccess;
+    c->errFetched = true;
+    return fetchWaitWord(c);
+}
+
 // withRetry (PagedAttentionEngine.swift:375-400): up to maxRetries attempts,
 // a back-off of 10 ms * 2^attempt from the second failure on, and a circuit
 // breaker after 2 * maxRetries consecutive failures.  `attempt` enqueues the
@@ -367,16 +412,15 @@ int32_t withRetry(Context* c, const char* operation, F attempt) {
             e = cudaErrorLaunchFailure;
             last = "injected launch failure";
         } else {
+            c->errFetched = false;
             e = attempt();
             if (e == cudaSuccess && !c->async) e = cudaStreamSynchronize(c->stream);
             if (e != cudaSuccess) { last = cudaGetErrorString(e); cudaGetLastError(); }
-            else if (!c->async && c->errPending) {
+            else if (c->errFetched) {
                 // a kernel gave up on a bounded wait and returned without finishing its work
-                c->errPending = false;
-                if (*c->hostErr != 0) {
-                    last = "a kernel's bounded wait ran out (site " + std::to_string(*c->hostErr) + ")";
-                    *c->hostErr = 0;
-                    cudaMemsetAsync(c->devErr, 0, sizeof(int), c->stream);
+                if (const int site = takeWaitWord(c)) {
+                    last = "a kernel's bounded wait ran out (site " + std::to_string(site) + ")";
+                    if (c->errRecorded) c->earlierSite = site;           // (a replay on another stream may have set it)
                     e = cudaErrorLaunchTimeout;
                 }
             }
@@ -784,13 +828,11 @@ int32_t prefillImpl(Context* c, const PamLayerSpec& l, const PamBuffer& q, const
                 p.poolBlocks = n * maxCount;
             }
         }
-        cudaError_t e = pam::launchPrefill(p, c->smCount, c->stream, &launches, &tensorPath);
+        const bool capturing = isCapturing(c);
+        cudaError_t e = beforeBounded(c, capturing);
+        if (e == cudaSuccess) e = pam::launchPrefill(p, c->smCount, c->stream, &launches, &tensorPath);
         c->launches += launches;
-        if (e == cudaSuccess && tensorPath) {
-            // the flag is fetched now when the call waits for the GPU anyway, else by pamc_synchronize
-            if (!c->async) e = cudaMemcpyAsync(c->hostErr, c->devErr, sizeof(int), cudaMemcpyDeviceToHost, c->stream);
-            c->errPending = true;
-        }
+        if (e == cudaSuccess && tensorPath) e = afterBounded(c, capturing);
         if (e == cudaSuccess) e = st.copyBack();
         // `meta` is read by an async copy from pageable memory, which the
         // runtime stages before returning; nothing else outlives this scope.
@@ -840,19 +882,16 @@ Cache* createCache(Context* c, int32_t maxBlocks, int32_t blockSize, int32_t hea
 
 int32_t syncContext(Context* c) {
     cudaError_t e = cudaSuccess;
-    if (c->errPending) e = cudaMemcpyAsync(c->hostErr, c->devErr, sizeof(int), cudaMemcpyDeviceToHost, c->stream);
+    const bool fetch = c->errPending || c->errRecorded;
+    if (fetch) e = fetchWaitWord(c);
     if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
     if (e != cudaSuccess) { cudaGetLastError(); return c->fail(PAM_ERR_COMMAND_EXECUTION, commandExecutionFailed(cudaGetErrorString(e))); }
-    if (c->errPending) {
-        c->errPending = false;
-        if (*c->hostErr != 0) {
-            const int site = *c->hostErr;
-            *c->hostErr = 0;
-            cudaMemsetAsync(c->devErr, 0, sizeof(int), c->stream);
-            return c->fail(PAM_ERR_COMMAND_EXECUTION, commandExecutionFailed("a kernel's bounded wait ran out (site " + std::to_string(site) + ")"));
-        }
-    }
-    return 0;
+    int site = fetch ? takeWaitWord(c) : 0;
+    if (site != 0) cudaStreamSynchronize(c->stream);       // (the next replay may be on another stream)
+    if (site == 0) site = c->earlierSite;
+    c->earlierSite = 0;
+    if (site == 0) return 0;
+    return c->fail(PAM_ERR_COMMAND_EXECUTION, commandExecutionFailed("a kernel's bounded wait ran out (site " + std::to_string(site) + ")"));
 }
 
 // The *Layers calls (PagedAttentionEngine.swift:1433-1895) run the same operation once per
@@ -1256,6 +1295,7 @@ int32_t pamc_set_async(void* ctx, int32_t enabled) { if (!ctx) return -1; asCtx(
 int32_t pamc_synchronize(void* ctx) {
     if (!ctx) return -1;
     Context* c = asCtx(ctx);
+    std::lock_guard<std::mutex> g(c->mu);
     DeviceGuard dg(c->device);
     if (c->device < 0) return noGpu(c);
     return syncContext(c);

@@ -26,12 +26,6 @@ bool stepSizes(Context* c, StepArg* args, int n) {
     return true;
 }
 
-bool isCapturing(Context* c) {
-    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(c->stream, &s) != cudaSuccess) { cudaGetLastError(); return false; }
-    return s != cudaStreamCaptureStatusNone;
-}
-
 // Where every buffer lives.  Memory of another GPU is refused (the kernels would fault on it, or
 // read it over the link without being asked to); a host buffer cannot be staged in a capture.
 bool stepPlaces(Context* c, StepArg* args, int n, bool capturing) {
@@ -577,13 +571,9 @@ int32_t pamc_tree_attention(void* ctx, const PamTreeAttentionRequest* request) {
         p.workspace = static_cast<float*>(rq.workspace.ptr ? rq.workspace.ptr : c->arena.take(need));
         if (!p.workspace) return cudaErrorMemoryAllocation;
         bool bounded = false;
-        cudaError_t e = pam::launchTreeAttention(p, c->smCount, c->stream, launches, &bounded);
-        if (e == cudaSuccess && bounded) {
-            // as in prefillImpl: fetched now when the call waits for the GPU, else by pamc_synchronize
-            if (!c->async && !capturing) e = cudaMemcpyAsync(c->hostErr, c->devErr, sizeof(int), cudaMemcpyDeviceToHost, c->stream);
-            c->errPending = true;
-        }
-        return e;
+        cudaError_t e = beforeBounded(c, capturing);
+        if (e == cudaSuccess) e = pam::launchTreeAttention(p, c->smCount, c->stream, launches, &bounded);
+        return e == cudaSuccess && bounded ? afterBounded(c, capturing) : e;
     });
     if (rc != 0) {
         if (!c->graceful || capturing) return rc;

@@ -190,6 +190,8 @@ class PagedAttentionEngine:
         lib.pamc_set_async(self._ctx, 1 if enabled else 0)
 
     def synchronize(self) -> None:
+        """Waits for the engine's stream; raises when a bounded wait of an asynchronous or
+        replayed call ran out (pamc_synchronize)."""
         _check(self._ctx, lib.pamc_synchronize(self._ctx))
 
     def setPrefillTensorPath(self, on: bool) -> None:
@@ -203,7 +205,7 @@ class PagedAttentionEngine:
         lib.pamc_inject_launch_failures(self._ctx, n)
 
     def setWaitLimit(self, smCycles: int) -> None:
-        """Bound of every wait inside the tensor-core prefill kernel, in SM clock
+        """Bound of every wait inside the tensor-core kernels, in SM clock
         cycles (0: the default, about 0.2 s); see pamc_set_wait_limit."""
         _check(self._ctx, lib.pamc_set_wait_limit(self._ctx, int(smCycles)))
 
