@@ -128,9 +128,11 @@ int32_t stepRun(Context* c, const char* name, StepArg* args, int n, bool capturi
 
 int32_t badStep(Context* c, const std::string& m) { return c->fail(PAM_ERR_INVALID_CONFIGURATION, invalidConfiguration(m)); }
 
-// Bytes from the first element of a strided array of rows to its last.
+// Bytes from the first element of a strided array of rows to its last; more than any buffer has where they pass
+// 64 bits.
 size_t rowSpan(int64_t rows, int64_t stride, int64_t width, int elem) {
-    return static_cast<size_t>((rows - 1) * stride + width) * elem;
+    const unsigned __int128 bytes = (static_cast<unsigned __int128>(rows - 1) * stride + width) * elem;
+    return bytes < kUnknownBytes ? static_cast<size_t>(bytes) : kUnknownBytes - 1;
 }
 StepRows stridedRows(int64_t rows, int64_t stride, int64_t width, int elem) {
     return {static_cast<size_t>(rows), static_cast<size_t>(width) * elem, static_cast<size_t>(stride) * elem};

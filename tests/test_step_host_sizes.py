@@ -1,0 +1,24 @@
+"""Refusals of the calls of a speculative step that come from arithmetic on large sizes, without a GPU."""
+import pytest
+
+from pagedattentionmetal_b200._cabi import lib
+from test_step_host import CALLS, TOO_SMALL, ctx, norm, norm_backward, tree      # noqa: F401
+
+FAR = 1 << 40                     # the largest stride that is taken, in elements
+ROWS = (1 << 24) + 1              # (ROWS - 1) * FAR = 2^64
+
+
+@pytest.mark.parametrize("make,stride,text", [
+    (norm, "qStride", b"Q"), (norm, "kStride", b"K"), (norm, "vStride", b"V"), (norm, "qOutStride", b"qOut"),
+    (norm, "kOutStride", b"kOut"), (norm_backward, "dQStride", b"dQ"), (norm_backward, "dKStride", b"dK"),
+    (tree, "qStride", b"Q"), (tree, "kStride", b"K"), (tree, "vStride", b"V")])
+def test_rows_whose_extent_passes_64_bits(ctx, make, stride, text):     # noqa: F811
+    """The extent of the strided rows must not wrap round to one that fits their buffer."""
+    request = make(numRows=ROWS, **{stride: FAR})
+    buffers = {norm: ("q", "k", "v", "qOut", "kOut", "slots", "positions"),
+               norm_backward: ("q", "k", "dQOut", "dKOut", "dQ", "dK", "positions"), tree: ("q", "k", "v", "output", "masks")}[make]
+    for name in buffers:
+        getattr(request._c, request._fields[name][0]).bytes = 1 << (20 if name == stride.removesuffix("Stride") else 50)
+    assert CALLS[type(request)](ctx, request) == -1
+    assert lib.pamc_last_error_code(ctx) == TOO_SMALL
+    assert lib.pam_last_error(ctx).startswith(text + b" buffer is too small")
