@@ -354,13 +354,14 @@ int32_t pamc_norm_rotate(void* ctx, const PamNormRotateRequest* request, void* c
             return pam::launchNormRotate(p, c->stream, launches);
         }
         // FP8: the scale of a block needs every new row of it first, so the rows go through the append
-        // kernels, which take them back to back: from kOut and V where they are, else from scratch that the
-        // same launch writes beside kOut (one launch, since the outputs may lie over the inputs).  Skipped
-        // rows lose their slot.
+        // kernels, which take them back to back from a 16-byte boundary on: kOut and V where they are that,
+        // else scratch that the same launch writes beside kOut (one launch, since the outputs may lie over the
+        // inputs).  Skipped rows lose their slot.
         const size_t bytes = static_cast<size_t>(R) * kWide * io;
         const void *keys = p.kOut, *values = p.v;
-        if (!p.kOut || ko != kWide) keys = p.kPool = c->arena.take(bytes);
-        if (vs != kWide) values = p.vPool = c->arena.take(bytes);
+        auto aligned = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; };
+        if (!p.kOut || ko != kWide || !aligned(keys)) keys = p.kPool = c->arena.take(bytes);
+        if (vs != kWide || !aligned(values)) values = p.vPool = c->arena.take(bytes);
         p.slotsOut = static_cast<int64_t*>(c->arena.take(static_cast<size_t>(R) * 8));
         if (!keys || !values || !p.slotsOut) return cudaErrorMemoryAllocation;
         cudaError_t e = nextAbsmaxEpoch(k, c->stream);

@@ -103,3 +103,27 @@ def test_gradient_into_columns_of_one_host_array(engine, dtype, pages):
     assert np.array_equal(host.numpy(), base.download(case.io, fill.shape))
     for a, b in zip(weights, host_weights):
         assert np.array_equal(a.download(np.float32, (case.D,)), b)
+
+
+@pytest.mark.parametrize("shape", [dict(heads=8, kv_heads=2, dim=64), dict(heads=4, kv_heads=2, dim=24, rotary=16)], ids=lambda s: f"dim{s['dim']}")
+@pytest.mark.parametrize("off", ["v", "kOut", "both"])
+def test_float8_append_of_rows_off_the_16_byte_grid(engine, shape, off):
+    """Back-to-back values and key rows that start one element into their buffers: the pages equal those of
+    reshapeAndCache over aligned copies of the same rows."""
+    case = NormCase(65, rows=30, dtype=DT.float8, fused=False, **shape)
+    one, two = (pam.KVCacheManager(engine, case.blocks, case.block, case.D, case.KVH, DT.float8) for _ in range(2))
+    n = case.R * case.KVH * case.D
+    shifted = lambda values, by: engine.makeBufferFrom(np.concatenate([np.zeros(by, np.float16), values.reshape(-1)]))
+    v_by, k_by = int(off in ("v", "both")), int(off in ("kOut", "both"))
+    inputs, keep = case.inputs(engine)
+    v_base, k_base = shifted(case.v, v_by), shifted(np.zeros(n, np.float16), k_by)
+    inputs["v"] = pam_buffer(v_base, 2 * v_by, 2 * n)
+    engine.normRotate(pam.PagedNormRotateRequest(
+        **inputs, **case.common(engine), qOut=engine.makeBuffer(case.R * case.H * case.D * 2), kOut=pam_buffer(k_base, 2 * k_by, 2 * n),
+        slots=engine.makeBufferFrom(case.slots)), one)
+    keys = engine.makeBufferFrom(k_base.download(np.float16, (n,), 2 * k_by))
+    engine.reshapeAndCache(two, keys, engine.makeBufferFrom(np.ascontiguousarray(case.v)),
+                           engine.makeBufferFrom(np.where(case.live, case.slots, -1)), case.R)
+    pools_equal(one, two)
+    one.close()
+    two.close()
