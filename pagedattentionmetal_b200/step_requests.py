@@ -25,6 +25,17 @@ def _span(x) -> _cabi.PamBuffer:
     return _cabi.PamBuffer(x.data_ptr(), elements * x.element_size())
 
 
+# What the index, scale and frequency buffers hold; arrays and tensors of another type are refused (rows, pages and
+# weights hold what the layer says).
+_HOLDS = {**{name: "int32" for name in (
+              "blockLists", "listIndex", "lengths", "newTokens", "parents", "tables", "totalLengths", "rowStarts", "positions",
+              "masks", "draftTokens", "targetTokens", "blockTables", "cacheLengths", "acceptedCounts", "acceptedRows",
+              "nextTokens", "newLengths")},
+          "slots": "int64", "invFreq": "float32", "dQWeight": "float32", "dKWeight": "float32",
+          "kScaleBuffer": "float16", "vScaleBuffer": "float16"}
+_TAKEN = {"int32": ("int32", "uint32"), "int64": ("int64", "uint64")}
+
+
 class _Request:
     """Fields by their Python names; `_fields` maps them to the struct's, with the default of a plain number."""
     _struct: type
@@ -52,6 +63,11 @@ class _Request:
             raise AttributeError(f"{type(self).__name__} has no field {name}")
         field, default = self._fields[name]
         if default is None:
+            holds = _HOLDS.get(name)
+            if holds and hasattr(value, "dtype"):
+                held = str(value.dtype).rpartition(".")[2]           # ("torch.int32")
+                if held != holds and held not in _TAKEN.get(holds, ()):
+                    raise TypeError(f"{type(self).__name__}.{name} holds {holds}, not {held}")
             c = _span(value)
         elif isinstance(value, PagedLayerSpec):
             c = _cabi.PamLayerSpec(value.headDim, value.numHeads, value.numKVHeads, value.blockSize,
