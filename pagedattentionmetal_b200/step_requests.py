@@ -13,16 +13,28 @@ from . import _cabi
 from .api_types import PagedLayerSpec
 
 
-def _span(x) -> _cabi.PamBuffer:
-    """A buffer argument with its length; a strided torch view reaches from its first to its last element."""
+# Buffers of rows that may start a stride apart.
+_ROWS = {"q", "k", "v", "qOut", "kOut", "dQ", "dK", "dV"}
+
+
+def _span(x, name: str) -> _cabi.PamBuffer:
+    """A buffer argument with its length; a view of strided rows reaches from its first to its last element."""
     if x is None:
         return _cabi.PamBuffer(None, 0)
-    if not hasattr(x, "is_contiguous"):
+    if hasattr(x, "is_contiguous"):
+        if x.is_contiguous():
+            return _cabi.PamBuffer(x.data_ptr(), x.numel() * x.element_size())
+        row = name in _ROWS and x[0].is_contiguous()
+        strides, size = x.stride(), x.element_size()
+    elif hasattr(x, "flags") and hasattr(x, "strides") and not x.flags.c_contiguous:
+        row = name in _ROWS and x.strides[0] > 0 and x[0].flags.c_contiguous
+        strides, size = [s // x.itemsize for s in x.strides], x.itemsize
+    else:
         return _cabi.buffer(x)
-    elements = x.numel()
-    if elements and not x.is_contiguous():
-        elements = 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
-    return _cabi.PamBuffer(x.data_ptr(), elements * x.element_size())
+    if not row:
+        raise ValueError(f"{name} must be contiguous" + (" within a row" if name in _ROWS else ""))
+    elements = 1 + sum((n - 1) * s for n, s in zip(x.shape, strides)) if all(x.shape) else 0
+    return _cabi.PamBuffer(_cabi.address(x), elements * size)
 
 
 # What the index, scale and frequency buffers hold; arrays and tensors of another type are refused (rows, pages and
@@ -68,7 +80,7 @@ class _Request:
                 held = str(value.dtype).rpartition(".")[2]           # ("torch.int32")
                 if held != holds and held not in _TAKEN.get(holds, ()):
                     raise TypeError(f"{type(self).__name__}.{name} holds {holds}, not {held}")
-            c = _span(value)
+            c = _span(value, name)
         elif isinstance(value, PagedLayerSpec):
             c = _cabi.PamLayerSpec(value.headDim, value.numHeads, value.numKVHeads, value.blockSize,
                                    int(value.dataType), value.windowSize)

@@ -41,3 +41,38 @@ def test_buffers_without_a_type_are_taken():
     assert request._c.cache_lengths.bytes == 64
     request.q = np.zeros(64, np.uint16)                 # (rows: the layer says what they hold)
     assert isinstance(request, pam.PagedTreeAttentionRequest)
+
+
+def views():
+    torch = pytest.importorskip("torch")
+    wide = np.zeros((6, 512), np.float16)
+    return wide, torch.from_numpy(wide)
+
+
+def test_views_of_rows_reach_from_their_first_to_their_last_element():
+    for wide in views():
+        address = wide.ctypes.data if isinstance(wide, np.ndarray) else wide.data_ptr()
+        for view in (wide[:, 128:256], wide[:, 128:256].reshape(6, 2, 64)):
+            request = tree(v=view, vStride=512)
+            assert request._c.v.ptr == address + 256 and request._c.v.bytes == (5 * 512 + 128) * 2
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+def test_rows_that_are_not_in_one_piece_are_refused(name):
+    for wide in views():
+        for view in (wide[:, ::2], wide.T, wide.reshape(6, 8, 64)[:, ::2], wide.reshape(6, 8, 64)[:, :, :32]):
+            with pytest.raises(ValueError, match=name):
+                tree(**{name: view})
+    with pytest.raises(ValueError, match=name):
+        tree(**{name: np.zeros((6, 512), np.float16)[::-1]})
+
+
+@pytest.mark.parametrize("make,name", [(make, name) for make, _, name in CASES] +
+                         [(tree, "output"), (tree, "kPool"), (tree, "vPool"), (norm, "qWeight"), (norm_backward, "dQOut"), (norm_backward, "dKOut")])
+def test_views_of_anything_but_rows_are_refused(make, name):
+    """They have no stride in the request: every other element would be read in their place."""
+    torch = pytest.importorskip("torch")
+    kind = next((k for m, k, n in CASES if m is make and n == name), "float16")
+    for value in (np.zeros((64, 64), kind)[:, 0], torch.zeros(64, 64, dtype=getattr(torch, kind))[:, 0]):
+        with pytest.raises(ValueError, match=name):
+            make(**{name: value})
