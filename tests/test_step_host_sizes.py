@@ -1,6 +1,7 @@
 """Refusals of the calls of a speculative step that come from arithmetic on large sizes, without a GPU."""
 import pytest
 
+import pagedattentionmetal_b200 as pam
 from pagedattentionmetal_b200._cabi import lib
 from test_step_host import CALLS, TOO_SMALL, ctx, norm, norm_backward, tree      # noqa: F401
 
@@ -22,3 +23,13 @@ def test_rows_whose_extent_passes_64_bits(ctx, make, stride, text):     # noqa: 
     assert CALLS[type(request)](ctx, request) == -1
     assert lib.pamc_last_error_code(ctx) == TOO_SMALL
     assert lib.pam_last_error(ctx).startswith(text + b" buffer is too small")
+
+
+def test_lists_of_tiles_that_a_blocks_share_would_push_past_31_bits(ctx):     # noqa: F811
+    """A block's piece of the list ends at its begin plus its share; begin + share must not pass 2^31."""
+    text = b"split the batch"
+    for blocks, refused in ((1073741820, True), (1 << 30, True), ((1 << 30) - (1 << 23) - 16, False)):
+        request = tree(batchSize=1, numRows=4, maxNewTokens=4, maxNumBlocks=blocks)
+        request.layer = pam.PagedLayerSpec(64, 2, 2, 32, pam.PagedAttentionDataType.float16, 0)     # (a tile for each block and head)
+        assert CALLS[type(request)](ctx, request) == -1
+        assert (text in lib.pam_last_error(ctx)) == refused, blocks
