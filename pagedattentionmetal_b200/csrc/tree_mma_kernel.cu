@@ -39,6 +39,9 @@ using namespace tree;
 constexpr int kThreads = 128, kKeys = 64;
 constexpr int kShortKeys = 256;
 constexpr float kRaise = 6.f;             // the running maximum moves when it is passed by 2^6
+// Weights are kept times 2^9, as far up as that leaves float16 room (2^15): those down to 2^-23 of a row's reference
+// then keep all their bits, not those down to 2^-14 alone.  (bfloat16 has float32's range.)
+template <typename T> constexpr float kWeightLift = std::is_same<T, __half>::value ? 9.f : 0.f;
 
 __device__ __forceinline__ uint32_t smemAddr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void ldmatrixX4(uint32_t (&r)[4], uint32_t addr) {
@@ -400,7 +403,7 @@ treeMmaKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
 #pragma unroll
             for (int n = 0; n < HD / 8; ++n) { o[n][0] *= c0; o[n][1] *= c0; o[n][2] *= c1; o[n][3] *= c1; }
         }
-        const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+        const float b0 = m0 == -INFINITY ? 0.f : m0 - kWeightLift<T>, b1 = m1 == -INFINITY ? 0.f : m1 - kWeightLift<T>;
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             s[n][0] = ex2(s[n][0] - b0); s[n][1] = ex2(s[n][1] - b0);

@@ -57,6 +57,9 @@ constexpr int kRows = 128, kKeys = 128, kHd = 128;
 constexpr int kTileBytes = kKeys * kHd * 2, kHalfBytes = kTileBytes / 2;      // a 64-dim block of a tile
 constexpr int kVHalfBytes = kTileBytes / 2, kVBlockBytes = kVHalfBytes / 2;   // 64 keys of V, a 64-dim block of them
 constexpr float kRescaleThreshold = 8.0f;
+// Weights are kept times 2^7, as far up as the threshold leaves float16 room (2^15): those down to 2^-21 of a row's
+// reference then keep all their bits, not those down to 2^-14 alone.  (bfloat16 has float32's range.)
+template <bool BF16> constexpr float kWeightLift = BF16 ? 0.f : 7.f;
 constexpr int kShortKeys = 256;                        // bfloat16: fewer visible keys carry the weights as two operands
 constexpr long long kWaitCycles = 400000000LL;
 constexpr long long kDrainCycles = 4000000LL;          // for the copies in flight when a wait ran out
@@ -956,7 +959,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                     tmemStWait();
                     l *= corr;
                 }
-                const float negM = mUsed == -INFINITY ? 0.f : -mUsed;
+                const float negM = mUsed == -INFINITY ? 0.f : kWeightLift<BF16> - mUsed;
                 if constexpr (FP8) {
                     // (a quarter at a time: there are fewer registers)
 #pragma unroll 1
