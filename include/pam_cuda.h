@@ -171,11 +171,12 @@ int32_t pamc_set_default_chunk(void *ctx, int32_t tokens);     /* defaultChunkSi
  * The reference picks its prefill variant the same way, by type and head_dim
  * (PagedAttentionEngine.swift:420-434). */
 int32_t pamc_set_prefill_tensor_path(void *ctx, int32_t on);
-/* bfloat16 tensor-core prefill: how the softmax weights are carried into the
- * second product.  0: one bfloat16 operand (8 significant bits, what bfloat16
- * attention kernels usually do); 1 (default): two operands, 16 bits, on query
- * tiles whose rows see fewer than 256 keys, where 8 bits can miss the 2e-3
- * bound; 2: two operands everywhere (about 1.5x the tensor work).  No
+/* bfloat16 tensor-core prefill and tree attention: how the softmax weights are
+ * carried into the second product.  0: one bfloat16 operand (8 significant bits,
+ * what bfloat16 attention kernels usually do); 1 (default): two operands, 16 bits,
+ * on query tiles (tree attention: requests) whose rows see fewer than 256 keys,
+ * where 8 bits can miss the 2e-3 bound; 2: two operands everywhere (about 1.5x
+ * the tensor work).  float16 weights (float16 and FP8 caches) keep 11 bits.  No
  * counterpart in the reference, which has no bfloat16. */
 int32_t pamc_set_prefill_exact_weights(void *ctx, int32_t mode);
 /* Host-side fault injection for tests of the retry loop, circuit breaker and
@@ -576,7 +577,9 @@ int64_t pamc_norm_rotate_backward_workspace(void *ctx, const PamNormRotateBackwa
  * stands at cache_lengths[b] + i).  A row that sees nothing is written as zero; values and (FP8)
  * scales a row does not see do not reach it, whatever they hold; a key scale that is not a finite
  * number makes the rows that see its page NaN.  Rows outside every request stay as they
- * were.  Requests beyond max_new_tokens rows are cut off there. */
+ * were.  Requests beyond max_new_tokens rows are cut off there.
+ * Scores, sums and accumulators are float32; with 16-bit and FP8 pages the softmax weights are
+ * rounded to 16 bits for their product with the values (pamc_set_prefill_exact_weights). */
 typedef struct PamTreeAttentionRequest {
     PamBuffer q, k, v, k_pool, v_pool;
     PamBuffer block_tables;       /* int32 [batch][max_num_blocks] */

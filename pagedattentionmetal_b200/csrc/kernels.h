@@ -278,6 +278,7 @@ struct TreeParams {
     int64_t qStride, kStride, vStride;   // elements between rows
     int batch, heads, kvHeads, headDim, blockSize, maxNumBlocks, numRows, maxNew, maskWords, window, dtype;
     int poolBlocks;               // table entries are clamped into [0, poolBlocks)
+    int exactWeights;             // bfloat16 weights as in PrefillParams: 0 = 8 bits, 1 = 16 for requests with few keys, 2 = 16 always
     float* workspace;             // treeWorkspaceBytes()
     int* errFlag;                 // device word the tensor-core kernel sets when a bounded wait runs out
     long long waitCycles;         // that bound; 0: the default

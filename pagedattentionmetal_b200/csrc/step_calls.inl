@@ -496,7 +496,7 @@ static bool treeShape(Context* c, const PamTreeAttentionRequest& rq, pam::TreePa
     p->q = rq.q.ptr; p->kNew = rq.k.ptr; p->vNew = rq.v.ptr; p->kPool = rq.k_pool.ptr; p->vPool = rq.v_pool.ptr; p->out = rq.output.ptr;
     p->batch = rq.batch_size; p->heads = l.num_heads; p->kvHeads = l.num_kv_heads; p->headDim = l.head_dim; p->blockSize = l.block_size;
     p->maxNumBlocks = rq.max_num_blocks; p->numRows = rq.num_rows; p->maxNew = std::min(rq.max_new_tokens, rq.num_rows);
-    p->maskWords = rq.mask_words; p->window = window; p->dtype = l.data_type;
+    p->maskWords = rq.mask_words; p->window = window; p->dtype = l.data_type; p->exactWeights = c->exactWeights;
     // (tiles are counted in 32 bits up to a block's begin plus its share, of which there is at least one for each SM)
     if (pam::treeTileBound(*p) >= INT32_MAX - INT32_MAX / std::max(c->smCount, 1) - 1)
         return bad("batchSize, maxNumBlocks and maxNewTokens span more work than one call takes; split the batch.");

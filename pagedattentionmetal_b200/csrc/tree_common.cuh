@@ -45,6 +45,13 @@ struct SeqInfo {
     __device__ __forceinline__ int rowTiles(int group, int mr) const { return (n * group + mr - 1) / mr; }
 };
 
+// bfloat16 keeps 8 bits of a weight, which shows when few keys carry the result: requests that see fewer keys than
+// this, and all if the caller wants it so, carry the weights into the second product as two operands (16 bits).
+constexpr uint32_t kShortKeys = 256;
+__device__ __forceinline__ bool twoOperands(const TreeParams& p, const SeqInfo& s) {
+    return p.exactWeights == 2 || (p.exactWeights == 1 && s.held - s.lo + static_cast<uint32_t>(s.n) < kShortKeys);
+}
+
 // Position of a row (node i of its tree); one below the cache length counts as the cache length.
 __device__ __forceinline__ long long positionOf(const TreeParams& p, const SeqInfo& s, int i) {
     if (!p.positions) return static_cast<long long>(s.len) + i;

@@ -21,9 +21,7 @@
 // into the second product as float16 then stay near 1 however small the scales are.
 //
 // The weights go into the second product in the type of the values: half a step of it per weight,
-// at random, against the half step of the result itself.  For bfloat16 that is 2^-8 and shows when
-// few keys carry the result, so that requests that see fewer than 256 keys carry the weights as two
-// operands (16 bits).
+// at random, against the half step of the result itself.  For bfloat16 that is 2^-8 (see twoOperands).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -37,7 +35,6 @@ namespace {
 using namespace tree;
 
 constexpr int kThreads = 128, kKeys = 64;
-constexpr int kShortKeys = 256;
 constexpr float kRaise = 6.f;             // the running maximum moves when it is passed by 2^6
 // Weights are kept times 2^9, as far up as that leaves float16 room (2^15): those down to 2^-23 of a row's reference
 // then keep all their bits, not those down to 2^-14 alone.  (bfloat16 has float32's range.)
@@ -264,7 +261,7 @@ treeMmaKernel(const __grid_constant__ TreeParams p, float scaleLog2) {
             m0 = m1 = -INFINITY;
             l0 = l1 = 0.f;
             odd = false;
-            two = std::is_same<T, __nv_bfloat16>::value && g.s.held - g.s.lo + g.s.n < kShortKeys;
+            two = std::is_same<T, __nv_bfloat16>::value && twoOperands(p, g.s);
         }
         const int cacheTiles = g.s.cacheTiles<kKeys>();
         const bool inTree = j >= cacheTiles;

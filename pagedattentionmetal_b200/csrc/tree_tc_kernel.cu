@@ -60,7 +60,6 @@ constexpr float kRescaleThreshold = 8.0f;
 // Weights are kept times 2^7, as far up as the threshold leaves float16 room (2^15): those down to 2^-21 of a row's
 // reference then keep all their bits, not those down to 2^-14 alone.  (bfloat16 has float32's range.)
 template <bool BF16> constexpr float kWeightLift = BF16 ? 0.f : 7.f;
-constexpr int kShortKeys = 256;                        // bfloat16: fewer visible keys carry the weights as two operands
 constexpr long long kWaitCycles = 400000000LL;
 constexpr long long kDrainCycles = 4000000LL;          // for the copies in flight when a wait ran out
 constexpr int kKProducerWarp = 8, kVProducerWarp = 9, kMmaWarp = 10, kPlanWarp = 11, kOutputWarp0 = 12;
@@ -80,7 +79,6 @@ struct Span {
     // tiles of group x
     __device__ __forceinline__ int tilesOf(int x) const { return dual ? last - first : (last - first + 1 - x) >> 1; }
     __device__ __forceinline__ bool whole() const { return first == 0 && last == nT; }
-    __device__ __forceinline__ bool shortKeys() const { return s.held - s.lo + static_cast<uint32_t>(s.n) < kShortKeys; }
 };
 
 constexpr int kSpans = 8;        // of the ring: no warp needs a span more than five behind the oldest one in use
@@ -477,7 +475,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             at.x = 0;
             at.valid = sp && sp->valid;
             if (!sp) ok = false;
-            if (at.valid) { at.first = at.j = sp->first; at.last = sp->last; at.dual = sp->dual != 0; at.lo = sp->shortKeys(); }
+            if (at.valid) { at.first = at.j = sp->first; at.last = sp->last; at.dual = sp->dual != 0; at.lo = twoOperands(p, sp->s); }
         };
         auto advance = [&](Step& at) {
             const bool sameTile = at.dual && at.x == 0;
@@ -882,7 +880,7 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
                 s->rowNode[x][t] = node;
                 s->rowFrom[x][t] = max(firstOf(p, g.s, node), g.s.lo);
             }
-            const bool useLo = BF16 && g.shortKeys();
+            const bool useLo = BF16 && twoOperands(p, g.s);
             float mUsed = -INFINITY, l = 0.f;
             int odd = 0;
             const int j0 = g.first + (g.dual ? 0 : x);

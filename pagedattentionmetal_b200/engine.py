@@ -198,7 +198,7 @@ class PagedAttentionEngine:
         lib.pamc_set_prefill_tensor_path(self._ctx, 1 if on else 0)
 
     def setPrefillExactWeights(self, mode: int) -> None:
-        """0 / 1 / 2, see pamc_set_prefill_exact_weights."""
+        """0 / 1 / 2, for bfloat16 prefill and tree attention; see pamc_set_prefill_exact_weights."""
         lib.pamc_set_prefill_exact_weights(self._ctx, mode)
 
     def injectLaunchFailures(self, n: int) -> None:
