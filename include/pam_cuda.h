@@ -481,7 +481,8 @@ int32_t pamc_append_layers(void *ctx, const PamAppendRequest *requests, int32_t 
  * "Rows" are the new tokens of all requests back to back; request b owns rows
  * [row_starts[b], row_starts[b + 1]).  Buffers may be device memory of the
  * context's GPU or host memory (staged inside the call; the pools are device
- * memory always); memory of another GPU is refused.  While the context's stream
+ * memory always); memory of another GPU is refused.  Outputs do not overlap inputs
+ * or one another but where a call says so.  While the context's stream
  * is being captured the calls only record their launches: every buffer must then
  * be device memory, and the calls that take a workspace must be given one (make one
  * eager call of each kind first: it loads the kernels).  Two graphs (or streams) that
@@ -604,7 +605,7 @@ int64_t pamc_tree_attention_workspace(void *ctx, const PamTreeAttentionRequest *
  *   accepted_counts[b]  nodes on the path (0 for a request without rows)
  *   accepted_rows[b]    their rows, root first, -1 behind them; the first max_path of them
  *   next_tokens[b]      target_tokens of the path's end, -1 for a request without rows
- *   new_lengths[b]      lengths[b] + accepted_counts[b]
+ *   new_lengths[b]      lengths[b] + accepted_counts[b]; may lie over lengths
  *   slots[r]            slot of position lengths[b] + depth for rows on the path, -1 for all others
  *                       (pamc_reshape_and_cache skips those); needs block_tables; -1 too where the
  *                       table ends or its entry is negative

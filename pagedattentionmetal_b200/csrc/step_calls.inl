@@ -167,6 +167,8 @@ int32_t pamc_plan_step(void* ctx, const PamStepPlanRequest* request) {
     if (rq.tables.ptr && (rq.max_num_blocks <= 0 || rq.max_num_blocks > (1 << 26))) return badStep(c, "maxNumBlocks must be in 1 ... 2^26.");
     if (rq.max_new_tokens > (1 << 26)) return badStep(c, "maxNewTokens must be at most 2^26.");
     if (rq.parents.ptr && rq.max_new_tokens > pam::kMaxTreeNodes) return badStep(c, "a tree has at most " + std::to_string(pam::kMaxTreeNodes) + " nodes: maxNewTokens is too large.");
+    if (rq.total_lengths.ptr && rq.total_lengths.ptr == rq.lengths.ptr)
+        return badStep(c, "totalLengths must not lie over lengths (every block of the plan reads them).");
     if (rq.parents.ptr && rq.slots.ptr) return badStep(c, "the nodes of a tree have no slots before they are accepted (see pamc_accept_tree).");
     if (rq.masks.ptr && (rq.mask_words <= 0 || rq.mask_words > (1 << 20) || rq.max_new_tokens > 32ll * rq.mask_words))
         return badStep(c, "maskWords must hold one bit for each of maxNewTokens rows.");

@@ -132,6 +132,7 @@ acceptTreeKernel(const AcceptParams p) {
     const int start = min(max(p.rowStarts[b], 0), p.numRows);
     const int end = min(max(p.rowStarts[b + 1], start), p.numRows);
     const int n = min(end - start, p.maxTree);
+    const int len = max(p.lengths[b], 0);         // (read by all before the barriers: newLengths may lie over lengths)
     constexpr int kDisagrees = 1 << 30;
     if (tid == 0) best = 0;
     for (int i = tid; i < n; i += threads) {
@@ -158,7 +159,6 @@ acceptTreeKernel(const AcceptParams p) {
     __syncthreads();
     const int count = static_cast<int>(best >> 11);
     const int node = count ? kMaxTreeNodes - 1 - static_cast<int>(best & 2047u) : 0;
-    const int len = max(p.lengths[b], 0);
     if (tid == 0) {
         int j = node;
         for (int d = count - 1; d >= 0; --d) {

@@ -3,7 +3,7 @@ import pytest
 
 import pagedattentionmetal_b200 as pam
 from pagedattentionmetal_b200._cabi import lib
-from test_step_host import CALLS, TOO_SMALL, ctx, norm, norm_backward, tree      # noqa: F401
+from test_step_host import CALLS, TOO_SMALL, ctx, norm, norm_backward, plan, tree      # noqa: F401
 
 FAR = 1 << 40                     # the largest stride that is taken, in elements
 ROWS = (1 << 24) + 1              # (ROWS - 1) * FAR = 2^64
@@ -33,3 +33,9 @@ def test_lists_of_tiles_that_a_blocks_share_would_push_past_31_bits(ctx):     # 
         request.layer = pam.PagedLayerSpec(64, 2, 2, 32, pam.PagedAttentionDataType.float16, 0)     # (a tile for each block and head)
         assert CALLS[type(request)](ctx, request) == -1
         assert (text in lib.pam_last_error(ctx)) == refused, blocks
+
+
+def test_total_lengths_over_lengths_are_refused(ctx):     # noqa: F811
+    request = plan()
+    request.totalLengths = request.lengths
+    assert CALLS[type(request)](ctx, request) == -1 and b"totalLengths" in lib.pam_last_error(ctx)
