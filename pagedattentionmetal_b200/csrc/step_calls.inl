@@ -485,6 +485,7 @@ static bool treeShape(Context* c, const PamTreeAttentionRequest& rq, pam::TreePa
     auto bad = [&](const std::string& m) { badStep(c, m); return false; };
     if (l.head_dim > 256) { c->fail(PAM_ERR_UNSUPPORTED, "Unsupported paged attention path: headDim above 256."); return false; }
     if (rq.batch_size <= 0 || rq.batch_size > pam::kTreeMaxBatch) return bad("batchSize must be in 1 ... " + std::to_string(pam::kTreeMaxBatch) + ".");
+    if (static_cast<int64_t>(l.num_kv_heads) * l.block_size > INT32_MAX) return bad("numKVHeads times blockSize is out of range.");
     if (rq.max_num_blocks <= 0) return bad("maxNumBlocks must be positive.");
     if (rq.num_rows <= 0) return bad("numRows must be positive.");
     if (rq.max_new_tokens <= 0) return bad("maxNewTokens must be positive.");

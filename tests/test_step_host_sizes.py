@@ -39,3 +39,12 @@ def test_total_lengths_over_lengths_are_refused(ctx):     # noqa: F811
     request = plan()
     request.totalLengths = request.lengths
     assert CALLS[type(request)](ctx, request) == -1 and b"totalLengths" in lib.pam_last_error(ctx)
+
+
+def test_pages_of_more_than_31_bits_of_tokens_are_refused(ctx):     # noqa: F811
+    """numKVHeads * blockSize is counted in 32 bits: at 2^32 it was the zero that the launch divided by."""
+    request = tree(batchSize=1, numRows=1, maxNewTokens=1, maxNumBlocks=1)
+    for heads, block, refused in ((1 << 16, 1 << 16, True), (1 << 15, 1 << 16, True), (1 << 14, 1 << 16, False)):
+        request.layer = pam.PagedLayerSpec(64, heads, heads, block, pam.PagedAttentionDataType.float16, 0)
+        assert CALLS[type(request)](ctx, request) == -1
+        assert (b"numKVHeads times blockSize" in lib.pam_last_error(ctx)) == refused
