@@ -243,7 +243,7 @@ struct NormRotateParams {
     int numRows, heads, kvHeads, headDim, blockSize, rotaryDim, interleaved, ioType;
     float eps;
 };
-cudaError_t launchNormRotate(const NormRotateParams& p, cudaStream_t stream, int* launches);
+cudaError_t launchNormRotate(const NormRotateParams& p, int smCount, cudaStream_t stream, int* launches);
 
 struct NormRotateBackwardParams {
     const void *q, *k, *qWeight, *kWeight;

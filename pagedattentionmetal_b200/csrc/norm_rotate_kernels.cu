@@ -58,26 +58,25 @@ __device__ __forceinline__ float2 turnOf(int position, float freq) {
     return cs;
 }
 
-// BYTES (8 or 16) of a row: E elements.
-template <typename T, int BYTES>
+// 16 bytes of a row: E elements.
+template <typename T>
 struct Piece {
-    static constexpr int E = BYTES / sizeof(T);
-    using Vec = std::conditional_t<BYTES == 16, uint4, uint2>;
+    static constexpr int E = 16 / sizeof(T);
     union {
-        Vec raw;
-        uint32_t word[BYTES / 4];
+        uint4 raw;
+        uint32_t word[4];
     };
     __device__ __forceinline__ Piece() {
 #pragma unroll
-        for (int i = 0; i < BYTES / 4; ++i) word[i] = 0u;
+        for (int i = 0; i < 4; ++i) word[i] = 0u;
     }
-    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const Vec*>(p); }
-    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Vec*>(p) = raw; }
+    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = raw; }
     // The compiler may not keep what was unpacked before: unpacking again costs less than the registers
     // that hold it (more rows in flight).
     __device__ __forceinline__ void forget() {
 #pragma unroll
-        for (int i = 0; i < BYTES / 4; ++i) asm volatile("" : "+r"(word[i]));
+        for (int i = 0; i < 4; ++i) asm volatile("" : "+r"(word[i]));
     }
     __device__ __forceinline__ void unpack(F2 (&f)[E / 2]) const {
 #pragma unroll
@@ -227,10 +226,10 @@ constexpr int kForwardStages = 4;        // rows in shared memory or on their wa
 // 5.8 TB/s, 0.89 of the copy rate; two rows ahead 142 us, 96 registers (one block less on an SM) 195 us, 56
 // 154 us; one row ahead in registers 155 us; one row a block with a division per head 277 us; 8-byte
 // pieces 242 us (twice the instructions per byte).
-template <typename T, int BYTES>
+template <typename T>
 __global__ void __maxnreg__(80)
 normRotateKernel(const __grid_constant__ NormRotateParams p, const Layout l, int rowsPer) {
-    using P = Piece<T, BYTES>;
+    using P = Piece<T>;
     constexpr int E = P::E;
     extern __shared__ __align__(16) unsigned char rowSmem[];
     unsigned char* ring = rowSmem;                                        // [kForwardStages][2][threads][16]
@@ -249,84 +248,82 @@ normRotateKernel(const __grid_constant__ NormRotateParams p, const Layout l, int
     const bool hasA = pa < l.pieces, hasB = pb < l.pieces;
     const float invDim = 1.f / static_cast<float>(p.headDim);
     // (whole warps stay in the loops for the shuffles)
-    {
-        const int h = static_cast<int>(blockIdx.y) * groups + group;
-        const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads;
-        const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
-        const bool wanted = h < perRow && !(isV && !p.vPool);
-        const T* src = isQ ? static_cast<const T*>(p.q) + static_cast<int64_t>(h) * p.headDim
-                     : isV ? static_cast<const T*>(p.v) + static_cast<int64_t>(kvh) * p.headDim
-                           : static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * p.headDim;
-        const int64_t stride = isQ ? p.qStride : isV ? p.vStride : p.kStride;
-        T* rows = static_cast<T*>(isQ ? p.qOut : isV ? nullptr : p.kOut);
-        const int64_t rowsStride = isQ ? p.qOutStride : p.kOutStride;
-        if (rows) rows += static_cast<int64_t>(isQ ? h : kvh) * p.headDim;
-        T* pool = isQ ? nullptr : static_cast<T*>(isV ? p.vPool : p.kPool);
-        if (pool) pool += static_cast<int64_t>(kvh) * (p.slotsOut ? 1 : p.blockSize) * p.headDim;
-        P wa, wb;
-        if (wanted && !isV && hasA) {
-            const T* weight = static_cast<const T*>(isQ ? p.qWeight : p.kWeight);
-            wa.load(weight + pa * E);
-            if (hasB) wb.load(weight + pb * E);
+    const int h = static_cast<int>(blockIdx.y) * groups + group;
+    const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads;
+    const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
+    const bool wanted = h < perRow && !(isV && !p.vPool);
+    const T* src = isQ ? static_cast<const T*>(p.q) + static_cast<int64_t>(h) * p.headDim
+                 : isV ? static_cast<const T*>(p.v) + static_cast<int64_t>(kvh) * p.headDim
+                       : static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * p.headDim;
+    const int64_t stride = isQ ? p.qStride : isV ? p.vStride : p.kStride;
+    T* rows = static_cast<T*>(isQ ? p.qOut : isV ? nullptr : p.kOut);
+    const int64_t rowsStride = isQ ? p.qOutStride : p.kOutStride;
+    if (rows) rows += static_cast<int64_t>(isQ ? h : kvh) * p.headDim;
+    T* pool = isQ ? nullptr : static_cast<T*>(isV ? p.vPool : p.kPool);
+    if (pool) pool += static_cast<int64_t>(kvh) * (p.slotsOut ? 1 : p.blockSize) * p.headDim;
+    P wa, wb;
+    if (wanted && !isV && hasA) {
+        const T* weight = static_cast<const T*>(isQ ? p.qWeight : p.kWeight);
+        wa.load(weight + pa * E);
+        if (hasB) wb.load(weight + pb * E);
+    }
+    auto place = [&](int r, int which) { return ring + static_cast<size_t>(((r % kForwardStages) * 2 + which) * blockDim.x + tid) * 16; };
+    auto fetch = [&](int r) {
+        if (wanted && hasA && r < n && info[r].position >= 0) {
+            const T* at = src + (row0 + r) * stride;
+            copyAhead(place(r, 0), at + pa * E, true);
+            copyAhead(place(r, 1), at + (hasB ? pb : pa) * E, hasB);
         }
-        auto place = [&](int r, int which) { return ring + static_cast<size_t>(((r % kForwardStages) * 2 + which) * blockDim.x + tid) * 16; };
-        auto fetch = [&](int r) {
-            if (wanted && hasA && r < n && info[r].position >= 0) {
-                const T* at = src + (row0 + r) * stride;
-                copyAhead(place(r, 0), at + pa * E, true);
-                copyAhead(place(r, 1), at + (hasB ? pb : pa) * E, hasB);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
 #pragma unroll
-        for (int r = 0; r < kForwardStages - 1; ++r) fetch(r);
+    for (int r = 0; r < kForwardStages - 1; ++r) fetch(r);
 #pragma unroll 1
-        for (int r = 0; r < n; ++r) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kForwardStages - 2) : "memory");
-            P a, b;
-            if (hasA) {                               // (lanes without a piece add zeros)
-                a.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 0));
-                b.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 1));
-            }
-            fetch(r + kForwardStages - 1);            // (where the row before this one was)
-            F2 sq = 0ull;
-            {
-                F2 fa[E / 2], fb[E / 2];
+    for (int r = 0; r < n; ++r) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kForwardStages - 2) : "memory");
+        P a, b;
+        if (hasA) {                               // (lanes without a piece add zeros)
+            a.raw = *reinterpret_cast<const uint4*>(place(r, 0));
+            b.raw = *reinterpret_cast<const uint4*>(place(r, 1));
+        }
+        fetch(r + kForwardStages - 1);            // (where the row before this one was)
+        F2 sq = 0ull;
+        {
+            F2 fa[E / 2], fb[E / 2];
+            a.unpack(fa);
+            b.unpack(fb);
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) sq = fma2(fb[e], fb[e], fma2(fa[e], fa[e], sq));
+        }
+        float sum = sumOf(sq);
+        for (int o = l.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        a.forget(); b.forget(); wa.forget(); wb.forget();
+        if (wanted && hasA && info[r].position >= 0) {
+            if (!isV) {
+                F2 fa[E / 2], fb[E / 2], ga[E / 2], gb[E / 2];
                 a.unpack(fa);
                 b.unpack(fb);
+                wa.unpack(ga);
+                wb.unpack(gb);
+                const float root = rsqrtf(sum * invDim + p.eps);
+                const F2 scale = pack2(root, root);
 #pragma unroll
-                for (int e = 0; e < E / 2; ++e) sq = fma2(fb[e], fb[e], fma2(fa[e], fa[e], sq));
+                for (int e = 0; e < E / 2; ++e) {
+                    fa[e] = mul2(mul2(fa[e], scale), ga[e]);
+                    fb[e] = mul2(mul2(fb[e], scale), gb[e]);
+                }
+                turnPieces<E>(fa, fb, l, lane, pa, pb, p.rotaryDim, turns + r * 2 * half, 1.f);
+                a.pack(fa);
+                b.pack(fb);
             }
-            float sum = sumOf(sq);
-            for (int o = l.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-            a.forget(); b.forget(); wa.forget(); wb.forget();
-            if (wanted && hasA && info[r].position >= 0) {
-                if (!isV) {
-                    F2 fa[E / 2], fb[E / 2], ga[E / 2], gb[E / 2];
-                    a.unpack(fa);
-                    b.unpack(fb);
-                    wa.unpack(ga);
-                    wb.unpack(gb);
-                    const float root = rsqrtf(sum * invDim + p.eps);
-                    const F2 scale = pack2(root, root);
-#pragma unroll
-                    for (int e = 0; e < E / 2; ++e) {
-                        fa[e] = mul2(mul2(fa[e], scale), ga[e]);
-                        fb[e] = mul2(mul2(fb[e], scale), gb[e]);
-                    }
-                    turnPieces<E>(fa, fb, l, lane, pa, pb, p.rotaryDim, turns + r * 2 * half, 1.f);
-                    a.pack(fa);
-                    b.pack(fb);
-                }
-                const int64_t row = row0 + r, at = info[r].pool;
-                if (rows) {
-                    a.store(rows + row * rowsStride + pa * E);
-                    if (hasB) b.store(rows + row * rowsStride + pb * E);
-                }
-                if (pool && at >= 0) {
-                    a.store(pool + at + pa * E);
-                    if (hasB) b.store(pool + at + pb * E);
-                }
+            const int64_t row = row0 + r, at = info[r].pool;
+            if (rows) {
+                a.store(rows + row * rowsStride + pa * E);
+                if (hasB) b.store(rows + row * rowsStride + pb * E);
+            }
+            if (pool && at >= 0) {
+                a.store(pool + at + pa * E);
+                if (hasB) b.store(pool + at + pb * E);
             }
         }
     }
@@ -424,8 +421,8 @@ inline void headChunks(int perRow, int lanes, int* chunks, int* threads) {
 }
 
 template <typename T>
-cudaError_t normRotateOf(const NormRotateParams& p, cudaStream_t stream, int* launches) {
-    constexpr int BYTES = 16, E = BYTES / sizeof(T);
+cudaError_t normRotateOf(const NormRotateParams& p, int smCount, cudaStream_t stream, int* launches) {
+    constexpr int E = Piece<T>::E;
     const void* ptrs[] = {p.q, p.k, p.v, p.qWeight, p.kWeight, p.qOut, p.kOut, p.kPool, p.vPool};
     bool pieces = piecesApply<E>(p.headDim, p.rotaryDim, p.interleaved);
     for (const void* ptr : ptrs) pieces = pieces && aligned16(ptr);
@@ -433,20 +430,20 @@ cudaError_t normRotateOf(const NormRotateParams& p, cudaStream_t stream, int* la
     const int perRow = p.heads + 2 * p.kvHeads;
     if (!pieces) {
         const int64_t warps = static_cast<int64_t>(p.numRows) * perRow;
-        normRotateAnyKernel<T><<<static_cast<unsigned>(std::min<int64_t>((warps + 3) / 4, 148 * 16)), 128, 0, stream>>>(p);
+        normRotateAnyKernel<T><<<static_cast<unsigned>(std::min<int64_t>((warps + 3) / 4, smCount * 16)), 128, 0, stream>>>(p);
     } else {
         const Layout l = layoutOf<E>(p.headDim, p.rotaryDim, p.interleaved);
         int chunks, threads;
         headChunks(perRow, l.lanes, &chunks, &threads);
         // enough blocks for every SM first, then rows to share the look-ups and the weights
-        const int rowsPer = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kForwardRows, p.numRows / (148 * 4))));
+        const int rowsPer = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kForwardRows, p.numRows / (smCount * 4))));
         const size_t smem = static_cast<size_t>(threads) * kForwardStages * 2 * 16 + static_cast<size_t>(rowsPer) * (sizeof(RowInfo) + (p.rotaryDim / 2) * sizeof(float2));
         // (at most 544 threads, 68 KB of rows, and 16 KB of turns)
         static std::atomic<unsigned long long> done{0};
-        const cudaError_t allowed = allowSmem(normRotateKernel<T, BYTES>, 100 * 1024, done);
+        const cudaError_t allowed = allowSmem(normRotateKernel<T>, 100 * 1024, done);
         if (allowed != cudaSuccess) return allowed;
         const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.numRows) + rowsPer - 1) / rowsPer), chunks);
-        normRotateKernel<T, BYTES><<<grid, threads, smem, stream>>>(p, l, rowsPer);
+        normRotateKernel<T><<<grid, threads, smem, stream>>>(p, l, rowsPer);
     }
     *launches += 1;
     return cudaGetLastError();
@@ -468,10 +465,10 @@ constexpr int kBackwardStages = 3;       // rows in shared memory or on their wa
 // rows of 32 + 8 heads of 128, bfloat16 (252 MB): 55.5 us = 4.5 TB/s, 0.69 of the copy rate, bound by the
 // issue of some 250 instructions per 16 elements; one row ahead in registers, with look-ups for 8 rows at
 // a time, 76 us; three rows ahead 55.5 us; 80 registers, with spills, 61 us; four blocks on an SM 59 us.
-template <typename T, int BYTES>
+template <typename T>
 __global__ void __maxnreg__(96)
 normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, const Layout l, int share) {
-    using P = Piece<T, BYTES>;
+    using P = Piece<T>;
     constexpr int E = P::E;
     extern __shared__ __align__(16) unsigned char rowSmem[];
     const int tid = threadIdx.x, half = p.rotaryDim / 2, threads = blockDim.x;
@@ -487,137 +484,135 @@ normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, con
     l.lane(lane, pa, pb);
     const bool hasA = pa < l.pieces, hasB = pb < l.pieces;
     const float invDim = 1.f / static_cast<float>(p.headDim);
-    {
-        const int h0 = static_cast<int>(blockIdx.y) * groups, h = h0 + group;
-        const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads, wanted = h < perRow;
-        const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
-        const T* src = isQ ? static_cast<const T*>(p.q) + static_cast<int64_t>(h) * p.headDim : static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * p.headDim;
-        const int64_t srcStride = isQ ? p.qStride : p.kStride;
-        // the gradient with respect to the rotated row: rows, or (keys and values) pages
-        const T* up = isQ ? static_cast<const T*>(p.dQOut) + static_cast<int64_t>(h) * p.headDim
-                    : !isV && p.dKOut ? static_cast<const T*>(p.dKOut) + static_cast<int64_t>(kvh) * p.headDim
-                    : static_cast<const T*>(isV ? p.dVPool : p.dKPool) + static_cast<int64_t>(kvh) * p.blockSize * p.headDim;
-        const int64_t upStride = static_cast<int64_t>(isQ ? p.heads : p.kvHeads) * p.headDim;
-        const bool fromPool = !isQ && (isV || !p.dKOut);
-        T* dst = static_cast<T*>(isQ ? p.dQ : isV ? p.dV : p.dK) + static_cast<int64_t>(isQ ? h : kvh) * p.headDim;
-        const int64_t dstStride = isQ ? p.dQStride : isV ? p.dVStride : p.dKStride;
-        P wa, wb;
-        if (wanted && !isV && hasA) {
-            const T* weight = static_cast<const T*>(isQ ? p.qWeight : p.kWeight);
-            wa.load(weight + pa * E);
-            if (hasB) wb.load(weight + pb * E);
-        }
-        F2 accA[E / 2], accB[E / 2];
+    const int h0 = static_cast<int>(blockIdx.y) * groups, h = h0 + group;
+    const bool isQ = h < p.heads, isV = h >= p.heads + p.kvHeads, wanted = h < perRow;
+    const int kvh = isQ ? 0 : isV ? h - p.heads - p.kvHeads : h - p.heads;
+    const T* src = isQ ? static_cast<const T*>(p.q) + static_cast<int64_t>(h) * p.headDim : static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * p.headDim;
+    const int64_t srcStride = isQ ? p.qStride : p.kStride;
+    // the gradient with respect to the rotated row: rows, or (keys and values) pages
+    const T* up = isQ ? static_cast<const T*>(p.dQOut) + static_cast<int64_t>(h) * p.headDim
+                : !isV && p.dKOut ? static_cast<const T*>(p.dKOut) + static_cast<int64_t>(kvh) * p.headDim
+                : static_cast<const T*>(isV ? p.dVPool : p.dKPool) + static_cast<int64_t>(kvh) * p.blockSize * p.headDim;
+    const int64_t upStride = static_cast<int64_t>(isQ ? p.heads : p.kvHeads) * p.headDim;
+    const bool fromPool = !isQ && (isV || !p.dKOut);
+    T* dst = static_cast<T*>(isQ ? p.dQ : isV ? p.dV : p.dK) + static_cast<int64_t>(isQ ? h : kvh) * p.headDim;
+    const int64_t dstStride = isQ ? p.dQStride : isV ? p.dVStride : p.dKStride;
+    P wa, wb;
+    if (wanted && !isV && hasA) {
+        const T* weight = static_cast<const T*>(isQ ? p.qWeight : p.kWeight);
+        wa.load(weight + pa * E);
+        if (hasB) wb.load(weight + pb * E);
+    }
+    F2 accA[E / 2], accB[E / 2];
 #pragma unroll
-        for (int e = 0; e < E / 2; ++e) accA[e] = accB[e] = 0ull;
-        for (int64_t row0 = begin; row0 < end; row0 += kBackwardRows) {
-            const int n = static_cast<int>(min(static_cast<int64_t>(kBackwardRows), end - row0));
-            __syncthreads();
-            lookRowsUp(info, turns, row0, n, p.positions, p.slots, p.numSlots, p.invFreq, half, p.kvHeads, p.blockSize, p.headDim, false);
-            // A thread copies what it will read itself, two rows ahead; nobody waits for anybody.
-            auto place = [&](int r, int which) { return ring + static_cast<size_t>(((r % kBackwardStages) * 4 + which) * threads + tid) * 16; };
-            auto fetch = [&](int r) {
-                if (wanted && hasA && r < n && info[r].position >= 0) {
-                    if (!isV) {
-                        const T* at = src + (row0 + r) * srcStride;
-                        copyAhead(place(r, 0), at + pa * E, true);
-                        copyAhead(place(r, 1), at + (hasB ? pb : pa) * E, hasB);
-                    }
-                    const int64_t slot = info[r].pool;
-                    const T* from = fromPool ? up + (slot >= 0 ? slot : 0) : up + (row0 + r) * upStride;
-                    const bool there = !fromPool || slot >= 0;
-                    copyAhead(place(r, 2), from + pa * E, there);
-                    copyAhead(place(r, 3), from + (hasB ? pb : pa) * E, there && hasB);
+    for (int e = 0; e < E / 2; ++e) accA[e] = accB[e] = 0ull;
+    for (int64_t row0 = begin; row0 < end; row0 += kBackwardRows) {
+        const int n = static_cast<int>(min(static_cast<int64_t>(kBackwardRows), end - row0));
+        __syncthreads();
+        lookRowsUp(info, turns, row0, n, p.positions, p.slots, p.numSlots, p.invFreq, half, p.kvHeads, p.blockSize, p.headDim, false);
+        // A thread copies what it will read itself, two rows ahead; nobody waits for anybody.
+        auto place = [&](int r, int which) { return ring + static_cast<size_t>(((r % kBackwardStages) * 4 + which) * threads + tid) * 16; };
+        auto fetch = [&](int r) {
+            if (wanted && hasA && r < n && info[r].position >= 0) {
+                if (!isV) {
+                    const T* at = src + (row0 + r) * srcStride;
+                    copyAhead(place(r, 0), at + pa * E, true);
+                    copyAhead(place(r, 1), at + (hasB ? pb : pa) * E, hasB);
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
+                const int64_t slot = info[r].pool;
+                const T* from = fromPool ? up + (slot >= 0 ? slot : 0) : up + (row0 + r) * upStride;
+                const bool there = !fromPool || slot >= 0;
+                copyAhead(place(r, 2), from + pa * E, there);
+                copyAhead(place(r, 3), from + (hasB ? pb : pa) * E, there && hasB);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
 #pragma unroll
-            for (int r = 0; r < kBackwardStages - 1; ++r) fetch(r);
+        for (int r = 0; r < kBackwardStages - 1; ++r) fetch(r);
 #pragma unroll 1
-            for (int r = 0; r < n; ++r) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kBackwardStages - 2) : "memory");
-                struct { P xa, xb, ya, yb; } w;
-                if (hasA) {                           // (lanes without a piece add zeros)
-                    w.xa.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 0));
-                    w.xb.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 1));
-                    w.ya.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 2));
-                    w.yb.raw = *reinterpret_cast<const typename P::Vec*>(place(r, 3));
-                }
-                fetch(r + kBackwardStages - 1);       // (where the row before this one was)
-                const bool live = wanted && hasA && info[r].position >= 0;
-                T* to = dst + (row0 + r) * dstStride;
-                if (live && isV) {
-                    w.ya.store(to + pa * E);
-                    if (hasB) w.yb.store(to + pb * E);
-                }
-                F2 ga[E / 2], gb[E / 2], sq = 0ull, xg = 0ull;                // sums of x^2, and of x * g
-                w.ya.unpack(ga); w.yb.unpack(gb);
-                turnPieces<E>(ga, gb, l, lane, pa, pb, p.rotaryDim, turns + r * 2 * half, -1.f);
-                {
-                    F2 fa[E / 2], fb[E / 2], va[E / 2], vb[E / 2];
-                    w.xa.unpack(fa); w.xb.unpack(fb);
-                    wa.unpack(va); wb.unpack(vb);
+        for (int r = 0; r < n; ++r) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kBackwardStages - 2) : "memory");
+            struct { P xa, xb, ya, yb; } w;
+            if (hasA) {                           // (lanes without a piece add zeros)
+                w.xa.raw = *reinterpret_cast<const uint4*>(place(r, 0));
+                w.xb.raw = *reinterpret_cast<const uint4*>(place(r, 1));
+                w.ya.raw = *reinterpret_cast<const uint4*>(place(r, 2));
+                w.yb.raw = *reinterpret_cast<const uint4*>(place(r, 3));
+            }
+            fetch(r + kBackwardStages - 1);       // (where the row before this one was)
+            const bool live = wanted && hasA && info[r].position >= 0;
+            T* to = dst + (row0 + r) * dstStride;
+            if (live && isV) {
+                w.ya.store(to + pa * E);
+                if (hasB) w.yb.store(to + pb * E);
+            }
+            F2 ga[E / 2], gb[E / 2], sq = 0ull, xg = 0ull;                // sums of x^2, and of x * g
+            w.ya.unpack(ga); w.yb.unpack(gb);
+            turnPieces<E>(ga, gb, l, lane, pa, pb, p.rotaryDim, turns + r * 2 * half, -1.f);
+            {
+                F2 fa[E / 2], fb[E / 2], va[E / 2], vb[E / 2];
+                w.xa.unpack(fa); w.xb.unpack(fb);
+                wa.unpack(va); wb.unpack(vb);
 #pragma unroll
-                    for (int e = 0; e < E / 2; ++e) {
-                        sq = fma2(fb[e], fb[e], fma2(fa[e], fa[e], sq));
-                        xg = fma2(fb[e], mul2(gb[e], vb[e]), fma2(fa[e], mul2(ga[e], va[e]), xg));
-                    }
+                for (int e = 0; e < E / 2; ++e) {
+                    sq = fma2(fb[e], fb[e], fma2(fa[e], fa[e], sq));
+                    xg = fma2(fb[e], mul2(gb[e], vb[e]), fma2(fa[e], mul2(ga[e], va[e]), xg));
                 }
-                w.xa.forget(); w.xb.forget(); wa.forget(); wb.forget();
-                float sum = sumOf(sq), dot = sumOf(xg);
-                for (int o = l.lanes >> 1; o > 0; o >>= 1) {
-                    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-                    dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
-                }
-                if (live && !isV) {
-                    const float root = rsqrtf(sum * invDim + p.eps);
-                    const float mean = dot * root * invDim;               // of xhat * g
-                    const F2 scale = pack2(root, root), minusMean = pack2(-mean, -mean);
-                    F2 fa[E / 2], fb[E / 2], va[E / 2], vb[E / 2], ha[E / 2], hb[E / 2];
-                    w.xa.unpack(fa); w.xb.unpack(fb);
-                    wa.unpack(va); wb.unpack(vb);
+            }
+            w.xa.forget(); w.xb.forget(); wa.forget(); wb.forget();
+            float sum = sumOf(sq), dot = sumOf(xg);
+            for (int o = l.lanes >> 1; o > 0; o >>= 1) {
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+                dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+            }
+            if (live && !isV) {
+                const float root = rsqrtf(sum * invDim + p.eps);
+                const float mean = dot * root * invDim;               // of xhat * g
+                const F2 scale = pack2(root, root), minusMean = pack2(-mean, -mean);
+                F2 fa[E / 2], fb[E / 2], va[E / 2], vb[E / 2], ha[E / 2], hb[E / 2];
+                w.xa.unpack(fa); w.xb.unpack(fb);
+                wa.unpack(va); wb.unpack(vb);
 #pragma unroll
-                    for (int e = 0; e < E / 2; ++e) {
-                        const F2 ua = mul2(fa[e], scale), ub = mul2(fb[e], scale);        // xhat
-                        ha[e] = mul2(scale, fma2(ua, minusMean, mul2(ga[e], va[e])));
-                        hb[e] = mul2(scale, fma2(ub, minusMean, mul2(gb[e], vb[e])));
-                        accA[e] = fma2(ga[e], ua, accA[e]);
-                        accB[e] = fma2(gb[e], ub, accB[e]);
-                    }
-                    P out;
-                    out.pack(ha);
-                    out.store(to + pa * E);
-                    if (hasB) {
-                        out.pack(hb);
-                        out.store(to + pb * E);
-                    }
+                for (int e = 0; e < E / 2; ++e) {
+                    const F2 ua = mul2(fa[e], scale), ub = mul2(fb[e], scale);        // xhat
+                    ha[e] = mul2(scale, fma2(ua, minusMean, mul2(ga[e], va[e])));
+                    hb[e] = mul2(scale, fma2(ub, minusMean, mul2(gb[e], vb[e])));
+                    accA[e] = fma2(ga[e], ua, accA[e]);
+                    accB[e] = fma2(gb[e], ub, accB[e]);
+                }
+                P out;
+                out.pack(ha);
+                out.store(to + pa * E);
+                if (hasB) {
+                    out.pack(hb);
+                    out.store(to + pb * E);
                 }
             }
         }
-        if (!p.partials) return;
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();
+    }
+    if (!p.partials) return;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 #pragma unroll
-        for (int e = 0; e < E / 2; ++e) {
-            *reinterpret_cast<F2*>(sums + tid * 2 * E + 2 * e) = accA[e];
-            *reinterpret_cast<F2*>(sums + tid * 2 * E + E + 2 * e) = accB[e];
-        }
-        __syncthreads();
-        // element i of a head: the lane and place that hold it, its groups in order, queries and keys apart
-        for (int i = tid; i < l.lanes * 2 * E; i += threads) {
-            int a, b;
-            l.lane(i / (2 * E), a, b);
-            const int e = i % (2 * E), piece = e < E ? a : b;
-            if (piece >= l.pieces) continue;
-            const int d = piece * E + e % E, queries = min(max(p.heads - h0, 0), groups);
-            const int both = min(max(p.heads + p.kvHeads - h0, 0), groups);
-            float q = 0.f, k = 0.f;
-            for (int g = 0; g < queries; ++g) q += sums[g * l.lanes * 2 * E + i];
-            for (int g = queries; g < both; ++g) k += sums[g * l.lanes * 2 * E + i];
-            float* out = p.partials + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 2 * p.headDim;
-            out[d] = q;
-            out[p.headDim + d] = k;
-        }
+    for (int e = 0; e < E / 2; ++e) {
+        *reinterpret_cast<F2*>(sums + tid * 2 * E + 2 * e) = accA[e];
+        *reinterpret_cast<F2*>(sums + tid * 2 * E + E + 2 * e) = accB[e];
+    }
+    __syncthreads();
+    // element i of a head: the lane and place that hold it, its groups in order, queries and keys apart
+    for (int i = tid; i < l.lanes * 2 * E; i += threads) {
+        int a, b;
+        l.lane(i / (2 * E), a, b);
+        const int e = i % (2 * E), piece = e < E ? a : b;
+        if (piece >= l.pieces) continue;
+        const int d = piece * E + e % E, queries = min(max(p.heads - h0, 0), groups);
+        const int both = min(max(p.heads + p.kvHeads - h0, 0), groups);
+        float q = 0.f, k = 0.f;
+        for (int g = 0; g < queries; ++g) q += sums[g * l.lanes * 2 * E + i];
+        for (int g = queries; g < both; ++g) k += sums[g * l.lanes * 2 * E + i];
+        float* out = p.partials + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 2 * p.headDim;
+        out[d] = q;
+        out[p.headDim + d] = k;
     }
 }
 
@@ -718,11 +713,10 @@ weightGradientKernel(const float* __restrict__ partials, int blocks, int dim, fl
 int backwardBlocks(const NormRotateBackwardParams& p, int smCount) {
     return static_cast<int>(std::min<int64_t>((static_cast<int64_t>(p.numRows) + kBackwardShare - 1) / kBackwardShare, static_cast<int64_t>(smCount) * 2));
 }
-template <typename T> constexpr int backwardBytes() { return 16; }
 // Lanes and threads of the launch that the pieces allow (chunks 1, threads 0: the other kernel runs).
 template <typename T>
 int backwardChunks(const NormRotateBackwardParams& p, Layout* l, int* threads) {
-    constexpr int E = backwardBytes<T>() / sizeof(T);
+    constexpr int E = Piece<T>::E;
     *threads = 0;
     if (!piecesApply<E>(p.headDim, p.rotaryDim, p.interleaved)) return 1;
     *l = layoutOf<E>(p.headDim, p.rotaryDim, p.interleaved);
@@ -733,7 +727,7 @@ int backwardChunks(const NormRotateBackwardParams& p, Layout* l, int* threads) {
 
 template <typename T>
 cudaError_t normRotateBackwardOf(const NormRotateBackwardParams& p, int smCount, cudaStream_t stream, int* launches) {
-    constexpr int BYTES = backwardBytes<T>(), E = BYTES / sizeof(T);
+    constexpr int E = Piece<T>::E;
     const void* ptrs[] = {p.q, p.k, p.qWeight, p.kWeight, p.dQOut, p.dKOut, p.dKPool, p.dVPool, p.dQ, p.dK, p.dV};
     Layout l{};
     int threads, chunks = backwardChunks<T>(p, &l, &threads);
@@ -747,9 +741,9 @@ cudaError_t normRotateBackwardOf(const NormRotateBackwardParams& p, int smCount,
                             kBackwardRows * (sizeof(RowInfo) + (p.rotaryDim / 2) * sizeof(float2));
         // (at most 544 threads, 102 KB of rows, and 33 KB of turns)
         static std::atomic<unsigned long long> done{0};
-        const cudaError_t allowed = allowSmem(normRotateBackwardKernel<T, BYTES>, 160 * 1024, done);
+        const cudaError_t allowed = allowSmem(normRotateBackwardKernel<T>, 160 * 1024, done);
         if (allowed != cudaSuccess) return allowed;
-        normRotateBackwardKernel<T, BYTES><<<dim3(blocks, chunks), threads, smem, stream>>>(p, l, share);
+        normRotateBackwardKernel<T><<<dim3(blocks, chunks), threads, smem, stream>>>(p, l, share);
     } else {
         chunks = 1;
         normRotateBackwardAnyKernel<T><<<blocks, 128, static_cast<size_t>(16) * p.headDim * sizeof(float), stream>>>(p);
@@ -774,11 +768,11 @@ cudaError_t normRotateBackwardOf(const NormRotateBackwardParams& p, int smCount,
 
 }  // namespace
 
-cudaError_t launchNormRotate(const NormRotateParams& p, cudaStream_t stream, int* launches) {
+cudaError_t launchNormRotate(const NormRotateParams& p, int smCount, cudaStream_t stream, int* launches) {
     switch (p.ioType) {
-        case kF32: return normRotateOf<float>(p, stream, launches);
-        case kBF16: return normRotateOf<__nv_bfloat16>(p, stream, launches);
-        default: return normRotateOf<__half>(p, stream, launches);
+        case kF32: return normRotateOf<float>(p, smCount, stream, launches);
+        case kBF16: return normRotateOf<__nv_bfloat16>(p, smCount, stream, launches);
+        default: return normRotateOf<__half>(p, smCount, stream, launches);
     }
 }
 

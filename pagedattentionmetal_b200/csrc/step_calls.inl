@@ -353,7 +353,7 @@ int32_t pamc_norm_rotate(void* ctx, const PamNormRotateRequest* request, void* c
         p.numSlots = static_cast<int64_t>(poolBlocksOf(kPool, vPool, l)) * l.block_size;
         if (!fp8 || !pages) {
             p.kPool = args[9].device; p.vPool = args[10].device;
-            return pam::launchNormRotate(p, c->stream, launches);
+            return pam::launchNormRotate(p, c->smCount, c->stream, launches);
         }
         // FP8: the scale of a block needs every new row of it first, so the rows go through the append
         // kernels, which take them back to back from a 16-byte boundary on: kOut and V where they are that,
@@ -367,7 +367,7 @@ int32_t pamc_norm_rotate(void* ctx, const PamNormRotateRequest* request, void* c
         p.slotsOut = static_cast<int64_t*>(c->arena.take(static_cast<size_t>(R) * 8));
         if (!keys || !values || !p.slotsOut) return cudaErrorMemoryAllocation;
         cudaError_t e = nextAbsmaxEpoch(k, c->stream);
-        if (e == cudaSuccess) e = pam::launchNormRotate(p, c->stream, launches);
+        if (e == cudaSuccess) e = pam::launchNormRotate(p, c->smCount, c->stream, launches);
         if (e != cudaSuccess) return e;
         pam::SlotSource src;
         src.slots = p.slotsOut;
