@@ -24,17 +24,20 @@ def _span(x, name: str) -> _cabi.PamBuffer:
     if hasattr(x, "is_contiguous"):
         if x.is_contiguous():
             return _cabi.PamBuffer(x.data_ptr(), x.numel() * x.element_size())
-        row = name in _ROWS and x[0].is_contiguous()
         strides, size = x.stride(), x.element_size()
     elif hasattr(x, "flags") and hasattr(x, "strides") and not x.flags.c_contiguous:
-        row = name in _ROWS and x.strides[0] > 0 and x[0].flags.c_contiguous
         strides, size = [s // x.itemsize for s in x.strides], x.itemsize
     else:
         return _cabi.buffer(x)
-    if not row:
+    width, shape = 1, x.shape                        # (elements of a row)
+    for n, stride in zip(shape[:0:-1], strides[:0:-1]):
+        if stride != width and n != 1:
+            width = -1
+            break
+        width *= n
+    if name not in _ROWS or width < 0 or strides[0] < 0:
         raise ValueError(f"{name} must be contiguous" + (" within a row" if name in _ROWS else ""))
-    elements = 1 + sum((n - 1) * s for n, s in zip(x.shape, strides)) if all(x.shape) else 0
-    return _cabi.PamBuffer(_cabi.address(x), elements * size)
+    return _cabi.PamBuffer(_cabi.address(x), ((shape[0] - 1) * strides[0] + width) * size)
 
 
 # What the index, scale and frequency buffers hold; arrays and tensors of another type are refused (rows, pages and
@@ -45,7 +48,13 @@ _HOLDS = {**{name: "int32" for name in (
               "nextTokens", "newLengths")},
           "slots": "int64", "invFreq": "float32", "dQWeight": "float32", "dKWeight": "float32",
           "kScaleBuffer": "float16", "vScaleBuffer": "float16"}
-_TAKEN = {"int32": ("int32", "uint32"), "int64": ("int64", "uint64")}
+_TAKEN = {"uint32": "int32", "uint64": "int64"}
+_HELD: dict = {}                                     # dtype of an array or a tensor -> what it counts as
+
+
+def _held(dtype) -> str:
+    name = str(dtype).rpartition(".")[2]             # ("torch.int32")
+    return _HELD.setdefault(dtype, _TAKEN.get(name, name))
 
 
 class _Request:
@@ -75,11 +84,9 @@ class _Request:
             raise AttributeError(f"{type(self).__name__} has no field {name}")
         field, default = self._fields[name]
         if default is None:
-            holds = _HOLDS.get(name)
-            if holds and hasattr(value, "dtype"):
-                held = str(value.dtype).rpartition(".")[2]           # ("torch.int32")
-                if held != holds and held not in _TAKEN.get(holds, ()):
-                    raise TypeError(f"{type(self).__name__}.{name} holds {holds}, not {held}")
+            dtype = getattr(value, "dtype", None)
+            if dtype is not None and name in _HOLDS and (_HELD.get(dtype) or _held(dtype)) != _HOLDS[name]:
+                raise TypeError(f"{type(self).__name__}.{name} holds {_HOLDS[name]}, not {_held(dtype)}")
             c = _span(value, name)
         elif isinstance(value, PagedLayerSpec):
             c = _cabi.PamLayerSpec(value.headDim, value.numHeads, value.numKVHeads, value.blockSize,
