@@ -148,7 +148,9 @@ void *pamc_create_host_context(void);
 /* Class of the last error on this context (PAM_ERR_*), PAM_OK if none. */
 int32_t pamc_last_error_code(void *ctx);
 /* Run on a caller-owned CUDA stream (a cudaStream_t); NULL restores the
- * context's own stream, which is in order with the device's default stream. */
+ * context's own stream, which is in order with the device's default stream: each waits
+ * for what the other was given before.  Work that is to overlap with default-stream work
+ * needs a stream of the caller's (a non-blocking one). */
 int32_t pamc_set_stream(void *ctx, void *cuda_stream);
 /* 1: operations return after enqueueing; 0 (default): they wait for the GPU
  * like the reference's commitAndWait (PagedAttentionEngine.swift:2008-2015). */
@@ -579,6 +581,8 @@ int64_t pamc_norm_rotate_backward_workspace(void *ctx, const PamNormRotateBackwa
  * scales a row does not see do not reach it, whatever they hold; a key scale that is not a finite
  * number makes the rows that see its page NaN.  Rows outside every request stay as they
  * were.  Requests beyond max_new_tokens rows are cut off there.
+ * Pools of unknown length (bytes = (size_t)-1) are taken, but 16-bit ones not by the tcgen05
+ * kernel, which takes a fifth to a quarter of the time with many rows: give them their lengths.
  * Scores, sums and accumulators are float32; with 16-bit and FP8 pages the softmax weights are
  * rounded to 16 bits for their product with the values (pamc_set_prefill_exact_weights). */
 typedef struct PamTreeAttentionRequest {

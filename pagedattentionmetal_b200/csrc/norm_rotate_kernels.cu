@@ -222,10 +222,11 @@ constexpr int kForwardStages = 4;        // rows in shared memory or on their wa
 // A block takes `rowsPer` rows.  A group of l.lanes lanes keeps one head of them (of the queries,
 // keys and values of a row, one after the other), so that its weights stay in registers and nothing
 // is divided inside the loop; rows come to shared memory by asynchronous copies, three ahead, each
-// thread its own pieces.  Measured at 32768 rows of 32 + 8 + 8 heads of 128, float16 (806 MB): 139 us =
-// 5.8 TB/s, 0.89 of the copy rate; two rows ahead 142 us, 96 registers (one block less on an SM) 195 us, 56
-// 154 us; one row ahead in registers 155 us; one row a block with a division per head 277 us; 8-byte
-// pieces 242 us (twice the instructions per byte).
+// thread its own pieces.  Measured at 32768 rows of 32 + 8 + 8 heads of 128, float16 (806 MB), call after call on
+// the same buffers: 138 us = 5.8 TB/s, 0.89 of the copy rate (156 us, 0.79, where every call has buffers of its
+// own); two rows ahead 142 us, 96 registers (one block less on an SM) 195 us, 56 154 us; one row ahead in
+// registers 155 us; one row a block with a division per head 277 us; 8-byte pieces 242 us (twice the
+// instructions per byte).  float32 (1.6 GB) 255 us, 0.96 of the copy rate.
 template <typename T>
 __global__ void __maxnreg__(80)
 normRotateKernel(const __grid_constant__ NormRotateParams p, const Layout l, int rowsPer) {
@@ -339,7 +340,9 @@ constexpr int kForwardRows = 16;
 constexpr int kMaxDim = 256;
 
 // Any head_dim, rotaryDim and alignment: one warp per (row, head), element by element, the row
-// in shared memory so that outputs may lie over the inputs.
+// in shared memory so that outputs may lie over the inputs.  Cosine and sine are taken anew for every element of
+// every head: 8192 rows of 32 + 8 + 8 heads of 96, float16, with 24 rotated elements 195 us, where the pieces
+// (all 96 rotated) take 45 us.
 template <typename T>
 __global__ void __launch_bounds__(128)
 normRotateAnyKernel(const __grid_constant__ NormRotateParams p) {
@@ -462,9 +465,10 @@ constexpr int kBackwardStages = 3;       // rows in shared memory or on their wa
 // shared memory in a fixed order and the block writes its [2][dim] partial sums: no atomics, the same
 // bits for the same grid.  Rows come to shared memory by asynchronous copies, two ahead, each thread its
 // own pieces, so that no registers wait for them and no barrier stands in the loop.  Measured at 8192
-// rows of 32 + 8 heads of 128, bfloat16 (252 MB): 55.5 us = 4.5 TB/s, 0.69 of the copy rate, bound by the
-// issue of some 250 instructions per 16 elements; one row ahead in registers, with look-ups for 8 rows at
-// a time, 76 us; three rows ahead 55.5 us; 80 registers, with spills, 61 us; four blocks on an SM 59 us.
+// rows of 32 + 8 heads of 128, bfloat16 (252 MB): 55.4 us = 4.5 TB/s, 0.69 of the copy rate, bound by
+// instructions: 455 a warp for each 16 elements of its lanes, 67% of the issue slots taken with 4.4 warps a
+// scheduler; one row ahead in registers, with look-ups for 8 rows at a time, 76 us; three rows ahead 55.5 us;
+// 80 registers, with spills, 61 us; four blocks on an SM 59 us.
 template <typename T>
 __global__ void __maxnreg__(96)
 normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, const Layout l, int share) {
@@ -617,7 +621,9 @@ normRotateBackwardKernel(const __grid_constant__ NormRotateBackwardParams p, con
 }
 
 // Any shape and alignment, one warp per (row, head) at a time: the warp's share of the weight
-// gradients is added up in shared memory, each element by the lane that owns it.
+// gradients is added up in shared memory, each element by the lane that owns it.  As the forward one, and with the
+// few blocks that the partial sums are counted for: 8192 rows of 32 + 8 heads of 96, float16, with 24 rotated
+// elements 754 us, where the pieces (all 96 rotated) take 58 us.
 template <typename T>
 __global__ void __launch_bounds__(128)
 normRotateBackwardAnyKernel(const __grid_constant__ NormRotateBackwardParams p) {

@@ -358,7 +358,8 @@ int32_t pamc_norm_rotate(void* ctx, const PamNormRotateRequest* request, void* c
         // FP8: the scale of a block needs every new row of it first, so the rows go through the append
         // kernels, which take them back to back from a 16-byte boundary on: kOut and V where they are that,
         // else scratch that the same launch writes beside kOut (one launch, since the outputs may lie over the
-        // inputs).  Skipped rows lose their slot.
+        // inputs).  Skipped rows lose their slot.  32 + 8 + 8 heads of 128: 64 rows 12.7 us, 8192 rows 84 us, 32768
+        // rows 234 us (float16 pages 4.8, 45, 138 us): three launches, and keys and values are read twice more.
         const size_t bytes = static_cast<size_t>(R) * kWide * io;
         const void *keys = p.kOut, *values = p.v;
         auto aligned = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; };

@@ -27,7 +27,9 @@ using namespace tree;
 // those of rows z and z + 4.  RW 8 takes 12 loads of 16 bytes for 128 products where RW 4 takes 8 for
 // 64, and half the fetches of keys and values: chosen when a request can have more than 16 rows (32
 // float32 requests of 4096 tokens, 64 rows: 1.40 against 1.66 ms; half of the instructions are products).
-// HALVES: blocks of 128 dims.
+// HALVES: blocks of 128 dims.  Above head_dim 128 the 16-bit types run here too, and every tile of 16 rows fetches
+// the keys again: bfloat16 with head_dim 256, 32 requests of 4096 tokens, 16 rows 1.75 ms, 64 rows 6.8 ms, where the
+// bytes take 165 us.
 constexpr int kGenKeys = 32, kGenThreads = 128;
 
 struct GeneralSmem {
@@ -515,10 +517,11 @@ TreePlan generalPlan(const TreeParams& p, int smCount) {
     return t;
 }
 
-// The tcgen05 kernel wherever it applies: at 32 requests of 4096 tokens (head_dim 128) and 4, 64 and 256
-// rows under a KV head 100, 110 and 185 us against 134, 237 and 867 us of the mma kernel, on short lists too, with one request of 8192
-// tokens, 23, 23 and 34 against 23, 34 and 68.  But a call that cannot have work for every block, and few rows, is over
-// sooner in the kernel with the shorter way from start to end (1024 tokens, 4 rows: 12.6 against 15.9 us).
+// The tcgen05 kernel wherever it applies: at 32 requests of 4096 tokens (head_dim 128, bfloat16) and 4, 64 and 256
+// rows under a KV head 100, 109 and 178 us against 121, 231 and 821 us of the mma kernel, on short lists too, with
+// one request of 8192 tokens and 4, 24 and 96 rows, 23, 23 and 24 against 23, 27 and 43.  But a call that cannot have
+// work for every block, and few rows, is over sooner in the kernel with the shorter way from start to end (1024
+// tokens, 4 rows: 12.6 against 16.4 us).
 bool shortCall(const TreeParams& p, int smCount) {
     const int64_t tiles = static_cast<int64_t>(p.batch) * p.kvHeads * ((static_cast<int64_t>(p.maxNumBlocks) * p.blockSize + 127) / 128 + 1);
     return static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) <= 16 && tiles <= smCount;

@@ -1,10 +1,10 @@
 // Tree attention for 16-bit and FP8 pools where the tcgen05 kernel does not apply (head_dim below 64 or
-// not a multiple of 16, FP8 pages that are not multiples of 16 tokens, very large batches of FP8) and for calls
-// too short for it, on mma.sync.m16n8k16.  A key costs 4 head_dim bytes and 4 head_dim flops per
+// not a multiple of 16, FP8 pages that are not multiples of 16 tokens, very large batches of FP8, pools of unknown
+// length) and for calls too short for it, on mma.sync.m16n8k16.  A key costs 4 head_dim bytes and 4 head_dim flops per
 // row, so that 16 rows ask for 16 flops a byte, where the legacy tensor pipe gives several times that;
 // at 64 rows the two come close.  Measured with 32 requests of 4096 tokens, 8 KV heads of 128, bfloat16:
-// 4 rows 134 us = 0.61 of the copy rate, 64 rows 237 us, 256 rows 867 us (a row tile of 64 after the
-// other, each of which reads the keys again); one request of 1024 tokens, 4 rows, 12.5 us.
+// 4 rows 121 us = 0.68 of the copy rate, 64 rows 231 us, 256 rows 821 us (a row tile of 64 after the
+// other, each of which reads the keys again); one request of 1024 tokens, 4 rows, 12.6 us.
 //
 // A block has four warps and walks its piece of the tile list (tree_common.cuh) in key tiles of 64.
 // MR = 16, 32 or 64 rows: the warps split into MR / 16 row groups and, where there are fewer than

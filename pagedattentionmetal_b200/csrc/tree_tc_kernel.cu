@@ -33,9 +33,9 @@
 // query tile and room for three K stages and five half stages of V; else two query tiles, two and four.
 //
 // What bounds it, measured with 32 requests of 4096 tokens, 8 KV heads of 128, pages of 16: 4 rows,
-// bfloat16, 101 us = 0.81 of the copy rate, 64 rows 109 us = 0.76: HBM.  256 rows (dual) 180 us, 0.95 us a tile
+// bfloat16, 100 us = 0.82 of the copy rate, 64 rows 109 us = 0.77: HBM.  256 rows (dual) 178 us, 0.95 us a tile
 // and group: the chain S -> softmax -> P V of each group (some 3000 cycles), whose instructions come from
-// caches that six kinds of warps share; half of the tensor pipe's rate.  FP8 64 rows 114 us, the same
+// caches that six kinds of warps share; half of the tensor pipe's rate.  FP8 64 rows 116 us, the same
 // chain with scales in it, where the codes would take 38 us.  One request of 1024 tokens 16 us: 9 us of
 // a block's way from start to end, 5 us of the join, launches.
 //
@@ -1084,7 +1084,7 @@ bool treeTcSizes(const TreeParams& p) {
 bool treeTcApplies(const TreeParams& p) {
     if (!treeTcSizes(p)) return false;
     if (p.dtype == kFP8 && smemBytes<false, true>(p.batch) > kSmemLimit) return false;
-    // (rows of the pool are counted in 32 bits)
+    // (rows of the pool are counted in 32 bits; a pool of unknown length is not taken, since the tensor maps need one)
     if (p.poolBlocks <= 0 || p.poolBlocks >= (1 << 30) / (p.kvHeads * p.blockSize)) return false;
     for (int64_t s : {p.qStride, p.kStride, p.vStride})
         if (s % 8) return false;
@@ -1096,8 +1096,8 @@ bool treeTcApplies(const TreeParams& p) {
 // Two query tiles: when a request can have more than 128 rows under a KV head, or the batch's list does
 // not fit beside the longer rings.  Over FP8 pages row tiles are taken one after the other: the ring of
 // codes leaves room for two query tiles and one tile of V, which then waits for the products of the
-// tile before (32 requests of 4096 tokens, 256 rows: 201 us, against 207; one of 8192 tokens 37
-// against 31).
+// tile before (both measured before pages of odd scales were told apart: 32 requests of 4096 tokens, 256 rows: 201 us,
+// against 207, now 219; one of 8192 tokens 37 against 31).
 static bool takesWide(const TreeParams& p) {
     return p.dtype != kFP8 && (static_cast<int64_t>(p.maxNew) * (p.heads / p.kvHeads) > kRows || smemBytes<false, false>(p.batch) > kSmemLimit);
 }
