@@ -1038,9 +1038,9 @@ treeTcKernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ C
             }
             if (!ok) break;
             ++spans;
-            const int before = k;
+            // (given back first: a ring full of spans without tiles of this group would wait for it)
+            spanDone(k);
             k = seek(k + 1);
-            spanDone(before);
         }
     }
 
