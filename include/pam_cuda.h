@@ -579,7 +579,8 @@ int64_t pamc_norm_rotate_backward_workspace(void *ctx, const PamNormRotateBackwa
  * position below the cache length counts as the cache length; without masks and positions row i
  * stands at cache_lengths[b] + i).  A row that sees nothing is written as zero; values and (FP8)
  * scales a row does not see do not reach it, whatever they hold; a key scale that is not a finite
- * number makes the rows that see its page NaN.  Rows outside every request stay as they
+ * number makes the rows that see its page NaN, and a value that is not finite (code times scale)
+ * makes its element of the rows that see it infinite or NaN.  Rows outside every request stay as they
  * were.  Requests beyond max_new_tokens rows are cut off there.
  * Pools of unknown length (bytes = (size_t)-1) are taken, but 16-bit ones not by the tcgen05
  * kernel, which takes a fifth to a quarter of the time with many rows: give them their lengths.
