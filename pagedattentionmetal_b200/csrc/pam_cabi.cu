@@ -378,18 +378,19 @@ int takeWaitWord(Context* c) {
     return site;
 }
 
-// Before a kernel with bounded waits: a word that an earlier launch has set would keep it from starting, and is
-// kept for pamc_synchronize to report.
-cudaError_t beforeBounded(Context* c, bool capturing) {
-    if (c->async || capturing || !(c->errPending || c->errRecorded)) return cudaSuccess;
+// Before kernels with bounded waits that the call itself waits for: a word that an earlier launch has set would keep
+// them from starting, and is kept for pamc_synchronize to report.
+cudaError_t keepEarlierWait(Context* c) {
+    if (!(c->errPending || c->errRecorded)) return cudaSuccess;
     cudaError_t e = fetchWaitWord(c);
     if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
     if (e != cudaSuccess) return e;
     if (const int site = takeWaitWord(c)) c->earlierSite = site;
     return cudaSuccess;
 }
+cudaError_t beforeBounded(Context* c, bool capturing) { return c->async || capturing ? cudaSuccess : keepEarlierWait(c); }
 
-// Behind it.
+// Behind one.
 cudaError_t afterBounded(Context* c, bool capturing) {
     if (capturing) { c->errRecorded = true; return cudaSuccess; }
     c->errPending = true;
@@ -880,7 +881,9 @@ Cache* createCache(Context* c, int32_t maxBlocks, int32_t blockSize, int32_t hea
     return k;
 }
 
-int32_t syncContext(Context* c) {
+// Waits for the context's stream.  `earlier`: reports what earlier launches left, too (else the call has kept that
+// apart before its own).
+int32_t syncContext(Context* c, bool earlier) {
     cudaError_t e = cudaSuccess;
     const bool fetch = c->errPending || c->errRecorded;
     if (fetch) e = fetchWaitWord(c);
@@ -888,8 +891,12 @@ int32_t syncContext(Context* c) {
     if (e != cudaSuccess) { cudaGetLastError(); return c->fail(PAM_ERR_COMMAND_EXECUTION, commandExecutionFailed(cudaGetErrorString(e))); }
     int site = fetch ? takeWaitWord(c) : 0;
     if (site != 0) cudaStreamSynchronize(c->stream);       // (the next replay may be on another stream)
-    if (site == 0) site = c->earlierSite;
-    c->earlierSite = 0;
+    if (earlier) {
+        if (site == 0) site = c->earlierSite;
+        c->earlierSite = 0;
+    } else if (site != 0 && c->errRecorded) {
+        c->earlierSite = site;                             // (a replay on another stream may have set it)
+    }
     if (site == 0) return 0;
     return c->fail(PAM_ERR_COMMAND_EXECUTION, commandExecutionFailed("a kernel's bounded wait ran out (site " + std::to_string(site) + ")"));
 }
@@ -907,13 +914,18 @@ int32_t runLayers(void* ctx, const Rq* requests, int32_t numLayers, F one) {
     if (c->device < 0) return noGpu(c);
     if (!requests || numLayers <= 0) return c->fail(PAM_ERR_INVALID_CONFIGURATION, invalidConfiguration("buffer/layer count mismatch"));
     const bool wasAsync = c->async;
+    if (!wasAsync)
+        if (const cudaError_t e = keepEarlierWait(c); e != cudaSuccess) {
+            cudaGetLastError();
+            return c->fail(PAM_ERR_COMMAND_EXECUTION, commandExecutionFailed(cudaGetErrorString(e)));
+        }
     c->async = true;
     int32_t rc = 0;
     const double t0 = nowMs();
     for (int i = 0; i < numLayers && rc == 0; ++i) rc = one(c, requests[i], i);
     c->async = wasAsync;
     if (!wasAsync) {
-        const int32_t src = syncContext(c);
+        const int32_t src = syncContext(c, false);
         if (rc == 0) rc = src;
     }
     if (rc == 0) {
@@ -1298,7 +1310,7 @@ int32_t pamc_synchronize(void* ctx) {
     std::lock_guard<std::mutex> g(c->mu);
     DeviceGuard dg(c->device);
     if (c->device < 0) return noGpu(c);
-    return syncContext(c);
+    return syncContext(c, true);
 }
 int32_t pamc_set_max_retries(void* ctx, int32_t n) { if (!ctx || n < 0) return -1; asCtx(ctx)->maxRetries = n; return 0; }
 int32_t pamc_set_graceful_degradation(void* ctx, int32_t on) { if (!ctx) return -1; asCtx(ctx)->graceful = on != 0; return 0; }
@@ -2190,6 +2202,10 @@ static int32_t inferFlushPrefill(Inference* inf, std::vector<PendingPrefill>& pe
         std::lock_guard<std::mutex> g(c->mu);
         DeviceGuard dg(c->device);
         const bool wasAsync = c->async;
+        if (const cudaError_t e = keepEarlierWait(c); e != cudaSuccess) {
+            cudaGetLastError();
+            return c->fail(PAM_ERR_COMMAND_EXECUTION, commandExecutionFailed(cudaGetErrorString(e)));
+        }
         c->async = true;                                   // the layers are enqueued back to back, one wait at the end
         for (size_t l = 0; l < inf->layers.size() && rc == 0; ++l) {
             const size_t bytes = totalRows * ioBytesPerToken(inf->layers[l]);
@@ -2198,7 +2214,7 @@ static int32_t inferFlushPrefill(Inference* inf, std::vector<PendingPrefill>& pe
                              buf(k->kScale, k->scaleBytes), buf(k->vScale, k->scaleBytes), seqs, maxNumBlocks, true, "blockTables");
         }
         c->async = wasAsync;
-        const int32_t src = syncContext(c);                // `tables` is read by async copies: wait in either mode
+        const int32_t src = syncContext(c, false);         // `tables` is read by async copies: wait in either mode
         if (rc == 0) rc = src;
         if (rc == 0) c->clearError();
     }

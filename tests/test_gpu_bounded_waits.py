@@ -110,3 +110,24 @@ def test_asynchronous_calls_that_run_out_are_reported(waits, between):
     waits.clear()
     waits.engine.treeAttention(waits.request)
     assert np.array_equal(waits.result(), waits.want)
+
+
+def test_calls_for_several_layers_do_not_take_the_report(waits):
+    """They wait once at their end; a prefill on the tensor cores starts although an earlier wait ran out."""
+    engine, rng = waits.engine, np.random.default_rng(84)
+    up, rows = engine.makeBufferFrom, 40
+    layer = pam.PagedLayerSpec(128, 4, 2, 16, DT.float16)
+    q = up(rng.standard_normal((rows, 4, 128)).astype(np.float16))
+    pools = [up(rng.standard_normal((3, 2, 16, 128)).astype(np.float16)) for _ in range(2)]
+    table, outs = up(np.array([2, 0, 1], np.int32)), [up(np.zeros((rows, 4, 128), np.float16)) for _ in range(2)]
+    prefill = lambda out: engine.prefillLayers([q, q], *pools, table, [out, out], rows, [layer, layer])
+    prefill(outs[0])
+    graph = waits.record(1)
+    waits.replay(graph)
+    prefill(outs[1])
+    assert np.array_equal(*(x.download(np.float16, (rows, 4, 128)) for x in outs))
+    with pytest.raises(pam.PagedAttentionError, match=RAN_OUT):
+        engine.synchronize()
+    prefill(outs[1])
+    engine.synchronize()
+    del graph
