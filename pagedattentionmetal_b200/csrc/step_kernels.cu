@@ -5,8 +5,8 @@
 // Both kernels move a few hundred KB at most and are bound by latency: one launch each, every
 // block derives what it needs of the other requests by itself, no intermediate goes through
 // memory, nothing is synchronised between blocks.  Measured call after call: the plan of 256 requests
-// with one new token 5.0 us, of 64 trees of up to 64 nodes, masks included, 6.5 us; acceptance of 8 trees
-// of up to 16 nodes 5.0 us, of 256 of up to 64 nodes 6.1 us.  A launch and the checks before it
+// with one new token 5.0 us, of 64 trees of up to 64 nodes, masks included, 6.5 to 7.5 us; acceptance of 8 trees
+// of up to 16 nodes 5.0 to 5.6 us, of 256 of up to 64 nodes 6.1 us.  A launch and the checks before it
 // take about 5 us of a processor; what a step of kernels in a graph pays is less.
 #include <algorithm>
 

@@ -81,7 +81,9 @@ struct Span {
     __device__ __forceinline__ bool whole() const { return first == 0 && last == nT; }
 };
 
-constexpr int kSpans = 8;        // of the ring: no warp needs a span more than five behind the oldest one in use
+// Of the ring.  A warp keeps a span only while it works on it, and looks two ahead of that at most (the issuer): it may
+// not keep one while it looks for the next with work for it, since there may be any number of spans in between.
+constexpr int kSpans = 8;
 
 // FP8, of a key tile: per 16 keys (a page holds a multiple of them) the key scale times log2(e) /
 // sqrt(dim), the logarithm of the value scale, and one over it.  Pages with other than positive finite scales
